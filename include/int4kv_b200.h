@@ -423,6 +423,106 @@ cudaError_t int4kv_paged_decode_static_scratch(const float* query, const uint8_t
  * device with a torch copy (src/ops.py:307). */
 cudaError_t int4kv_stage_inputs(void* dst, const void* src, size_t bytes, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving with drafted tokens and sliding windows. No counterpart in the
+ * reference, whose decode takes one query per sequence over its whole cache.
+ * ------------------------------------------------------------------------- */
+
+/* Most drafted tokens of one sequence (one bit of a mask word each). */
+#define INT4KV_MAX_DRAFTS 64
+
+/* Append several tokens per sequence at any position, quantized as they are
+ * written: the general form of int4kv_cache_append. Sequence b holds
+ * start_pos[b] tokens and gets n = tok_offsets[b+1] - tok_offsets[b] <=
+ * max_rows_per_seq more (0: nothing of it is touched); new token i is row
+ * rows[tok_offsets[b] + i] of k / v [num_src, num_heads, head_dim] (type
+ * kv_dtype, INT4KV_VALUES_*; v nullable), or row tok_offsets[b] + i where
+ * `rows` is NULL. `rows` holds num_rows entries: the accepted path of a drafted
+ * tree is written straight from the rows of all drafts. Every touched group is
+ * quantized over all its rows, the first one over the staged rows too, so the
+ * pools equal a bulk int4kv_cache_write of the same tokens bit for bit; after
+ * the call stage slot stage_slots[b] of k_stage [num_slots, group_tokens,
+ * num_heads * head_dim] holds the float32 keys of the group left open (slots
+ * distinct; the pages of the new tokens must be in block_table). Malformed
+ * lengths skip the sequence and set INT4KV_STATUS_BAD_LENGTH, as does an entry of
+ * `rows` outside [0, num_src), whose token is written as zeros; pages outside
+ * the pool are not written (INT4KV_STATUS_BAD_PAGE). */
+cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int num_src,
+                                const int32_t* tok_offsets, const int32_t* start_pos,
+                                const int32_t* rows, int num_rows, const int32_t* stage_slots,
+                                float* k_stage, int num_slots, int batch, int max_rows_per_seq,
+                                int num_heads, int head_dim, int group_tokens, int page_tokens,
+                                const int32_t* block_table, int max_pages, int num_pages,
+                                uint8_t* k_pool, void* v_pool, int value_dtype, float* sz_pool,
+                                uint32_t* status, cudaStream_t stream);
+
+/* Read tokens start_pos[b] + [0, n), n = tok_offsets[b+1] - tok_offsets[b] <=
+ * max_rows_per_seq, of each sequence back into rows tok_offsets[b] .. of k_out /
+ * v_out [num_rows, num_heads, head_dim] of type out_dtype (INT4KV_VALUES_*):
+ * keys as code * s - zp * s in float32, rounded once to the output type, values
+ * widened or rounded (v_pool and v_out both NULL: keys only). Output rows no
+ * range covers, and ranges that do not lie in the table row or the outputs
+ * (INT4KV_STATUS_BAD_LENGTH), are left as they were; tokens of a page outside
+ * the pool read as zeros (INT4KV_STATUS_BAD_PAGE). */
+cudaError_t int4kv_cache_read(const uint8_t* k_pool, const void* v_pool, int value_dtype,
+                              const float* sz_pool, const int32_t* block_table,
+                              const int32_t* start_pos, const int32_t* tok_offsets, int batch,
+                              int num_rows, int max_rows_per_seq, int num_heads, int head_dim,
+                              int group_tokens, int page_tokens, int max_pages, int num_pages,
+                              int out_dtype, void* k_out, void* v_out, uint32_t* status,
+                              cudaStream_t stream);
+
+/* Workspace of the two attentions below, for at most max_drafts drafted tokens
+ * per sequence (1 for the window decode). It needs no initialisation and
+ * carries nothing between calls; calls that may overlap need one each (two
+ * captured graphs replayed at once, two streams). */
+cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                                                  int head_dim, int max_drafts, size_t* bytes);
+
+/* Attention of each sequence's drafted tokens over its cache and, through
+ * tree_mask, over one another: the verification step of speculative decoding.
+ * Rows draft_offsets[b] .. draft_offsets[b+1]-1 (at most max_drafts <=
+ * INT4KV_MAX_DRAFTS; rows of query / k_draft / v_draft / out past the last
+ * sequence's are left as they were) are the drafts of sequence b, whose cache
+ * holds seq_lens[b] tokens, none of them drafts. Draft t sees draft u of its
+ * sequence iff bit u of tree_mask[row of t] is set (its own bit included, if it
+ * is to see itself), and its position is seq_lens[b] + its ancestors, the
+ * other bits set. With window > 0 a query at position p sees position j only
+ * if j > p - window or j < sinks, cached and drafted alike; window 0: all. No
+ * softmax scale (the queries carry it); a row that sees nothing gives zeros.
+ * query / out [num_rows, num_q_heads, head_dim], k_draft / v_draft [num_rows,
+ * num_kv_heads, head_dim], all of type qkv_dtype: float32 with any value pool,
+ * or float16 / bfloat16 with a value pool of the same type (keys and softmax
+ * weights are then rounded to 16 bits for the tensor cores, sums stay
+ * float32). head_dim 64, 128 or 256, pages of 16 tokens, tensors 16-byte
+ * aligned. Cached values that some row of the sequence sees must be finite for
+ * the other rows' results to be. Bad pages are not read (their tokens are not seen); offsets outside
+ * [0, num_rows], too many drafts or bad lengths set INT4KV_STATUS_BAD_LENGTH
+ * and the sequence's drafts are skipped (a length is clamped). */
+cudaError_t int4kv_paged_tree_decode(const void* query, const void* k_draft, const void* v_draft,
+                                     int qkv_dtype, const int64_t* tree_mask,
+                                     const int32_t* draft_offsets, int num_rows, int max_drafts,
+                                     const uint8_t* k_pool, const void* v_pool, int value_dtype,
+                                     const float* sz_pool, const int32_t* block_table,
+                                     const int32_t* seq_lens, int batch, int num_q_heads,
+                                     int num_kv_heads, int head_dim, int page_tokens,
+                                     int group_tokens, int max_pages, int num_pages, int window,
+                                     int sinks, void* out, void* workspace, size_t workspace_bytes,
+                                     uint32_t* status, cudaStream_t stream);
+
+/* int4kv_paged_decode behind a sliding window: the query of each sequence
+ * (one token, already in the cache) sees its last `window` > 0 tokens and the
+ * first `sinks`; only their pages are read. Types, workspace and the rest as
+ * int4kv_paged_tree_decode; an empty cache gives zeros. */
+cudaError_t int4kv_paged_window_decode(const void* query, int query_dtype, const uint8_t* k_pool,
+                                       const void* v_pool, int value_dtype, const float* sz_pool,
+                                       const int32_t* block_table, const int32_t* seq_lens,
+                                       int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                       int page_tokens, int group_tokens, int max_pages,
+                                       int num_pages, int window, int sinks, void* out,
+                                       void* workspace, size_t workspace_bytes, uint32_t* status,
+                                       cudaStream_t stream);
+
 /* Library identification: returns a static string naming the build. */
 const char* int4kv_build_info(void);
 

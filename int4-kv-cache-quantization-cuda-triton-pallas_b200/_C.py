@@ -597,3 +597,253 @@ def paged_decode_split(query, k_pool, v_pool, sz_pool, block_table, seq_lens, pe
             workspace.numel() * workspace.element_size(), _p(status), _stream(query)),
             "paged_decode_split")
     return out
+
+
+# --------------------------------------------------------------------------
+# drafted tokens and sliding windows
+# --------------------------------------------------------------------------
+
+#: most drafted tokens of one sequence (INT4KV_MAX_DRAFTS)
+MAX_DRAFTS = 64
+
+
+def _check_int32(t, name, n=None):
+    _check_input(t, name)
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise RuntimeError(f"{name} must be int32 [{'entries' if n is None else n}]")
+
+
+def _check_status(status):
+    if status is not None and (not status.is_cuda or status.dtype != torch.int32 or status.numel() < 1):
+        raise RuntimeError("status must be an int32 CUDA tensor")
+
+
+def _check_groups(group_tokens, most=None):
+    if group_tokens <= 0 or group_tokens % PAGE_TOKENS or (most and group_tokens > most):
+        raise RuntimeError(f"group_tokens must be a positive multiple of {PAGE_TOKENS}"
+                           + (f" up to {most}" if most else "") + f", got {group_tokens}")
+
+
+def cache_extend(k, v, tok_offsets, start_pos, stage_slots, k_stage, block_table, k_pool, v_pool,
+                 sz_pool, max_rows_per_seq, group_tokens=128, rows=None, status=None):
+    """Append several tokens per sequence, quantized as they are written (int4kv_cache_extend).
+
+    Sequence b holds ``start_pos[b]`` tokens and gets ``tok_offsets[b+1] - tok_offsets[b]`` (at
+    most ``max_rows_per_seq``) rows of ``k`` / ``v`` [rows, kv_heads, head_dim] (float32, float16
+    or bfloat16); with ``rows`` (int32) new token i is input row ``rows[tok_offsets[b] + i]``, the
+    accepted path out of all drafted rows. ``k_stage`` keeps the float32 keys of the open groups,
+    as for ``cache_append``; the pools equal a bulk write of the same tokens bit for bit.
+    """
+    lib = _lib.load()
+    num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)
+    _check_input(k, "k")
+    if k.dtype not in VALUE_KINDS or k.dim() != 3 or tuple(k.shape[1:]) != (hkv, d):
+        raise RuntimeError(f"k must be float32, float16 or bfloat16 [rows, {hkv}, {d}]")
+    if v is not None:
+        _check_input(v, "v")
+        if v.dtype != k.dtype or v.shape != k.shape:
+            raise RuntimeError("v must have the type and shape of k")
+        if v_pool is None:
+            raise RuntimeError("v needs a v_pool")
+    _check_int32(tok_offsets, "tok_offsets")
+    b = tok_offsets.shape[0] - 1
+    if b <= 0:
+        raise RuntimeError("tok_offsets must describe at least one sequence")
+    _check_int32(start_pos, "start_pos", b)
+    _check_int32(stage_slots, "stage_slots", b)
+    if rows is not None:
+        _check_int32(rows, "rows")
+    _check_groups(group_tokens, 128)
+    if page != PAGE_TOKENS:
+        raise RuntimeError(f"cache_extend needs {PAGE_TOKENS}-token pages, got {page}")
+    _check_input(k_stage, "k_stage")
+    if k_stage.dtype != torch.float32 or k_stage.dim() != 3 or \
+            tuple(k_stage.shape[1:]) != (group_tokens, hkv * d):
+        raise RuntimeError(f"k_stage must be float32 [slots, {group_tokens}, {hkv * d}]")
+    if max_rows_per_seq < 0:
+        raise RuntimeError("max_rows_per_seq must not be negative")
+    max_pages = _check_table(block_table, b)
+    _check_status(status)
+    _same_device(k, v, tok_offsets, start_pos, stage_slots, rows, k_stage, block_table, k_pool,
+                 v_pool, sz_pool, status)
+    vk = VALUE_KINDS[v_pool.dtype] if v_pool is not None else 0
+    with torch.cuda.device(k.device):
+        _lib.check(lib.int4kv_cache_extend(
+            _p(k), _p(v), VALUE_KINDS[k.dtype], k.shape[0], _p(tok_offsets), _p(start_pos),
+            _p(rows), rows.shape[0] if rows is not None else k.shape[0],
+            _p(stage_slots), _p(k_stage), k_stage.shape[0], b, int(max_rows_per_seq), hkv, d,
+            group_tokens, page, _p(block_table), max_pages, num_pages, _p(k_pool), _p(v_pool), vk,
+            _p(sz_pool), _p(status), _stream(k)), "cache_extend")
+
+
+def cache_read(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, num_rows,
+               max_rows_per_seq, group_tokens=128, dtype=torch.float32, k_out=None, v_out=None,
+               status=None):
+    """Read tokens ``start_pos[b] + [0, tok_offsets[b+1] - tok_offsets[b])`` of each sequence back.
+
+    Returns dense keys and values [num_rows, kv_heads, head_dim] of ``dtype`` (int4kv_cache_read);
+    ``v_pool=None`` reads keys only (values None). Rows that no range covers keep what ``k_out`` /
+    ``v_out`` held (new outputs: unspecified).
+    """
+    lib = _lib.load()
+    num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)
+    _check_int32(start_pos, "start_pos")
+    b = start_pos.shape[0]
+    if b <= 0:
+        raise RuntimeError("start_pos must describe at least one sequence")
+    _check_int32(tok_offsets, "tok_offsets", b + 1)
+    max_pages = _check_table(block_table, b)
+    _check_groups(group_tokens)
+    if group_tokens % page:
+        raise RuntimeError(f"group_tokens must be a multiple of the page ({page})")
+    if num_rows < 0 or max_rows_per_seq < 0:
+        raise RuntimeError("num_rows and max_rows_per_seq must not be negative")
+    if dtype not in VALUE_KINDS:
+        raise RuntimeError(f"dtype must be one of {list(VALUE_KINDS)}")
+    if v_pool is None and v_out is not None:
+        raise RuntimeError("v_out needs a v_pool")
+    shape = (int(num_rows), hkv, d)
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is not None:
+            _check_input(t, name)
+            if t.dtype != dtype or tuple(t.shape) != shape:
+                raise RuntimeError(f"{name} must be {dtype} {list(shape)}")
+    _check_status(status)
+    _same_device(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, k_out, v_out, status)
+    with torch.cuda.device(k_pool.device):
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=dtype, device=k_pool.device)
+        if v_pool is not None and v_out is None:
+            v_out = torch.empty(shape, dtype=dtype, device=k_pool.device)
+        _lib.check(lib.int4kv_cache_read(
+            _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype] if v_pool is not None else 0,
+            _p(sz_pool), _p(block_table), _p(start_pos), _p(tok_offsets), b, shape[0],
+            int(max_rows_per_seq), hkv, d, group_tokens, page, max_pages, num_pages,
+            VALUE_KINDS[dtype], _p(k_out), _p(v_out), _p(status), _stream(k_pool)), "cache_read")
+    return k_out, v_out
+
+
+def paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_drafts=1, device=None):
+    """Workspace bytes of ``paged_tree_decode`` (``max_drafts`` per sequence) and
+    ``paged_window_decode`` (``max_drafts=1``); needs no initialisation."""
+    import ctypes
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        _lib.check(lib.int4kv_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim,
+                                                             max_drafts, ctypes.byref(need)),
+                   "paged_attention_workspace_size")
+    return need.value
+
+
+def _check_attention(query, hkv, d, page, v_pool, group_tokens, sinks):
+    if v_pool is None:
+        raise RuntimeError("v_pool is required")
+    _check_input(query, "query")
+    if query.dtype not in VALUE_KINDS or query.dim() != 3:
+        raise RuntimeError("query must be float32, float16 or bfloat16 [rows, heads, head_dim]")
+    if query.dtype != torch.float32 and v_pool.dtype != query.dtype:
+        raise RuntimeError(f"a {query.dtype} query needs a value pool of its type, got {v_pool.dtype}; "
+                           "a float32 query takes any value pool")
+    rows, hq, qd = query.shape
+    if qd != d:
+        raise RuntimeError(f"query head_dim {qd} != pool head_dim {d}")
+    if d not in (64, 128, 256):
+        raise RuntimeError(f"paged attention supports head_dim in (64, 128, 256), got {d}")
+    if page != PAGE_TOKENS:
+        raise RuntimeError(f"paged attention needs {PAGE_TOKENS}-token pages, got {page}")
+    if hq < hkv or hq % hkv:
+        raise RuntimeError(f"query heads ({hq}) must be a multiple of kv heads ({hkv})")
+    _check_groups(group_tokens)
+    if sinks < 0:
+        raise RuntimeError(f"sinks must not be negative, got {sinks}")
+    return rows, hq
+
+
+def _attention_buffers(query, out, workspace, need):
+    if out is None:
+        out = torch.empty_like(query)
+    elif out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous with the type and shape of query")
+    if workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=query.device)
+    elif not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise RuntimeError(f"workspace needs {need} contiguous bytes")
+    return out, workspace
+
+
+def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool, v_pool, sz_pool,
+                      block_table, seq_lens, max_drafts, group_tokens=128, window=None, sinks=0,
+                      out=None, workspace=None, status=None):
+    """Attention of drafted tokens over the paged INT4 cache and one another (int4kv_paged_tree_decode).
+
+    query [rows, heads, head_dim], k_draft / v_draft [rows, kv_heads, head_dim]: rows
+    ``draft_offsets[b] .. draft_offsets[b+1] - 1`` (at most ``max_drafts`` <= MAX_DRAFTS) are the
+    drafts of sequence b, none of them in its cache of ``seq_lens[b]`` tokens. Bit u of
+    ``tree_mask[row]`` (int64; ``paged.tree_mask``) lets a draft see draft u of its sequence. With
+    ``window`` a query at position p sees positions above p - window and the first ``sinks`` only.
+    float32 with any value pool, or float16 / bfloat16 with a value pool of the same type. Rows
+    past the last sequence's are left as ``out`` held them. A ``workspace`` belongs to one call at
+    a time; None allocates one.
+    """
+    lib = _lib.load()
+    num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)
+    _check_int32(seq_lens, "seq_lens")
+    b = seq_lens.shape[0]
+    rows, hq = _check_attention(query, hkv, d, page, v_pool, group_tokens, sinks)
+    for t, name in ((k_draft, "k_draft"), (v_draft, "v_draft")):
+        _check_input(t, name)
+        if t.dtype != query.dtype or tuple(t.shape) != (rows, hkv, d):
+            raise RuntimeError(f"{name} must be {query.dtype} [{rows}, {hkv}, {d}]")
+    _check_input(tree_mask, "tree_mask")
+    if tree_mask.dtype != torch.int64 or tuple(tree_mask.shape) != (rows,):
+        raise RuntimeError(f"tree_mask must be int64 [{rows}]")
+    _check_int32(draft_offsets, "draft_offsets", b + 1)
+    max_pages = _check_table(block_table, b)
+    if not 0 <= max_drafts <= MAX_DRAFTS:
+        raise RuntimeError(f"max_drafts must be in [0, {MAX_DRAFTS}], got {max_drafts}")
+    if window is not None and window <= 0:
+        raise RuntimeError(f"window must be positive (None: no window), got {window}")
+    _check_status(status)
+    _same_device(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool, v_pool, sz_pool,
+                 block_table, seq_lens, out, workspace, status)
+    with torch.cuda.device(query.device):
+        need = paged_attention_workspace_bytes(b, hq, hkv, d, max_drafts, query.device)
+        out, workspace = _attention_buffers(query, out, workspace, need)
+        _lib.check(lib.int4kv_paged_tree_decode(
+            _p(query), _p(k_draft), _p(v_draft), VALUE_KINDS[query.dtype], _p(tree_mask),
+            _p(draft_offsets), rows, int(max_drafts), _p(k_pool), _p(v_pool),
+            VALUE_KINDS[v_pool.dtype], _p(sz_pool), _p(block_table), _p(seq_lens), b, hq, hkv, d,
+            page, group_tokens, max_pages, num_pages, int(window or 0), int(sinks), _p(out),
+            _p(workspace), workspace.numel() * workspace.element_size(), _p(status),
+            _stream(query)), "paged_tree_decode")
+    return out
+
+
+def paged_window_decode(query, k_pool, v_pool, sz_pool, block_table, seq_lens, window, sinks=0,
+                        group_tokens=128, out=None, workspace=None, status=None):
+    """Decode over the last ``window`` and the first ``sinks`` tokens (int4kv_paged_window_decode).
+
+    query [batch, heads, head_dim], one token per sequence, already in its cache of ``seq_lens``
+    tokens (as for ``paged_decode``); only the visible pages are read. Types and ``workspace`` as
+    for ``paged_tree_decode``.
+    """
+    lib = _lib.load()
+    num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)
+    b, hq = _check_attention(query, hkv, d, page, v_pool, group_tokens, sinks)
+    _check_int32(seq_lens, "seq_lens", b)
+    max_pages = _check_table(block_table, b)
+    if window is None or window <= 0:
+        raise RuntimeError(f"window must be positive, got {window}")
+    _check_status(status)
+    _same_device(query, k_pool, v_pool, sz_pool, block_table, seq_lens, out, workspace, status)
+    with torch.cuda.device(query.device):
+        need = paged_attention_workspace_bytes(b, hq, hkv, d, 1, query.device)
+        out, workspace = _attention_buffers(query, out, workspace, need)
+        _lib.check(lib.int4kv_paged_window_decode(
+            _p(query), VALUE_KINDS[query.dtype], _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype],
+            _p(sz_pool), _p(block_table), _p(seq_lens), b, hq, hkv, d, page, group_tokens,
+            max_pages, num_pages, int(window), int(sinks), _p(out), _p(workspace),
+            workspace.numel() * workspace.element_size(), _p(status), _stream(query)),
+            "paged_window_decode")
+    return out

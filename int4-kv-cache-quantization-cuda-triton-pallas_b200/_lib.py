@@ -64,6 +64,19 @@ _PROTOS = {
     "int4kv_ipc_handle": [_c_void_p, _c_void_p],
     "int4kv_ipc_open": [_c_void_p, ctypes.POINTER(_c_void_p)],
     "int4kv_ipc_close": [_c_void_p],
+    "int4kv_cache_extend": [_c_void_p, _c_void_p, _c_int, _c_int] + [_c_void_p] * 3
+                           + [_c_int, _c_void_p, _c_void_p] + [_c_int] * 7
+                           + [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int]
+                           + [_c_void_p] * 3,
+    "int4kv_cache_read": [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 4 + [_c_int] * 10
+                         + [_c_void_p] * 4,
+    "int4kv_paged_attention_workspace_size": [_c_int] * 5 + [_c_size_p],
+    "int4kv_paged_tree_decode": [_c_void_p] * 3 + [_c_int] + [_c_void_p] * 2 + [_c_int] * 2
+                                + [_c_void_p, _c_void_p, _c_int] + [_c_void_p] * 3 + [_c_int] * 10
+                                + [_c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_void_p],
+    "int4kv_paged_window_decode": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int]
+                                  + [_c_void_p] * 3 + [_c_int] * 10
+                                  + [_c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_void_p],
     "int4kv_paged_decode_static_scratch": [_c_void_p] * 6 + [_c_int] * 8
                                           + [_c_void_p, _c_void_p, _c_size_p, _c_void_p],
 }

@@ -1,0 +1,376 @@
+// Work decomposition shared by the kernels in which several queries of a
+// sequence attend over its paged INT4 cache (drafted trees, sliding windows).
+//
+// Sequence b has `rows` query rows per kv head, row = draft * G + (query head
+// of the group), in chunks of NR rows; a stream is one (b, kv head, chunk). Its
+// work is a list of tiles: the visible pages of the cache, TP at a time (the
+// pages of the sinks and of the window are one list without the pages between
+// them), then the drafted tokens. The streams' tiles are laid end to end and
+// every CTA takes one contiguous run of equal length, so the CTAs do the same
+// number of tiles whatever the lengths are. A stream inside one run is finished
+// by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per row,
+// and merge_records_kernel, one block per run boundary, combines them. The
+// records need no counters, so the workspace carries nothing between launches,
+// and their order of combination is fixed: equal inputs give equal bits.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "../../include/int4kv_b200.h"
+
+namespace i4kv {
+
+constexpr int kMqPage = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMqMaxDrafts = INT4KV_MAX_DRAFTS;
+
+struct MultiQueryArgs {
+  const void* q;               // [rows, Hq, D] of kind qk
+  const void* kd;              // [rows, Hkv, D] drafted keys / values of kind qk (tree only)
+  const void* vd;
+  const int64_t* mask;         // [rows] bit u: draft u of the same sequence is visible (tree only)
+  const int32_t* offs;         // [B+1] rows of each sequence (null: one row each, already cached)
+  const uint8_t* k_pool;
+  const void* v_pool;
+  const float* sz_pool;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  void* out;                   // [rows, Hq, D] of kind qk
+  float* recs;                 // two records per CTA
+  uint32_t* status;
+  int qk, batch, kv_heads, group_q, total_rows, max_drafts;
+  int max_pages, num_pages, group_pages;
+  int window, sinks;           // window 0: the whole cache
+};
+
+// What one sequence asks for.
+struct SeqWork {
+  int len, drafts, row0, rows, chunks;
+  int pos0;                    // position of a query without drafted ancestors
+  int sink_pages, win_page;    // visible pages: [0, sink_pages) and [win_page, pages)
+  int vis_pages, cache_tiles, tiles;
+};
+
+I4KV_DEVINL void mq_status(uint32_t* status, uint32_t bits) {
+  if (status) atomicOr(status, bits);
+}
+
+template <int NR, int TP>
+I4KV_DEVINL SeqWork seq_work(const MultiQueryArgs& a, int b, bool report) {
+  SeqWork w;
+  const int cap = a.max_pages * kMqPage;  // < 2^31 - 128 (checked on the host)
+  int len = a.seq_lens[b];
+  bool bad = len < 0 || len > cap;
+  w.len = len < 0 ? 0 : (len > cap ? cap : len);
+  if (a.offs) {
+    const int lo = a.offs[b], hi = a.offs[b + 1];
+    const long long n = (long long)hi - lo;
+    const bool ok = lo >= 0 && n >= 0 && n <= a.max_drafts && hi <= a.total_rows;
+    bad |= !ok;
+    w.row0 = ok ? lo : 0;
+    w.drafts = ok ? (int)n : 0;
+    w.rows = w.drafts * a.group_q;
+    w.pos0 = w.len;
+  } else {
+    w.row0 = b;
+    w.drafts = 0;
+    w.rows = a.group_q;
+    w.pos0 = w.len - 1;
+  }
+  if (bad && report) mq_status(a.status, kStatusBadLength);
+  w.chunks = (w.rows + NR - 1) / NR;
+  const int pages = (w.len + kMqPage - 1) / kMqPage;
+  w.sink_pages = 0;
+  w.win_page = 0;
+  if (a.window > 0) {
+    const int lo = w.pos0 - a.window + 1;  // first windowed position of the lowest query
+    if (lo > 0) {
+      w.win_page = min(lo / kMqPage, pages);
+      const int sp = (int)(((long long)min(a.sinks, w.len) + kMqPage - 1) / kMqPage);
+      if (sp >= w.win_page) w.win_page = 0;
+      else w.sink_pages = sp;
+    }
+  }
+  w.vis_pages = w.sink_pages + pages - w.win_page;
+  w.cache_tiles = (w.vis_pages + TP - 1) / TP;
+  w.tiles = w.rows > 0 ? w.cache_tiles + (w.drafts + TP * kMqPage - 1) / (TP * kMqPage) : 0;
+  return w;
+}
+
+I4KV_DEVINL int visible_page(const SeqWork& w, int i) {
+  return i < w.sink_pages ? i : i - w.sink_pages + w.win_page;
+}
+
+// Place of one tile in the end-to-end order.
+struct TileAt {
+  int b, head, chunk, tile;
+};
+
+template <int NR, int TP>
+I4KV_DEVINL long long seq_units(const MultiQueryArgs& a, int b, bool report) {
+  const SeqWork w = seq_work<NR, TP>(a, b, report);
+  return (long long)w.tiles * w.chunks * a.kv_heads;
+}
+
+// Block-wide: total number of tiles, and the sequence that holds tile
+// pick(total) with the tiles before that sequence. `s_tmp`: 3 + warps int64 of
+// shared memory. Every thread of the block calls it.
+template <int NR, int TP, typename Pick>
+__device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, Pick pick, int& b_out,
+                                     long long& before_out) {
+  const int nt = blockDim.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int per = (a.batch + nt - 1) / nt;
+  const int lo = min(a.batch, t * per), hi = min(a.batch, lo + per);
+  long long local = 0;
+  for (int b = lo; b < hi; ++b) local += seq_units<NR, TP>(a, b, blockIdx.x == 0);
+  long long incl = local;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_tmp[3 + warp] = incl;
+  __syncthreads();
+  if (t == 0) {
+    long long run = 0;
+    for (int i = 0; i < nt / 32; ++i) {
+      const long long v = s_tmp[3 + i];
+      s_tmp[3 + i] = run;
+      run += v;
+    }
+    s_tmp[0] = run;
+    s_tmp[1] = 0;
+    s_tmp[2] = 0;
+  }
+  __syncthreads();
+  const long long total = s_tmp[0];
+  const long long u = pick(total);
+  long long base = s_tmp[3 + warp] + incl - local;
+  if (u >= base && u < base + local) {
+    for (int b = lo; b < hi; ++b) {
+      const long long n = seq_units<NR, TP>(a, b, false);
+      if (u < base + n) {
+        s_tmp[1] = b;
+        s_tmp[2] = base;
+        break;
+      }
+      base += n;
+    }
+  }
+  __syncthreads();
+  b_out = (int)s_tmp[1];
+  before_out = s_tmp[2];
+  __syncthreads();
+  return total;
+}
+
+// First tile of CTA c of n (n <= total): contiguous runs of equal length.
+I4KV_DEVINL long long run_start(long long c, long long total, long long n) { return c * total / n; }
+I4KV_DEVINL long long run_of(long long u, long long total, long long n) { return ((u + 1) * n - 1) / total; }
+
+I4KV_DEVINL TileAt tile_at(const MultiQueryArgs& a, const SeqWork& w, int b, long long rem) {
+  TileAt p;
+  const int per_head = w.tiles * w.chunks;
+  p.b = b;
+  p.head = (int)(rem / per_head);
+  const int r = (int)(rem - (long long)p.head * per_head);
+  p.chunk = r / w.tiles;
+  p.tile = r - p.chunk * w.tiles;
+  return p;
+}
+
+// Step to the next stream; `w` follows the sequence. False past the last one.
+template <int NR, int TP>
+I4KV_DEVINL bool next_stream(const MultiQueryArgs& a, SeqWork& w, TileAt& p) {
+  p.tile = 0;
+  if (++p.chunk < w.chunks) return true;
+  p.chunk = 0;
+  if (++p.head < a.kv_heads) return true;
+  p.head = 0;
+  while (++p.b < a.batch) {
+    w = seq_work<NR, TP>(a, p.b, false);
+    if (w.tiles > 0 && w.rows > 0) return true;
+  }
+  return false;
+}
+
+// Element offset of row r of a stream's chunk in q / out.
+I4KV_DEVINL size_t row_offset(const MultiQueryArgs& a, const SeqWork& w, int head, int rr, int D) {
+  const int t = rr / a.group_q, g = rr - t * a.group_q;
+  return ((size_t)(w.row0 + t) * a.kv_heads * a.group_q + (size_t)head * a.group_q + g) * D;
+}
+
+// Drafted ancestors of draft t (its position behind the cache).
+I4KV_DEVINL int draft_depth(uint64_t word, int t, int drafts) {
+  const uint64_t real = drafts >= 64 ? ~0ull : (1ull << drafts) - 1;
+  return __popcll(word & real & ~(1ull << t));
+}
+
+template <int N>
+I4KV_DEVINL void load_f32(const void* base, int kind, size_t i, float (&x)[N]) {
+  if (kind == INT4KV_VALUES_F32) {
+    const float* p = static_cast<const float*>(base) + i;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p + j);
+      x[j] = v.x;
+      x[j + 1] = v.y;
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + j);
+      if (kind == INT4KV_VALUES_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        x[j] = f.x;
+        x[j + 1] = f.y;
+      } else {
+        x[j] = __uint_as_float(w << 16);
+        x[j + 1] = __uint_as_float(w & 0xFFFF0000u);
+      }
+    }
+  }
+}
+
+I4KV_DEVINL void store2(void* base, int kind, size_t i, float x, float y) {
+  if (kind == INT4KV_VALUES_F32) {
+    *reinterpret_cast<float2*>(static_cast<float*>(base) + i) = make_float2(x, y);
+  } else if (kind == INT4KV_VALUES_F16) {
+    *reinterpret_cast<__half2*>(static_cast<__half*>(base) + i) = __floats2half2_rn(x, y);
+  } else {
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(base) + i) = __floats2bfloat162_rn(x, y);
+  }
+}
+
+// A CTA's record of one stream: m [NR] (natural units), l [NR], acc [NR, D].
+template <int NR, int D>
+struct Record {
+  static constexpr int kFloats = 2 * NR + NR * D;
+};
+
+// Rows of sequences that see nothing (a window over an empty cache) are zeros.
+template <int NR, int TP, int D>
+__device__ void zero_idle_rows(const MultiQueryArgs& a) {
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    const SeqWork w = seq_work<NR, TP>(a, b, false);
+    if (w.tiles > 0 || w.rows == 0) continue;
+    const int n = a.kv_heads * a.group_q * D;  // one row a sequence
+    for (int i = 2 * threadIdx.x; i < n; i += 2 * blockDim.x)
+      store2(a.out, a.qk, (size_t)w.row0 * n + i, 0.f, 0.f);
+  }
+}
+
+I4KV_DEVINL float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+constexpr int kMergeWarps = 8;
+
+// Combine the records of the streams that lie across run boundaries: block x
+// looks at the boundary between runs x and x + 1, and merges the stream there if
+// it is the stream's first boundary; blocks y take kMergeWarps rows each, one
+// warp a row. Plain float32 with weights e^(m_i - M): a handful of terms.
+template <int NR, int TP, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQueryArgs a, int runs) {
+  __shared__ long long s_tmp[3 + kMergeWarps];
+  grid_dependency_wait();
+  int b;
+  long long before;
+  const long long c = blockIdx.x;
+  const long long total = locate_sequence<NR, TP>(
+      a, s_tmp, [&](long long n) { return run_start(c + 1, n, min((long long)runs, n)) - 1; }, b, before);
+  const long long n = min((long long)runs, total);
+  if (c + 1 >= n) return;
+  const SeqWork w = seq_work<NR, TP>(a, b, false);
+  const long long edge = run_start(c + 1, total, n);
+  const TileAt p = tile_at(a, w, b, edge - 1 - before);
+  const long long s0 = edge - 1 - p.tile, s1 = s0 + w.tiles;
+  if (s1 == edge || s0 < run_start(c, total, n)) return;
+  const int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int rr = p.chunk * NR + r;
+  if (rr >= w.rows) return;
+  const long long last = run_of(s1 - 1, total, n);
+  constexpr int kRec = Record<NR, D>::kFloats;
+  auto record = [&](long long i) {
+    const bool tail = i == c && run_start(c, total, n) != s0;  // the stream begins inside run c
+    return a.recs + (2 * i + (tail ? 1 : 0)) * (size_t)kRec;
+  };
+  float M = -INFINITY;
+  for (long long i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(record(i) + r));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  float L = 0.f, o[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+  if (M != -INFINITY) {
+    for (long long i = c; i <= last; ++i) {
+      const float* rec = record(i);
+      const float e = exp2_fast((__ldcg(rec + r) - M) * kLog2e);
+      L = fmaf(__ldcg(rec + NR + r), e, L);
+      const float* acc = rec + 2 * NR + (size_t)r * D;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(acc + 64 * k + 2 * lane));
+        o[2 * k] = fmaf(x.x, e, o[2 * k]);
+        o[2 * k + 1] = fmaf(x.y, e, o[2 * k + 1]);
+      }
+    }
+  }
+  const float inv = 1.f / fmaxf(L, 1e-10f);
+  const size_t to = row_offset(a, w, p.head, rr, D);
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) store2(a.out, a.qk, to + 64 * k + 2 * lane, o[2 * k] * inv, o[2 * k + 1] * inv);
+}
+
+// Resident CTAs per SM of kernel Kern with `smem` dynamic bytes, once per kernel and
+// device (also raises the kernel's shared-memory limit there).
+template <auto Kern>
+cudaError_t mq_occupancy(int threads, size_t smem, int* per_sm) {
+  static std::mutex mu;
+  static int known[64];  // 0: not asked yet
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!known[dev]) {
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    int n = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, smem);
+    if (e != cudaSuccess) return e;
+    if (n < 1) return cudaErrorInvalidConfiguration;
+    known[dev] = n;
+  }
+  *per_sm = known[dev];
+  return cudaSuccess;
+}
+
+// Launch with programmatic stream serialization: the kernel's CTAs may be
+// placed while its predecessor ends; it waits for it before it reads.
+template <typename... KArgs, typename... Args>
+cudaError_t mq_launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          Args... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+}  // namespace i4kv

@@ -602,6 +602,174 @@ append_quant_kernel(AppendArgs ap, int C, int R, OutPaged op) {
   }
 }
 
+// Several tokens per sequence, quantized as they are written
+// (int4kv_cache_extend): the general form of append_quant_kernel. Sequence b's
+// n = tok_off[b+1] - tok_off[b] new rows take the positions start[b] ..; every
+// group they touch is quantized over all of its rows, the first one over its
+// staged rows as well, so the pools equal a bulk write of the same tokens bit
+// for bit. Row i of sequence b is input row rows[tok_off[b] + i] (rows NULL:
+// tok_off[b] + i): the accepted path of a drafted tree is taken from the rows
+// of all its drafts without a gather.
+//
+// Grid: x = 128-channel slabs, y = touched groups (the first is open groups'
+// common case, the rest only long chunks reach), z = sequences. A CTA holds
+// its group's rows in registers between the min / max and the codes. The
+// staged rows of the old open group are read by the y = 0 CTA alone, and the
+// same CTA writes those of the new one after the barrier that follows its
+// reads: when the rows cross a group boundary the slot is reused in place.
+// Bound by HBM bytes for long chunks, by launch and two dependent loads
+// (metadata, rows) for a few tokens.
+struct ExtendArgs {
+  const void* k;             // [num_src, C] keys of the kernel's input type
+  const void* v;             // [num_src, C] (nullable)
+  const int32_t* tok_off;    // [B+1]
+  const int32_t* start;      // [B] tokens already in each sequence
+  const int32_t* rows;       // [>= tok_off[B]] input row of each new token (nullable)
+  int num_src, num_rows;     // rows of k / v, entries of `rows` (or num_src)
+  const int32_t* slot;       // [B] staging slots, distinct
+  float* stage;              // [slots, R, C]
+  int num_slots, max_rows;
+};
+
+// Four consecutive input channels widened to float32 (kind INT4KV_VALUES_*).
+template <int KIND>
+__device__ __forceinline__ float4 load4_as_f32(const void* base, size_t i) {
+  if constexpr (KIND == INT4KV_VALUES_F32) {
+    return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + i));
+  } else {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + i));
+    if constexpr (KIND == INT4KV_VALUES_F16) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+      return make_float4(a.x, a.y, b.x, b.y);
+    } else {
+      return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u),
+                         __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+    }
+  }
+}
+
+// Store four values into the pool's kind, rounded to nearest even.
+__device__ __forceinline__ void store_value4(const OutPaged& op, size_t vi, const float4& vv) {
+  if (op.vk == INT4KV_VALUES_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(op.v_pool) + vi) = vv;
+  } else if (op.vk == INT4KV_VALUES_F16) {
+    const __half2 x = __floats2half2_rn(vv.x, vv.y), y = __floats2half2_rn(vv.z, vv.w);
+    *reinterpret_cast<uint2*>(static_cast<__half*>(op.v_pool) + vi) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  } else {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(vv.x, vv.y), y = __floats2bfloat162_rn(vv.z, vv.w);
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(op.v_pool) + vi) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+  }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kQuantThreads)
+extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
+  __shared__ __align__(16) float s_min[kQuantWarps * kSlab];
+  __shared__ __align__(16) float s_max[kQuantWarps * kSlab];
+  __shared__ __align__(16) float s_lo[kSlab];
+  __shared__ __align__(16) float s_sc[kSlab];
+  __shared__ __align__(16) float s_rc[kSlab];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slab_c0 = blockIdx.x * kSlab;
+  const int c0 = slab_c0 + lane * 4;
+  const int b = blockIdx.z;
+  const int off = ea.tok_off[b], n = ea.tok_off[b + 1] - off, start = ea.start[b], sl = ea.slot[b];
+  if (n == 0) return;  // takes no part: nothing of it is read or written
+  // 64-bit sums: malformed metadata must not wrap into range
+  const bool bad = n < 0 || n > ea.max_rows || off < 0 || (long long)off + n > ea.num_rows ||
+                   start < 0 || (long long)start + n > (long long)op.max_pages * op.page ||
+                   sl < 0 || sl >= ea.num_slots;
+  if (bad) {
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0 && op.status)
+      atomicOr(op.status, kStatusBadLength);
+    return;
+  }
+  const int end = start + n;
+  const int gpos = (start / R + (int)blockIdx.y) * R;  // the group's first token
+  if (gpos >= end) return;
+  const int rows = min(R, end - gpos);
+  const bool lane_ok = c0 < C;
+  float* stage = ea.stage + (size_t)sl * R * C;
+  auto source = [&](int pos) -> long long {  // input row of the new token at `pos`, -1 if malformed
+    const int i = off + pos - start;
+    const int r = ea.rows ? __ldg(ea.rows + i) : i;
+    return (r >= 0 && r < ea.num_src) ? (long long)r : -1;
+  };
+
+  float4 vals[kMaxRowsPerWarp];
+  float4 mn = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
+  float4 mx = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  bool lost = false;
+#pragma unroll
+  for (int i = 0; i < kMaxRowsPerWarp; ++i) {
+    const int r = warp + i * kQuantWarps;
+    if (r < rows && lane_ok) {
+      if (gpos + r < start) {
+        vals[i] = *reinterpret_cast<const float4*>(stage + (size_t)r * C + c0);
+      } else {
+        const long long src = source(gpos + r);
+        lost |= src < 0;
+        vals[i] = src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
+      }
+      minmax4(vals[i], mn, mx);
+    }
+  }
+  if (lost && op.status) atomicOr(op.status, kStatusBadLength);
+  const int32_t* row_bt = op.block_table + (size_t)b * op.max_pages;
+  int gslot = row_bt[gpos / op.page];
+  if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
+  // (its barriers also order this CTA's reads of the staged rows before the
+  // writes of the new open group's below)
+  reduce_params(mn, mx, s_min, s_max, s_lo, s_sc, s_rc, slab_c0, C, [&](int ch, float sc, float zp) {
+    if (gslot < 0) return;
+    const int h = ch / op.head_dim, d = ch - h * op.head_dim;
+    float* dst = op.sz_pool + ((size_t)gslot * op.heads + h) * 2 * op.head_dim;
+    dst[d] = sc;
+    dst[op.head_dim + d] = zp;
+  });
+  if (gslot < 0 && threadIdx.x == 0 && op.status) atomicOr(op.status, kStatusBadPage);
+  if (!lane_ok) return;
+  const int open0 = end - end % R;  // first token of the group left open (== end: none)
+  if (blockIdx.y == 0 && open0 >= gpos + R) {
+    // the rows crossed into another open group: its rows go over the old ones
+    for (int pos = open0 + warp; pos < end; pos += kQuantWarps) {
+      const long long src = source(pos);
+      *reinterpret_cast<float4*>(stage + (size_t)(pos - open0) * C + c0) =
+          src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
+    }
+  }
+  const float4 lo = reinterpret_cast<const float4*>(s_lo)[lane];
+  const float4 sc = reinterpret_cast<const float4*>(s_sc)[lane];
+  const float4 rc = reinterpret_cast<const float4*>(s_rc)[lane];
+  const int h = c0 / op.head_dim, d = c0 - h * op.head_dim;
+#pragma unroll
+  for (int i = 0; i < kMaxRowsPerWarp; ++i) {
+    const int r = warp + i * kQuantWarps;
+    if (r < rows) {
+      const int pos = gpos + r;
+      const bool fresh = pos >= start;
+      if (blockIdx.y == 0 && fresh && open0 == gpos)
+        *reinterpret_cast<float4*>(stage + (size_t)r * C + c0) = vals[i];
+      const int pg = pos / op.page, t = pos - pg * op.page;
+      const int phys = row_bt[pg];
+      if (phys < 0 || phys >= op.num_pages) {
+        if (op.status) atomicOr(op.status, kStatusBadPage);
+        continue;
+      }
+      const size_t ph = ((size_t)phys * op.heads + h) * op.page + t;
+      *reinterpret_cast<uint16_t*>(op.k_pool + ph * (op.head_dim / 2) + d / 2) = pack4(vals[i], lo, sc, rc);
+      if (fresh && ea.v) {
+        const long long src = source(pos);
+        store_value4(op, ph * op.head_dim + d,
+                     src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.v, (size_t)src * C + c0));
+      }
+    }
+  }
+}
+
 // Rotary embedding of rows x[rows, heads, head_dim] at positions[rows] into
 // out (a separate buffer: each channel reads its partner channel of x): the
 // prefill's keys before they are quantized, with the arithmetic of rope4.
@@ -1131,6 +1299,47 @@ cudaError_t int4kv_cache_append(const float* k_new, const float* v_new, const in
                                   num_heads, head_dim, group_tokens, page_tokens, block_table,
                                   max_pages, num_pages, k_pool, v_pool, value_dtype, sz_pool,
                                   nullptr, nullptr, 0, nullptr, nullptr, 0, status, stream);
+}
+
+cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int num_src,
+                                const int32_t* tok_offsets, const int32_t* start_pos,
+                                const int32_t* rows, int num_rows, const int32_t* stage_slots,
+                                float* k_stage, int num_slots, int batch, int max_rows_per_seq,
+                                int num_heads, int head_dim, int group_tokens, int page_tokens,
+                                const int32_t* block_table, int max_pages, int num_pages,
+                                uint8_t* k_pool, void* v_pool, int value_dtype, float* sz_pool,
+                                uint32_t* status, cudaStream_t stream) {
+  if (batch <= 0 || batch > 65535 || max_rows_per_seq < 0 || num_heads <= 0 || head_dim <= 0 ||
+      num_slots <= 0 || num_src < 0 || num_rows < 0)
+    return cudaErrorInvalidValue;
+  if (head_dim % 4 != 0 || page_tokens <= 0 || group_tokens <= 0) return cudaErrorInvalidValue;
+  if (group_tokens % page_tokens != 0 || group_tokens > kRegGroupMax) return cudaErrorInvalidValue;
+  for (int kind : {kv_dtype, value_dtype})
+    if (kind != INT4KV_VALUES_F32 && kind != INT4KV_VALUES_F16 && kind != INT4KV_VALUES_BF16)
+      return cudaErrorInvalidValue;
+  if (max_pages <= 0 || num_pages <= 0 || (long long)max_pages * page_tokens > 0x7fffffffll)
+    return cudaErrorInvalidValue;
+  if (!tok_offsets || !start_pos || !stage_slots || !k_stage || !block_table || !k_pool || !sz_pool)
+    return cudaErrorInvalidValue;
+  if (!aligned16(k_stage)) return cudaErrorInvalidValue;
+  const long long C = (long long)num_heads * head_dim;
+  if (C > (1 << 30)) return cudaErrorInvalidValue;
+  if (max_rows_per_seq == 0 || num_src == 0 || num_rows == 0) return cudaSuccess;
+  if (!k || !aligned16(k) || (v && (!v_pool || !aligned16(v) || !aligned16(v_pool))))
+    return cudaErrorInvalidValue;
+  // an open group's rows may come before the new ones: up to group_tokens - 1
+  const long long groups = ((long long)max_rows_per_seq + 2 * group_tokens - 2) / group_tokens;
+  if (groups > 65535) return cudaErrorInvalidValue;
+  dim3 grid((unsigned)((C + kSlab - 1) / kSlab), (unsigned)groups, batch);
+  ExtendArgs ea{k, v, tok_offsets, start_pos, rows, num_src, rows ? num_rows : num_src,
+                stage_slots, k_stage, num_slots, max_rows_per_seq};
+  OutPaged op{nullptr, nullptr, nullptr, block_table, max_pages, page_tokens, num_pages,
+              num_heads, head_dim, k_pool, v_pool, value_dtype, sz_pool, status};
+  auto kern = kv_dtype == INT4KV_VALUES_F32   ? extend_quant_kernel<INT4KV_VALUES_F32>
+              : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16>
+                                              : extend_quant_kernel<INT4KV_VALUES_BF16>;
+  kern<<<grid, kQuantThreads, 0, stream>>>(ea, (int)C, group_tokens, op);
+  return cudaGetLastError();
 }
 
 cudaError_t int4kv_cache_write(const float* k, const float* v, const int32_t* tok_offsets,

@@ -25,6 +25,26 @@ from . import _C
 PAGE_TOKENS = 16
 
 
+def tree_mask(parents: Sequence[Sequence[int]], device="cuda") -> torch.Tensor:
+    """Mask words (int64 [sum of lengths]) of drafted trees for ``tree_decode``.
+
+    ``parents[b][i]`` is the parent draft of draft i of sequence b, -1 for a
+    child of the cached context; parents come before their children. A draft
+    sees its ancestors and itself.
+    """
+    words: List[int] = []
+    for tree in parents:
+        rows: List[int] = []
+        if len(tree) > _C.MAX_DRAFTS:
+            raise ValueError(f"a tree has at most {_C.MAX_DRAFTS} drafts, got {len(tree)}")
+        for i, p in enumerate(tree):
+            if not -1 <= p < i:
+                raise ValueError(f"the parent of draft {i} must be -1 or an earlier draft, got {p}")
+            rows.append((rows[p] if p >= 0 else 0) | (1 << i))
+        words += rows
+    return torch.from_numpy(np.array(words, np.uint64).view(np.int64)).to(device)
+
+
 class PagedKVCache:
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int,
                  group_tokens: int = 128, device="cuda", seed: Optional[int] = None,
@@ -173,6 +193,55 @@ class PagedKVCache:
             self.lens[s] += 1
         return q_rot
 
+    def extend(self, seq_ids: Sequence[int], counts: Sequence[int], keys: torch.Tensor,
+               values: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None) -> None:
+        """Append ``counts[i]`` tokens to each sequence, quantized as they are written.
+
+        ``keys`` / ``values`` [n, heads, head_dim] (float32, float16 or bfloat16)
+        hold the sequences' new tokens one after another; with ``rows`` (int32
+        [sum of counts]) the new tokens are those rows of ``keys`` in that order:
+        the accepted paths out of all drafted rows. Sequences may be new. The
+        cache equals a bulk write of the same tokens bit for bit.
+        """
+        ids, n_new = list(seq_ids), [int(n) for n in counts]
+        if len(set(ids)) != len(ids):
+            raise ValueError("a sequence may be extended only once per call")
+        if len(ids) != len(n_new) or any(n < 0 for n in n_new):
+            raise ValueError("counts must give a number of new tokens for each sequence")
+        total = sum(n_new)
+        if keys.dim() != 3 or tuple(keys.shape[1:]) != (self.heads, self.head_dim):
+            raise ValueError(f"keys must be [rows, {self.heads}, {self.head_dim}]")
+        if values is not None and values.shape != keys.shape:
+            raise ValueError("values must have the shape of keys")
+        if (rows.shape[0] if rows is not None else keys.shape[0]) < total:
+            raise ValueError(f"{total} new tokens need as many rows")
+        if total == 0:
+            return
+        need = [-(-(self.lens.get(s, 0) + n) // PAGE_TOKENS) - len(self.pages.get(s, []))
+                for s, n in zip(ids, n_new)]
+        if sum(max(0, n) for n in need) > len(self._free):
+            raise MemoryError(f"paged KV cache out of pages: need {sum(need)}, {len(self._free)} free")
+        start = []
+        for s, n in zip(ids, need):
+            start.append(self.lens.setdefault(s, 0))
+            self.pages.setdefault(s, []).extend(self._alloc(max(0, n)))
+        # a sequence that takes no token has no open group to stage for: any slot names it
+        slots = [self._slot_of(s) if n else 0 for s, n in zip(ids, n_new)]
+        bt, _ = self.block_table(ids)
+        k = keys.to(self.device).contiguous()
+        v = None
+        if values is not None and self.v_pool is not None:
+            v = values.to(self.device, k.dtype).contiguous()
+        offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n_new)]).astype(np.int32))
+        _C.cache_extend(k, v, offs.to(self.device),
+                        torch.tensor(start, dtype=torch.int32, device=self.device),
+                        torch.tensor(slots, dtype=torch.int32, device=self.device), self.k_stage, bt,
+                        self.k_pool, self.v_pool, self.sz_pool, max_rows_per_seq=max(n_new),
+                        group_tokens=self.group_tokens,
+                        rows=rows.to(self.device, torch.int32).contiguous() if rows is not None else None)
+        for s, n in zip(ids, n_new):
+            self.lens[s] += n
+
     def decode_step(self, seq_ids: Sequence[int], query: torch.Tensor, keys: torch.Tensor,
                     values: torch.Tensor, rope) -> torch.Tensor:
         """One decode step of a Llama-style attention layer: RoPE of the step's
@@ -197,6 +266,51 @@ class PagedKVCache:
         bt, sl = self.block_table(seq_ids)
         return _C.paged_decode(query.to(self.device, torch.float32).contiguous(), self.k_pool,
                                self.v_pool, self.sz_pool, bt, sl, self.group_tokens)
+
+    def window_decode(self, query: torch.Tensor, seq_ids: Sequence[int], window: int,
+                      sinks: int = 0) -> torch.Tensor:
+        """``decode`` over each sequence's last ``window`` and first ``sinks`` tokens only.
+
+        query [B, heads, head_dim] float32, or of the value pool's 16-bit type.
+        """
+        bt, sl = self.block_table(seq_ids)
+        return _C.paged_window_decode(query.to(self.device).contiguous(), self.k_pool, self.v_pool,
+                                      self.sz_pool, bt, sl, window=window, sinks=sinks,
+                                      group_tokens=self.group_tokens)
+
+    def tree_decode(self, query: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor,
+                    seq_ids: Sequence[int], counts: Sequence[int], mask: torch.Tensor,
+                    window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
+        """Attention of each sequence's ``counts[i]`` drafted tokens over its cache and one another.
+
+        query [n, heads, head_dim], k_draft / v_draft [n, kv_heads, head_dim]
+        (rotated, not in the cache), ``mask`` from ``tree_mask``. float32, or of
+        the value pool's 16-bit type. ``extend`` then writes the accepted path.
+        """
+        n = [int(c) for c in counts]
+        if len(n) != len(list(seq_ids)) or any(c < 0 for c in n) or sum(n) > query.shape[0]:
+            raise ValueError("counts must give the number of drafts of each sequence")
+        bt, sl = self.block_table(seq_ids)
+        offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n)]).astype(np.int32))
+        return _C.paged_tree_decode(
+            query.to(self.device).contiguous(), k_draft.to(self.device).contiguous(),
+            v_draft.to(self.device).contiguous(), mask.to(self.device), offs.to(self.device),
+            self.k_pool, self.v_pool, self.sz_pool, bt, sl, max_drafts=max(n),
+            group_tokens=self.group_tokens, window=window, sinks=sinks)
+
+    def read(self, seq_id: int, start: int = 0, stop: Optional[int] = None,
+             dtype=torch.float32):
+        """Tokens start .. stop-1 of a sequence as dense (keys, values) [n, heads, head_dim]:
+        the keys as the cache holds them (dequantized), values None without a value pool."""
+        n = self.lens[seq_id]
+        stop = n if stop is None else stop
+        if not 0 <= start <= stop <= n:
+            raise ValueError(f"tokens {start} .. {stop} of a sequence of {n}")
+        bt, _ = self.block_table([seq_id])
+        one = torch.tensor([start, 0, stop - start], dtype=torch.int32, device=self.device)
+        return _C.cache_read(self.k_pool, self.v_pool, self.sz_pool, bt, one[:1], one[1:],
+                             num_rows=stop - start, max_rows_per_seq=stop - start,
+                             group_tokens=self.group_tokens, dtype=dtype)
 
     def memory_stats(self) -> dict:
         used = sum(len(p) for p in self.pages.values())
