@@ -10,6 +10,8 @@ namespace i4kv {
 size_t multi_query_f32_workspace(int dim, int sms);
 cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, size_t ws_bytes,
                             cudaStream_t stream);
+size_t multi_query_tc_workspace(int dim, long long rows, int sms);
+cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, size_t ws_bytes, cudaStream_t stream);
 }  // namespace i4kv
 
 namespace {
@@ -40,6 +42,7 @@ cudaError_t run(MultiQueryArgs a, int dim, int vk, void* workspace, size_t bytes
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   a.recs = static_cast<float*>(workspace);
+  if (a.qk != INT4KV_VALUES_F32) return multi_query_tc(a, dim, sms, bytes, stream);
   return multi_query_f32(a, dim, vk, sms, bytes, stream);
 }
 
@@ -54,7 +57,8 @@ cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, in
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  *bytes = multi_query_f32_workspace(head_dim, sms);
+  const long long rows = (long long)std::max(1, max_drafts) * (num_q_heads / num_kv_heads);
+  *bytes = std::max(multi_query_f32_workspace(head_dim, sms), multi_query_tc_workspace(head_dim, rows, sms));
   return cudaSuccess;
 }
 

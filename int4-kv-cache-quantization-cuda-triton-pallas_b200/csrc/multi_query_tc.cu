@@ -1,0 +1,985 @@
+// Several 16-bit queries of a sequence over its paged INT4 cache on the 5th
+// generation tensor cores: drafted trees and sliding windows in float16 and
+// bfloat16 (the float32 form is multi_query_f32.cu).
+//
+// Math: the logits are taken transposed, S^T[token, row] = K^ Q^T, and so are
+// the outputs, O^T[channel, row] += V^T P^T. Tokens and channels fill the 128
+// lanes of an MMA whatever the number of rows is, and its cost grows with the
+// rows (N = 16, 32, 64 or 128): a handful of drafted rows costs a handful of
+// columns, where rows in the lanes would pay for 128. A thread of the softmax
+// holds one token and half of the rows, so a row's sum of weights stays in one
+// register per thread until the stream ends. The running maximum is kept
+// lazily: weights are 2^(x - ref) against a reference that is raised to the
+// true maximum only when some logit exceeds it by more than 8 (in log2), so
+// the outputs are rescaled a few times per stream instead of every tile; sums
+// and outputs are float32 in registers and tensor memory.
+//
+// Numerics: keys are dequantized as code * s - zp * s in float32, scaled by a
+// power of two that brings the largest channel of their group to [1, 2), and
+// rounded once to float16 (relative step 2^-11; bfloat16 would lose 3 bits of
+// the logits); queries (exact in float16 after their own power of two) likewise;
+// the scales return in the float32 logits. Weights are rounded to the value
+// pool's type, which the tensor cores multiply with the stored values as they
+// are.
+//
+// A tile is 128 cached tokens (8 pages) or the drafts. Roles of the 18 warps:
+//   0-7   softmax: S^T from tensor memory, mask, weights to shared memory,
+//         the rare rescale of O^T, and the stream's epilogue
+//   8-15  conversion: packed codes to float16 keys (K-major, 128-byte swizzle),
+//         a stream's queries, drafted keys
+//   16    copies: pages by bulk (codes, scales) and tensor copies (values, in
+//         the swizzled layout the MMA reads: V is stored token-major, which is
+//         the transposed operand's contiguous side, so nothing is rearranged)
+//   17    MMA issue, one thread: S^T of tile i, then O^T of tile i - 1
+// One persistent CTA per SM; work decomposition and merge: multi_query.cuh.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "multi_query.cuh"
+
+using namespace i4kv;
+
+namespace {
+
+constexpr int kSoftWarps = 8, kConvWarps = 8;
+constexpr int kThreadsTc = 32 * (kSoftWarps + kConvWarps + 2);
+constexpr int kTile = 128, kTilePages = kTile / kMqPage;
+constexpr int kDesc = 4;                        // tiles in flight between the roles
+constexpr uint64_t kTcWaitNs = 2000000000ull;   // bounded waits: 2 s
+constexpr float kLazy = 8.f;                    // weights reach 2^8 before a rescale
+
+// ---- tcgen05 ----
+I4KV_DEVINL void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+I4KV_DEVINL void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+I4KV_DEVINL void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+I4KV_DEVINL void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+// N columns of the warp's 32 lanes; the wait is part of the statement, so no use
+// of the registers can be scheduled before it.
+template <int N>
+I4KV_DEVINL void tc_ld(uint32_t (&r)[N], uint32_t addr) {
+  static_assert(N == 8 || N == 16, "columns per load");
+  if constexpr (N == 8) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+        : "r"(addr)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+  }
+}
+I4KV_DEVINL void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
+I4KV_DEVINL void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// One page of values: box of 64 channels x 16 rows x D / 64 chunks at the pool's
+// page-head slab `slab` (or, of the drafts, 16 rows from `row` of head `slab`).
+I4KV_DEVINL void tma_page(void* dst, const CUtensorMap* map, int row, int slab, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4}], "
+      "[%5];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(slab), "r"(smem_addr(bar))
+      : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle (lbo / sbo in bytes).
+I4KV_DEVINL uint64_t mat_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor of kind::f16 with float32 accumulators; `fmt` 0
+// float16, 1 bfloat16, `mn` set where both operands are contiguous along M / N.
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, int fmt, bool mn) {
+  return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | (mn ? (3u << 15) : 0u) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+template <int D, int NR>
+struct Tc {
+  static constexpr int CH = D / 64;                        // 64-channel chunks
+  static constexpr int PAGE_V = kMqPage * D * 2;           // value bytes of a page
+  static constexpr int UNIT = 16384, PPU = UNIT / PAGE_V;  // value ring: units of PPU pages
+  static constexpr int UNITS = kTilePages / PPU;           // units of a full tile
+  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 5 : 6);
+  static constexpr int NK = D == 256 ? 1 : 2;              // stages of packed codes
+  static constexpr int NP = (NR > 64 || D == 256) ? 1 : 2; // weight buffers
+  static constexpr int PC = (NR + 63) / 64;                // 64-row chunks of the weights
+  static constexpr int NO = D == 256 ? 2 : 1;              // 128-channel blocks of O^T
+  static constexpr int KH = kTile * D * 2, Q = NR * D * 2, P = PC * kTile * 128;
+  static constexpr int KC = kTile * D / 2, SZ = kTilePages * 2 * D * 4;
+  static constexpr int KH_OFF = 0, V_OFF = KH_OFF + KH, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q;
+  static constexpr int KC_OFF = P_OFF + NP * P, SZ_OFF = KC_OFF + NK * KC, END = SZ_OFF + NK * SZ;
+  static constexpr int BYTES = END + 1024;                 // the base is rounded up to 1024
+  static constexpr int COLS_O = 2 * NR, COLS = 512;
+  static_assert(Q % 1024 == 0 && P % 1024 == 0 && COLS_O + NO * NR <= COLS, "layout");
+};
+
+struct TileDesc {
+  int flags, pages, len, drafts;
+  int row0, rows, chunk, head;
+  int seg, slot;                // segment ring entry; record of a shared stream
+  int low_edge;                 // no row sees cached positions <= low_edge (but the sinks)
+  int at[kTilePages];           // position of each page's first token, -1: not there
+  int sz[kTilePages];           // scale slot of each page
+};
+enum : int { kDraftTile = 1, kMasked = 2, kFirst = 4, kLast = 8, kWhole = 16 };
+
+template <int NR>
+struct TcShared {
+  uint64_t desc_full[kDesc], desc_empty[kDesc], kc_full[2], kc_empty[2], v_full[6], v_empty[6];
+  uint64_t kh_full, kh_empty, s_full[2], s_empty[2], p_full[2], p_empty[2];
+  TileDesc desc[kDesc];
+  uint64_t word[kDesc][NR];     // visible drafts of each row, per segment
+  int edge[kDesc][NR];          // last position a row does not see (-1: none)
+  int depth[kDesc][kMqMaxDrafts];
+  float qscale[kDesc];
+  float kscale[kDesc][kTile];
+  float ref[NR], sub[NR], alpha[NR], part[4][NR], lsum[4][NR];
+  float qmax[kConvWarps];
+  unsigned long long odd;       // drafts of the segment whose values are not all finite
+  uint32_t tmem;
+  int dead;
+  long long scan[3 + kThreadsTc / 32];
+};
+
+// Bounded wait; false after a timeout here or in another role.
+template <typename Sh>
+I4KV_DEVINL bool tc_wait(Sh& sh, uint64_t* bar, uint32_t parity, uint32_t* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_wait_bounded(bar, parity, kTcWaitNs)) return true;
+  *(volatile int*)&sh.dead = 1;
+  mq_status(status, kStatusWaitTimeout);
+  return false;
+}
+
+template <int VK>
+I4KV_DEVINL uint32_t pack16(float x, float y) {
+  if constexpr (VK == INT4KV_VALUES_F16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// Power of two that brings |x| <= top to [1, 2) (1 for 0), and its inverse.
+I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
+  const int e = top > 0.f ? (int)((__float_as_uint(top) >> 23) & 0xFF) : 127;
+  const int c = min(max(e, 2), 252);
+  down = __uint_as_float((uint32_t)(254 - c) << 23);
+  up = __uint_as_float((uint32_t)c << 23);
+}
+
+template <int D, int NR, int VK>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ CUtensorMap dmap) {
+  using T = Tc<D, NR>;
+  extern __shared__ char smem_raw[];
+  __shared__ TcShared<NR> sh;
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  grid_dependency_wait();
+  allow_dependent_launch();
+  if (tid == 0) {
+    for (int i = 0; i < kDesc; ++i) {
+      mbar_init(&sh.desc_full[i], 1);
+      mbar_init(&sh.desc_empty[i], kSoftWarps + kConvWarps + 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.kc_full[i], kTilePages);
+      mbar_init(&sh.kc_empty[i], kConvWarps);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_empty[i], kSoftWarps);
+      mbar_init(&sh.p_full[i], kSoftWarps);
+      mbar_init(&sh.p_empty[i], 1);
+    }
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&sh.v_full[i], T::PPU);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    mbar_init(&sh.kh_full, kConvWarps);
+    mbar_init(&sh.kh_empty, 1);
+    sh.dead = 0;
+    sh.odd = 0;
+    fence_barrier_init();
+  }
+  zero_idle_rows<NR, kTilePages, D>(a);
+  int b0;
+  long long before;
+  const long long cta = blockIdx.x, ctas = gridDim.x;
+  const long long total = locate_sequence<NR, kTilePages>(
+      a, sh.scan, [&](long long n) { return n > cta ? run_start(cta, n, min(ctas, n)) : 0ll; }, b0, before);
+  const long long runs = min(ctas, total);
+  if (cta >= runs) return;
+  const long long u0 = run_start(cta, total, runs), u1 = run_start(cta + 1, total, runs);
+  const int n_tiles = (int)(u1 - u0);
+  if (warp == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)),
+                 "n"(T::COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = sh.tmem;
+
+  if (warp == 16) {
+    // ------------------------------------------------------------ copies
+    SeqWork w = seq_work<NR, kTilePages>(a, b0, false);
+    TileAt p = tile_at(a, w, b0, u0 - before);
+    int seg = -1, high_edge = 0;
+    uint32_t kc = 0, vu = 0;  // stages used so far
+    bool ok = true;
+    for (int i = 0; i < n_tiles && ok; ++i) {
+      const int ds = i % kDesc;
+      if (i >= kDesc) ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.desc_empty[ds], (i / kDesc - 1) & 1, a.status));
+      if (!ok) break;
+      const bool first = i == 0 || p.tile == 0;
+      if (first) {
+        ++seg;
+        const int sg = seg % kDesc;
+        int top = 0;
+        if (a.mask) {
+          for (int t = lane; t < w.drafts; t += 32) {
+            const int dp = draft_depth((uint64_t)a.mask[w.row0 + t], t, w.drafts);
+            sh.depth[sg][t] = dp;
+            top = max(top, dp);
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+        }
+        high_edge = w.pos0 + top - a.window;
+        for (int r = lane; r < NR; r += 32) {
+          const int t = min(p.chunk * NR + r, w.rows - 1) / a.group_q;
+          const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
+          sh.word[sg][r] = word;
+          sh.edge[sg][r] = a.window > 0 ? w.pos0 + (a.mask ? draft_depth(word, t, w.drafts) : 0) - a.window : -1;
+        }
+      }
+      const bool draft = p.tile >= w.cache_tiles;
+      const int here = draft ? (w.drafts + kMqPage - 1) / kMqPage
+                             : min(kTilePages, w.vis_pages - p.tile * kTilePages);
+      int phys = 0, home = -1, at = -1;
+      bool live = false, clean = true;  // the page is read; every row sees all of it
+      if (lane < here) {
+        if (draft) {
+          at = lane * kMqPage;
+          live = true;
+          clean = false;
+        } else {
+          const int pg = visible_page(w, p.tile * kTilePages + lane);
+          const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
+          phys = __ldg(bt + pg);
+          home = __ldg(bt + pg / a.group_pages * a.group_pages);
+          live = phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages;
+          if (!live) mq_status(a.status, kStatusBadPage);
+          at = live ? pg * kMqPage : -1;
+          clean = live && at + kMqPage <= w.len &&
+                  (a.window == 0 || at > high_edge || at + kMqPage <= a.sinks);
+          if (!live) home = -1;
+        }
+      }
+      const bool masked = !__all_sync(0xffffffffu, clean) || here < kTilePages;
+      // pages of one group share a scale slot: the slot of the group's first page here
+      const int prev = __shfl_up_sync(0xffffffffu, home, 1);
+      const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || home != prev);
+      const int slot = 31 - __clz(starts & ((2u << lane) - 1));
+      if (lane < kTilePages) {
+        sh.desc[ds].at[lane] = at;
+        sh.desc[ds].sz[lane] = slot;
+      }
+      if (lane == 0) {
+        TileDesc& d = sh.desc[ds];
+        const long long first_u = u0 + i - p.tile;  // the stream's first tile
+        const bool ends = p.tile + 1 == w.tiles;
+        d.flags = (draft ? kDraftTile : 0) | (masked ? kMasked : 0) | (first ? kFirst : 0) |
+                  ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= u0) ? kWhole : 0);
+        d.pages = here;
+        d.len = w.len;
+        d.drafts = w.drafts;
+        d.row0 = w.row0;
+        d.rows = w.rows;
+        d.chunk = p.chunk;
+        d.head = p.head;
+        d.seg = seg % kDesc;
+        d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
+        d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
+      // packed codes and scales
+      if (!draft) {
+        const int ks = kc % T::NK;
+        if (kc >= T::NK)
+          ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.kc_empty[ks], (kc / T::NK - 1) & 1, a.status));
+        if (!ok) break;
+        if (lane < kTilePages) {
+          const bool sz = live && slot == lane;
+          mbar_arrive_expect_tx(&sh.kc_full[ks], live ? kMqPage * D / 2 + (sz ? 2 * D * 4 : 0) : 0);
+          if (live)
+            bulk_g2s(smem + T::KC_OFF + ks * T::KC + lane * (kMqPage * D / 2),
+                     a.k_pool + ((size_t)phys * a.kv_heads + p.head) * (kMqPage * D / 2), kMqPage * D / 2,
+                     &sh.kc_full[ks]);
+          if (sz)
+            bulk_g2s(smem + T::SZ_OFF + ks * T::SZ + lane * (2 * D * 4),
+                     a.sz_pool + ((size_t)home * a.kv_heads + p.head) * 2 * D, 2 * D * 4, &sh.kc_full[ks]);
+        }
+        ++kc;
+      }
+      // values, a unit of pages at a time
+      for (int q = 0; q * T::PPU < here; ++q) {
+        const int vs = vu % T::NV;
+        if (vu >= T::NV)
+          ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.v_empty[vs], (vu / T::NV - 1) & 1, a.status));
+        if (!ok) break;
+        if (lane / T::PPU == q) {
+          mbar_arrive_expect_tx(&sh.v_full[vs], live ? T::PAGE_V : 0);
+          if (live) {
+            char* dst = smem + T::V_OFF + vs * T::UNIT + (lane % T::PPU) * T::PAGE_V;
+            if (draft) tma_page(dst, &dmap, w.row0 + lane * kMqPage, p.head, &sh.v_full[vs]);
+            else tma_page(dst, &vmap, 0, phys * a.kv_heads + p.head, &sh.v_full[vs]);
+          }
+        }
+        ++vu;
+      }
+      if (++p.tile >= w.tiles) next_stream<NR, kTilePages>(a, w, p);
+    }
+    // after a timeout: the copies issued so far land (or a bound passes) before the CTA ends
+    if (!ok && lane == 0) {
+      for (uint32_t s = kc > T::NK ? kc - T::NK : 0; s < kc; ++s)
+        mbar_wait_bounded(&sh.kc_full[s % T::NK], (s / T::NK) & 1, 10000000ull);
+      for (uint32_t s = vu > T::NV ? vu - T::NV : 0; s < vu; ++s)
+        mbar_wait_bounded(&sh.v_full[s % T::NV], (s / T::NV) & 1, 10000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 17) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      constexpr uint32_t kQk = mma_desc(128, NR, 0, false);
+      constexpr uint32_t kPv = mma_desc(128, NR, VK == INT4KV_VALUES_BF16 ? 1 : 0, true);
+      const uint32_t base = smem_addr(smem);
+      uint32_t vu = 0;
+      int pages = 0;       // of tile i - 1
+      bool fresh = true;   // tile i - 1 starts its segment
+      bool ok = true;
+      for (int i = 0; i <= n_tiles && ok; ++i) {
+        int next_pages = 0;
+        bool next_fresh = false;
+        if (i < n_tiles) {
+          const int ds = i % kDesc;
+          ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status);
+          if (!ok) break;
+          next_pages = sh.desc[ds].pages;
+          next_fresh = sh.desc[ds].flags & kFirst;
+          mbar_arrive(&sh.desc_empty[ds]);
+          ok = tc_wait(sh, &sh.kh_full, i & 1, a.status) &&
+               (i < 2 || tc_wait(sh, &sh.s_empty[i & 1], (i / 2 - 1) & 1, a.status));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t in = (k % 4) * 32;
+            tc_mma(tm + (i & 1) * NR, mat_desc(base + T::KH_OFF + (k / 4) * (kTile * 128) + in, 16, 1024),
+                   mat_desc(base + T::Q_OFF + (k / 4) * (NR * 128) + in, 16, 1024), kQk, k > 0);
+          }
+          tc_commit(&sh.s_full[i & 1]);
+          tc_commit(&sh.kh_empty);
+        }
+        if (i > 0) {
+          const int j = i - 1, pb = j % T::NP;
+          ok = tc_wait(sh, &sh.p_full[pb], (j / T::NP) & 1, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          for (int g = 0; g < pages; ++g) {
+            const int vs = vu % T::NV;
+            if (g % T::PPU == 0) {
+              ok = tc_wait(sh, &sh.v_full[vs], (vu / T::NV) & 1, a.status);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            const uint32_t va = base + T::V_OFF + vs * T::UNIT + (g % T::PPU) * T::PAGE_V;
+            const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P + g * 2048, kTile * 128, 1024);
+#pragma unroll
+            for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
+              tc_mma(tm + T::COLS_O + o * NR, mat_desc(va + o * 2 * 2048, 2048, 1024), pd, kPv,
+                     !(fresh && g == 0));
+            if (g % T::PPU == T::PPU - 1 || g == pages - 1) {
+              tc_commit(&sh.v_empty[vs]);
+              ++vu;
+            }
+          }
+          if (!ok) break;
+          tc_commit(&sh.p_empty[pb]);
+        }
+        pages = next_pages;
+        fresh = next_fresh;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kSoftWarps) {
+    // ------------------------------------------------------------ conversion
+    constexpr int LPT = D / 16;          // lanes of a token, 16 channels each
+    constexpr int TPW = 32 / LPT;        // tokens of a warp at a time
+    const int cw = warp - kSoftWarps, ct = tid - 32 * kSoftWarps;
+    const int c = lane % LPT;
+    const int chunk = c / 4, flip = chunk & 1;  // 64-channel chunk; order of the two 16-byte stores
+    uint32_t kc = 0;
+    // 16 channels of token / row `r` of an operand with `rows` rows
+    auto put = [&](char* op, int rows, int r, const uint32_t (&h)[8]) {
+      char* row = op + chunk * (rows * 128) + r * 128;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = j ^ flip, piece = 2 * (c % 4) + s;
+        const uint4 v = s ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = v;
+      }
+    };
+    // 16 consecutive 16-bit inputs widened to float32
+    auto get = [&](const void* src, size_t i, float (&x)[16]) {
+      const uint4* p4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + i);
+      const uint4 u = __ldg(p4), v = __ldg(p4 + 1);
+      const uint32_t wd[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (VK == INT4KV_VALUES_F16) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&wd[j]));
+          x[2 * j] = f.x;
+          x[2 * j + 1] = f.y;
+        } else {
+          x[2 * j] = __uint_as_float(wd[j] << 16);
+          x[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
+        }
+      }
+    };
+    auto top_of = [&](const float (&x)[16]) {  // largest finite magnitude
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float y = fabsf(x[j]);
+        m = fmaxf(m, y <= 3.4e38f ? y : 0.f);
+      }
+      return m;
+    };
+    for (int i = 0; i < n_tiles; ++i) {
+      const int ds = i % kDesc;
+      bool ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status);
+      const TileDesc& d = sh.desc[ds];
+      const int flags = d.flags, pages = d.pages;
+      const int ks = kc % T::NK;
+      if (ok && !(flags & kDraftTile)) ok = tc_wait(sh, &sh.kc_full[ks], (kc / T::NK) & 1, a.status);
+      if (ok && i > 0) ok = tc_wait(sh, &sh.kh_empty, (i - 1) & 1, a.status);
+      // (uniform over the role: its warps meet in named barriers)
+      if (named_bar_or(1, 32 * kConvWarps, !ok)) break;
+      if (flags & kFirst) {
+        // the stream's queries: two passes, the first for the common scale
+        float top = 0.f;
+        for (int r = cw * TPW + lane / LPT; r < NR; r += kConvWarps * TPW) {
+          const int rr = d.chunk * NR + r;
+          if (rr >= d.rows) continue;
+          SeqWork w;
+          w.row0 = d.row0;
+          float x[16];
+          get(a.q, row_offset(a, w, d.head, rr, D) + 16 * c, x);
+          top = fmaxf(top, top_of(x));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) sh.qmax[cw] = top;
+        named_bar_sync(1, 32 * kConvWarps);
+#pragma unroll
+        for (int j = 0; j < kConvWarps; ++j) top = fmaxf(top, sh.qmax[j]);
+        float down, up;
+        unit_scale(top, down, up);
+        if (ct == 0) sh.qscale[d.seg] = up;
+        for (int r = cw * TPW + lane / LPT; r < NR; r += kConvWarps * TPW) {
+          const int rr = d.chunk * NR + r;
+          uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (rr < d.rows) {
+            SeqWork w;
+            w.row0 = d.row0;
+            float x[16];
+            get(a.q, row_offset(a, w, d.head, rr, D) + 16 * c, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+          }
+          put(smem + T::Q_OFF, NR, r, h);
+        }
+        named_bar_sync(1, 32 * kConvWarps);  // qmax is free again
+      }
+      if (flags & kDraftTile) {
+        for (int t = cw * TPW + lane / LPT; t < pages * kMqPage; t += kConvWarps * TPW) {
+          float x[16];
+          const bool real = t < d.drafts;
+          if (real) {
+            get(a.kd, ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 16 * c, x);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = 0.f;
+          }
+          float top = top_of(x), down, up;
+#pragma unroll
+          for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          unit_scale(top, down, up);
+          uint32_t h[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+          put(smem + T::KH_OFF, kTile, t, h);
+          if (c == 0) sh.kscale[ds][t] = up;
+        }
+      } else {
+        const char* codes = smem + T::KC_OFF + ks * T::KC;
+        float s[16], z[16];
+        float up = 1.f;
+        int have = -1;
+        for (int t = cw * TPW + lane / LPT; t < pages * kMqPage; t += kConvWarps * TPW) {
+          const int slot = d.sz[t / kMqPage];  // uniform in the warp: its tokens lie in one page
+          if (slot != have) {
+            have = slot;
+            const float* p4 = reinterpret_cast<const float*>(smem + T::SZ_OFF + ks * T::SZ + slot * (2 * D * 4)) + 16 * c;
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(p4 + j);
+              const float4 y = *reinterpret_cast<const float4*>(p4 + D + j);
+              s[j] = x.x; s[j + 1] = x.y; s[j + 2] = x.z; s[j + 3] = x.w;
+              z[j] = -y.x * x.x; z[j + 1] = -y.y * x.y; z[j + 2] = -y.z * x.z; z[j + 3] = -y.w * x.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float y = fmaxf(fabsf(z[j]), fabsf(fmaf(15.f, s[j], z[j])));
+              top = fmaxf(top, y <= 3.4e38f ? y : 0.f);
+            }
+#pragma unroll
+            for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float down;
+            unit_scale(top, down, up);
+            // code c enters as 1 + c / 128 (its bits in the mantissa)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float e = s[j] * down * 128.f;
+              z[j] = fmaf(z[j], down, -e);
+              s[j] = e;
+            }
+          }
+          const uint2 wd = *reinterpret_cast<const uint2*>(codes + t * (D / 2) + 8 * c);
+          uint32_t h[8];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t x = k ? wd.y : wd.x;
+            const uint32_t lo = (x & 0x0F0F0F0Fu) | 0x80808080u, hi = ((x >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float e = __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8)));
+              const float o = __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8)));
+              const int q = 8 * k + 2 * j;
+              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(fmaf(e, s[q], z[q]), fmaf(o, s[q + 1], z[q + 1]));
+            }
+          }
+          put(smem + T::KH_OFF, kTile, t, h);
+          if (c == 0) sh.kscale[ds][t] = up;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh.kh_full);
+        if (!(flags & kDraftTile)) mbar_arrive(&sh.kc_empty[ks]);
+        mbar_arrive(&sh.desc_empty[ds]);
+      }
+      if (!(flags & kDraftTile)) ++kc;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    constexpr int NC = NR / 2;                 // rows (columns of S^T) of a thread
+    constexpr int LD = NC < 16 ? 8 : 16;       // columns per tensor-memory load
+    const int wg = warp / 4, tok = (warp % 4) * 32 + lane, c0 = wg * NC, wt = tid % 128;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const int bar = 2 + wg;
+    float l[NC];
+    uint32_t vu = 0;                           // value units before this tile
+    bool failed = false, started = false;      // a wait ran out; O^T of the segment holds something
+#pragma unroll
+    for (int j = 0; j < NC; ++j) l[j] = 0.f;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int ds = i % kDesc, sb = i & 1, pb = i % T::NP;
+      // Every thread waits. A timeout is made uniform over both warpgroups here
+      // alone: until then the tile goes on with what it has, so no barrier of the
+      // softmax ever waits for a warp that has left.
+      const bool ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status) &&
+                      tc_wait(sh, &sh.s_full[sb], (i / 2) & 1, a.status);
+      failed |= !ok;
+      const TileDesc& d = sh.desc[ds];
+      const int flags = ok ? d.flags : 0, pages = ok ? d.pages : 0, sg = ok ? d.seg : 0;
+      if (flags & kFirst) {
+        started = false;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) l[j] = 0.f;
+        if (wt < NC) {
+          sh.ref[c0 + wt] = -INFINITY;
+          sh.sub[c0 + wt] = 0.f;
+        }
+      }
+      if (named_bar_or(4, 256, failed)) break;
+      tc_fence_after();
+      // the token of this thread
+      const int at0 = d.at[tok / kMqPage], at = at0 + tok % kMqPage;
+      const bool draft = flags & kDraftTile;
+      bool real = tok < pages * kMqPage && at0 >= 0 && at < (draft ? d.drafts : d.len);
+      if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
+      const float f = real ? sh.qscale[sg] * sh.kscale[ds][tok] * kLog2e : 0.f;
+      int behind = at;
+      if (draft && real && a.window > 0) behind = d.len + sh.depth[sg][at];
+      const bool masked = flags & kMasked;
+      auto sees = [&](int r) -> bool {
+        bool s = real;
+        if (draft) s = s && (sh.word[sg][r] >> (at & 63) & 1);
+        if (a.window > 0) s = s && (behind > sh.edge[sg][r] || behind < a.sinks);
+        return s;
+      };
+      const uint32_t s_addr = tm + lanes + sb * NR + c0;
+
+      // pass 1: does some logit exceed its row's reference by more than kLazy?
+      float over = -INFINITY;
+#pragma unroll
+      for (int j0 = 0; j0 < NC; j0 += LD) {
+        uint32_t x[LD];
+        tc_ld<LD>(x, s_addr + j0);
+#pragma unroll
+        for (int j = 0; j < LD; j += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(&sh.ref[c0 + j0 + j]);
+          const float y0 = fmaf(__uint_as_float(x[j]), f, -m.x), y1 = fmaf(__uint_as_float(x[j + 1]), f, -m.y);
+          const float y2 = fmaf(__uint_as_float(x[j + 2]), f, -m.z), y3 = fmaf(__uint_as_float(x[j + 3]), f, -m.w);
+          if (masked) {
+            if (sees(c0 + j0 + j)) over = fmaxf(over, y0);
+            if (sees(c0 + j0 + j + 1)) over = fmaxf(over, y1);
+            if (sees(c0 + j0 + j + 2)) over = fmaxf(over, y2);
+            if (sees(c0 + j0 + j + 3)) over = fmaxf(over, y3);
+          } else {
+            over = fmax3f(fmax3f(over, y0, y1), y2, y3);
+          }
+        }
+      }
+      if (named_bar_or(bar, 128, over > kLazy)) {
+        // raise the references to the true maxima, rescale sums and outputs
+#pragma unroll
+        for (int j0 = 0; j0 < NC; j0 += LD) {
+          uint32_t x[LD];
+          tc_ld<LD>(x, s_addr + j0);
+#pragma unroll
+          for (int j = 0; j < LD; ++j) {
+            float y = __uint_as_float(x[j]) * f;
+            if (masked && !sees(c0 + j0 + j)) y = -INFINITY;
+            const uint32_t k = __reduce_max_sync(0xffffffffu, ordered_key(fmaxf(y, -INFINITY)));
+            if (lane == 0) sh.part[warp % 4][c0 + j0 + j] = from_ordered_key(k);
+          }
+        }
+        named_bar_sync(bar, 128);
+        if (wt < NC) {
+          const int r = c0 + wt;
+          const float old = sh.ref[r];
+          const float m = fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
+          sh.ref[r] = m;
+          sh.sub[r] = m == -INFINITY ? 0.f : m;
+          sh.alpha[r] = m == -INFINITY ? 1.f : exp2_fast(old - m);
+        }
+        if (started)  // the weights of tile i - 1 have been multiplied
+          failed |= !tc_wait(sh, &sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status);
+        named_bar_sync(bar, 128);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) l[j] *= sh.alpha[c0 + j];
+        if (started) {
+          tc_fence_after();
+#pragma unroll
+          for (int o = 0; o < T::NO; ++o)
+#pragma unroll
+            for (int j0 = 0; j0 < NC; j0 += 8) {
+              uint32_t x[8];
+              const uint32_t at_o = tm + lanes + T::COLS_O + o * NR + c0 + j0;
+              tc_ld<8>(x, at_o);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sh.alpha[c0 + j0 + j]);
+              tc_st8(at_o, x);
+            }
+          tc_wait_st();
+          tc_fence_before();
+        }
+      }
+      // pass 2: weights
+      if (i >= T::NP) failed |= !tc_wait(sh, &sh.p_empty[pb], (i / T::NP - 1) & 1, a.status);
+      char* prow = smem + T::P_OFF + pb * T::P + tok * 128;
+#pragma unroll
+      for (int j0 = 0; j0 < NC; j0 += LD) {
+        uint32_t x[LD], h[LD / 2];
+        tc_ld<LD>(x, s_addr + j0);
+#pragma unroll
+        for (int j = 0; j < LD; j += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(&sh.sub[c0 + j0 + j]);
+          float e[4] = {exp2_fast(fmaf(__uint_as_float(x[j]), f, -m.x)),
+                        exp2_fast(fmaf(__uint_as_float(x[j + 1]), f, -m.y)),
+                        exp2_fast(fmaf(__uint_as_float(x[j + 2]), f, -m.z)),
+                        exp2_fast(fmaf(__uint_as_float(x[j + 3]), f, -m.w))};
+          if (masked) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (!sees(c0 + j0 + j + q)) e[q] = 0.f;
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) l[j0 + j + q] += e[q];
+          h[j / 2] = pack16<VK>(e[0], e[1]);
+          h[j / 2 + 1] = pack16<VK>(e[2], e[3]);
+        }
+#pragma unroll
+        for (int j = 0; j < LD; j += 8) {
+          const int col = c0 + j0 + j;
+          *reinterpret_cast<uint4*>(prow + (col / 64) * (kTile * 128) + (((col / 8) % 8 ^ (tok & 7)) << 4)) =
+              make_uint4(h[j / 2], h[j / 2 + 1], h[j / 2 + 2], h[j / 2 + 3]);
+        }
+      }
+      // Values that no row sees must not reach the product (0 * NaN): cleared.
+      // A drafted value that is not finite is taken out too and added for the
+      // rows that see it when the stream ends.
+      const int units = (pages + T::PPU - 1) / T::PPU;
+      if (masked && wg == 0 && tok < pages * kMqPage) {
+        const uint32_t mine = vu + tok / (kMqPage * T::PPU);
+        if (!real || draft) {
+          failed |= !tc_wait(sh, &sh.v_full[mine % T::NV], (mine / T::NV) & 1, a.status);
+          char* row = smem + T::V_OFF + (mine % T::NV) * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V +
+                      (tok % kMqPage) * 128;
+          bool bad = false;
+#pragma unroll
+          for (int q = 0; q < T::CH; ++q) {
+            for (int j = 0; j < 8; ++j) {
+              uint4* v = reinterpret_cast<uint4*>(row + q * (kMqPage * 128) + 16 * j);
+              if (!real) {
+                *v = make_uint4(0, 0, 0, 0);
+              } else {
+                uint4 y = *v;
+                uint32_t* e = reinterpret_cast<uint32_t*>(&y);
+                constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
+                bool hit = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
+                  if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
+                }
+                if (hit) { *v = y; bad = true; }
+              }
+            }
+          }
+          if (bad) atomicOr(&sh.odd, 1ull << (at & 63));
+        }
+      }
+      vu += units;
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      const bool last = flags & kLast, whole = flags & kWhole;
+      const int row0 = d.row0, rows = d.rows, chunk = d.chunk, head = d.head, slot = d.slot, drafts = d.drafts;
+      if (lane == 0) {
+        mbar_arrive(&sh.s_empty[sb]);
+        mbar_arrive(&sh.p_full[pb]);
+        if (!last) mbar_arrive(&sh.desc_empty[ds]);
+      }
+      started = true;
+      if (last) {
+        // ---- epilogue: sums over the tokens, then O^T, a lane a channel ----
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          float x = l[j];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+          if (lane == 0) sh.lsum[warp % 4][c0 + j] = x;
+        }
+        failed |= !tc_wait(sh, &sh.p_empty[pb], (i / T::NP) & 1, a.status);
+        named_bar_sync(4, 256);  // both warpgroups' sums and the list of odd values are complete
+        tc_fence_after();
+        const unsigned long long odd = sh.odd;
+        float* rec = a.recs + (size_t)slot * Record<NR, D>::kFloats;
+        SeqWork w;
+        w.row0 = row0;
+        for (int o = 0; o < T::NO; ++o) {
+          const int ch = o * 128 + (warp % 4) * 32 + lane;
+#pragma unroll
+          for (int j0 = 0; j0 < NC; j0 += 8) {
+            uint32_t x[8];
+            tc_ld<8>(x, tm + lanes + T::COLS_O + o * NR + c0 + j0);
+            if (odd && ch < D) {
+              for (unsigned long long left = odd; left; left &= left - 1) {
+                const int u = __ffsll(left) - 1;
+                float v[2];
+                load_f32<2>(a.vd, VK, ((size_t)(row0 + u) * a.kv_heads + head) * D + (ch & ~1), v);
+                const float y = v[ch & 1];
+                if (fabsf(y) <= 3.4e38f) continue;
+                const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const int r = c0 + j0 + j;
+                  if ((sh.word[sg][r] >> u & 1) && (a.window == 0 || pos > sh.edge[sg][r] || pos < a.sinks))
+                    x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+                }
+              }
+            }
+            if (ch < D) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = c0 + j0 + j, rr = chunk * NR + r;
+                if (rr >= rows) continue;
+                const float v = __uint_as_float(x[j]);
+                if (whole) {
+                  const float sum = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
+                  const float y = v * (1.f / fmaxf(sum, 1e-10f));
+                  const size_t to = row_offset(a, w, head, rr, D) + ch;
+                  if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y);
+                  else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y);
+                } else {
+                  rec[2 * NR + r * D + ch] = v;
+                  if (ch == 0) {
+                    rec[r] = sh.ref[r] * 0.6931471805599453f;
+                    rec[NR + r] = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
+                  }
+                }
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        named_bar_sync(4, 256);  // lsum, odd and the references are free
+        if (tid == 0) sh.odd = 0;
+        if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
+      }
+    }
+  }
+  // all roles meet; tensor memory is freed on every path
+  __syncthreads();
+  if (warp == 17) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(T::COLS));
+  }
+}
+
+cudaError_t encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
+  static std::mutex mu;
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!encode) {
+    cudaDriverEntryPointQueryResult qr;
+    void* p = nullptr;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr);
+    if (e != cudaSuccess) return e;
+    if (qr != cudaDriverEntryPointSuccess || !p) return cudaErrorNotSupported;
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }
+  *fn = encode;
+  return cudaSuccess;
+}
+
+// [outer][rows][chunks of 64 channels] 16-bit values as boxes of one outer
+// entry, 16 rows and every chunk, 128-byte swizzled.
+cudaError_t value_map(CUtensorMap* map, const void* base, int vk, int dim, uint64_t rows, uint64_t row_bytes,
+                      uint64_t outer, uint64_t outer_bytes) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode;
+  const cudaError_t e = encoder(&encode);
+  if (e != cudaSuccess) return e;
+  const cuuint64_t dims[4] = {64, rows, (cuuint64_t)dim / 64, outer};
+  const cuuint64_t strides[3] = {row_bytes, 128, outer_bytes};
+  const cuuint32_t box[4] = {64, kMqPage, (cuuint32_t)dim / 64, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, vk == INT4KV_VALUES_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                            4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+template <int D, int NR, int VK>
+cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream_t stream) {
+  using T = Tc<D, NR>;
+  static_assert(T::BYTES + sizeof(TcShared<NR>) <= 227 * 1024, "shared memory");
+  constexpr auto kern = multi_query_tc_kernel<D, NR, VK>;
+  int per_sm = 0;
+  cudaError_t e = mq_occupancy<kern>(kThreadsTc, T::BYTES, &per_sm);
+  if (e != cudaSuccess) return e;
+  if (ws_bytes < (size_t)sms * 2 * Record<NR, D>::kFloats * 4) return cudaErrorInvalidValue;
+  CUtensorMap vmap, dmap;
+  const uint64_t row = (uint64_t)D * 2;
+  if ((long long)a.num_pages * a.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;  // a TMA coordinate
+  e = value_map(&vmap, a.v_pool, VK, D, kMqPage, row, (uint64_t)a.num_pages * a.kv_heads, kMqPage * row);
+  if (e != cudaSuccess) return e;
+  if (a.vd) e = value_map(&dmap, a.vd, VK, D, a.total_rows, row * a.kv_heads, a.kv_heads, row);
+  else dmap = vmap;
+  if (e != cudaSuccess) return e;
+  e = mq_launch_pdl(kern, dim3(sms), dim3(kThreadsTc), T::BYTES, stream, a, vmap, dmap);
+  if (e != cudaSuccess) return e;
+  return mq_launch_pdl(merge_records_kernel<NR, kTilePages, D>, dim3(sms - 1, (NR + kMergeWarps - 1) / kMergeWarps),
+                       dim3(kMergeWarps * 32), 0, stream, a, sms);
+}
+
+// Rows of one kv head's chunk: the smallest of 16, 32, 64, 128 that holds them
+// (head_dim 256: at most 64, the most its shared memory holds).
+int rows_of(long long rows, int dim) {
+  if (rows <= 16) return 16;
+  if (rows <= 32) return 32;
+  return rows <= 64 || dim == 256 ? 64 : 128;
+}
+
+template <int D, int NR>
+cudaError_t launch_kind(const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
+  return a.qk == INT4KV_VALUES_F16 ? launch<D, NR, INT4KV_VALUES_F16>(a, sms, ws, st)
+                                   : launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, st);
+}
+
+template <int D>
+cudaError_t launch_rows(int nr, const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
+  if (nr == 16) return launch_kind<D, 16>(a, sms, ws, st);
+  if (nr == 32) return launch_kind<D, 32>(a, sms, ws, st);
+  if constexpr (D < 256) {
+    if (nr == 128) return launch_kind<D, 128>(a, sms, ws, st);
+  }
+  return launch_kind<D, 64>(a, sms, ws, st);
+}
+
+}  // namespace
+
+namespace i4kv {
+
+size_t multi_query_tc_workspace(int dim, long long rows, int sms) {
+  const int nr = rows_of(rows, dim);
+  return (size_t)sms * 2 * (2 * nr + (size_t)nr * dim) * 4;
+}
+
+cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, size_t ws_bytes, cudaStream_t stream) {
+  const int nr = rows_of((long long)std::max(1, a.max_drafts) * a.group_q, dim);
+  if (dim == 64) return launch_rows<64>(nr, a, sms, ws_bytes, stream);
+  if (dim == 128) return launch_rows<128>(nr, a, sms, ws_bytes, stream);
+  return launch_rows<256>(nr, a, sms, ws_bytes, stream);
+}
+
+}  // namespace i4kv
