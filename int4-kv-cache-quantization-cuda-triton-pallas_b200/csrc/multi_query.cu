@@ -39,6 +39,7 @@ bool sizes_ok(int batch, int hq, int hkv, int dim, int page, int group, int max_
 cudaError_t run(MultiQueryArgs a, int dim, int vk, void* workspace, size_t bytes, cudaStream_t stream) {
   if (!aligned16(workspace) || !workspace) return cudaErrorInvalidValue;
   int sms = 0;
+  if ((long long)a.total_rows * a.kv_heads * a.group_q > 0x7fffffffll) return cudaErrorInvalidValue;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   a.recs = static_cast<float*>(workspace);

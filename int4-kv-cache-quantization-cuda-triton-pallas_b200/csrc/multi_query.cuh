@@ -61,8 +61,10 @@ I4KV_DEVINL void mq_status(uint32_t* status, uint32_t bits) {
   if (status) atomicOr(status, bits);
 }
 
+// (Not inlined: it runs once per sequence, and every kernel calls it from
+// several places.)
 template <int NR, int TP>
-I4KV_DEVINL SeqWork seq_work(const MultiQueryArgs& a, int b, bool report) {
+__device__ __noinline__ SeqWork seq_work(const MultiQueryArgs& a, int b, bool report) {
   SeqWork w;
   const int cap = a.max_pages * kMqPage;  // < 2^31 - 128 (checked on the host)
   int len = a.seq_lens[b];
@@ -128,6 +130,7 @@ __device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, 
   const int per = (a.batch + nt - 1) / nt;
   const int lo = min(a.batch, t * per), hi = min(a.batch, lo + per);
   long long local = 0;
+#pragma unroll 1
   for (int b = lo; b < hi; ++b) local += seq_units<NR, TP>(a, b, blockIdx.x == 0);
   long long incl = local;
 #pragma unroll
@@ -139,6 +142,7 @@ __device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, 
   __syncthreads();
   if (t == 0) {
     long long run = 0;
+#pragma unroll 1
     for (int i = 0; i < nt / 32; ++i) {
       const long long v = s_tmp[3 + i];
       s_tmp[3 + i] = run;
@@ -153,6 +157,7 @@ __device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, 
   const long long u = pick(total);
   long long base = s_tmp[3 + warp] + incl - local;
   if (u >= base && u < base + local) {
+#pragma unroll 1
     for (int b = lo; b < hi; ++b) {
       const long long n = seq_units<NR, TP>(a, b, false);
       if (u < base + n) {
@@ -171,14 +176,15 @@ __device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, 
 }
 
 // First tile of CTA c of n (n <= total): contiguous runs of equal length.
-I4KV_DEVINL long long run_start(long long c, long long total, long long n) { return c * total / n; }
-I4KV_DEVINL long long run_of(long long u, long long total, long long n) { return ((u + 1) * n - 1) / total; }
+static __device__ __noinline__ long long tile_div(long long x, long long n) { return floor_div_s52(x, n); }
+I4KV_DEVINL long long run_start(long long c, long long total, long long n) { return tile_div(c * total, n); }
+I4KV_DEVINL long long run_of(long long u, long long total, long long n) { return tile_div((u + 1) * n - 1, total); }
 
 I4KV_DEVINL TileAt tile_at(const MultiQueryArgs& a, const SeqWork& w, int b, long long rem) {
   TileAt p;
   const int per_head = w.tiles * w.chunks;
   p.b = b;
-  p.head = (int)(rem / per_head);
+  p.head = (int)tile_div(rem, per_head);
   const int r = (int)(rem - (long long)p.head * per_head);
   p.chunk = r / w.tiles;
   p.tile = r - p.chunk * w.tiles;
@@ -258,10 +264,12 @@ struct Record {
 // Rows of sequences that see nothing (a window over an empty cache) are zeros.
 template <int NR, int TP, int D>
 __device__ void zero_idle_rows(const MultiQueryArgs& a) {
+#pragma unroll 1
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     const SeqWork w = seq_work<NR, TP>(a, b, false);
     if (w.tiles > 0 || w.rows == 0) continue;
     const int n = a.kv_heads * a.group_q * D;  // one row a sequence
+#pragma unroll 1
     for (int i = 2 * threadIdx.x; i < n; i += 2 * blockDim.x)
       store2(a.out, a.qk, (size_t)w.row0 * n + i, 0.f, 0.f);
   }
@@ -305,6 +313,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQu
     return a.recs + (2 * i + (tail ? 1 : 0)) * (size_t)kRec;
   };
   float M = -INFINITY;
+#pragma unroll 1
   for (long long i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(record(i) + r));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -312,6 +321,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQu
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
   if (M != -INFINITY) {
+#pragma unroll 2
     for (long long i = c; i <= last; ++i) {
       const float* rec = record(i);
       const float e = exp2_fast((__ldcg(rec + r) - M) * kLog2e);

@@ -22,15 +22,17 @@
 // pool's type, which the tensor cores multiply with the stored values as they
 // are.
 //
-// A tile is 128 cached tokens (8 pages) or the drafts. Roles of the 18 warps:
-//   0-7   softmax: S^T from tensor memory, mask, weights to shared memory,
-//         the rare rescale of O^T, and the stream's epilogue
-//   8-15  conversion: packed codes to float16 keys (K-major, 128-byte swizzle),
-//         a stream's queries, drafted keys
-//   16    copies: pages by bulk (codes, scales) and tensor copies (values, in
-//         the swizzled layout the MMA reads: V is stored token-major, which is
-//         the transposed operand's contiguous side, so nothing is rearranged)
-//   17    MMA issue, one thread: S^T of tile i, then O^T of tile i - 1
+// A tile is 128 cached tokens (8 pages) or the drafts. Roles of the warps:
+//   softmax (8, or 16 for 128 rows): S^T from tensor memory, mask, weights to
+//       shared memory, the rare rescale of O^T, and the stream's epilogue
+//   conversion (8 or 5): packed codes to float16 keys (K-major, 128-byte
+//       swizzle), a stream's queries, drafted keys
+//   MMA issue (1): S^T of tile i, then O^T of tile i - 1
+//   copies (2): pages by bulk (codes, scales) and tensor copies (values, in the
+//       swizzled layout the MMA reads: V is stored token-major, which is the
+//       transposed operand's contiguous side, so nothing is rearranged)
+// What runs once per stream is kept out of the tile's straight line: the roles
+// run different code side by side, and the instruction caches are small.
 // One persistent CTA per SM; work decomposition and merge: multi_query.cuh.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -43,8 +45,6 @@ using namespace i4kv;
 
 namespace {
 
-constexpr int kSoftWarps = 8, kConvWarps = 8;
-constexpr int kThreadsTc = 32 * (kSoftWarps + kConvWarps + 2);
 constexpr int kTile = 128, kTilePages = kTile / kMqPage;
 constexpr int kDesc = 4;                        // tiles in flight between the roles
 constexpr uint64_t kTcWaitNs = 2000000000ull;   // bounded waits: 2 s
@@ -94,6 +94,12 @@ I4KV_DEVINL void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
 }
 I4KV_DEVINL void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of a converged warp (the same one every time).
+I4KV_DEVINL bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -120,20 +126,35 @@ __host__ __device__ constexpr uint32_t mma_desc(int m, int n, int fmt, bool mn) 
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// A ring position: stage and the parity of its current use.
+struct Ring {
+  uint32_t s = 0, ph = 0;
+  template <int N>
+  I4KV_DEVINL void next() {
+    if (++s == N) { s = 0; ph ^= 1; }
+  }
+};
+
 template <int D, int NR>
 struct Tc {
   static constexpr int CH = D / 64;                        // 64-channel chunks
   static constexpr int PAGE_V = kMqPage * D * 2;           // value bytes of a page
   static constexpr int UNIT = 16384, PPU = UNIT / PAGE_V;  // value ring: units of PPU pages
-  static constexpr int UNITS = kTilePages / PPU;           // units of a full tile
-  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 5 : 6);
-  static constexpr int NK = D == 256 ? 1 : 2;              // stages of packed codes
-  static constexpr int NP = (NR > 64 || D == 256) ? 1 : 2; // weight buffers
+  // Stages. One buffer of dequantized keys or of weights makes its writer wait
+  // for the MMA that reads it, so there are two of each where they fit.
+  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : 5;
+  static constexpr int NK = D == 256 ? 1 : 2;              // packed codes and scales
+  static constexpr int NH = (D == 64 || (D == 128 && NR <= 64)) ? 2 : 1;  // dequantized keys
+  static constexpr int NP = (D == 256 || NR > 32) ? 1 : 2; // weights
+  // Softmax warpgroups share the rows: at most 32 of them (and as many sums) a
+  // thread. 24 warps leave 80 registers a thread, 19 leave 96.
+  static constexpr int WG = NR > 64 ? 4 : 2, SOFT = 4 * WG, CONV = NR > 64 ? 5 : 8;
+  static constexpr int THREADS = 32 * (SOFT + CONV + 3);
   static constexpr int PC = (NR + 63) / 64;                // 64-row chunks of the weights
   static constexpr int NO = D == 256 ? 2 : 1;              // 128-channel blocks of O^T
   static constexpr int KH = kTile * D * 2, Q = NR * D * 2, P = PC * kTile * 128;
   static constexpr int KC = kTile * D / 2, SZ = kTilePages * 2 * D * 4;
-  static constexpr int KH_OFF = 0, V_OFF = KH_OFF + KH, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q;
+  static constexpr int KH_OFF = 0, V_OFF = KH_OFF + NH * KH, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q;
   static constexpr int KC_OFF = P_OFF + NP * P, SZ_OFF = KC_OFF + NK * KC, END = SZ_OFF + NK * SZ;
   static constexpr int BYTES = END + 1024;                 // the base is rounded up to 1024
   static constexpr int COLS_O = 2 * NR, COLS = 512;
@@ -142,7 +163,7 @@ struct Tc {
 
 struct TileDesc {
   int flags, pages, len, drafts;
-  int row0, rows, chunk, head;
+  int row0, head;
   int seg, slot;                // segment ring entry; record of a shared stream
   int low_edge;                 // no row sees cached positions <= low_edge (but the sinks)
   int at[kTilePages];           // position of each page's first token, -1: not there
@@ -153,29 +174,31 @@ enum : int { kDraftTile = 1, kMasked = 2, kFirst = 4, kLast = 8, kWhole = 16 };
 template <int NR>
 struct TcShared {
   uint64_t desc_full[kDesc], desc_empty[kDesc], kc_full[2], kc_empty[2], v_full[6], v_empty[6];
-  uint64_t kh_full, kh_empty, s_full[2], s_empty[2], p_full[2], p_empty[2];
+  uint64_t kh_full[2], kh_empty[2], s_full[2], s_empty[2], p_full[2], p_empty[2];
   TileDesc desc[kDesc];
-  uint64_t word[kDesc][NR];     // visible drafts of each row, per segment
-  int edge[kDesc][NR];          // last position a row does not see (-1: none)
-  int depth[kDesc][kMqMaxDrafts];
+  uint64_t word[kDesc][kMqMaxDrafts];  // per segment: the drafts each draft sees,
+  int depth[kDesc][kMqMaxDrafts];      // its ancestors,
+  int row[kDesc][NR];                  // each row's row of the outputs [rows * heads], -1: none,
+  uint8_t draft[kDesc][NR];            // and its draft
   float qscale[kDesc];
+  int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
-  float ref[NR], sub[NR], alpha[NR], part[4][NR], lsum[4][NR];
-  float qmax[kConvWarps];
+  float ref[NR], sub[NR], alpha[NR], inv[NR];
+  float part[4][NR];            // maxima, or sums, of the four quarters of a tile's tokens
+  float qmax[8];
   unsigned long long odd;       // drafts of the segment whose values are not all finite
   uint32_t tmem;
-  int dead;
-  long long scan[3 + kThreadsTc / 32];
+  long long scan[3 + 32];
 };
 
-// Bounded wait; false after a timeout here or in another role.
-template <typename Sh>
-I4KV_DEVINL bool tc_wait(Sh& sh, uint64_t* bar, uint32_t parity, uint32_t* status) {
-  if (mbar_try_wait(bar, parity)) return true;
+// Bounded wait: false (and a status bit) when its limit passes.
+__device__ __noinline__ bool tc_wait_slow(uint64_t* bar, uint32_t parity, uint32_t* status) {
   if (mbar_wait_bounded(bar, parity, kTcWaitNs)) return true;
-  *(volatile int*)&sh.dead = 1;
   mq_status(status, kStatusWaitTimeout);
   return false;
+}
+I4KV_DEVINL bool tc_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return mbar_try_wait(bar, parity) || tc_wait_slow(bar, parity, status);
 }
 
 template <int VK>
@@ -189,6 +212,14 @@ I4KV_DEVINL uint32_t pack16(float x, float y) {
   }
 }
 
+// (d0, d1) = (a0 b0 + c0, a1 b1 + c1), each rounded once.
+I4KV_DEVINL void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 c, a, b, c;\n\tmov.b64 {%0, %1}, c;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
 // Power of two that brings |x| <= top to [1, 2) (1 for 0), and its inverse.
 I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
   const int e = top > 0.f ? (int)((__float_as_uint(top) >> 23) & 0xFF) : 127;
@@ -196,278 +227,311 @@ I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
   down = __uint_as_float((uint32_t)(254 - c) << 23);
   up = __uint_as_float((uint32_t)c << 23);
 }
+constexpr float kHalfRoom = 32768.f;  // magnitudes up to here are kept as float16 unscaled
+I4KV_DEVINL float finite_abs(float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; }
 
 template <int D, int NR, int VK>
-__global__ void __launch_bounds__(kThreadsTc, 1)
+__global__ void __launch_bounds__(Tc<D, NR>::THREADS, 1)
 multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ CUtensorMap dmap) {
   using T = Tc<D, NR>;
+  constexpr int kSoftWarps = T::SOFT, kConvWarps = T::CONV;
+  constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;  // two copy warps
+  constexpr int kBarConv = 1, kBarSoft = 2, kBarGroup = 3;  // named barriers (one per warpgroup from kBarGroup on)
   extern __shared__ char smem_raw[];
   __shared__ TcShared<NR> sh;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
-  grid_dependency_wait();
-  allow_dependent_launch();
-  if (tid == 0) {
-    for (int i = 0; i < kDesc; ++i) {
-      mbar_init(&sh.desc_full[i], 1);
-      mbar_init(&sh.desc_empty[i], kSoftWarps + kConvWarps + 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.kc_full[i], kTilePages);
-      mbar_init(&sh.kc_empty[i], kConvWarps);
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.s_empty[i], kSoftWarps);
-      mbar_init(&sh.p_full[i], kSoftWarps);
-      mbar_init(&sh.p_empty[i], 1);
-    }
-    for (int i = 0; i < 6; ++i) {
-      mbar_init(&sh.v_full[i], T::PPU);
-      mbar_init(&sh.v_empty[i], 1);
-    }
-    mbar_init(&sh.kh_full, kConvWarps);
-    mbar_init(&sh.kh_empty, 1);
-    sh.dead = 0;
-    sh.odd = 0;
-    fence_barrier_init();
-  }
-  zero_idle_rows<NR, kTilePages, D>(a);
-  int b0;
-  long long before;
-  const long long cta = blockIdx.x, ctas = gridDim.x;
-  const long long total = locate_sequence<NR, kTilePages>(
-      a, sh.scan, [&](long long n) { return n > cta ? run_start(cta, n, min(ctas, n)) : 0ll; }, b0, before);
-  const long long runs = min(ctas, total);
-  if (cta >= runs) return;
-  const long long u0 = run_start(cta, total, runs), u1 = run_start(cta + 1, total, runs);
-  const int n_tiles = (int)(u1 - u0);
-  if (warp == 17) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)),
                  "n"(T::COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     tc_fence_before();
   }
-  __syncthreads();
+  if (tid == 0) {
+    for (int i = 0; i < kDesc; ++i) {
+      mbar_init(&sh.desc_full[i], 1);
+      mbar_init(&sh.desc_empty[i], kSoftWarps + kConvWarps + 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.kc_full[i], 1);
+      mbar_init(&sh.kc_empty[i], kConvWarps);
+      mbar_init(&sh.kh_full[i], kConvWarps);
+      mbar_init(&sh.kh_empty[i], 1);
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.s_empty[i], kSoftWarps);
+      mbar_init(&sh.p_full[i], kSoftWarps);
+      mbar_init(&sh.p_empty[i], 1);
+    }
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    sh.odd = 0;
+    fence_barrier_init();
+  }
+  grid_dependency_wait();
+  allow_dependent_launch();
+  if (!a.offs) zero_idle_rows<NR, kTilePages, D>(a);
+  int b0;
+  long long before;
+  const long long cta = blockIdx.x, ctas = gridDim.x;
+  const long long total = locate_sequence<NR, kTilePages>(
+      a, sh.scan, [&](long long n) { return n > cta ? run_start(cta, n, min(ctas, n)) : 0ll; }, b0, before);
+  const long long runs = min(ctas, total);
+  const long long u0 = cta < runs ? run_start(cta, total, runs) : 0;
+  const int n_tiles = cta < runs ? (int)(run_start(cta + 1, total, runs) - u0) : 0;
   tc_fence_after();
   const uint32_t tm = sh.tmem;
 
-  if (warp == 16) {
+  if (n_tiles == 0) {
+  } else if (warp >= kCopyWarp) {
     // ------------------------------------------------------------ copies
+    // Both warps walk the tiles; the first publishes their descriptors and copies
+    // codes and scales, the second the values.
+    const bool values = warp > kCopyWarp;
     SeqWork w = seq_work<NR, kTilePages>(a, b0, false);
     TileAt p = tile_at(a, w, b0, u0 - before);
     int seg = -1, high_edge = 0;
-    uint32_t kc = 0, vu = 0;  // stages used so far
+    Ring kc, v;
     bool ok = true;
+    // this lane's page of tile p: loaded one tile ahead of its use
+    int pg = 0, phys = -1, home = -1;
+    auto fetch = [&]() {
+      const int i = p.tile * kTilePages + lane;
+      phys = home = -1;
+      if (lane < kTilePages && p.tile < w.cache_tiles && i < w.vis_pages) {
+        pg = visible_page(w, i);
+        const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
+        phys = __ldg(bt + pg);
+        home = __ldg(bt + pg / a.group_pages * a.group_pages);
+      }
+    };
+    fetch();
+#pragma unroll 1
     for (int i = 0; i < n_tiles && ok; ++i) {
       const int ds = i % kDesc;
-      if (i >= kDesc) ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.desc_empty[ds], (i / kDesc - 1) & 1, a.status));
-      if (!ok) break;
-      const bool first = i == 0 || p.tile == 0;
-      if (first) {
-        ++seg;
-        const int sg = seg % kDesc;
-        int top = 0;
-        if (a.mask) {
-          for (int t = lane; t < w.drafts; t += 32) {
-            const int dp = draft_depth((uint64_t)a.mask[w.row0 + t], t, w.drafts);
+      const bool draft = p.tile >= w.cache_tiles;
+      const int here = draft ? (w.drafts + kMqPage - 1) / kMqPage
+                             : min(kTilePages, w.vis_pages - p.tile * kTilePages);
+      const bool mine = lane < here;
+      const bool live = mine && (draft || (phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages));
+      const uint32_t lives = __ballot_sync(0xffffffffu, live);
+      if (!values) {
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.desc_empty[ds], (i / kDesc + 1) & 1, a.status));
+        if (!ok) break;
+        const bool first = i == 0 || p.tile == 0;
+        if (first) {
+          ++seg;
+          const int sg = seg % kDesc;
+          int top = 0;
+#pragma unroll 1
+          for (int t = lane; t < max(w.drafts, 1); t += 32) {
+            const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
+            const int dp = a.mask ? draft_depth(word, t, w.drafts) : 0;
+            sh.word[sg][t] = word;
             sh.depth[sg][t] = dp;
             top = max(top, dp);
           }
           top = __reduce_max_sync(0xffffffffu, top);
-        }
-        high_edge = w.pos0 + top - a.window;
-        for (int r = lane; r < NR; r += 32) {
-          const int t = min(p.chunk * NR + r, w.rows - 1) / a.group_q;
-          const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
-          sh.word[sg][r] = word;
-          sh.edge[sg][r] = a.window > 0 ? w.pos0 + (a.mask ? draft_depth(word, t, w.drafts) : 0) - a.window : -1;
-        }
-      }
-      const bool draft = p.tile >= w.cache_tiles;
-      const int here = draft ? (w.drafts + kMqPage - 1) / kMqPage
-                             : min(kTilePages, w.vis_pages - p.tile * kTilePages);
-      int phys = 0, home = -1, at = -1;
-      bool live = false, clean = true;  // the page is read; every row sees all of it
-      if (lane < here) {
-        if (draft) {
-          at = lane * kMqPage;
-          live = true;
-          clean = false;
-        } else {
-          const int pg = visible_page(w, p.tile * kTilePages + lane);
-          const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
-          phys = __ldg(bt + pg);
-          home = __ldg(bt + pg / a.group_pages * a.group_pages);
-          live = phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages;
-          if (!live) mq_status(a.status, kStatusBadPage);
-          at = live ? pg * kMqPage : -1;
-          clean = live && at + kMqPage <= w.len &&
-                  (a.window == 0 || at > high_edge || at + kMqPage <= a.sinks);
-          if (!live) home = -1;
-        }
-      }
-      const bool masked = !__all_sync(0xffffffffu, clean) || here < kTilePages;
-      // pages of one group share a scale slot: the slot of the group's first page here
-      const int prev = __shfl_up_sync(0xffffffffu, home, 1);
-      const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || home != prev);
-      const int slot = 31 - __clz(starts & ((2u << lane) - 1));
-      if (lane < kTilePages) {
-        sh.desc[ds].at[lane] = at;
-        sh.desc[ds].sz[lane] = slot;
-      }
-      if (lane == 0) {
-        TileDesc& d = sh.desc[ds];
-        const long long first_u = u0 + i - p.tile;  // the stream's first tile
-        const bool ends = p.tile + 1 == w.tiles;
-        d.flags = (draft ? kDraftTile : 0) | (masked ? kMasked : 0) | (first ? kFirst : 0) |
-                  ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= u0) ? kWhole : 0);
-        d.pages = here;
-        d.len = w.len;
-        d.drafts = w.drafts;
-        d.row0 = w.row0;
-        d.rows = w.rows;
-        d.chunk = p.chunk;
-        d.head = p.head;
-        d.seg = seg % kDesc;
-        d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
-        d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
-      // packed codes and scales
-      if (!draft) {
-        const int ks = kc % T::NK;
-        if (kc >= T::NK)
-          ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.kc_empty[ks], (kc / T::NK - 1) & 1, a.status));
-        if (!ok) break;
-        if (lane < kTilePages) {
-          const bool sz = live && slot == lane;
-          mbar_arrive_expect_tx(&sh.kc_full[ks], live ? kMqPage * D / 2 + (sz ? 2 * D * 4 : 0) : 0);
-          if (live)
-            bulk_g2s(smem + T::KC_OFF + ks * T::KC + lane * (kMqPage * D / 2),
-                     a.k_pool + ((size_t)phys * a.kv_heads + p.head) * (kMqPage * D / 2), kMqPage * D / 2,
-                     &sh.kc_full[ks]);
-          if (sz)
-            bulk_g2s(smem + T::SZ_OFF + ks * T::SZ + lane * (2 * D * 4),
-                     a.sz_pool + ((size_t)home * a.kv_heads + p.head) * 2 * D, 2 * D * 4, &sh.kc_full[ks]);
-        }
-        ++kc;
-      }
-      // values, a unit of pages at a time
-      for (int q = 0; q * T::PPU < here; ++q) {
-        const int vs = vu % T::NV;
-        if (vu >= T::NV)
-          ok = __all_sync(0xffffffffu, tc_wait(sh, &sh.v_empty[vs], (vu / T::NV - 1) & 1, a.status));
-        if (!ok) break;
-        if (lane / T::PPU == q) {
-          mbar_arrive_expect_tx(&sh.v_full[vs], live ? T::PAGE_V : 0);
-          if (live) {
-            char* dst = smem + T::V_OFF + vs * T::UNIT + (lane % T::PPU) * T::PAGE_V;
-            if (draft) tma_page(dst, &dmap, w.row0 + lane * kMqPage, p.head, &sh.v_full[vs]);
-            else tma_page(dst, &vmap, 0, phys * a.kv_heads + p.head, &sh.v_full[vs]);
+          high_edge = w.pos0 + top - a.window;
+#pragma unroll 1
+          for (int r = lane; r < NR; r += 32) {
+            const int rr = p.chunk * NR + r, t = min(rr, w.rows - 1) / a.group_q;
+            sh.draft[sg][r] = (uint8_t)t;
+            sh.row[sg][r] = rr < w.rows ? ((w.row0 + t) * a.kv_heads + p.head) * a.group_q + rr - t * a.group_q : -1;
           }
         }
-        ++vu;
+        int at = -1;
+        bool clean = true;  // every row sees all of the page
+        if (mine) {
+          if (draft) {
+            at = lane * kMqPage;
+            clean = false;
+          } else {
+            if (!live) mq_status(a.status, kStatusBadPage);
+            at = live ? pg * kMqPage : -1;
+            clean = live && at + kMqPage <= w.len &&
+                    (a.window == 0 || at > high_edge || at + kMqPage <= a.sinks);
+          }
+        }
+        const bool masked = !__all_sync(0xffffffffu, clean) || here < kTilePages;
+        // pages of one group share a scale slot: the slot of the group's first page here
+        if (!live) home = -1;
+        const int prev = __shfl_up_sync(0xffffffffu, home, 1);
+        const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || home != prev);
+        const int slot = 31 - __clz(starts & ((2u << lane) - 1));
+        if (lane < kTilePages) {
+          sh.desc[ds].at[lane] = at;
+          sh.desc[ds].sz[lane] = slot;
+        }
+        if (lane == 0) {
+          TileDesc& d = sh.desc[ds];
+          const long long first_u = u0 + i - p.tile;  // the stream's first tile
+          const bool ends = p.tile + 1 == w.tiles;
+          d.flags = (draft ? kDraftTile : 0) | (masked ? kMasked : 0) | (first ? kFirst : 0) |
+                    ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= u0) ? kWhole : 0);
+          d.pages = here;
+          d.len = w.len;
+          d.drafts = w.drafts;
+          d.row0 = w.row0;
+          d.head = p.head;
+          d.seg = seg % kDesc;
+          d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
+          d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
+        if (!draft) {
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.kc_empty[kc.s], kc.ph ^ 1, a.status));
+          if (!ok) break;
+          const uint32_t szs = lives & starts;
+          uint64_t* bar = &sh.kc_full[kc.s];
+          char* kdst = smem + T::KC_OFF + kc.s * T::KC;
+          char* zdst = smem + T::SZ_OFF + kc.s * T::SZ;
+          if (lane == 0)
+            mbar_arrive_expect_tx(bar, __popc(lives) * (kMqPage * D / 2) + __popc(szs) * (2 * D * 4));
+          __syncwarp();
+#pragma unroll 1
+          for (int g = 0; g < here; ++g) {
+            const int ph = __shfl_sync(0xffffffffu, phys, g), hm = __shfl_sync(0xffffffffu, home, g);
+            if (!(lives >> g & 1)) continue;
+            if (elect_one()) {
+              bulk_g2s(kdst + g * (kMqPage * D / 2),
+                       a.k_pool + ((size_t)ph * a.kv_heads + p.head) * (kMqPage * D / 2), kMqPage * D / 2, bar);
+              if (szs >> g & 1)
+                bulk_g2s(zdst + g * (2 * D * 4), a.sz_pool + ((size_t)hm * a.kv_heads + p.head) * 2 * D, 2 * D * 4,
+                         bar);
+            }
+          }
+          kc.next<T::NK>();
+        }
+      } else {
+        const CUtensorMap* map = draft ? &dmap : &vmap;
+#pragma unroll 1
+        for (int g0 = 0; g0 < here; g0 += T::PPU) {
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.v_empty[v.s], v.ph ^ 1, a.status));
+          if (!ok) break;
+          uint64_t* bar = &sh.v_full[v.s];
+          const int g1 = min(g0 + T::PPU, here);
+          const uint32_t unit = lives >> g0 & ((1u << (g1 - g0)) - 1);
+          if (lane == 0) mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
+          __syncwarp();
+          char* dst = smem + T::V_OFF + v.s * T::UNIT;
+#pragma unroll 1
+          for (int g = g0; g < g1; ++g) {
+            const int ph = __shfl_sync(0xffffffffu, phys, g);
+            if ((lives >> g & 1) && elect_one())
+              tma_page(dst + (g - g0) * T::PAGE_V, map, draft ? w.row0 + g * kMqPage : 0,
+                       draft ? p.head : ph * a.kv_heads + p.head, bar);
+            __syncwarp();
+          }
+          v.next<T::NV>();
+        }
+        if (!ok) break;
       }
       if (++p.tile >= w.tiles) next_stream<NR, kTilePages>(a, w, p);
+      if (i + 1 < n_tiles) fetch();
     }
     // after a timeout: the copies issued so far land (or a bound passes) before the CTA ends
     if (!ok && lane == 0) {
-      for (uint32_t s = kc > T::NK ? kc - T::NK : 0; s < kc; ++s)
-        mbar_wait_bounded(&sh.kc_full[s % T::NK], (s / T::NK) & 1, 10000000ull);
-      for (uint32_t s = vu > T::NV ? vu - T::NV : 0; s < vu; ++s)
-        mbar_wait_bounded(&sh.v_full[s % T::NV], (s / T::NV) & 1, 10000000ull);
+      for (int s = 0; s < T::NK && !values; ++s) mbar_wait_bounded(&sh.kc_full[s], s < (int)kc.s ? kc.ph : kc.ph ^ 1, 10000000ull);
+      for (int s = 0; s < T::NV && values; ++s) mbar_wait_bounded(&sh.v_full[s], s < (int)v.s ? v.ph : v.ph ^ 1, 10000000ull);
     }
     __syncwarp();
-  } else if (warp == 17) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      constexpr uint32_t kQk = mma_desc(128, NR, 0, false);
-      constexpr uint32_t kPv = mma_desc(128, NR, VK == INT4KV_VALUES_BF16 ? 1 : 0, true);
-      const uint32_t base = smem_addr(smem);
-      uint32_t vu = 0;
-      int pages = 0;       // of tile i - 1
-      bool fresh = true;   // tile i - 1 starts its segment
-      bool ok = true;
-      for (int i = 0; i <= n_tiles && ok; ++i) {
-        int next_pages = 0;
-        bool next_fresh = false;
-        if (i < n_tiles) {
-          const int ds = i % kDesc;
-          ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status);
-          if (!ok) break;
-          next_pages = sh.desc[ds].pages;
-          next_fresh = sh.desc[ds].flags & kFirst;
-          mbar_arrive(&sh.desc_empty[ds]);
-          ok = tc_wait(sh, &sh.kh_full, i & 1, a.status) &&
-               (i < 2 || tc_wait(sh, &sh.s_empty[i & 1], (i / 2 - 1) & 1, a.status));
-          if (!ok) break;
-          tc_fence_after();
+    constexpr uint32_t kQk = mma_desc(128, NR, 0, false);
+    constexpr uint32_t kPv = mma_desc(128, NR, VK == INT4KV_VALUES_BF16 ? 1 : 0, true);
+    const uint32_t base = smem_addr(smem);
+    Ring v;
+    int pages = 0;       // of tile i - 1
+    bool fresh = true;   // tile i - 1 starts its segment
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i <= n_tiles && ok; ++i) {
+      int next_pages = 0;
+      bool next_fresh = false;
+      if (i < n_tiles) {
+        const int ds = i % kDesc, hb = i % T::NH;
+        ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
+        next_pages = sh.desc[ds].pages;
+        next_fresh = sh.desc[ds].flags & kFirst;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
+        ok = ok && tc_wait(&sh.kh_full[hb], (i / T::NH) & 1, a.status) &&
+             tc_wait(&sh.s_empty[i & 1], (i / 2 + 1) & 1, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t kd = mat_desc(base + T::KH_OFF + hb * T::KH, 16, 1024), qd = mat_desc(base + T::Q_OFF, 16, 1024);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t in = (k % 4) * 32;
-            tc_mma(tm + (i & 1) * NR, mat_desc(base + T::KH_OFF + (k / 4) * (kTile * 128) + in, 16, 1024),
-                   mat_desc(base + T::Q_OFF + (k / 4) * (NR * 128) + in, 16, 1024), kQk, k > 0);
-          }
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma(tm + (i & 1) * NR, kd + (k / 4) * (kTile * 128 / 16) + (k % 4) * 2,
+                   qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
           tc_commit(&sh.s_full[i & 1]);
-          tc_commit(&sh.kh_empty);
+          tc_commit(&sh.kh_empty[hb]);
         }
-        if (i > 0) {
-          const int j = i - 1, pb = j % T::NP;
-          ok = tc_wait(sh, &sh.p_full[pb], (j / T::NP) & 1, a.status);
+        __syncwarp();
+      }
+      if (i > 0) {
+        const int j = i - 1, pb = j % T::NP;
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.p_full[pb], (j / T::NP) & 1, a.status));
+        if (!ok) break;
+        const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P, kTile * 128, 1024);
+#pragma unroll 1
+        for (int g0 = 0; g0 < pages; g0 += T::PPU) {
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.v_full[v.s], v.ph, a.status));
           if (!ok) break;
           tc_fence_after();
-          for (int g = 0; g < pages; ++g) {
-            const int vs = vu % T::NV;
-            if (g % T::PPU == 0) {
-              ok = tc_wait(sh, &sh.v_full[vs], (vu / T::NV) & 1, a.status);
-              if (!ok) break;
-              tc_fence_after();
-            }
-            const uint32_t va = base + T::V_OFF + vs * T::UNIT + (g % T::PPU) * T::PAGE_V;
-            const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P + g * 2048, kTile * 128, 1024);
+          if (elect_one()) {
+            const uint64_t vd = mat_desc(base + T::V_OFF + v.s * T::UNIT, 2048, 1024);
 #pragma unroll
-            for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
-              tc_mma(tm + T::COLS_O + o * NR, mat_desc(va + o * 2 * 2048, 2048, 1024), pd, kPv,
-                     !(fresh && g == 0));
-            if (g % T::PPU == T::PPU - 1 || g == pages - 1) {
-              tc_commit(&sh.v_empty[vs]);
-              ++vu;
+            for (int q = 0; q < T::PPU; ++q) {
+              if (g0 + q < pages) {
+#pragma unroll
+                for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
+                  tc_mma(tm + T::COLS_O + o * NR, vd + (q * T::PAGE_V + o * 4096) / 16, pd + (g0 + q) * (2048 / 16),
+                         kPv, !(fresh && g0 + q == 0));
+              }
             }
+            tc_commit(&sh.v_empty[v.s]);
           }
-          if (!ok) break;
-          tc_commit(&sh.p_empty[pb]);
+          __syncwarp();
+          v.next<T::NV>();
         }
-        pages = next_pages;
-        fresh = next_fresh;
+        if (!ok) break;
+        if (elect_one()) tc_commit(&sh.p_empty[pb]);
+        __syncwarp();
       }
+      pages = next_pages;
+      fresh = next_fresh;
     }
-    __syncwarp();
   } else if (warp >= kSoftWarps) {
     // ------------------------------------------------------------ conversion
-    constexpr int LPT = D / 16;          // lanes of a token, 16 channels each
+    constexpr int LPT = D / 16;          // lanes of a token: 8 channels at 8 c and 8 at 8 (c + LPT)
     constexpr int TPW = 32 / LPT;        // tokens of a warp at a time
     const int cw = warp - kSoftWarps, ct = tid - 32 * kSoftWarps;
-    const int c = lane % LPT;
-    const int chunk = c / 4, flip = chunk & 1;  // 64-channel chunk; order of the two 16-byte stores
-    uint32_t kc = 0;
-    // 16 channels of token / row `r` of an operand with `rows` rows
+    const int c = lane % LPT, t_lane = cw * TPW + lane / LPT;
+    const int ca = 8 * c, cb = 8 * (c + LPT);
+    Ring kc;
+    // The lane's 16 channels of token / row r of an operand with `rows` rows.
     auto put = [&](char* op, int rows, int r, const uint32_t (&h)[8]) {
-      char* row = op + chunk * (rows * 128) + r * 128;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int s = j ^ flip, piece = 2 * (c % 4) + s;
-        const uint4 v = s ? make_uint4(h[4], h[5], h[6], h[7]) : make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(row + ((piece ^ (r & 7)) << 4)) = v;
-      }
+      char* at = op + r * 128;
+      *reinterpret_cast<uint4*>(at + (ca / 64) * (rows * 128) + ((((ca / 8) & 7) ^ (r & 7)) << 4)) =
+          make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(at + (cb / 64) * (rows * 128) + ((((cb / 8) & 7) ^ (r & 7)) << 4)) =
+          make_uint4(h[4], h[5], h[6], h[7]);
     };
-    // 16 consecutive 16-bit inputs widened to float32
+    // ... of a row of 16-bit inputs, widened to float32
     auto get = [&](const void* src, size_t i, float (&x)[16]) {
-      const uint4* p4 = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + i);
-      const uint4 u = __ldg(p4), v = __ldg(p4 + 1);
-      const uint32_t wd[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      const uint16_t* p16 = static_cast<const uint16_t*>(src) + i;
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p16 + ca));
+      const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(p16 + cb));
+      const uint32_t wd[8] = {u.x, u.y, u.z, u.w, w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (VK == INT4KV_VALUES_F16) {
@@ -480,165 +544,210 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
       }
     };
-    auto top_of = [&](const float (&x)[16]) {  // largest finite magnitude
-      float m = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float y = fabsf(x[j]);
-        m = fmaxf(m, y <= 3.4e38f ? y : 0.f);
-      }
-      return m;
-    };
+#pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
-      const int ds = i % kDesc;
-      bool ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status);
+      const int ds = i % kDesc, hb = i % T::NH;
+      bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
       const TileDesc& d = sh.desc[ds];
       const int flags = d.flags, pages = d.pages;
-      const int ks = kc % T::NK;
-      if (ok && !(flags & kDraftTile)) ok = tc_wait(sh, &sh.kc_full[ks], (kc / T::NK) & 1, a.status);
-      if (ok && i > 0) ok = tc_wait(sh, &sh.kh_empty, (i - 1) & 1, a.status);
-      // (uniform over the role: its warps meet in named barriers)
-      if (named_bar_or(1, 32 * kConvWarps, !ok)) break;
-      if (flags & kFirst) {
-        // the stream's queries: two passes, the first for the common scale
-        float top = 0.f;
-        for (int r = cw * TPW + lane / LPT; r < NR; r += kConvWarps * TPW) {
-          const int rr = d.chunk * NR + r;
-          if (rr >= d.rows) continue;
-          SeqWork w;
-          w.row0 = d.row0;
-          float x[16];
-          get(a.q, row_offset(a, w, d.head, rr, D) + 16 * c, x);
-          top = fmaxf(top, top_of(x));
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) sh.qmax[cw] = top;
-        named_bar_sync(1, 32 * kConvWarps);
-#pragma unroll
-        for (int j = 0; j < kConvWarps; ++j) top = fmaxf(top, sh.qmax[j]);
-        float down, up;
-        unit_scale(top, down, up);
-        if (ct == 0) sh.qscale[d.seg] = up;
-        for (int r = cw * TPW + lane / LPT; r < NR; r += kConvWarps * TPW) {
-          const int rr = d.chunk * NR + r;
-          uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          if (rr < d.rows) {
-            SeqWork w;
-            w.row0 = d.row0;
-            float x[16];
-            get(a.q, row_offset(a, w, d.head, rr, D) + 16 * c, x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+      const bool draft = flags & kDraftTile;
+      if (ok && !draft) ok = tc_wait(&sh.kc_full[kc.s], kc.ph, a.status);
+      // A new stream's queries replace the last one's: every product with those
+      // is done. Otherwise the buffer of tile i - NH has been read.
+      if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) % T::NH], ((i - 1) / T::NH) & 1, a.status);
+      if (ok && i >= T::NH) ok = tc_wait(&sh.kh_empty[hb], (i / T::NH + 1) & 1, a.status);
+      // keys beyond float16's range take a scale per group (checked a channel a thread)
+      const float* scales = reinterpret_cast<const float*>(smem + T::SZ_OFF + kc.s * T::SZ);
+      float key_top = 0.f;
+      if (ok && !draft) {
+        int last = -1;
+#pragma unroll 1
+        for (int g = 0; g < pages; ++g) {
+          const int slot = d.sz[g];
+          if (slot == last) continue;
+          last = slot;
+          for (int ch = ct; ch < D; ch += 32 * kConvWarps) {
+            const float s = scales[slot * (2 * D) + ch], z = -scales[slot * (2 * D) + D + ch] * s;
+            key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
           }
-          put(smem + T::Q_OFF, NR, r, h);
         }
-        named_bar_sync(1, 32 * kConvWarps);  // qmax is free again
       }
-      if (flags & kDraftTile) {
-        for (int t = cw * TPW + lane / LPT; t < pages * kMqPage; t += kConvWarps * TPW) {
-          float x[16];
-          const bool real = t < d.drafts;
-          if (real) {
-            get(a.kd, ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 16 * c, x);
+      bool scaled = false;
+      if (named_bar_or(kBarConv, 32 * kConvWarps, !ok || key_top > kHalfRoom)) {
+        // (uniform over the role: its warps meet in named barriers)
+        if (named_bar_or(kBarConv, 32 * kConvWarps, !ok)) break;
+        scaled = true;
+      }
+      if (flags & kFirst) {
+        // The stream's queries, as they are: a magnitude below float16's range
+        // loses nothing that a logit could show. Only one above it (a bfloat16
+        // input) takes the second pass, with a common power of two.
+        float top = 0.f, down = 1.f, up = 1.f;
+#pragma unroll 1
+        for (int pass = 0;; ++pass) {
+#pragma unroll 2
+          for (int r = t_lane; r < NR; r += kConvWarps * TPW) {
+            const int row = sh.row[d.seg][r];
+            uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (row >= 0) {
+              float x[16];
+              get(a.q, (size_t)row * D, x);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                if (VK == INT4KV_VALUES_BF16) top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+                h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+              }
+            }
+            put(smem + T::Q_OFF, NR, r, h);
+          }
+          if (VK == INT4KV_VALUES_F16 || pass == 1) break;
+          if (!named_bar_or(kBarConv, 32 * kConvWarps, top > kHalfRoom)) break;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (lane == 0) sh.qmax[cw] = top;
+          named_bar_sync(kBarConv, 32 * kConvWarps);
+#pragma unroll 1
+          for (int j = 0; j < kConvWarps; ++j) top = fmaxf(top, sh.qmax[j]);
+          named_bar_sync(kBarConv, 32 * kConvWarps);  // qmax is free again
+          unit_scale(top, down, up);
+        }
+        if (ct == 0) sh.qscale[d.seg] = up;
+      }
+      char* kh = smem + T::KH_OFF + hb * T::KH;
+      if (draft) {
+#pragma unroll 1
+        for (int t = t_lane; t < pages * kMqPage; t += kConvWarps * TPW) {
+          float x[16], top = 0.f, down, up;
+          if (t < d.drafts) {
+            get(a.kd, ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D, x);
           } else {
 #pragma unroll
             for (int j = 0; j < 16; ++j) x[j] = 0.f;
           }
-          float top = top_of(x), down, up;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_abs(x[j]));
 #pragma unroll
           for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           unit_scale(top, down, up);
           uint32_t h[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
-          put(smem + T::KH_OFF, kTile, t, h);
+          put(kh, kTile, t, h);
           if (c == 0) sh.kscale[ds][t] = up;
         }
       } else {
-        const char* codes = smem + T::KC_OFF + ks * T::KC;
+        const char* codes = smem + T::KC_OFF + kc.s * T::KC;
         float s[16], z[16];
         float up = 1.f;
         int have = -1;
-        for (int t = cw * TPW + lane / LPT; t < pages * kMqPage; t += kConvWarps * TPW) {
+#pragma unroll 1
+        for (int t = t_lane; t < pages * kMqPage; t += kConvWarps * TPW) {
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(codes + t * (D / 2) + ca / 2);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(codes + t * (D / 2) + cb / 2);
           const int slot = d.sz[t / kMqPage];  // uniform in the warp: its tokens lie in one page
           if (slot != have) {
             have = slot;
-            const float* p4 = reinterpret_cast<const float*>(smem + T::SZ_OFF + ks * T::SZ + slot * (2 * D * 4)) + 16 * c;
-            float top = 0.f;
+            const float* p4 = scales + slot * (2 * D);
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(p4 + j);
-              const float4 y = *reinterpret_cast<const float4*>(p4 + D + j);
+              const int ch = j < 8 ? ca + j : cb + j - 8;
+              const float4 x = *reinterpret_cast<const float4*>(p4 + ch);
+              const float4 y = *reinterpret_cast<const float4*>(p4 + D + ch);
               s[j] = x.x; s[j + 1] = x.y; s[j + 2] = x.z; s[j + 3] = x.w;
               z[j] = -y.x * x.x; z[j + 1] = -y.y * x.y; z[j + 2] = -y.z * x.z; z[j + 3] = -y.w * x.w;
             }
+            float down = 1.f;
+            if (scaled) {
+              float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float y = fmaxf(fabsf(z[j]), fabsf(fmaf(15.f, s[j], z[j])));
-              top = fmaxf(top, y <= 3.4e38f ? y : 0.f);
+              for (int j = 0; j < 16; ++j)
+                top = fmaxf(top, fmaxf(finite_abs(z[j]), finite_abs(fmaf(15.f, s[j], z[j]))));
+#pragma unroll
+              for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              unit_scale(top, down, up);
             }
-#pragma unroll
-            for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float down;
-            unit_scale(top, down, up);
             // code c enters as 1 + c / 128 (its bits in the mantissa)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float e = s[j] * down * 128.f;
+              const float e = s[j] * (down * 128.f);
               z[j] = fmaf(z[j], down, -e);
               s[j] = e;
             }
           }
-          const uint2 wd = *reinterpret_cast<const uint2*>(codes + t * (D / 2) + 8 * c);
           uint32_t h[8];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint32_t x = k ? wd.y : wd.x;
+            const uint32_t x = k ? wb : wa;
             const uint32_t lo = (x & 0x0F0F0F0Fu) | 0x80808080u, hi = ((x >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float e = __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8)));
-              const float o = __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8)));
               const int q = 8 * k + 2 * j;
-              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(fmaf(e, s[q], z[q]), fmaf(o, s[q + 1], z[q + 1]));
+              float e0, e1;
+              fma2(e0, e1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
+                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), s[q], s[q + 1], z[q], z[q + 1]);
+              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(e0, e1);
             }
           }
-          put(smem + T::KH_OFF, kTile, t, h);
-          if (c == 0) sh.kscale[ds][t] = up;
+          put(kh, kTile, t, h);
+          if (scaled && c == 0) sh.kscale[ds][t] = up;
         }
       }
+      if (ct == 0) sh.scaled[ds] = scaled || draft;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&sh.kh_full);
-        if (!(flags & kDraftTile)) mbar_arrive(&sh.kc_empty[ks]);
+        mbar_arrive(&sh.kh_full[hb]);
+        if (!draft) mbar_arrive(&sh.kc_empty[kc.s]);
         mbar_arrive(&sh.desc_empty[ds]);
       }
-      if (!(flags & kDraftTile)) ++kc;
+      if (!draft) kc.next<T::NK>();
     }
   } else {
     // ------------------------------------------------------------ softmax
-    constexpr int NC = NR / 2;                 // rows (columns of S^T) of a thread
+    constexpr int NC = NR / T::WG;             // rows (columns of S^T) of a thread
     constexpr int LD = NC < 16 ? 8 : 16;       // columns per tensor-memory load
-    const int wg = warp / 4, tok = (warp % 4) * 32 + lane, c0 = wg * NC, wt = tid % 128;
-    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
-    const int bar = 2 + wg;
+    const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC, wt = tid % 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int bar = kBarGroup + wg;
     float l[NC];
-    uint32_t vu = 0;                           // value units before this tile
+    Ring v;                                    // first value unit of the tile
     bool failed = false, started = false;      // a wait ran out; O^T of the segment holds something
 #pragma unroll
     for (int j = 0; j < NC; ++j) l[j] = 0.f;
+#pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int ds = i % kDesc, sb = i & 1, pb = i % T::NP;
-      // Every thread waits. A timeout is made uniform over both warpgroups here
+      // Every thread waits. A timeout is made uniform over the whole role here
       // alone: until then the tile goes on with what it has, so no barrier of the
       // softmax ever waits for a warp that has left.
-      const bool ok = tc_wait(sh, &sh.desc_full[ds], (i / kDesc) & 1, a.status) &&
-                      tc_wait(sh, &sh.s_full[sb], (i / 2) & 1, a.status);
+      const bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
       failed |= !ok;
       const TileDesc& d = sh.desc[ds];
       const int flags = ok ? d.flags : 0, pages = ok ? d.pages : 0, sg = ok ? d.seg : 0;
+      const bool draft = flags & kDraftTile, masked = flags & kMasked;
+      // the token of this thread, and (bits) the rows that see it
+      const int at = d.at[tok / kMqPage] + tok % kMqPage;
+      bool real = true;
+      uint32_t vis = 0xffffffffu;
+      if (masked) {
+        real = tok < pages * kMqPage && d.at[tok / kMqPage] >= 0 && at < (draft ? d.drafts : d.len);
+        if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
+        if (real && draft) {
+#pragma unroll 4
+          for (int j = 0; j < NC; ++j)
+            vis &= ~((uint32_t)(~(sh.word[sg][sh.draft[sg][c0 + j]] >> (at & 63)) & 1) << j);
+        }
+        if (real && a.window > 0) {
+          const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
+          if (behind >= a.sinks) {
+#pragma unroll 4
+            for (int j = 0; j < NC; ++j)
+              vis &= ~((uint32_t)(behind <= d.low_edge + sh.depth[sg][sh.draft[sg][c0 + j]]) << j);
+          }
+        }
+        if (!real) vis = 0;
+      }
+      failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
       if (flags & kFirst) {
         started = false;
 #pragma unroll
@@ -648,23 +757,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           sh.sub[c0 + wt] = 0.f;
         }
       }
-      if (named_bar_or(4, 256, failed)) break;
+      if (named_bar_or(kBarSoft, 32 * kSoftWarps, failed)) break;
       tc_fence_after();
-      // the token of this thread
-      const int at0 = d.at[tok / kMqPage], at = at0 + tok % kMqPage;
-      const bool draft = flags & kDraftTile;
-      bool real = tok < pages * kMqPage && at0 >= 0 && at < (draft ? d.drafts : d.len);
-      if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
-      const float f = real ? sh.qscale[sg] * sh.kscale[ds][tok] * kLog2e : 0.f;
-      int behind = at;
-      if (draft && real && a.window > 0) behind = d.len + sh.depth[sg][at];
-      const bool masked = flags & kMasked;
-      auto sees = [&](int r) -> bool {
-        bool s = real;
-        if (draft) s = s && (sh.word[sg][r] >> (at & 63) & 1);
-        if (a.window > 0) s = s && (behind > sh.edge[sg][r] || behind < a.sinks);
-        return s;
-      };
+      float f = sh.qscale[sg] * kLog2e;
+      if (sh.scaled[ds]) f = real ? f * sh.kscale[ds][tok] : 0.f;
       const uint32_t s_addr = tm + lanes + sb * NR + c0;
 
       // pass 1: does some logit exceed its row's reference by more than kLazy?
@@ -676,30 +772,29 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll
         for (int j = 0; j < LD; j += 4) {
           const float4 m = *reinterpret_cast<const float4*>(&sh.ref[c0 + j0 + j]);
-          const float y0 = fmaf(__uint_as_float(x[j]), f, -m.x), y1 = fmaf(__uint_as_float(x[j + 1]), f, -m.y);
-          const float y2 = fmaf(__uint_as_float(x[j + 2]), f, -m.z), y3 = fmaf(__uint_as_float(x[j + 3]), f, -m.w);
+          float y[4];
+          fma2(y[0], y[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, -m.x, -m.y);
+          fma2(y[2], y[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, -m.z, -m.w);
           if (masked) {
-            if (sees(c0 + j0 + j)) over = fmaxf(over, y0);
-            if (sees(c0 + j0 + j + 1)) over = fmaxf(over, y1);
-            if (sees(c0 + j0 + j + 2)) over = fmaxf(over, y2);
-            if (sees(c0 + j0 + j + 3)) over = fmaxf(over, y3);
-          } else {
-            over = fmax3f(fmax3f(over, y0, y1), y2, y3);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (!(vis >> (j0 + j + q) & 1)) y[q] = -INFINITY;
           }
+          over = fmax3f(fmax3f(over, y[0], y[1]), y[2], y[3]);
         }
       }
       if (named_bar_or(bar, 128, over > kLazy)) {
         // raise the references to the true maxima, rescale sums and outputs
+#pragma unroll 1
+        for (int j0 = 0; j0 < NC; j0 += 8) {
+          uint32_t x[8];
+          tc_ld<8>(x, s_addr + j0);
 #pragma unroll
-        for (int j0 = 0; j0 < NC; j0 += LD) {
-          uint32_t x[LD];
-          tc_ld<LD>(x, s_addr + j0);
-#pragma unroll
-          for (int j = 0; j < LD; ++j) {
+          for (int j = 0; j < 8; ++j) {
             float y = __uint_as_float(x[j]) * f;
-            if (masked && !sees(c0 + j0 + j)) y = -INFINITY;
+            if (!(vis >> (j0 + j) & 1)) y = -INFINITY;
             const uint32_t k = __reduce_max_sync(0xffffffffu, ordered_key(fmaxf(y, -INFINITY)));
-            if (lane == 0) sh.part[warp % 4][c0 + j0 + j] = from_ordered_key(k);
+            if (lane == j) sh.part[quarter][c0 + j0 + j] = from_ordered_key(k);
           }
         }
         named_bar_sync(bar, 128);
@@ -712,29 +807,28 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           sh.alpha[r] = m == -INFINITY ? 1.f : exp2_fast(old - m);
         }
         if (started)  // the weights of tile i - 1 have been multiplied
-          failed |= !tc_wait(sh, &sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status);
+          failed |= !tc_wait(&sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
 #pragma unroll
         for (int j = 0; j < NC; ++j) l[j] *= sh.alpha[c0 + j];
         if (started) {
           tc_fence_after();
+#pragma unroll 1
+          for (int j0 = 0; j0 < T::NO * NC; j0 += 8) {
+            uint32_t x[8];
+            const int col = j0 % NC;
+            const uint32_t at_o = tm + lanes + T::COLS_O + (j0 / NC) * NR + c0 + col;
+            tc_ld<8>(x, at_o);
 #pragma unroll
-          for (int o = 0; o < T::NO; ++o)
-#pragma unroll
-            for (int j0 = 0; j0 < NC; j0 += 8) {
-              uint32_t x[8];
-              const uint32_t at_o = tm + lanes + T::COLS_O + o * NR + c0 + j0;
-              tc_ld<8>(x, at_o);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sh.alpha[c0 + j0 + j]);
-              tc_st8(at_o, x);
-            }
+            for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sh.alpha[c0 + col + j]);
+            tc_st8(at_o, x);
+          }
           tc_wait_st();
           tc_fence_before();
         }
       }
       // pass 2: weights
-      if (i >= T::NP) failed |= !tc_wait(sh, &sh.p_empty[pb], (i / T::NP - 1) & 1, a.status);
+      failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP + 1) & 1, a.status);
       char* prow = smem + T::P_OFF + pb * T::P + tok * 128;
 #pragma unroll
       for (int j0 = 0; j0 < NC; j0 += LD) {
@@ -743,17 +837,18 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll
         for (int j = 0; j < LD; j += 4) {
           const float4 m = *reinterpret_cast<const float4*>(&sh.sub[c0 + j0 + j]);
-          float e[4] = {exp2_fast(fmaf(__uint_as_float(x[j]), f, -m.x)),
-                        exp2_fast(fmaf(__uint_as_float(x[j + 1]), f, -m.y)),
-                        exp2_fast(fmaf(__uint_as_float(x[j + 2]), f, -m.z)),
-                        exp2_fast(fmaf(__uint_as_float(x[j + 3]), f, -m.w))};
+          float e[4];
+          fma2(e[0], e[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, -m.x, -m.y);
+          fma2(e[2], e[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, -m.z, -m.w);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) e[q] = exp2_fast(e[q]);
           if (masked) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              if (!sees(c0 + j0 + j + q)) e[q] = 0.f;
+              if (!(vis >> (j0 + j + q) & 1)) e[q] = 0.f;
           }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) l[j0 + j + q] += e[q];
+          add2_rn(l[j0 + j], l[j0 + j + 1], l[j0 + j], l[j0 + j + 1], e[0], e[1]);
+          add2_rn(l[j0 + j + 2], l[j0 + j + 3], l[j0 + j + 2], l[j0 + j + 3], e[2], e[3]);
           h[j / 2] = pack16<VK>(e[0], e[1]);
           h[j / 2 + 1] = pack16<VK>(e[2], e[3]);
         }
@@ -767,43 +862,40 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       // Values that no row sees must not reach the product (0 * NaN): cleared.
       // A drafted value that is not finite is taken out too and added for the
       // rows that see it when the stream ends.
-      const int units = (pages + T::PPU - 1) / T::PPU;
-      if (masked && wg == 0 && tok < pages * kMqPage) {
-        const uint32_t mine = vu + tok / (kMqPage * T::PPU);
-        if (!real || draft) {
-          failed |= !tc_wait(sh, &sh.v_full[mine % T::NV], (mine / T::NV) & 1, a.status);
-          char* row = smem + T::V_OFF + (mine % T::NV) * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V +
-                      (tok % kMqPage) * 128;
-          bool bad = false;
+      if (masked && wg == 0 && tok < pages * kMqPage && (!real || draft)) {
+        Ring u = v;
+#pragma unroll 1
+        for (int k = tok / (kMqPage * T::PPU); k > 0; --k) u.next<T::NV>();
+        failed |= !tc_wait(&sh.v_full[u.s], u.ph, a.status);
+        char* row = smem + T::V_OFF + u.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+        bool bad = false;
+#pragma unroll 1
+        for (int q = 0; q < 8 * T::CH; ++q) {
+          uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
+          uint4 y = make_uint4(0, 0, 0, 0);
+          bool hit = !real;
+          if (real) {
+            y = *at16;
+            uint32_t e[4] = {y.x, y.y, y.z, y.w};
+            constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
 #pragma unroll
-          for (int q = 0; q < T::CH; ++q) {
-            for (int j = 0; j < 8; ++j) {
-              uint4* v = reinterpret_cast<uint4*>(row + q * (kMqPage * 128) + 16 * j);
-              if (!real) {
-                *v = make_uint4(0, 0, 0, 0);
-              } else {
-                uint4 y = *v;
-                uint32_t* e = reinterpret_cast<uint32_t*>(&y);
-                constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
-                bool hit = false;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-                  if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
-                }
-                if (hit) { *v = y; bad = true; }
-              }
+            for (int k = 0; k < 4; ++k) {
+              if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
+              if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
             }
+            bad |= hit;
+            y = make_uint4(e[0], e[1], e[2], e[3]);
           }
-          if (bad) atomicOr(&sh.odd, 1ull << (at & 63));
+          if (hit) *at16 = y;
         }
+        if (bad) atomicOr(&sh.odd, 1ull << (at & 63));
       }
-      vu += units;
+#pragma unroll 1
+      for (int g = 0; g < pages; g += T::PPU) v.next<T::NV>();
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
-      const bool last = flags & kLast, whole = flags & kWhole;
-      const int row0 = d.row0, rows = d.rows, chunk = d.chunk, head = d.head, slot = d.slot, drafts = d.drafts;
+      const bool last = flags & kLast;
       if (lane == 0) {
         mbar_arrive(&sh.s_empty[sb]);
         mbar_arrive(&sh.p_full[pb]);
@@ -812,67 +904,76 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       started = true;
       if (last) {
         // ---- epilogue: sums over the tokens, then O^T, a lane a channel ----
+        // Each step of the butterfly halves the rows a lane holds: lane k ends
+        // with the sum of row k / (32 / NC) over the warp's tokens.
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-          float x = l[j];
+        for (int st = 0; st < 5; ++st) {
+          const int o = 16 >> st, half = (NC >> st) / 2;
+          if (half >= 1) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-          if (lane == 0) sh.lsum[warp % 4][c0 + j] = x;
-        }
-        failed |= !tc_wait(sh, &sh.p_empty[pb], (i / T::NP) & 1, a.status);
-        named_bar_sync(4, 256);  // both warpgroups' sums and the list of odd values are complete
-        tc_fence_after();
-        const unsigned long long odd = sh.odd;
-        float* rec = a.recs + (size_t)slot * Record<NR, D>::kFloats;
-        SeqWork w;
-        w.row0 = row0;
-        for (int o = 0; o < T::NO; ++o) {
-          const int ch = o * 128 + (warp % 4) * 32 + lane;
-#pragma unroll
-          for (int j0 = 0; j0 < NC; j0 += 8) {
-            uint32_t x[8];
-            tc_ld<8>(x, tm + lanes + T::COLS_O + o * NR + c0 + j0);
-            if (odd && ch < D) {
-              for (unsigned long long left = odd; left; left &= left - 1) {
-                const int u = __ffsll(left) - 1;
-                float v[2];
-                load_f32<2>(a.vd, VK, ((size_t)(row0 + u) * a.kv_heads + head) * D + (ch & ~1), v);
-                const float y = v[ch & 1];
-                if (fabsf(y) <= 3.4e38f) continue;
-                const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const int r = c0 + j0 + j;
-                  if ((sh.word[sg][r] >> u & 1) && (a.window == 0 || pos > sh.edge[sg][r] || pos < a.sinks))
-                    x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
-                }
-              }
+            for (int j = 0; j < half; ++j) {
+              const bool up = lane & o;
+              const float send = up ? l[j] : l[j + half], keep = up ? l[j + half] : l[j];
+              l[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
             }
-            if (ch < D) {
+          } else {
+            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+          }
+        }
+        if (lane % (32 / NC) == 0) sh.part[quarter][c0 + lane / (32 / NC)] = l[0];
+        failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
+        named_bar_sync(kBarSoft, 32 * kSoftWarps);  // all sums, and the list of odd values, are complete
+        tc_fence_after();
+        const bool whole = flags & kWhole;
+        float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
+        if (wt < NC) {
+          const int r = c0 + wt;
+          const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+          sh.inv[r] = 1.f / fmaxf(sum, 1e-10f);
+          if (!whole) {
+            rec[r] = sh.ref[r] * 0.6931471805599453f;
+            rec[NR + r] = sum;
+          }
+        }
+        named_bar_sync(bar, 128);
+        const unsigned long long odd = sh.odd;
+#pragma unroll 1
+        for (int j0 = 0; j0 < T::NO * NC; j0 += 8) {
+          const int ch = (j0 / NC) * 128 + tok, col = c0 + j0 % NC;
+          uint32_t x[8];
+          tc_ld<8>(x, tm + lanes + T::COLS_O + (j0 / NC) * NR + col);
+          if (ch >= D) continue;
+#pragma unroll 1
+          for (unsigned long long left = odd; left; left &= left - 1) {
+            const int u = __ffsll(left) - 1;
+            float y2[2];
+            load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
+            const float y = y2[ch & 1];
+            if (fabsf(y) <= 3.4e38f) continue;
+            const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = c0 + j0 + j, rr = chunk * NR + r;
-                if (rr >= rows) continue;
-                const float v = __uint_as_float(x[j]);
-                if (whole) {
-                  const float sum = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
-                  const float y = v * (1.f / fmaxf(sum, 1e-10f));
-                  const size_t to = row_offset(a, w, head, rr, D) + ch;
-                  if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y);
-                  else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y);
-                } else {
-                  rec[2 * NR + r * D + ch] = v;
-                  if (ch == 0) {
-                    rec[r] = sh.ref[r] * 0.6931471805599453f;
-                    rec[NR + r] = (sh.lsum[0][r] + sh.lsum[1][r]) + (sh.lsum[2][r] + sh.lsum[3][r]);
-                  }
-                }
-              }
+            for (int j = 0; j < 8; ++j) {
+              const int t = sh.draft[sg][col + j];
+              if ((sh.word[sg][t] >> u & 1) && (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
+                x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = col + j, row = sh.row[sg][r];
+            if (row < 0) continue;
+            const float y = __uint_as_float(x[j]);
+            if (whole) {
+              const size_t to = (size_t)row * D + ch;
+              if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.inv[r]);
+              else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.inv[r]);
+            } else {
+              rec[2 * NR + r * D + ch] = y;
             }
           }
         }
         tc_fence_before();
-        named_bar_sync(4, 256);  // lsum, odd and the references are free
+        named_bar_sync(kBarSoft, 32 * kSoftWarps);  // sums, references and odd values are free
         if (tid == 0) sh.odd = 0;
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
       }
@@ -880,7 +981,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   }
   // all roles meet; tensor memory is freed on every path
   __syncthreads();
-  if (warp == 17) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(T::COLS));
   }
@@ -925,7 +1026,7 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   static_assert(T::BYTES + sizeof(TcShared<NR>) <= 227 * 1024, "shared memory");
   constexpr auto kern = multi_query_tc_kernel<D, NR, VK>;
   int per_sm = 0;
-  cudaError_t e = mq_occupancy<kern>(kThreadsTc, T::BYTES, &per_sm);
+  cudaError_t e = mq_occupancy<kern>(T::THREADS, T::BYTES, &per_sm);
   if (e != cudaSuccess) return e;
   if (ws_bytes < (size_t)sms * 2 * Record<NR, D>::kFloats * 4) return cudaErrorInvalidValue;
   CUtensorMap vmap, dmap;
@@ -936,7 +1037,7 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   if (a.vd) e = value_map(&dmap, a.vd, VK, D, a.total_rows, row * a.kv_heads, a.kv_heads, row);
   else dmap = vmap;
   if (e != cudaSuccess) return e;
-  e = mq_launch_pdl(kern, dim3(sms), dim3(kThreadsTc), T::BYTES, stream, a, vmap, dmap);
+  e = mq_launch_pdl(kern, dim3(sms), dim3(T::THREADS), T::BYTES, stream, a, vmap, dmap);
   if (e != cudaSuccess) return e;
   return mq_launch_pdl(merge_records_kernel<NR, kTilePages, D>, dim3(sms - 1, (NR + kMergeWarps - 1) / kMergeWarps),
                        dim3(kMergeWarps * 32), 0, stream, a, sms);
