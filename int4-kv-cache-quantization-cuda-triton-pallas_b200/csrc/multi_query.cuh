@@ -3,9 +3,10 @@
 //
 // Sequence b has `rows` query rows per kv head, row = draft * G + (query head
 // of the group), in chunks of NR rows; a stream is one (b, kv head, chunk). Its
-// work is a list of tiles: the visible pages of the cache, TP at a time (the
-// pages of the sinks and of the window are one list without the pages between
-// them), then the drafted tokens. The streams' tiles are laid end to end and
+// work is a list of tiles: the blocks of TP pages (from multiples of TP, so that a
+// block lies in one quantization group wherever groups are that long) that hold
+// visible pages, those of the sinks and those of the window, then the drafted
+// tokens. The streams' tiles are laid end to end and
 // every CTA takes one contiguous run of equal length, so the CTAs do the same
 // number of tiles whatever the lengths are. A stream inside one run is finished
 // by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per row,
@@ -53,8 +54,9 @@ struct MultiQueryArgs {
 struct SeqWork {
   int len, drafts, row0, rows, chunks;
   int pos0;                    // position of a query without drafted ancestors
-  int sink_pages, win_page;    // visible pages: [0, sink_pages) and [win_page, pages)
-  int vis_pages, cache_tiles, tiles;
+  int pages, sink_pages, win_page;  // visible pages: [0, sink_pages) and [win_page, pages)
+  int sink_blocks, win_block;       // and the blocks that hold them: [0, sink_blocks), [win_block, ..)
+  int cache_tiles, tiles;
 };
 
 I4KV_DEVINL void mq_status(uint32_t* status, uint32_t bits) {
@@ -87,26 +89,36 @@ __device__ __noinline__ SeqWork seq_work(const MultiQueryArgs& a, int b, bool re
   }
   if (bad && report) mq_status(a.status, kStatusBadLength);
   w.chunks = (w.rows + NR - 1) / NR;
-  const int pages = (w.len + kMqPage - 1) / kMqPage;
+  w.pages = (w.len + kMqPage - 1) / kMqPage;
   w.sink_pages = 0;
   w.win_page = 0;
   if (a.window > 0) {
     const int lo = w.pos0 - a.window + 1;  // first windowed position of the lowest query
     if (lo > 0) {
-      w.win_page = min(lo / kMqPage, pages);
-      const int sp = (int)(((long long)min(a.sinks, w.len) + kMqPage - 1) / kMqPage);
-      if (sp >= w.win_page) w.win_page = 0;
-      else w.sink_pages = sp;
+      w.win_page = min(lo / kMqPage, w.pages);
+      w.sink_pages = (int)(((long long)min(a.sinks, w.len) + kMqPage - 1) / kMqPage);
     }
   }
-  w.vis_pages = w.sink_pages + pages - w.win_page;
-  w.cache_tiles = (w.vis_pages + TP - 1) / TP;
+  w.sink_blocks = (w.sink_pages + TP - 1) / TP;
+  w.win_block = w.win_page / TP;
+  const int blocks = (w.pages + TP - 1) / TP;
+  if (w.win_page >= w.pages) w.win_block = blocks;  // nothing in the window
+  if (w.sink_blocks >= w.win_block) {                // one run of blocks
+    w.sink_blocks = 0;
+    if (w.sink_pages > 0) w.win_block = 0;
+  }
+  w.cache_tiles = w.sink_blocks + blocks - w.win_block;
   w.tiles = w.rows > 0 ? w.cache_tiles + (w.drafts + TP * kMqPage - 1) / (TP * kMqPage) : 0;
   return w;
 }
 
-I4KV_DEVINL int visible_page(const SeqWork& w, int i) {
-  return i < w.sink_pages ? i : i - w.sink_pages + w.win_page;
+// Page j of cache tile i, and whether some query sees it.
+template <int TP>
+I4KV_DEVINL int tile_page(const SeqWork& w, int i, int j) {
+  return (i < w.sink_blocks ? i : i - w.sink_blocks + w.win_block) * TP + j;
+}
+I4KV_DEVINL bool page_visible(const SeqWork& w, int pg) {
+  return pg < w.pages && (pg < w.sink_pages || pg >= w.win_page);
 }
 
 // Place of one tile in the end-to-end order.

@@ -91,12 +91,11 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   // Copies of tile `np` into stage st (lanes < TP of warp 0, a page each).
   auto issue = [&](int st) {
     if (lane < TP) {
-      const int i = np.tile * TP + lane;
       uint32_t bytes = 0;
       int phys = 0, home = 0, rows = 0;
       bool ok = false;
-      if (np.tile < nw.cache_tiles && i < nw.vis_pages) {
-        const int pg = visible_page(nw, i);
+      const int pg = tile_page<TP>(nw, np.tile, lane);
+      if (np.tile < nw.cache_tiles && page_visible(nw, pg)) {
         const int32_t* bt = a.block_table + (size_t)np.b * a.max_pages;
         phys = __ldg(bt + pg);
         home = __ldg(bt + pg / a.group_pages * a.group_pages);
@@ -215,9 +214,8 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         int at;        // position of the token (cache), or index of the draft
         bool real;
         if (in_cache) {
-          const int i = p.tile * TP + tok / kMqPage;
-          at = visible_page(w, i) * kMqPage + tok % kMqPage;
-          real = i < w.vis_pages && at < w.len && (s_pages[st] >> (tok / kMqPage) & 1);
+          at = tile_page<TP>(w, p.tile, tok / kMqPage) * kMqPage + tok % kMqPage;
+          real = at < w.len && (s_pages[st] >> (tok / kMqPage) & 1);
           const char* krow = base + S::V_BYTES + tok * (D / 2);
           const float* sz = reinterpret_cast<const float*>(base + S::V_BYTES + S::K_BYTES) + tok / kMqPage * 2 * D;
           if (real) {

@@ -23,14 +23,14 @@
 // are.
 //
 // A tile is 128 cached tokens (8 pages) or the drafts. Roles of the warps:
-//   softmax (8, or 16 for 128 rows): S^T from tensor memory, mask, weights to
+//   softmax (4 for each 32 rows): S^T from tensor memory, mask, weights to
 //       shared memory, the rare rescale of O^T, and the stream's epilogue
-//   conversion (8 or 5): packed codes to float16 keys (K-major, 128-byte
-//       swizzle), a stream's queries, drafted keys
-//   MMA issue (1): S^T of tile i, then O^T of tile i - 1
-//   copies (2): pages by bulk (codes, scales) and tensor copies (values, in the
-//       swizzled layout the MMA reads: V is stored token-major, which is the
-//       transposed operand's contiguous side, so nothing is rearranged)
+//   conversion (4 to 16): packed codes, loaded a tile ahead, to float16 keys
+//       (K-major, 128-byte swizzle), a stream's queries, drafted keys
+//   MMA issue (1): S^T of tile i and O^T of tile i - 1, the one that can go first
+//   copies (2): the tiles' descriptors; values by tensor copies, in the swizzled
+//       layout the MMA reads (V is stored token-major, which is the transposed
+//       operand's contiguous side, so nothing is rearranged)
 // What runs once per stream is kept out of the tile's straight line: the roles
 // run different code side by side, and the instruction caches are small.
 // One persistent CTA per SM; work decomposition and merge: multi_query.cuh.
@@ -100,6 +100,16 @@ I4KV_DEVINL bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
+// Whether a phase is over, without waiting.
+I4KV_DEVINL bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -142,20 +152,20 @@ struct Tc {
   static constexpr int UNIT = 16384, PPU = UNIT / PAGE_V;  // value ring: units of PPU pages
   // Stages. One buffer of dequantized keys or of weights makes its writer wait
   // for the MMA that reads it, so there are two of each where they fit.
-  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : 5;
-  static constexpr int NK = D == 256 ? 1 : 2;              // packed codes and scales
-  static constexpr int NH = (D == 64 || (D == 128 && NR <= 64)) ? 2 : 1;  // dequantized keys
-  static constexpr int NP = (D == 256 || NR > 32) ? 1 : 2; // weights
-  // Softmax warpgroups share the rows: at most 32 of them (and as many sums) a
-  // thread. 24 warps leave 80 registers a thread, 19 leave 96.
-  static constexpr int WG = NR > 64 ? 4 : 2, SOFT = 4 * WG, CONV = NR > 64 ? 5 : 8;
-  static constexpr int THREADS = 32 * (SOFT + CONV + 3);
+  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 4 : 5);
+  static constexpr int NH = D == 256 ? 1 : 2;              // dequantized keys
+  static constexpr int NP = (D == 256 || NR > 64) ? 1 : 2; // weights
+  // Warps: a softmax warpgroup for each 32 rows (16 or 32 rows, and as many
+  // sums, a thread), conversion warps as registers allow.
+  static constexpr int WG = NR / 32 > 0 ? NR / 32 : 1, SOFT = 4 * WG;
+  static constexpr int CONV = NR == 16 ? 16 : (NR > 64 ? 4 : 8);
+  static constexpr int WARPS = SOFT + CONV + 3, THREADS = 32 * WARPS;
   static constexpr int PC = (NR + 63) / 64;                // 64-row chunks of the weights
   static constexpr int NO = D == 256 ? 2 : 1;              // 128-channel blocks of O^T
   static constexpr int KH = kTile * D * 2, Q = NR * D * 2, P = PC * kTile * 128;
-  static constexpr int KC = kTile * D / 2, SZ = kTilePages * 2 * D * 4;
+  static constexpr int SZ = kTilePages * 2 * D * 4;        // a tile's scales, two tiles
   static constexpr int KH_OFF = 0, V_OFF = KH_OFF + NH * KH, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q;
-  static constexpr int KC_OFF = P_OFF + NP * P, SZ_OFF = KC_OFF + NK * KC, END = SZ_OFF + NK * SZ;
+  static constexpr int SZ_OFF = P_OFF + NP * P, END = SZ_OFF + 2 * SZ;
   static constexpr int BYTES = END + 1024;                 // the base is rounded up to 1024
   static constexpr int COLS_O = 2 * NR, COLS = 512;
   static_assert(Q % 1024 == 0 && P % 1024 == 0 && COLS_O + NO * NR <= COLS, "layout");
@@ -167,13 +177,16 @@ struct TileDesc {
   int seg, slot;                // segment ring entry; record of a shared stream
   int low_edge;                 // no row sees cached positions <= low_edge (but the sinks)
   int at[kTilePages];           // position of each page's first token, -1: not there
-  int sz[kTilePages];           // scale slot of each page
+  int slab[kTilePages];         // its page-head slab in the pools, -1: not there
+  int sz[kTilePages];           // its scale slot (the first page here of its group),
+  int home[kTilePages];         // and a slot's slab in the scale pool
+  uint32_t slots;               // slots in use (a bit each)
 };
 enum : int { kDraftTile = 1, kMasked = 2, kFirst = 4, kLast = 8, kWhole = 16 };
 
 template <int NR>
 struct TcShared {
-  uint64_t desc_full[kDesc], desc_empty[kDesc], kc_full[2], kc_empty[2], v_full[6], v_empty[6];
+  uint64_t desc_full[kDesc], desc_empty[kDesc], v_full[6], v_empty[6];
   uint64_t kh_full[2], kh_empty[2], s_full[2], s_empty[2], p_full[2], p_empty[2];
   TileDesc desc[kDesc];
   uint64_t word[kDesc][kMqMaxDrafts];  // per segment: the drafts each draft sees,
@@ -183,10 +196,11 @@ struct TcShared {
   float qscale[kDesc];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
-  float ref[NR], sub[NR], alpha[NR], inv[NR];
+  float nref[NR], nsub[NR];     // minus the reference; minus what logits are taken relative to
+  float alpha[NR], inv[NR];
   float part[4][NR];            // maxima, or sums, of the four quarters of a tile's tokens
-  float qmax[8];
-  unsigned long long odd;       // drafts of the segment whose values are not all finite
+  float qmax[16];
+  unsigned long long odd[kDesc];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
   long long scan[3 + 32];
 };
@@ -237,7 +251,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   using T = Tc<D, NR>;
   constexpr int kSoftWarps = T::SOFT, kConvWarps = T::CONV;
   constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;  // two copy warps
-  constexpr int kBarConv = 1, kBarSoft = 2, kBarGroup = 3;  // named barriers (one per warpgroup from kBarGroup on)
+  constexpr int kBarConv = 1, kBarGroup = 2;  // named barriers (one per softmax warpgroup from kBarGroup on)
   extern __shared__ char smem_raw[];
   __shared__ TcShared<NR> sh;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -256,8 +270,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       mbar_init(&sh.desc_empty[i], kSoftWarps + kConvWarps + 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.kc_full[i], 1);
-      mbar_init(&sh.kc_empty[i], kConvWarps);
       mbar_init(&sh.kh_full[i], kConvWarps);
       mbar_init(&sh.kh_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
@@ -269,7 +281,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_empty[i], 1);
     }
-    sh.odd = 0;
     fence_barrier_init();
   }
   grid_dependency_wait();
@@ -289,21 +300,20 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   if (n_tiles == 0) {
   } else if (warp >= kCopyWarp) {
     // ------------------------------------------------------------ copies
-    // Both warps walk the tiles; the first publishes their descriptors and copies
-    // codes and scales, the second the values.
+    // Both warps walk the tiles; the first publishes their descriptors, the second
+    // copies the values.
     const bool values = warp > kCopyWarp;
     SeqWork w = seq_work<NR, kTilePages>(a, b0, false);
     TileAt p = tile_at(a, w, b0, u0 - before);
     int seg = -1, high_edge = 0;
-    Ring kc, v;
+    Ring v;
     bool ok = true;
     // this lane's page of tile p: loaded one tile ahead of its use
     int pg = 0, phys = -1, home = -1;
     auto fetch = [&]() {
-      const int i = p.tile * kTilePages + lane;
       phys = home = -1;
-      if (lane < kTilePages && p.tile < w.cache_tiles && i < w.vis_pages) {
-        pg = visible_page(w, i);
+      pg = tile_page<kTilePages>(w, p.tile, lane);
+      if (lane < kTilePages && p.tile < w.cache_tiles && page_visible(w, pg)) {
         const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
         phys = __ldg(bt + pg);
         home = __ldg(bt + pg / a.group_pages * a.group_pages);
@@ -315,8 +325,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       const int ds = i % kDesc;
       const bool draft = p.tile >= w.cache_tiles;
       const int here = draft ? (w.drafts + kMqPage - 1) / kMqPage
-                             : min(kTilePages, w.vis_pages - p.tile * kTilePages);
-      const bool mine = lane < here;
+                             : min(kTilePages, w.pages - tile_page<kTilePages>(w, p.tile, 0));
+      const bool mine = lane < here && (draft || page_visible(w, pg));
       const bool live = mine && (draft || (phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages));
       const uint32_t lives = __ballot_sync(0xffffffffu, live);
       if (!values) {
@@ -345,11 +355,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
         int at = -1;
-        bool clean = true;  // every row sees all of the page
+        bool clean = lane >= here;  // every row sees all of the page
         if (mine) {
           if (draft) {
             at = lane * kMqPage;
-            clean = false;
           } else {
             if (!live) mq_status(a.status, kStatusBadPage);
             at = live ? pg * kMqPage : -1;
@@ -361,11 +370,13 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         // pages of one group share a scale slot: the slot of the group's first page here
         if (!live) home = -1;
         const int prev = __shfl_up_sync(0xffffffffu, home, 1);
-        const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || home != prev);
-        const int slot = 31 - __clz(starts & ((2u << lane) - 1));
+        const uint32_t starts = __ballot_sync(0xffffffffu, live && (lane == 0 || home != prev));
         if (lane < kTilePages) {
-          sh.desc[ds].at[lane] = at;
-          sh.desc[ds].sz[lane] = slot;
+          TileDesc& d = sh.desc[ds];
+          d.at[lane] = at;
+          d.slab[lane] = live && !draft ? phys * a.kv_heads + p.head : -1;
+          d.home[lane] = live && !draft ? home * a.kv_heads + p.head : -1;
+          d.sz[lane] = max(0, 31 - __clz(starts & ((2u << lane) - 1)));
         }
         if (lane == 0) {
           TileDesc& d = sh.desc[ds];
@@ -381,53 +392,36 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.seg = seg % kDesc;
           d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
+          d.slots = draft ? 0 : starts;
+          if (first) sh.odd[seg % kDesc] = 0;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
-        if (!draft) {
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.kc_empty[kc.s], kc.ph ^ 1, a.status));
-          if (!ok) break;
-          const uint32_t szs = lives & starts;
-          uint64_t* bar = &sh.kc_full[kc.s];
-          char* kdst = smem + T::KC_OFF + kc.s * T::KC;
-          char* zdst = smem + T::SZ_OFF + kc.s * T::SZ;
-          if (lane == 0)
-            mbar_arrive_expect_tx(bar, __popc(lives) * (kMqPage * D / 2) + __popc(szs) * (2 * D * 4));
-          __syncwarp();
-#pragma unroll 1
-          for (int g = 0; g < here; ++g) {
-            const int ph = __shfl_sync(0xffffffffu, phys, g), hm = __shfl_sync(0xffffffffu, home, g);
-            if (!(lives >> g & 1)) continue;
-            if (elect_one()) {
-              bulk_g2s(kdst + g * (kMqPage * D / 2),
-                       a.k_pool + ((size_t)ph * a.kv_heads + p.head) * (kMqPage * D / 2), kMqPage * D / 2, bar);
-              if (szs >> g & 1)
-                bulk_g2s(zdst + g * (2 * D * 4), a.sz_pool + ((size_t)hm * a.kv_heads + p.head) * 2 * D, 2 * D * 4,
-                         bar);
-            }
-          }
-          kc.next<T::NK>();
-        }
       } else {
         const CUtensorMap* map = draft ? &dmap : &vmap;
-#pragma unroll 1
-        for (int g0 = 0; g0 < here; g0 += T::PPU) {
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.v_empty[v.s], v.ph ^ 1, a.status));
+        const int row = draft ? w.row0 + lane * kMqPage : 0, slab = draft ? p.head : phys * a.kv_heads + p.head;
+        int rows[kTilePages], slabs[kTilePages];
+#pragma unroll
+        for (int g = 0; g < kTilePages; ++g) {
+          rows[g] = __shfl_sync(0xffffffffu, row, g);
+          slabs[g] = __shfl_sync(0xffffffffu, slab, g);
+        }
+#pragma unroll
+        for (int g0 = 0; g0 < kTilePages; g0 += T::PPU) {
+          if (g0 >= here) break;
+          ok = ok && tc_wait(&sh.v_empty[v.s], v.ph ^ 1, a.status);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          uint64_t* bar = &sh.v_full[v.s];
-          const int g1 = min(g0 + T::PPU, here);
-          const uint32_t unit = lives >> g0 & ((1u << (g1 - g0)) - 1);
-          if (lane == 0) mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
-          __syncwarp();
-          char* dst = smem + T::V_OFF + v.s * T::UNIT;
-#pragma unroll 1
-          for (int g = g0; g < g1; ++g) {
-            const int ph = __shfl_sync(0xffffffffu, phys, g);
-            if ((lives >> g & 1) && elect_one())
-              tma_page(dst + (g - g0) * T::PAGE_V, map, draft ? w.row0 + g * kMqPage : 0,
-                       draft ? p.head : ph * a.kv_heads + p.head, bar);
-            __syncwarp();
+          if (elect_one()) {
+            uint64_t* bar = &sh.v_full[v.s];
+            const uint32_t unit = lives >> g0 & ((1u << T::PPU) - 1);
+            mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
+            char* dst = smem + T::V_OFF + v.s * T::UNIT;
+#pragma unroll
+            for (int q = 0; q < T::PPU; ++q)
+              if (unit >> q & 1) tma_page(dst + q * T::PAGE_V, map, rows[g0 + q], slabs[g0 + q], bar);
           }
+          __syncwarp();
           v.next<T::NV>();
         }
         if (!ok) break;
@@ -437,7 +431,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     }
     // after a timeout: the copies issued so far land (or a bound passes) before the CTA ends
     if (!ok && lane == 0) {
-      for (int s = 0; s < T::NK && !values; ++s) mbar_wait_bounded(&sh.kc_full[s], s < (int)kc.s ? kc.ph : kc.ph ^ 1, 10000000ull);
       for (int s = 0; s < T::NV && values; ++s) mbar_wait_bounded(&sh.v_full[s], s < (int)v.s ? v.ph : v.ph ^ 1, 10000000ull);
     }
     __syncwarp();
@@ -450,34 +443,42 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     int pages = 0;       // of tile i - 1
     bool fresh = true;   // tile i - 1 starts its segment
     bool ok = true;
+    auto logits = [&](int i) {  // S^T of tile i
+      const int hb = i % T::NH;
+      ok = ok && tc_wait(&sh.kh_full[hb], (i / T::NH) & 1, a.status) &&
+           tc_wait(&sh.s_empty[i & 1], (i / 2 + 1) & 1, a.status);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t kd = mat_desc(base + T::KH_OFF + hb * T::KH, 16, 1024), qd = mat_desc(base + T::Q_OFF, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma(tm + (i & 1) * NR, kd + (k / 4) * (kTile * 128 / 16) + (k % 4) * 2,
+                 qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
+        tc_commit(&sh.s_full[i & 1]);
+        tc_commit(&sh.kh_empty[hb]);
+      }
+      __syncwarp();
+    };
 #pragma unroll 1
     for (int i = 0; i <= n_tiles && ok; ++i) {
       int next_pages = 0;
-      bool next_fresh = false;
+      bool next_fresh = false, waiting = i < n_tiles;  // the logits of tile i are still to be issued
       if (i < n_tiles) {
-        const int ds = i % kDesc, hb = i % T::NH;
+        const int ds = i % kDesc;
         ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
         next_pages = sh.desc[ds].pages;
         next_fresh = sh.desc[ds].flags & kFirst;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
-        ok = ok && tc_wait(&sh.kh_full[hb], (i / T::NH) & 1, a.status) &&
-             tc_wait(&sh.s_empty[i & 1], (i / 2 + 1) & 1, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t kd = mat_desc(base + T::KH_OFF + hb * T::KH, 16, 1024), qd = mat_desc(base + T::Q_OFF, 16, 1024);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma(tm + (i & 1) * NR, kd + (k / 4) * (kTile * 128 / 16) + (k % 4) * 2,
-                   qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
-          tc_commit(&sh.s_full[i & 1]);
-          tc_commit(&sh.kh_empty[hb]);
+        // the outputs of tile i - 1 go first where the keys of tile i are not there yet
+        if (i == 0 || __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i % T::NH], (i / T::NH) & 1))) {
+          logits(i);
+          waiting = false;
         }
-        __syncwarp();
       }
-      if (i > 0) {
+      if (i > 0 && ok) {
         const int j = i - 1, pb = j % T::NP;
         ok = __all_sync(0xffffffffu, tc_wait(&sh.p_full[pb], (j / T::NP) & 1, a.status));
         if (!ok) break;
@@ -507,6 +508,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         if (elect_one()) tc_commit(&sh.p_empty[pb]);
         __syncwarp();
       }
+      if (waiting && ok) logits(i);
       pages = next_pages;
       fresh = next_fresh;
     }
@@ -517,7 +519,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     const int cw = warp - kSoftWarps, ct = tid - 32 * kSoftWarps;
     const int c = lane % LPT, t_lane = cw * TPW + lane / LPT;
     const int ca = 8 * c, cb = 8 * (c + LPT);
-    Ring kc;
+    constexpr int kStep = kConvWarps * TPW, kPasses = kTile / kStep;  // tokens at a time, times
+    static_assert(kStep * kPasses == kTile, "whole tiles");
     // The lane's 16 channels of token / row r of an operand with `rows` rows.
     auto put = [&](char* op, int rows, int r, const uint32_t (&h)[8]) {
       char* at = op + r * 128;
@@ -544,34 +547,80 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
       }
     };
+    // Codes of a tile and the scales of its first group travel in registers, loaded
+    // while the tile before is converted: 8 KB a tile need no copies of their own.
+    uint32_t na[kPasses], nb[kPasses];
+    float ns = 0.f, nz = 0.f;
+    auto codes_at = [&](int slab, int t, uint32_t& x, uint32_t& y) {
+      const uint8_t* src = a.k_pool + ((size_t)slab * kMqPage + t % kMqPage) * (D / 2);
+      x = __ldg(reinterpret_cast<const uint32_t*>(src + ca / 2));
+      y = __ldg(reinterpret_cast<const uint32_t*>(src + cb / 2));
+    };
+    auto prefetch = [&](const TileDesc& d) {
+#pragma unroll
+      for (int q = 0; q < kPasses; ++q) {
+        const int t = t_lane + q * kStep, slab = d.slab[t / kMqPage];
+        na[q] = nb[q] = 0;
+        if (slab >= 0) codes_at(slab, t, na[q], nb[q]);
+      }
+      if (d.slots && ct < D) {
+        const float* sz = a.sz_pool + (size_t)d.home[__ffs(d.slots) - 1] * (2 * D) + ct;
+        ns = __ldg(sz);
+        nz = __ldg(sz + D);
+      }
+    };
+    bool ok = tc_wait(&sh.desc_full[0], 0, a.status);
+    if (ok) prefetch(sh.desc[0]);
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int ds = i % kDesc, hb = i % T::NH;
-      bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
       const TileDesc& d = sh.desc[ds];
       const int flags = d.flags, pages = d.pages;
       const bool draft = flags & kDraftTile;
-      if (ok && !draft) ok = tc_wait(&sh.kc_full[kc.s], kc.ph, a.status);
+      // Scale and zero point become what the conversion uses: a code c enters as
+      // 1 + c / 128 (its bits in the mantissa), so a key is (1 + c / 128) e + z
+      // with e = 128 s, z = -zp s - e. Keys beyond float16's range (checked on the
+      // way) take a power of two per group.
+      float* scales = reinterpret_cast<float*>(smem + T::SZ_OFF + (i & 1) * T::SZ);
+      float key_top = 0.f;
+      if (ok && d.slots) {
+        auto params = [&](int slot, int ch, float s, float zp) {
+          const float z = -zp * s;
+          key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
+          scales[slot * (2 * D) + ch] = 128.f * s;
+          scales[slot * (2 * D) + D + ch] = fmaf(-128.f, s, z);
+        };
+        const int one = __ffs(d.slots) - 1;
+        if (ct < D) params(one, ct, ns, nz);
+#pragma unroll 1
+        for (int ch = ct + 32 * kConvWarps; ch < D; ch += 32 * kConvWarps) {
+          const float* sz = a.sz_pool + (size_t)d.home[one] * (2 * D) + ch;
+          params(one, ch, __ldg(sz), __ldg(sz + D));
+        }
+#pragma unroll 1
+        for (uint32_t left = d.slots & (d.slots - 1); left; left &= left - 1) {
+          const int slot = __ffs(left) - 1;
+          const float* sz = a.sz_pool + (size_t)d.home[slot] * (2 * D);
+#pragma unroll 1
+          for (int ch = ct; ch < D; ch += 32 * kConvWarps) params(slot, ch, __ldg(sz + ch), __ldg(sz + D + ch));
+        }
+      }
+      uint32_t wa[kPasses], wb[kPasses];
+#pragma unroll
+      for (int q = 0; q < kPasses; ++q) {
+        wa[q] = na[q];
+        wb[q] = nb[q];
+      }
+      const bool more = i + 1 < n_tiles;
+      bool next_ok = true;
+      if (more) {
+        next_ok = tc_wait(&sh.desc_full[(i + 1) % kDesc], ((i + 1) / kDesc) & 1, a.status);
+        if (next_ok) prefetch(sh.desc[(i + 1) % kDesc]);
+      }
       // A new stream's queries replace the last one's: every product with those
       // is done. Otherwise the buffer of tile i - NH has been read.
       if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) % T::NH], ((i - 1) / T::NH) & 1, a.status);
       if (ok && i >= T::NH) ok = tc_wait(&sh.kh_empty[hb], (i / T::NH + 1) & 1, a.status);
-      // keys beyond float16's range take a scale per group (checked a channel a thread)
-      const float* scales = reinterpret_cast<const float*>(smem + T::SZ_OFF + kc.s * T::SZ);
-      float key_top = 0.f;
-      if (ok && !draft) {
-        int last = -1;
-#pragma unroll 1
-        for (int g = 0; g < pages; ++g) {
-          const int slot = d.sz[g];
-          if (slot == last) continue;
-          last = slot;
-          for (int ch = ct; ch < D; ch += 32 * kConvWarps) {
-            const float s = scales[slot * (2 * D) + ch], z = -scales[slot * (2 * D) + D + ch] * s;
-            key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
-          }
-        }
-      }
       bool scaled = false;
       if (named_bar_or(kBarConv, 32 * kConvWarps, !ok || key_top > kHalfRoom)) {
         // (uniform over the role: its warps meet in named barriers)
@@ -586,7 +635,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll 1
         for (int pass = 0;; ++pass) {
 #pragma unroll 2
-          for (int r = t_lane; r < NR; r += kConvWarps * TPW) {
+          for (int r = t_lane; r < NR; r += kStep) {
             const int row = sh.row[d.seg][r];
             uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             if (row >= 0) {
@@ -616,7 +665,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       char* kh = smem + T::KH_OFF + hb * T::KH;
       if (draft) {
 #pragma unroll 1
-        for (int t = t_lane; t < pages * kMqPage; t += kConvWarps * TPW) {
+        for (int t = t_lane; t < pages * kMqPage; t += kStep) {
           float x[16], top = 0.f, down, up;
           if (t < d.drafts) {
             get(a.kd, ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D, x);
@@ -636,48 +685,23 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           if (c == 0) sh.kscale[ds][t] = up;
         }
       } else {
-        const char* codes = smem + T::KC_OFF + kc.s * T::KC;
-        float s[16], z[16];
-        float up = 1.f;
-        int have = -1;
-#pragma unroll 1
-        for (int t = t_lane; t < pages * kMqPage; t += kConvWarps * TPW) {
-          const uint32_t wa = *reinterpret_cast<const uint32_t*>(codes + t * (D / 2) + ca / 2);
-          const uint32_t wb = *reinterpret_cast<const uint32_t*>(codes + t * (D / 2) + cb / 2);
-          const int slot = d.sz[t / kMqPage];  // uniform in the warp: its tokens lie in one page
-          if (slot != have) {
-            have = slot;
-            const float* p4 = scales + slot * (2 * D);
+        float s[16], z[16], up = 1.f;
+        auto load = [&](int slot) {
+          const float* p4 = scales + slot * (2 * D);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const int ch = j < 8 ? ca + j : cb + j - 8;
-              const float4 x = *reinterpret_cast<const float4*>(p4 + ch);
-              const float4 y = *reinterpret_cast<const float4*>(p4 + D + ch);
-              s[j] = x.x; s[j + 1] = x.y; s[j + 2] = x.z; s[j + 3] = x.w;
-              z[j] = -y.x * x.x; z[j + 1] = -y.y * x.y; z[j + 2] = -y.z * x.z; z[j + 3] = -y.w * x.w;
-            }
-            float down = 1.f;
-            if (scaled) {
-              float top = 0.f;
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                top = fmaxf(top, fmaxf(finite_abs(z[j]), finite_abs(fmaf(15.f, s[j], z[j]))));
-#pragma unroll
-              for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              unit_scale(top, down, up);
-            }
-            // code c enters as 1 + c / 128 (its bits in the mantissa)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float e = s[j] * (down * 128.f);
-              z[j] = fmaf(z[j], down, -e);
-              s[j] = e;
-            }
+          for (int j = 0; j < 16; j += 4) {
+            const int ch = j < 8 ? ca + j : cb + j - 8;
+            const float4 x = *reinterpret_cast<const float4*>(p4 + ch);
+            const float4 y = *reinterpret_cast<const float4*>(p4 + D + ch);
+            s[j] = x.x; s[j + 1] = x.y; s[j + 2] = x.z; s[j + 3] = x.w;
+            z[j] = y.x; z[j + 1] = y.y; z[j + 2] = y.z; z[j + 3] = y.w;
           }
+        };
+        auto convert = [&](int t, uint32_t ka, uint32_t kb) {
           uint32_t h[8];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint32_t x = k ? wb : wa;
+            const uint32_t x = k ? kb : ka;
             const uint32_t lo = (x & 0x0F0F0F0Fu) | 0x80808080u, hi = ((x >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -689,7 +713,39 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             }
           }
           put(kh, kTile, t, h);
-          if (scaled && c == 0) sh.kscale[ds][t] = up;
+        };
+        if (!scaled && !(d.slots & (d.slots - 1))) {  // one group: the usual tile
+          load(__ffs(d.slots | 1u << 31) - 1 & (kTilePages - 1));
+#pragma unroll
+          for (int q = 0; q < kPasses; ++q) convert(t_lane + q * kStep, wa[q], wb[q]);
+        } else {
+          int have = -1;
+#pragma unroll 1
+          for (int t = t_lane; t < pages * kMqPage; t += kStep) {
+            const int slot = d.sz[t / kMqPage], slab = d.slab[t / kMqPage];  // uniform in the warp
+            if (slot != have) {
+              have = slot;
+              load(slot);
+              if (scaled) {
+                float top = 0.f, down;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  top = fmaxf(top, fmaxf(finite_abs(s[j] + z[j]), finite_abs(fmaf(143.f / 128.f, s[j], z[j]))));
+#pragma unroll
+                for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                unit_scale(top, down, up);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  s[j] *= down;
+                  z[j] *= down;
+                }
+              }
+            }
+            uint32_t ka = 0, kb = 0;
+            if (slab >= 0) codes_at(slab, t, ka, kb);
+            convert(t, ka, kb);
+            if (scaled && c == 0) sh.kscale[ds][t] = up;
+          }
         }
       }
       if (ct == 0) sh.scaled[ds] = scaled || draft;
@@ -697,15 +753,14 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sh.kh_full[hb]);
-        if (!draft) mbar_arrive(&sh.kc_empty[kc.s]);
         mbar_arrive(&sh.desc_empty[ds]);
       }
-      if (!draft) kc.next<T::NK>();
+      ok = next_ok;
     }
   } else {
     // ------------------------------------------------------------ softmax
     constexpr int NC = NR / T::WG;             // rows (columns of S^T) of a thread
-    constexpr int LD = NC < 16 ? 8 : 16;       // columns per tensor-memory load
+    constexpr int LD = 16;       // columns per tensor-memory load
     const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC, wt = tid % 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
@@ -717,9 +772,9 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int ds = i % kDesc, sb = i & 1, pb = i % T::NP;
-      // Every thread waits. A timeout is made uniform over the whole role here
+      // Every thread waits. A timeout is made uniform over the warpgroup here
       // alone: until then the tile goes on with what it has, so no barrier of the
-      // softmax ever waits for a warp that has left.
+      // warpgroup (they share none) ever waits for a warp that has left.
       const bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
       failed |= !ok;
       const TileDesc& d = sh.desc[ds];
@@ -753,11 +808,11 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll
         for (int j = 0; j < NC; ++j) l[j] = 0.f;
         if (wt < NC) {
-          sh.ref[c0 + wt] = -INFINITY;
-          sh.sub[c0 + wt] = 0.f;
+          sh.nref[c0 + wt] = INFINITY;
+          sh.nsub[c0 + wt] = 0.f;
         }
       }
-      if (named_bar_or(kBarSoft, 32 * kSoftWarps, failed)) break;
+      if (named_bar_or(bar, 128, failed)) break;
       tc_fence_after();
       float f = sh.qscale[sg] * kLog2e;
       if (sh.scaled[ds]) f = real ? f * sh.kscale[ds][tok] : 0.f;
@@ -771,10 +826,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         tc_ld<LD>(x, s_addr + j0);
 #pragma unroll
         for (int j = 0; j < LD; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(&sh.ref[c0 + j0 + j]);
+          const float4 m = *reinterpret_cast<const float4*>(&sh.nref[c0 + j0 + j]);
           float y[4];
-          fma2(y[0], y[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, -m.x, -m.y);
-          fma2(y[2], y[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, -m.z, -m.w);
+          fma2(y[0], y[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, m.x, m.y);
+          fma2(y[2], y[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, m.z, m.w);
           if (masked) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -800,10 +855,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         named_bar_sync(bar, 128);
         if (wt < NC) {
           const int r = c0 + wt;
-          const float old = sh.ref[r];
+          const float old = -sh.nref[r];
           const float m = fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
-          sh.ref[r] = m;
-          sh.sub[r] = m == -INFINITY ? 0.f : m;
+          sh.nref[r] = -m;
+          sh.nsub[r] = m == -INFINITY ? 0.f : -m;
           sh.alpha[r] = m == -INFINITY ? 1.f : exp2_fast(old - m);
         }
         if (started)  // the weights of tile i - 1 have been multiplied
@@ -836,10 +891,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         tc_ld<LD>(x, s_addr + j0);
 #pragma unroll
         for (int j = 0; j < LD; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(&sh.sub[c0 + j0 + j]);
+          const float4 m = *reinterpret_cast<const float4*>(&sh.nsub[c0 + j0 + j]);
           float e[4];
-          fma2(e[0], e[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, -m.x, -m.y);
-          fma2(e[2], e[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, -m.z, -m.w);
+          fma2(e[0], e[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, m.x, m.y);
+          fma2(e[2], e[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, m.z, m.w);
 #pragma unroll
           for (int q = 0; q < 4; ++q) e[q] = exp2_fast(e[q]);
           if (masked) {
@@ -888,10 +943,15 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
           if (hit) *at16 = y;
         }
-        if (bad) atomicOr(&sh.odd, 1ull << (at & 63));
+        if (bad) atomicOr(&sh.odd[sg], 1ull << (at & 63));
       }
+      if (masked) {
 #pragma unroll 1
-      for (int g = 0; g < pages; g += T::PPU) v.next<T::NV>();
+        for (int g = 0; g < pages; g += T::PPU) v.next<T::NV>();
+      } else {
+        v.s += kTilePages / T::PPU;
+        if (v.s >= T::NV) { v.s -= T::NV; v.ph ^= 1; }
+      }
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
@@ -904,8 +964,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       started = true;
       if (last) {
         // ---- epilogue: sums over the tokens, then O^T, a lane a channel ----
-        // Each step of the butterfly halves the rows a lane holds: lane k ends
-        // with the sum of row k / (32 / NC) over the warp's tokens.
+        // Each step of the butterfly halves the rows a lane holds: it ends with
+        // the sum over the warp's tokens of row NC k / 32.
 #pragma unroll
         for (int st = 0; st < 5; ++st) {
           const int o = 16 >> st, half = (NC >> st) / 2;
@@ -920,9 +980,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
           }
         }
-        if (lane % (32 / NC) == 0) sh.part[quarter][c0 + lane / (32 / NC)] = l[0];
+        sh.part[quarter][c0 + lane * NC / 32] = l[0];
+        // (the product waited for every warp's weights: the list of odd values is complete)
         failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
-        named_bar_sync(kBarSoft, 32 * kSoftWarps);  // all sums, and the list of odd values, are complete
+        named_bar_sync(bar, 128);
         tc_fence_after();
         const bool whole = flags & kWhole;
         float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
@@ -931,12 +992,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
           sh.inv[r] = 1.f / fmaxf(sum, 1e-10f);
           if (!whole) {
-            rec[r] = sh.ref[r] * 0.6931471805599453f;
+            rec[r] = -sh.nref[r] * 0.6931471805599453f;
             rec[NR + r] = sum;
           }
         }
         named_bar_sync(bar, 128);
-        const unsigned long long odd = sh.odd;
+        const unsigned long long odd = sh.odd[sg];
 #pragma unroll 1
         for (int j0 = 0; j0 < T::NO * NC; j0 += 8) {
           const int ch = (j0 / NC) * 128 + tok, col = c0 + j0 % NC;
@@ -973,8 +1034,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
         tc_fence_before();
-        named_bar_sync(kBarSoft, 32 * kSoftWarps);  // sums, references and odd values are free
-        if (tid == 0) sh.odd = 0;
+        __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
       }
     }
