@@ -6,13 +6,16 @@
 // the outputs, O^T[channel, row] += V^T P^T. Tokens and channels fill the 128
 // lanes of an MMA whatever the number of rows is, and its cost grows with the
 // rows (N = 16, 32, 64 or 128): a handful of drafted rows costs a handful of
-// columns, where rows in the lanes would pay for 128. A thread of the softmax
-// holds one token and half of the rows, so a row's sum of weights stays in one
-// register per thread until the stream ends. The running maximum is kept
-// lazily: weights are 2^(x - ref) against a reference that is raised to the
-// true maximum only when some logit exceeds it by more than 8 (in log2), so
-// the outputs are rescaled a few times per stream instead of every tile; sums
-// and outputs are float32 in registers and tensor memory.
+// columns, where rows in the lanes would pay for 128. An MMA with few columns is
+// bound by the shared memory its 128-lane operand is read from (42 cycles at N =
+// 16, 67 at 128, measured), so the dequantized keys never go there: they are
+// written to tensor memory, the other place that operand may come from. A thread
+// of the softmax holds one token and up to 32 rows, so a row's sum of weights
+// stays in one register per thread until the stream ends. The running maximum is
+// kept lazily: weights are 2^(x - ref) against a reference that is raised to the
+// true maximum only when some logit exceeds it by more than 8 (in log2), so the
+// outputs are rescaled a few times per stream instead of every tile; sums and
+// outputs are float32 in registers and tensor memory.
 //
 // Numerics: keys are dequantized as code * s - zp * s in float32, scaled by a
 // power of two that brings the largest channel of their group to [1, 2), and
@@ -23,10 +26,12 @@
 // are.
 //
 // A tile is 128 cached tokens (8 pages) or the drafts. Roles of the warps:
-//   softmax (4 for each 32 rows): S^T from tensor memory, mask, weights to
-//       shared memory, the rare rescale of O^T, and the stream's epilogue
-//   conversion (4 to 16): packed codes, loaded a tile ahead, to float16 keys
-//       (K-major, 128-byte swizzle), a stream's queries, drafted keys
+//   softmax (a warpgroup for up to 32 rows): S^T from tensor memory, mask, weights
+//       to shared memory, the rare rescale of O^T, and the stream's epilogue
+//   conversion (two warpgroups, a tile each in turn): packed codes, copied a tile
+//       ahead, to float16 keys, a thread a token; a stream's queries; drafted
+//       keys. A tile's way through a group is a chain of waits, loads and
+//       arithmetic; two chains side by side keep the arithmetic busy.
 //   MMA issue (1): S^T of tile i and O^T of tile i - 1, the one that can go first
 //   copies (2): the tiles' descriptors; values by tensor copies, in the swizzled
 //       layout the MMA reads (V is stored token-major, which is the transposed
@@ -64,6 +69,14 @@ I4KV_DEVINL void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
+// The same with the first operand in tensor memory (two 16-bit elements a column).
+I4KV_DEVINL void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
 // N columns of the warp's 32 lanes; the wait is part of the statement, so no use
 // of the registers can be scheduled before it.
 template <int N>
@@ -92,8 +105,19 @@ I4KV_DEVINL void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
                : "memory");
 }
+I4KV_DEVINL void tc_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
 I4KV_DEVINL void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 4-byte asynchronous global -> shared copy.
+I4KV_DEVINL void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
 // One lane of a converged warp (the same one every time).
 I4KV_DEVINL bool elect_one() {
   uint32_t p;
@@ -150,30 +174,27 @@ struct Tc {
   static constexpr int CH = D / 64;                        // 64-channel chunks
   static constexpr int PAGE_V = kMqPage * D * 2;           // value bytes of a page
   static constexpr int UNIT = 16384, PPU = UNIT / PAGE_V;  // value ring: units of PPU pages
-  // Stages. One buffer of dequantized keys or of weights makes its writer wait
-  // for the MMA that reads it, so there are two of each where they fit.
-  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 4 : 5);
-  static constexpr int NH = D == 256 ? 1 : 2;              // dequantized keys
-  static constexpr int NP = (D == 256 || NR > 64) ? 1 : 2; // weights
-  // Warps: a softmax warpgroup for each 32 rows (16 or 32 rows, and as many
-  // sums, a thread), conversion warps as registers allow.
-  static constexpr int WG = NR / 32 > 0 ? NR / 32 : 1, SOFT = 4 * WG;
-  static constexpr int CONV = NR == 16 ? 16 : (NR > 64 ? 4 : 8);
+  static constexpr int NC = NR < 32 ? NR : 32;             // rows of a softmax thread
+  static constexpr int WG = NR / NC, SOFT = 4 * WG;        // softmax warpgroups, warps
+  static constexpr int CONV = 8;                           // two conversion groups of four warps
   static constexpr int WARPS = SOFT + CONV + 3, THREADS = 32 * WARPS;
+  // Stages, as shared memory allows.
+  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 4 : (NR > 32 ? 7 : 8));  // value units
+  static constexpr int NP = D == 256 ? 1 : 2;              // weights
   static constexpr int PC = (NR + 63) / 64;                // 64-row chunks of the weights
   static constexpr int NO = D == 256 ? 2 : 1;              // 128-channel blocks of O^T
-  static constexpr int KH = kTile * D * 2, Q = NR * D * 2, P = PC * kTile * 128;
-  static constexpr int SZ = kTilePages * 2 * D * 4;        // a tile's scales, two tiles
-  static constexpr int KH_OFF = 0, V_OFF = KH_OFF + NH * KH, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q;
-  static constexpr int SZ_OFF = P_OFF + NP * P, END = SZ_OFF + 2 * SZ;
-  static constexpr int BYTES = END + 1024;                 // the base is rounded up to 1024
-  static constexpr int COLS_O = 2 * NR, COLS = 512;
-  static_assert(Q % 1024 == 0 && P % 1024 == 0 && COLS_O + NO * NR <= COLS, "layout");
+  static constexpr int Q = NR * D * 2, P = PC * kTile * 128;
+  static constexpr int KC = kTile * D / 2, SZ = kTilePages * 2 * D * 4;  // a tile's codes, and scales
+  static constexpr int V_OFF = 0, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q, KC_OFF = P_OFF + NP * P;
+  static constexpr int SZ_OFF = KC_OFF + 2 * KC, END = SZ_OFF + 4 * SZ;
+  // Tensor memory: two tiles of S^T, O^T, two tiles of keys.
+  static constexpr int COLS_O = 2 * NR, COLS_K = COLS_O + NO * NR, COLS = 512;
+  static_assert(Q % 1024 == 0 && P % 1024 == 0 && COLS_K + D <= COLS, "layout");
 };
 
 struct TileDesc {
   int flags, pages, len, drafts;
-  int row0, head;
+  int row0, head, rows, first_row;  // rows of the sequence; the chunk's first
   int seg, slot;                // segment ring entry; record of a shared stream
   int low_edge;                 // no row sees cached positions <= low_edge (but the sinks)
   int at[kTilePages];           // position of each page's first token, -1: not there
@@ -186,20 +207,19 @@ enum : int { kDraftTile = 1, kMasked = 2, kFirst = 4, kLast = 8, kWhole = 16 };
 
 template <int NR>
 struct TcShared {
-  uint64_t desc_full[kDesc], desc_empty[kDesc], v_full[6], v_empty[6];
+  uint64_t desc_full[kDesc], desc_empty[kDesc], v_full[8], v_empty[8];
   uint64_t kh_full[2], kh_empty[2], s_full[2], s_empty[2], p_full[2], p_empty[2];
   TileDesc desc[kDesc];
   uint64_t word[kDesc][kMqMaxDrafts];  // per segment: the drafts each draft sees,
   int depth[kDesc][kMqMaxDrafts];      // its ancestors,
-  int row[kDesc][NR];                  // each row's row of the outputs [rows * heads], -1: none,
-  uint8_t draft[kDesc][NR];            // and its draft
+  uint8_t draft[kDesc][NR];            // and each row's draft
   float qscale[kDesc];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
   float nref[NR], nsub[NR];     // minus the reference; minus what logits are taken relative to
-  float alpha[NR], inv[NR];
-  float part[4][NR];            // maxima, or sums, of the four quarters of a tile's tokens
-  float qmax[16];
+  float alpha[NR];
+  float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
+  float qmax[2][4];
   unsigned long long odd[kDesc];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
   long long scan[3 + 32];
@@ -234,6 +254,24 @@ I4KV_DEVINL void fma2(float& d0, float& d1, float a0, float a1, float b0, float 
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
+// 8 consecutive 16-bit inputs widened to float32.
+template <int VK>
+I4KV_DEVINL void load8(const void* base, size_t i, float (&x)[8]) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
+  const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (VK == INT4KV_VALUES_F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&wd[j]));
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
+    } else {
+      x[2 * j] = __uint_as_float(wd[j] << 16);
+      x[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
+    }
+  }
+}
+
 // Power of two that brings |x| <= top to [1, 2) (1 for 0), and its inverse.
 I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
   const int e = top > 0.f ? (int)((__float_as_uint(top) >> 23) & 0xFF) : 127;
@@ -244,6 +282,11 @@ I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
 constexpr float kHalfRoom = 32768.f;  // magnitudes up to here are kept as float16 unscaled
 I4KV_DEVINL float finite_abs(float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; }
 
+// Row of the outputs [rows * heads] of a sequence's row rr, one of draft t's.
+I4KV_DEVINL size_t out_row(const MultiQueryArgs& a, int row0, int head, int t, int rr) {
+  return ((size_t)(row0 + t) * a.kv_heads + head) * a.group_q + (rr - t * a.group_q);
+}
+
 template <int D, int NR, int VK>
 __global__ void __launch_bounds__(Tc<D, NR>::THREADS, 1)
 multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_constant__ CUtensorMap vmap,
@@ -251,10 +294,9 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   using T = Tc<D, NR>;
   constexpr int kSoftWarps = T::SOFT, kConvWarps = T::CONV;
   constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;  // two copy warps
-  constexpr int kBarConv = 1, kBarGroup = 2;  // named barriers (one per softmax warpgroup from kBarGroup on)
-  extern __shared__ char smem_raw[];
-  __shared__ TcShared<NR> sh;
-  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int kBarConv = 1, kBarGroup = 3;  // named barriers: one per conversion group, one per softmax warpgroup
+  extern __shared__ __align__(1024) char smem[];  // (no static shared memory: it starts on a 1024-byte boundary)
+  TcShared<NR>& sh = *reinterpret_cast<TcShared<NR>*>(smem + T::END);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (warp == kMmaWarp) {
@@ -267,17 +309,17 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   if (tid == 0) {
     for (int i = 0; i < kDesc; ++i) {
       mbar_init(&sh.desc_full[i], 1);
-      mbar_init(&sh.desc_empty[i], kSoftWarps + kConvWarps + 1);
+      mbar_init(&sh.desc_empty[i], kSoftWarps + 4 + 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.kh_full[i], kConvWarps);
+      mbar_init(&sh.kh_full[i], 4);
       mbar_init(&sh.kh_empty[i], 1);
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.s_empty[i], kSoftWarps);
       mbar_init(&sh.p_full[i], kSoftWarps);
       mbar_init(&sh.p_empty[i], 1);
     }
-    for (int i = 0; i < 6; ++i) {
+    for (int i = 0; i < 8; ++i) {
       mbar_init(&sh.v_full[i], 1);
       mbar_init(&sh.v_empty[i], 1);
     }
@@ -348,11 +390,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           top = __reduce_max_sync(0xffffffffu, top);
           high_edge = w.pos0 + top - a.window;
 #pragma unroll 1
-          for (int r = lane; r < NR; r += 32) {
-            const int rr = p.chunk * NR + r, t = min(rr, w.rows - 1) / a.group_q;
-            sh.draft[sg][r] = (uint8_t)t;
-            sh.row[sg][r] = rr < w.rows ? ((w.row0 + t) * a.kv_heads + p.head) * a.group_q + rr - t * a.group_q : -1;
-          }
+          for (int r = lane; r < NR; r += 32)
+            sh.draft[sg][r] = (uint8_t)(min(p.chunk * NR + r, w.rows - 1) / a.group_q);
         }
         int at = -1;
         bool clean = lane >= here;  // every row sees all of the page
@@ -389,6 +428,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.drafts = w.drafts;
           d.row0 = w.row0;
           d.head = p.head;
+          d.rows = w.rows;
+          d.first_row = p.chunk * NR;
           d.seg = seg % kDesc;
           d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
@@ -444,18 +485,19 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     bool fresh = true;   // tile i - 1 starts its segment
     bool ok = true;
     auto logits = [&](int i) {  // S^T of tile i
-      const int hb = i % T::NH;
-      ok = ok && tc_wait(&sh.kh_full[hb], (i / T::NH) & 1, a.status) &&
+      const int hb = i & 1;
+      ok = ok && tc_wait(&sh.kh_full[hb], (i / 2) & 1, a.status) &&
            tc_wait(&sh.s_empty[i & 1], (i / 2 + 1) & 1, a.status);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) return;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t kd = mat_desc(base + T::KH_OFF + hb * T::KH, 16, 1024), qd = mat_desc(base + T::Q_OFF, 16, 1024);
+        const uint32_t keys = tm + T::COLS_K + hb * (D / 2);
+        const uint64_t qd = mat_desc(base + T::Q_OFF, 16, 1024);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          tc_mma(tm + (i & 1) * NR, kd + (k / 4) * (kTile * 128 / 16) + (k % 4) * 2,
-                 qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
+          tc_mma_ts(tm + (i & 1) * NR, keys + k * 8,
+                    qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
         tc_commit(&sh.s_full[i & 1]);
         tc_commit(&sh.kh_empty[hb]);
       }
@@ -473,7 +515,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
         // the outputs of tile i - 1 go first where the keys of tile i are not there yet
-        if (i == 0 || __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i % T::NH], (i / T::NH) & 1))) {
+        if (i == 0 || __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i & 1], (i / 2) & 1))) {
           logits(i);
           waiting = false;
         }
@@ -514,253 +556,205 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     }
   } else if (warp >= kSoftWarps) {
     // ------------------------------------------------------------ conversion
-    constexpr int LPT = D / 16;          // lanes of a token: 8 channels at 8 c and 8 at 8 (c + LPT)
-    constexpr int TPW = 32 / LPT;        // tokens of a warp at a time
-    const int cw = warp - kSoftWarps, ct = tid - 32 * kSoftWarps;
-    const int c = lane % LPT, t_lane = cw * TPW + lane / LPT;
-    const int ca = 8 * c, cb = 8 * (c + LPT);
-    constexpr int kStep = kConvWarps * TPW, kPasses = kTile / kStep;  // tokens at a time, times
-    static_assert(kStep * kPasses == kTile, "whole tiles");
-    // The lane's 16 channels of token / row r of an operand with `rows` rows.
-    auto put = [&](char* op, int rows, int r, const uint32_t (&h)[8]) {
-      char* at = op + r * 128;
-      *reinterpret_cast<uint4*>(at + (ca / 64) * (rows * 128) + ((((ca / 8) & 7) ^ (r & 7)) << 4)) =
-          make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(at + (cb / 64) * (rows * 128) + ((((cb / 8) & 7) ^ (r & 7)) << 4)) =
-          make_uint4(h[4], h[5], h[6], h[7]);
+    const int grp = (warp - kSoftWarps) / 4, ct = (warp - kSoftWarps) % 4 * 32 + lane;
+    const int bar = kBarConv + grp;
+    // (a warp reaches the lanes of tensor memory that its number within the
+    // warpgroup names: kSoftWarps is a multiple of 4)
+    const uint32_t lanes = (uint32_t)(ct & 96) << 16;
+    // A tile's codes (a thread's token's row) and scales are copied ahead, each
+    // thread into words of its own, where it also turns the scales into what the
+    // conversion uses; the group meets once before it reads them.
+    char* codes = smem + T::KC_OFF + grp * T::KC + 16 * ct;  // 16 bytes of each 2048
+    auto scales_of = [&](int i) {
+      return reinterpret_cast<float*>(smem + T::SZ_OFF + (2 * grp + (i >> 1 & 1)) * T::SZ);
     };
-    // ... of a row of 16-bit inputs, widened to float32
-    auto get = [&](const void* src, size_t i, float (&x)[16]) {
-      const uint16_t* p16 = static_cast<const uint16_t*>(src) + i;
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p16 + ca));
-      const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(p16 + cb));
-      const uint32_t wd[8] = {u.x, u.y, u.z, u.w, w4.x, w4.y, w4.z, w4.w};
+    auto prefetch = [&](const TileDesc& d, int i) {
+      const int slab = d.slab[ct / kMqPage];
+      if (slab >= 0) {
+        const uint8_t* src = a.k_pool + ((size_t)slab * kMqPage + ct % kMqPage) * (D / 2);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if constexpr (VK == INT4KV_VALUES_F16) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&wd[j]));
-          x[2 * j] = f.x;
-          x[2 * j + 1] = f.y;
-        } else {
-          x[2 * j] = __uint_as_float(wd[j] << 16);
-          x[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
+        for (int q = 0; q < D / 32; ++q) cp_async16(codes + q * 2048, src + 16 * q);
+      }
+      float* sz = scales_of(i);
+#pragma unroll 1
+      for (uint32_t left = d.slots; left; left &= left - 1) {
+        const int slot = __ffs(left) - 1;
+        const float* src = a.sz_pool + (size_t)d.home[slot] * (2 * D);
+#pragma unroll
+        for (int ch = 0; ch < D; ch += 128) {
+          if (D >= 128 || ct < D) {
+            cp_async4(sz + slot * (2 * D) + ch + ct, src + ch + ct);
+            cp_async4(sz + slot * (2 * D) + D + ch + ct, src + D + ch + ct);
+          }
         }
       }
+      cp_async_commit();
     };
-    // Codes of a tile and the scales of its first group travel in registers, loaded
-    // while the tile before is converted: 8 KB a tile need no copies of their own.
-    uint32_t na[kPasses], nb[kPasses];
-    float ns = 0.f, nz = 0.f;
-    auto codes_at = [&](int slab, int t, uint32_t& x, uint32_t& y) {
-      const uint8_t* src = a.k_pool + ((size_t)slab * kMqPage + t % kMqPage) * (D / 2);
-      x = __ldg(reinterpret_cast<const uint32_t*>(src + ca / 2));
-      y = __ldg(reinterpret_cast<const uint32_t*>(src + cb / 2));
-    };
-    auto prefetch = [&](const TileDesc& d) {
-#pragma unroll
-      for (int q = 0; q < kPasses; ++q) {
-        const int t = t_lane + q * kStep, slab = d.slab[t / kMqPage];
-        na[q] = nb[q] = 0;
-        if (slab >= 0) codes_at(slab, t, na[q], nb[q]);
-      }
-      if (d.slots && ct < D) {
-        const float* sz = a.sz_pool + (size_t)d.home[__ffs(d.slots) - 1] * (2 * D) + ct;
-        ns = __ldg(sz);
-        nz = __ldg(sz + D);
-      }
-    };
-    bool ok = tc_wait(&sh.desc_full[0], 0, a.status);
-    if (ok) prefetch(sh.desc[0]);
+    bool ok = true;
+    if (grp < n_tiles) {
+      ok = tc_wait(&sh.desc_full[grp], 0, a.status);
+      if (ok) prefetch(sh.desc[grp], grp);
+    }
 #pragma unroll 1
-    for (int i = 0; i < n_tiles; ++i) {
-      const int ds = i % kDesc, hb = i % T::NH;
+    for (int i = grp; i < n_tiles; i += 2) {
+      const int ds = i % kDesc;
       const TileDesc& d = sh.desc[ds];
-      const int flags = d.flags, pages = d.pages;
+      const int flags = d.flags;
       const bool draft = flags & kDraftTile;
-      // Scale and zero point become what the conversion uses: a code c enters as
-      // 1 + c / 128 (its bits in the mantissa), so a key is (1 + c / 128) e + z
-      // with e = 128 s, z = -zp s - e. Keys beyond float16's range (checked on the
-      // way) take a power of two per group.
-      float* scales = reinterpret_cast<float*>(smem + T::SZ_OFF + (i & 1) * T::SZ);
+      // Scale and zero point, in place: a code c enters as 1 + c / 128 (its bits in
+      // the mantissa), so a key is (1 + c / 128) e + z with e = 128 s, z = -zp s - e.
+      float* scales = scales_of(i);
       float key_top = 0.f;
-      if (ok && d.slots) {
-        auto params = [&](int slot, int ch, float s, float zp) {
-          const float z = -zp * s;
-          key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
-          scales[slot * (2 * D) + ch] = 128.f * s;
-          scales[slot * (2 * D) + D + ch] = fmaf(-128.f, s, z);
-        };
-        const int one = __ffs(d.slots) - 1;
-        if (ct < D) params(one, ct, ns, nz);
+      cp_async_wait<0>();
 #pragma unroll 1
-        for (int ch = ct + 32 * kConvWarps; ch < D; ch += 32 * kConvWarps) {
-          const float* sz = a.sz_pool + (size_t)d.home[one] * (2 * D) + ch;
-          params(one, ch, __ldg(sz), __ldg(sz + D));
-        }
-#pragma unroll 1
-        for (uint32_t left = d.slots & (d.slots - 1); left; left &= left - 1) {
-          const int slot = __ffs(left) - 1;
-          const float* sz = a.sz_pool + (size_t)d.home[slot] * (2 * D);
-#pragma unroll 1
-          for (int ch = ct; ch < D; ch += 32 * kConvWarps) params(slot, ch, __ldg(sz + ch), __ldg(sz + D + ch));
-        }
-      }
-      uint32_t wa[kPasses], wb[kPasses];
+      for (uint32_t left = ok ? d.slots : 0u; left; left &= left - 1) {
+        float* sz = scales + (__ffs(left) - 1) * (2 * D) + ct;
 #pragma unroll
-      for (int q = 0; q < kPasses; ++q) {
-        wa[q] = na[q];
-        wb[q] = nb[q];
-      }
-      const bool more = i + 1 < n_tiles;
-      bool next_ok = true;
-      if (more) {
-        next_ok = tc_wait(&sh.desc_full[(i + 1) % kDesc], ((i + 1) / kDesc) & 1, a.status);
-        if (next_ok) prefetch(sh.desc[(i + 1) % kDesc]);
+        for (int ch = 0; ch < D; ch += 128) {
+          if (D >= 128 || ct < D) {
+            const float s = sz[ch], z = -sz[D + ch] * s;
+            key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
+            sz[ch] = 128.f * s;
+            sz[D + ch] = fmaf(-128.f, s, z);
+          }
+        }
       }
       // A new stream's queries replace the last one's: every product with those
-      // is done. Otherwise the buffer of tile i - NH has been read.
-      if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) % T::NH], ((i - 1) / T::NH) & 1, a.status);
-      if (ok && i >= T::NH) ok = tc_wait(&sh.kh_empty[hb], (i / T::NH + 1) & 1, a.status);
+      // is done. Otherwise the keys of tile i - 2 have been multiplied.
+      if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
+      ok = ok && tc_wait(&sh.kh_empty[i & 1], (i / 2 + 1) & 1, a.status);
+      // Keys beyond float16's range take a power of two per group.
       bool scaled = false;
-      if (named_bar_or(kBarConv, 32 * kConvWarps, !ok || key_top > kHalfRoom)) {
-        // (uniform over the role: its warps meet in named barriers)
-        if (named_bar_or(kBarConv, 32 * kConvWarps, !ok)) break;
+      if (named_bar_or(bar, 128, !ok || key_top > kHalfRoom)) {
+        // (uniform over the group: its warps meet in named barriers)
+        if (named_bar_or(bar, 128, !ok)) break;
         scaled = true;
       }
+      tc_fence_after();
       if (flags & kFirst) {
         // The stream's queries, as they are: a magnitude below float16's range
         // loses nothing that a logit could show. Only one above it (a bfloat16
-        // input) takes the second pass, with a common power of two.
+        // input) takes the second pass, with a common power of two. A thread
+        // takes 8 channels of a row.
         float top = 0.f, down = 1.f, up = 1.f;
 #pragma unroll 1
         for (int pass = 0;; ++pass) {
-#pragma unroll 2
-          for (int r = t_lane; r < NR; r += kStep) {
-            const int row = sh.row[d.seg][r];
-            uint32_t h[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (row >= 0) {
-              float x[16];
-              get(a.q, (size_t)row * D, x);
+#pragma unroll 4
+          for (int k = ct; k < NR * (D / 8); k += 128) {
+            const int r = k / (D / 8), c8 = k % (D / 8), rr = d.first_row + r;
+            uint32_t h[4] = {0, 0, 0, 0};
+            if (rr < d.rows) {
+              float x[8];
+              load8<VK>(a.q, out_row(a, d.row0, d.head, sh.draft[d.seg][r], rr) * D + 8 * c8, x);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+              for (int j = 0; j < 4; ++j) {
                 if (VK == INT4KV_VALUES_BF16) top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
                 h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
               }
             }
-            put(smem + T::Q_OFF, NR, r, h);
+            *reinterpret_cast<uint4*>(smem + T::Q_OFF + (c8 / 8) * (NR * 128) + r * 128 + ((c8 % 8 ^ (r & 7)) << 4)) =
+                make_uint4(h[0], h[1], h[2], h[3]);
           }
           if (VK == INT4KV_VALUES_F16 || pass == 1) break;
-          if (!named_bar_or(kBarConv, 32 * kConvWarps, top > kHalfRoom)) break;
+          if (!named_bar_or(bar, 128, top > kHalfRoom)) break;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (lane == 0) sh.qmax[cw] = top;
-          named_bar_sync(kBarConv, 32 * kConvWarps);
-#pragma unroll 1
-          for (int j = 0; j < kConvWarps; ++j) top = fmaxf(top, sh.qmax[j]);
-          named_bar_sync(kBarConv, 32 * kConvWarps);  // qmax is free again
+          if (lane == 0) sh.qmax[grp][ct / 32] = top;
+          named_bar_sync(bar, 128);
+          top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
+          named_bar_sync(bar, 128);  // qmax is free again
           unit_scale(top, down, up);
         }
         if (ct == 0) sh.qscale[d.seg] = up;
+        fence_proxy_async_smem();
       }
-      char* kh = smem + T::KH_OFF + hb * T::KH;
+      const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
+      float up = 1.f, down = 1.f;
       if (draft) {
+        const bool real = ct < d.drafts;
+        const size_t row = ((size_t)(d.row0 + ct) * a.kv_heads + d.head) * D;
+        float top = 0.f;
 #pragma unroll 1
-        for (int t = t_lane; t < pages * kMqPage; t += kStep) {
-          float x[16], top = 0.f, down, up;
-          if (t < d.drafts) {
-            get(a.kd, ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D, x);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) top = fmaxf(top, finite_abs(x[j]));
-#pragma unroll
-          for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          unit_scale(top, down, up);
-          uint32_t h[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
-          put(kh, kTile, t, h);
-          if (c == 0) sh.kscale[ds][t] = up;
-        }
-      } else {
-        float s[16], z[16], up = 1.f;
-        auto load = [&](int slot) {
-          const float* p4 = scales + slot * (2 * D);
-#pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const int ch = j < 8 ? ca + j : cb + j - 8;
-            const float4 x = *reinterpret_cast<const float4*>(p4 + ch);
-            const float4 y = *reinterpret_cast<const float4*>(p4 + D + ch);
-            s[j] = x.x; s[j + 1] = x.y; s[j + 2] = x.z; s[j + 3] = x.w;
-            z[j] = y.x; z[j + 1] = y.y; z[j + 2] = y.z; z[j + 3] = y.w;
-          }
-        };
-        auto convert = [&](int t, uint32_t ka, uint32_t kb) {
-          uint32_t h[8];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t x = k ? kb : ka;
-            const uint32_t lo = (x & 0x0F0F0F0Fu) | 0x80808080u, hi = ((x >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int q = 8 * k + 2 * j;
-              float e0, e1;
-              fma2(e0, e1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
-                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), s[q], s[q + 1], z[q], z[q + 1]);
-              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(e0, e1);
-            }
-          }
-          put(kh, kTile, t, h);
-        };
-        if (!scaled && !(d.slots & (d.slots - 1))) {  // one group: the usual tile
-          load(__ffs(d.slots | 1u << 31) - 1 & (kTilePages - 1));
-#pragma unroll
-          for (int q = 0; q < kPasses; ++q) convert(t_lane + q * kStep, wa[q], wb[q]);
-        } else {
-          int have = -1;
+        for (int pass = 0; pass < 2; ++pass) {  // the row's scale, then its keys
 #pragma unroll 1
-          for (int t = t_lane; t < pages * kMqPage; t += kStep) {
-            const int slot = d.sz[t / kMqPage], slab = d.slab[t / kMqPage];  // uniform in the warp
-            if (slot != have) {
-              have = slot;
-              load(slot);
-              if (scaled) {
-                float top = 0.f, down;
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t h[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  top = fmaxf(top, fmaxf(finite_abs(s[j] + z[j]), finite_abs(fmaf(143.f / 128.f, s[j], z[j]))));
+            for (int e = 0; e < 4; ++e) {
+              float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+              if (real) load8<VK>(a.kd, row + 32 * q + 8 * e, x);
 #pragma unroll
-                for (int o = 1; o < LPT; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                unit_scale(top, down, up);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  s[j] *= down;
-                  z[j] *= down;
-                }
+              for (int j = 0; j < 4; ++j) {
+                top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+                h[4 * e + j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
               }
             }
-            uint32_t ka = 0, kb = 0;
-            if (slab >= 0) codes_at(slab, t, ka, kb);
-            convert(t, ka, kb);
-            if (scaled && c == 0) sh.kscale[ds][t] = up;
+            __syncwarp();
+            if (pass) tc_st16(keys + 16 * q, h);
           }
+          if (!pass) unit_scale(top, down, up);
+        }
+      } else {
+        const float* sz = scales + d.sz[ct / kMqPage] * (2 * D);
+        if (scaled) {
+          float top = 0.f;
+#pragma unroll 1
+          for (int ch = 0; ch < D; ++ch) {
+            const float e = sz[ch], z = sz[D + ch];  // code 0: e + z; 15: 143/128 e + z
+            top = fmaxf(top, fmaxf(finite_abs(e + z), finite_abs(fmaf(143.f / 128.f, e, z))));
+          }
+          unit_scale(top, down, up);
+        }
+        uint4 next = *reinterpret_cast<const uint4*>(codes);
+#pragma unroll 2
+        for (int q = 0; q < D / 32; ++q) {  // 32 channels
+          const uint32_t wd[4] = {next.x, next.y, next.z, next.w};
+          if (q + 1 < D / 32) next = *reinterpret_cast<const uint4*>(codes + (q + 1) * 2048);
+          uint32_t h[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = (wd[k] & 0x0F0F0F0Fu) | 0x80808080u, hi = ((wd[k] >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
+            const float* p4 = sz + 32 * q + 8 * k;
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+              const float4 e = *reinterpret_cast<const float4*>(p4 + 2 * j);
+              const float4 z = *reinterpret_cast<const float4*>(p4 + D + 2 * j);
+              float x0, x1, x2, x3;
+              fma2(x0, x1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
+                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), e.x, e.y, z.x, z.y);
+              fma2(x2, x3, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | ((j + 1) << 8))),
+                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | ((j + 1) << 8))), e.z, e.w, z.z, z.w);
+              if (scaled) {
+                x0 *= down; x1 *= down; x2 *= down; x3 *= down;
+              }
+              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(x0, x1);
+              h[4 * k + j + 1] = pack16<INT4KV_VALUES_F16>(x2, x3);
+            }
+          }
+          tc_st16(keys + 16 * q, h);
         }
       }
+      if (scaled || draft) sh.kscale[ds][ct] = up;
       if (ct == 0) sh.scaled[ds] = scaled || draft;
-      fence_proxy_async_smem();
+      const int next = i + 2;
+      tc_wait_st();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&sh.kh_full[hb]);
+        mbar_arrive(&sh.kh_full[i & 1]);
         mbar_arrive(&sh.desc_empty[ds]);
       }
-      ok = next_ok;
+      // (the thread has read its codes: their words are free)
+      if (next < n_tiles) {
+        ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+        if (ok) prefetch(sh.desc[next % kDesc], next);
+      }
     }
+    cp_async_wait<0>();
   } else {
     // ------------------------------------------------------------ softmax
-    constexpr int NC = NR / T::WG;             // rows (columns of S^T) of a thread
-    constexpr int LD = 16;       // columns per tensor-memory load
+    constexpr int NC = T::NC;                  // rows (columns of S^T) of a thread
+    constexpr int LD = NR > 64 ? 8 : 16;       // columns per tensor-memory load (72 registers a thread at 128 rows)
     const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC, wt = tid % 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
@@ -803,6 +797,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         if (!real) vis = 0;
       }
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
+      if (named_bar_or(bar, 128, failed)) break;
       if (flags & kFirst) {
         started = false;
 #pragma unroll
@@ -811,8 +806,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           sh.nref[c0 + wt] = INFINITY;
           sh.nsub[c0 + wt] = 0.f;
         }
+        named_bar_sync(bar, 128);
       }
-      if (named_bar_or(bar, 128, failed)) break;
       tc_fence_after();
       float f = sh.qscale[sg] * kLog2e;
       if (sh.scaled[ds]) f = real ? f * sh.kscale[ds][tok] : 0.f;
@@ -963,7 +958,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       }
       started = true;
       if (last) {
-        // ---- epilogue: sums over the tokens, then O^T, a lane a channel ----
+        // ---- epilogue: O^T, a lane a channel, over the sums of the weights ----
         // Each step of the butterfly halves the rows a lane holds: it ends with
         // the sum over the warp's tokens of row NC k / 32.
 #pragma unroll
@@ -984,52 +979,57 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         // (the product waited for every warp's weights: the list of odd values is complete)
         failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
+        if (wt < NC) {
+          const int r = c0 + wt;
+          sh.alpha[r] = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+        }
+        named_bar_sync(bar, 128);
         tc_fence_after();
         const bool whole = flags & kWhole;
         float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
-        if (wt < NC) {
-          const int r = c0 + wt;
-          const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
-          sh.inv[r] = 1.f / fmaxf(sum, 1e-10f);
-          if (!whole) {
-            rec[r] = -sh.nref[r] * 0.6931471805599453f;
-            rec[NR + r] = sum;
-          }
-        }
-        named_bar_sync(bar, 128);
         const unsigned long long odd = sh.odd[sg];
 #pragma unroll 1
-        for (int j0 = 0; j0 < T::NO * NC; j0 += 8) {
-          const int ch = (j0 / NC) * 128 + tok, col = c0 + j0 % NC;
-          uint32_t x[8];
-          tc_ld<8>(x, tm + lanes + T::COLS_O + (j0 / NC) * NR + col);
-          if (ch >= D) continue;
+        for (int j0 = 0; j0 < NC; j0 += 8) {
+          const int col = c0 + j0;
 #pragma unroll 1
-          for (unsigned long long left = odd; left; left &= left - 1) {
-            const int u = __ffsll(left) - 1;
-            float y2[2];
-            load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
-            const float y = y2[ch & 1];
-            if (fabsf(y) <= 3.4e38f) continue;
-            const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
+          for (int o = 0; o < T::NO; ++o) {
+            const int ch = o * 128 + tok;
+            uint32_t x[8];
+            tc_ld<8>(x, tm + lanes + T::COLS_O + o * NR + col);
+            if (ch >= D) continue;
+#pragma unroll 1
+            for (unsigned long long left = odd; left; left &= left - 1) {
+              const int u = __ffsll(left) - 1;
+              float y2[2];
+              load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
+              const float y = y2[ch & 1];
+              if (fabsf(y) <= 3.4e38f) continue;
+              const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int t = sh.draft[sg][col + j];
+                if ((sh.word[sg][t] >> u & 1) &&
+                    (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
+                  x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+              }
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int t = sh.draft[sg][col + j];
-              if ((sh.word[sg][t] >> u & 1) && (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
-                x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = col + j, row = sh.row[sg][r];
-            if (row < 0) continue;
-            const float y = __uint_as_float(x[j]);
-            if (whole) {
-              const size_t to = (size_t)row * D + ch;
-              if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.inv[r]);
-              else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.inv[r]);
-            } else {
-              rec[2 * NR + r * D + ch] = y;
+              const int r = col + j, rr = d.first_row + r;
+              if (rr >= d.rows) continue;
+              const float y = __uint_as_float(x[j]), sum = sh.alpha[r];
+              if (whole) {
+                const size_t to = out_row(a, d.row0, d.head, sh.draft[sg][r], rr) * D + ch;
+                const float q = y * (1.f / fmaxf(sum, 1e-10f));
+                if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(q);
+                else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(q);
+              } else {
+                rec[2 * NR + r * D + ch] = y;
+                if (ch == 0) {
+                  rec[r] = -sh.nref[r] * 0.6931471805599453f;
+                  rec[NR + r] = sum;
+                }
+              }
             }
           }
         }
@@ -1083,10 +1083,11 @@ cudaError_t value_map(CUtensorMap* map, const void* base, int vk, int dim, uint6
 template <int D, int NR, int VK>
 cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream_t stream) {
   using T = Tc<D, NR>;
-  static_assert(T::BYTES + sizeof(TcShared<NR>) <= 227 * 1024, "shared memory");
+  constexpr size_t kBytes = T::END + sizeof(TcShared<NR>);
+  static_assert(T::END + sizeof(TcShared<NR>) <= 227 * 1024, "shared memory");
   constexpr auto kern = multi_query_tc_kernel<D, NR, VK>;
   int per_sm = 0;
-  cudaError_t e = mq_occupancy<kern>(T::THREADS, T::BYTES, &per_sm);
+  cudaError_t e = mq_occupancy<kern>(T::THREADS, kBytes, &per_sm);
   if (e != cudaSuccess) return e;
   if (ws_bytes < (size_t)sms * 2 * Record<NR, D>::kFloats * 4) return cudaErrorInvalidValue;
   CUtensorMap vmap, dmap;
@@ -1097,7 +1098,7 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   if (a.vd) e = value_map(&dmap, a.vd, VK, D, a.total_rows, row * a.kv_heads, a.kv_heads, row);
   else dmap = vmap;
   if (e != cudaSuccess) return e;
-  e = mq_launch_pdl(kern, dim3(sms), dim3(T::THREADS), T::BYTES, stream, a, vmap, dmap);
+  e = mq_launch_pdl(kern, dim3(sms), dim3(T::THREADS), kBytes, stream, a, vmap, dmap);
   if (e != cudaSuccess) return e;
   return mq_launch_pdl(merge_records_kernel<NR, kTilePages, D>, dim3(sms - 1, (NR + kMergeWarps - 1) / kMergeWarps),
                        dim3(kMergeWarps * 32), 0, stream, a, sms);
