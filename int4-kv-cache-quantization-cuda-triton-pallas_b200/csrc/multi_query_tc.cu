@@ -77,39 +77,53 @@ I4KV_DEVINL void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, b
       "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
 }
-// N columns of the warp's 32 lanes; the wait is part of the statement, so no use
-// of the registers can be scheduled before it.
-template <int N>
-I4KV_DEVINL void tc_ld(uint32_t (&r)[N], uint32_t addr) {
-  static_assert(N == 8 || N == 16, "columns per load");
-  if constexpr (N == 8) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-        : "r"(addr)
-        : "memory");
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr)
-        : "memory");
-  }
+// 8 columns of the warp's 32 lanes. (The waits are part of the loads' statements, so
+// no use of the registers can be scheduled before them.)
+I4KV_DEVINL void tc_ld8(uint32_t (&r)[8], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr)
+      : "memory");
 }
-I4KV_DEVINL void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
+// 16 lanes x 8 N columns in the layout of mma fragments: thread (g, t) = (lane / 4,
+// lane % 4) holds columns 8 j + 2 t, + 1 of lane g in r[4 j], r[4 j + 1] and of lane
+// g + 8 in r[4 j + 2], r[4 j + 3].
+I4KV_DEVINL void tc_st_frag(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
+I4KV_DEVINL void tc_st_frag(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
                : "memory");
 }
-I4KV_DEVINL void tc_st16(uint32_t addr, const uint32_t (&r)[16]) {
+// Two such blocks (lanes 0-15 and 16-31 of the warp's 32) and the wait for both.
+I4KV_DEVINL void tc_ld_frag(uint32_t (&a)[16], uint32_t (&b)[16], uint32_t addr) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
-      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(a[8]),
+        "=r"(a[9]), "=r"(a[10]), "=r"(a[11]), "=r"(a[12]), "=r"(a[13]), "=r"(a[14]), "=r"(a[15]), "=r"(b[0]), "=r"(b[1]),
+        "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7]), "=r"(b[8]), "=r"(b[9]), "=r"(b[10]),
+        "=r"(b[11]), "=r"(b[12]), "=r"(b[13]), "=r"(b[14]), "=r"(b[15])
+      : "r"(addr), "r"(addr + (16u << 16))
+      : "memory");
+}
+I4KV_DEVINL void tc_ld_frag(uint32_t (&a)[8], uint32_t (&b)[8], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(b[0]),
+        "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7])
+      : "r"(addr), "r"(addr + (16u << 16))
       : "memory");
 }
 I4KV_DEVINL void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -174,19 +188,21 @@ struct Tc {
   static constexpr int CH = D / 64;                        // 64-channel chunks
   static constexpr int PAGE_V = kMqPage * D * 2;           // value bytes of a page
   static constexpr int UNIT = 16384, PPU = UNIT / PAGE_V;  // value ring: units of PPU pages
-  static constexpr int NC = NR < 32 ? NR : 32;             // rows of a softmax thread
+  static constexpr int NC = NR > 64 ? 64 : (NR < 32 ? NR : 32);  // rows of a softmax warpgroup
   static constexpr int WG = NR / NC, SOFT = 4 * WG;        // softmax warpgroups, warps
   static constexpr int CONV = 8;                           // two conversion groups of four warps
   static constexpr int WARPS = SOFT + CONV + 3, THREADS = 32 * WARPS;
   // Stages, as shared memory allows.
-  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 4 : (NR > 32 ? 7 : 8));  // value units
-  static constexpr int NP = D == 256 ? 1 : 2;              // weights
+  static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 3 : (NR > 32 ? 6 : 7));  // value units
+  static constexpr int NP = 2;                             // weights
+  static constexpr int NB = D == 256 ? 1 : 2;              // codes and scales of a conversion group
+  static_assert(NV * PPU >= kTilePages, "a whole tile's values fit (the softmax may wait for its last ones)");
   static constexpr int PC = (NR + 63) / 64;                // 64-row chunks of the weights
   static constexpr int NO = D == 256 ? 2 : 1;              // 128-channel blocks of O^T
   static constexpr int Q = NR * D * 2, P = PC * kTile * 128;
   static constexpr int KC = kTile * D / 2, SZ = kTilePages * 2 * D * 4;  // a tile's codes, and scales
   static constexpr int V_OFF = 0, Q_OFF = V_OFF + NV * UNIT, P_OFF = Q_OFF + Q, KC_OFF = P_OFF + NP * P;
-  static constexpr int SZ_OFF = KC_OFF + 2 * KC, END = SZ_OFF + 4 * SZ;
+  static constexpr int SZ_OFF = KC_OFF + 2 * NB * KC, END = SZ_OFF + 2 * NB * SZ;
   // Tensor memory: two tiles of S^T, O^T, two tiles of keys.
   static constexpr int COLS_O = 2 * NR, COLS_K = COLS_O + NO * NR, COLS = 512;
   static_assert(Q % 1024 == 0 && P % 1024 == 0 && COLS_K + D <= COLS, "layout");
@@ -216,8 +232,7 @@ struct TcShared {
   float qscale[kDesc];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
-  float nref[NR], nsub[NR];     // minus the reference; minus what logits are taken relative to
-  float alpha[NR];
+  float ref[NR], sum[NR];       // a finished stream's references and sums
   float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
   float qmax[2][4];
   unsigned long long odd[kDesc];  // per segment: drafts whose values are not all finite
@@ -561,19 +576,25 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // (a warp reaches the lanes of tensor memory that its number within the
     // warpgroup names: kSoftWarps is a multiple of 4)
     const uint32_t lanes = (uint32_t)(ct & 96) << 16;
-    // A tile's codes (a thread's token's row) and scales are copied ahead, each
-    // thread into words of its own, where it also turns the scales into what the
-    // conversion uses; the group meets once before it reads them.
-    char* codes = smem + T::KC_OFF + grp * T::KC + 16 * ct;  // 16 bytes of each 2048
+    // A tile's codes and scales are copied ahead into one of two buffers; a thread
+    // turns the scales it copied into what the conversion uses, and the group meets
+    // once before it reads either. (The other buffer is free by then: every warp
+    // has left the tile that used it. With one buffer, at head_dim 256, the group
+    // meets again before the next copies.) Rows of codes are swizzled by 16 bytes, as
+    // the threads of a warp read 8 rows at a time.
+    constexpr int kRow = D / 2;  // bytes of a row of codes
+    auto codes_of = [&](int i) { return smem + T::KC_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::KC; };
+    auto swizzle = [](int t) { return D == 64 ? (t >> 2 & 1) : (D == 128 ? (t >> 1 & 3) : (t & 7)); };
     auto scales_of = [&](int i) {
-      return reinterpret_cast<float*>(smem + T::SZ_OFF + (2 * grp + (i >> 1 & 1)) * T::SZ);
+      return reinterpret_cast<float*>(smem + T::SZ_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::SZ);
     };
     auto prefetch = [&](const TileDesc& d, int i) {
       const int slab = d.slab[ct / kMqPage];
       if (slab >= 0) {
         const uint8_t* src = a.k_pool + ((size_t)slab * kMqPage + ct % kMqPage) * (D / 2);
 #pragma unroll
-        for (int q = 0; q < D / 32; ++q) cp_async16(codes + q * 2048, src + 16 * q);
+        for (int q = 0; q < D / 32; ++q)
+          cp_async16(codes_of(i) + ct * kRow + ((q ^ swizzle(ct)) << 4), src + 16 * q);
       }
       float* sz = scales_of(i);
 #pragma unroll 1
@@ -631,6 +652,13 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         scaled = true;
       }
       tc_fence_after();
+      // the next tile's copies, now if its descriptor is there (else at the end)
+      const int next = i + 2;
+      bool ahead = false;
+      if (T::NB > 1 && next < n_tiles && mbar_test(&sh.desc_full[next % kDesc], (next / kDesc) & 1)) {
+        prefetch(sh.desc[next % kDesc], next);
+        ahead = true;
+      }
       if (flags & kFirst) {
         // The stream's queries, as they are: a magnitude below float16's range
         // loses nothing that a logit could show. Only one above it (a bfloat16
@@ -652,8 +680,14 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
                 h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
               }
             }
-            *reinterpret_cast<uint4*>(smem + T::Q_OFF + (c8 / 8) * (NR * 128) + r * 128 + ((c8 % 8 ^ (r & 7)) << 4)) =
-                make_uint4(h[0], h[1], h[2], h[3]);
+            // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
+            char* row = smem + T::Q_OFF + (c8 / 8) * (NR * 128) + r * 128;
+            const int q = c8 % 8 / 2, j = c8 % 2 * 2;
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              const int at = 32 * (j + o) + 8 * q;  // byte of the row
+              *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
+            }
           }
           if (VK == INT4KV_VALUES_F16 || pass == 1) break;
           if (!named_bar_or(bar, 128, top > kHalfRoom)) break;
@@ -668,75 +702,123 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         if (ct == 0) sh.qscale[d.seg] = up;
         fence_proxy_async_smem();
       }
+      // Keys: thread (g, t) of a warp takes tokens g, g + 8 of each of the warp's two
+      // pages and 16 channels 64 b + 16 t of each block b of 64: its parameters stay
+      // in registers over the tokens, and the fragments go to tensor memory as they are.
       const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
-      float up = 1.f, down = 1.f;
+      const int g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
       if (draft) {
-        const bool real = ct < d.drafts;
-        const size_t row = ((size_t)(d.row0 + ct) * a.kv_heads + d.head) * D;
-        float top = 0.f;
 #pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {  // the row's scale, then its keys
+        for (int p = 0; p < 2; ++p) {
+          const int ta = (page0 + p) * kMqPage + g, tb = ta + 8;
+          float top[2] = {0.f, 0.f}, down[2] = {1.f, 1.f}, up[2] = {1.f, 1.f};
 #pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t h[16];
+          for (int pass = 0; pass < 2; ++pass) {  // the rows' scales, then their keys
+#pragma unroll 1
+            for (int blk = 0; blk < D / 64; ++blk) {
+              uint32_t h[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-              if (real) load8<VK>(a.kd, row + 32 * q + 8 * e, x);
+              for (int r = 0; r < 2; ++r) {
+                const int t = r ? tb : ta;
+                const size_t row = ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 64 * blk + 16 * t4;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-                h[4 * e + j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+                for (int e = 0; e < 2; ++e) {
+                  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                  if (t < d.drafts) load8<VK>(a.kd, row + 8 * e, x);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    top[r] = fmaxf(top[r], fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+                    // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
+                    h[4 * (2 * e + j / 2) + 2 * r + j % 2] =
+                        pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
+                  }
+                }
+              }
+              __syncwarp();
+              if (pass) tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
+            }
+            if (!pass) {
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                unit_scale(top[r], down[r], up[r]);
               }
             }
-            __syncwarp();
-            if (pass) tc_st16(keys + 16 * q, h);
           }
-          if (!pass) unit_scale(top, down, up);
+          if (t4 == 0) {
+            sh.kscale[ds][ta] = up[0];
+            sh.kscale[ds][tb] = up[1];
+          }
         }
       } else {
-        const float* sz = scales + d.sz[ct / kMqPage] * (2 * D);
+        const char* codes = codes_of(i) + 8 * (t4 & 1);
+        const int slot_a = d.sz[page0], slot_b = d.sz[page0 + 1];  // (uniform in the warp)
+        float down[2] = {1.f, 1.f};
         if (scaled) {
-          float top = 0.f;
 #pragma unroll 1
-          for (int ch = 0; ch < D; ++ch) {
-            const float e = sz[ch], z = sz[D + ch];  // code 0: e + z; 15: 143/128 e + z
-            top = fmaxf(top, fmaxf(finite_abs(e + z), finite_abs(fmaf(143.f / 128.f, e, z))));
-          }
-          unit_scale(top, down, up);
-        }
-        uint4 next = *reinterpret_cast<const uint4*>(codes);
-#pragma unroll 2
-        for (int q = 0; q < D / 32; ++q) {  // 32 channels
-          const uint32_t wd[4] = {next.x, next.y, next.z, next.w};
-          if (q + 1 < D / 32) next = *reinterpret_cast<const uint4*>(codes + (q + 1) * 2048);
-          uint32_t h[16];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = (wd[k] & 0x0F0F0F0Fu) | 0x80808080u, hi = ((wd[k] >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
-            const float* p4 = sz + 32 * q + 8 * k;
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-              const float4 e = *reinterpret_cast<const float4*>(p4 + 2 * j);
-              const float4 z = *reinterpret_cast<const float4*>(p4 + D + 2 * j);
-              float x0, x1, x2, x3;
-              fma2(x0, x1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
-                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), e.x, e.y, z.x, z.y);
-              fma2(x2, x3, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | ((j + 1) << 8))),
-                   __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | ((j + 1) << 8))), e.z, e.w, z.z, z.w);
-              if (scaled) {
-                x0 *= down; x1 *= down; x2 *= down; x3 *= down;
-              }
-              h[4 * k + j] = pack16<INT4KV_VALUES_F16>(x0, x1);
-              h[4 * k + j + 1] = pack16<INT4KV_VALUES_F16>(x2, x3);
+          for (int p = 0; p < 2; ++p) {
+            const float* sz = scales + (p ? slot_b : slot_a) * (2 * D);
+            float top = 0.f, up;
+#pragma unroll 1
+            for (int ch = lane; ch < D; ch += 32) {
+              const float e = sz[ch], z = sz[D + ch];  // code 0: e + z; 15: 143/128 e + z
+              top = fmaxf(top, fmaxf(finite_abs(e + z), finite_abs(fmaf(143.f / 128.f, e, z))));
             }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            unit_scale(top, down[p], up);
+            if (lane < kMqPage) sh.kscale[ds][(page0 + p) * kMqPage + lane] = up;
           }
-          tc_st16(keys + 16 * q, h);
+        }
+#pragma unroll 1
+        for (int blk = 0; blk < D / 64; ++blk) {
+          float e[16], z[16];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            if (p == 0 || slot_b != slot_a || scaled) {
+              const float* sz = scales + (p ? slot_b : slot_a) * (2 * D) + 64 * blk + 16 * t4;
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(sz + j);
+                const float4 y = *reinterpret_cast<const float4*>(sz + D + j);
+                e[j] = x.x; e[j + 1] = x.y; e[j + 2] = x.z; e[j + 3] = x.w;
+                z[j] = y.x; z[j + 1] = y.y; z[j + 2] = y.z; z[j + 3] = y.w;
+              }
+              if (scaled) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  e[j] *= down[p];
+                  z[j] *= down[p];
+                }
+              }
+            }
+            uint32_t h[16];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int t = (page0 + p) * kMqPage + g + 8 * r;
+              // 16 channels: 8 bytes, half of the row's 16-byte piece 2 blk + t4 / 2
+              const uint2 wd =
+                  *reinterpret_cast<const uint2*>(codes + t * kRow + (((2 * blk + (t4 >> 1)) ^ swizzle(t)) << 4));
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t w4 = k ? wd.y : wd.x;
+                const uint32_t lo = (w4 & 0x0F0F0F0Fu) | 0x80808080u, hi = ((w4 >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int c = 8 * k + 2 * j;
+                  float x0, x1;
+                  fma2(x0, x1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
+                       __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), e[c], e[c + 1], z[c], z[c + 1]);
+                  h[4 * (2 * k + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x0, x1);
+                }
+              }
+            }
+            tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
+          }
         }
       }
-      if (scaled || draft) sh.kscale[ds][ct] = up;
       if (ct == 0) sh.scaled[ds] = scaled || draft;
-      const int next = i + 2;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -744,8 +826,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         mbar_arrive(&sh.kh_full[i & 1]);
         mbar_arrive(&sh.desc_empty[ds]);
       }
-      // (the thread has read its codes: their words are free)
-      if (next < n_tiles) {
+      if (T::NB == 1) named_bar_sync(bar, 128);
+      if (next < n_tiles && !ahead) {
         ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
         if (ok) prefetch(sh.desc[next % kDesc], next);
       }
@@ -753,16 +835,25 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     cp_async_wait<0>();
   } else {
     // ------------------------------------------------------------ softmax
-    constexpr int NC = T::NC;                  // rows (columns of S^T) of a thread
-    constexpr int LD = NR > 64 ? 8 : 16;       // columns per tensor-memory load (72 registers a thread at 128 rows)
+    // Logits are read as fragments: thread (g, t) of a warp holds tokens g, g + 8 of
+    // the warp's two pages and rows 8 i + 2 t, + 1, so a thread's rows are few: their
+    // references and sums stay in its registers (as broadcasts from shared memory they
+    // would cost a cycle per row and warp, as many as the exponentials do).
+    constexpr int NC = T::NC, NI = NC / 8;     // rows of the warpgroup; pairs of rows of a thread
+    constexpr int LI = NI < 4 ? NI : 4;        // pairs per load
     const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC, wt = tid % 128;
+    const int g = lane >> 2, t4 = lane & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
-    float l[NC];
+    constexpr float kNone = -1e30f;            // the reference of a row that has seen nothing
+    float nref[NI][2], l[NI][2];               // minus the references; sums
     Ring v;                                    // first value unit of the tile
     bool failed = false, started = false;      // a wait ran out; O^T of the segment holds something
 #pragma unroll
-    for (int j = 0; j < NC; ++j) l[j] = 0.f;
+    for (int j = 0; j < NI; ++j) {
+      nref[j][0] = nref[j][1] = -kNone;
+      l[j][0] = l[j][1] = 0.f;
+    }
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int ds = i % kDesc, sb = i & 1, pb = i % T::NP;
@@ -774,179 +865,198 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       const TileDesc& d = sh.desc[ds];
       const int flags = ok ? d.flags : 0, pages = ok ? d.pages : 0, sg = ok ? d.seg : 0;
       const bool draft = flags & kDraftTile, masked = flags & kMasked;
-      // the token of this thread, and (bits) the rows that see it
-      const int at = d.at[tok / kMqPage] + tok % kMqPage;
-      bool real = true;
-      uint32_t vis = 0xffffffffu;
+      // rows that see a token: a bit each, for tokens g, g + 8 of the first page and
+      // of the second
+      uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (masked) {
-        real = tok < pages * kMqPage && d.at[tok / kMqPage] >= 0 && at < (draft ? d.drafts : d.len);
-        if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
-        if (real && draft) {
-#pragma unroll 4
-          for (int j = 0; j < NC; ++j)
-            vis &= ~((uint32_t)(~(sh.word[sg][sh.draft[sg][c0 + j]] >> (at & 63)) & 1) << j);
-        }
-        if (real && a.window > 0) {
-          const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
-          if (behind >= a.sinks) {
-#pragma unroll 4
-            for (int j = 0; j < NC; ++j)
-              vis &= ~((uint32_t)(behind <= d.low_edge + sh.depth[sg][sh.draft[sg][c0 + j]]) << j);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int page = 2 * quarter + q / 2, at = d.at[page] + g + 8 * (q % 2);
+          bool real = page < pages && d.at[page] >= 0 && at < (draft ? d.drafts : d.len);
+          if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
+          uint32_t bits = real ? ~0u : 0u;
+          if (real && (draft || a.window > 0)) {
+            const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
+            const bool edge = a.window > 0 && behind >= a.sinks;
+#pragma unroll 1
+            for (int j = 0; j < 2 * NI; ++j) {
+              const int t = sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2];
+              const bool sees = (!draft || (sh.word[sg][t] >> (at & 63) & 1)) &&
+                                (!edge || behind > d.low_edge + sh.depth[sg][t]);
+              bits &= ~((uint32_t)!sees << j);
+            }
           }
+          vis[q] = bits;
         }
-        if (!real) vis = 0;
       }
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
       if (named_bar_or(bar, 128, failed)) break;
+      tc_fence_after();
       if (flags & kFirst) {
         started = false;
 #pragma unroll
-        for (int j = 0; j < NC; ++j) l[j] = 0.f;
-        if (wt < NC) {
-          sh.nref[c0 + wt] = INFINITY;
-          sh.nsub[c0 + wt] = 0.f;
+        for (int j = 0; j < NI; ++j) {
+          nref[j][0] = nref[j][1] = -kNone;
+          l[j][0] = l[j][1] = 0.f;
         }
-        named_bar_sync(bar, 128);
       }
-      tc_fence_after();
-      float f = sh.qscale[sg] * kLog2e;
-      if (sh.scaled[ds]) f = real ? f * sh.kscale[ds][tok] : 0.f;
+      float f[4];
+      f[0] = f[1] = f[2] = f[3] = sh.qscale[sg] * kLog2e;
+      if (sh.scaled[ds]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f[q] *= sh.kscale[ds][quarter * 32 + 8 * q + g];
+      }
       const uint32_t s_addr = tm + lanes + sb * NR + c0;
 
       // pass 1: does some logit exceed its row's reference by more than kLazy?
       float over = -INFINITY;
 #pragma unroll
-      for (int j0 = 0; j0 < NC; j0 += LD) {
-        uint32_t x[LD];
-        tc_ld<LD>(x, s_addr + j0);
+      for (int j0 = 0; j0 < NI; j0 += LI) {
+        uint32_t x[2][4 * LI];
+        tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
 #pragma unroll
-        for (int j = 0; j < LD; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(&sh.nref[c0 + j0 + j]);
-          float y[4];
-          fma2(y[0], y[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, m.x, m.y);
-          fma2(y[2], y[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, m.z, m.w);
-          if (masked) {
+        for (int j = 0; j < LI; ++j) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (!(vis >> (j0 + j + q) & 1)) y[q] = -INFINITY;
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* xx = &x[q / 2][4 * j + 2 * (q % 2)];
+            float y0, y1;
+            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
+            if (masked) {
+              if (!(vis[q] >> (2 * (j0 + j)) & 1)) y0 = -INFINITY;
+              if (!(vis[q] >> (2 * (j0 + j) + 1) & 1)) y1 = -INFINITY;
+            }
+            over = fmax3f(over, y0, y1);
           }
-          over = fmax3f(fmax3f(over, y[0], y[1]), y[2], y[3]);
         }
       }
       if (named_bar_or(bar, 128, over > kLazy)) {
         // raise the references to the true maxima, rescale sums and outputs
-#pragma unroll 1
-        for (int j0 = 0; j0 < NC; j0 += 8) {
-          uint32_t x[8];
-          tc_ld<8>(x, s_addr + j0);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float y = __uint_as_float(x[j]) * f;
-            if (!(vis >> (j0 + j) & 1)) y = -INFINITY;
-            const uint32_t k = __reduce_max_sync(0xffffffffu, ordered_key(fmaxf(y, -INFINITY)));
-            if (lane == j) sh.part[quarter][c0 + j0 + j] = from_ordered_key(k);
+        for (int j0 = 0; j0 < NI; j0 += LI) {
+          uint32_t x[2][4 * LI];
+          tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
+#pragma unroll
+          for (int j = 0; j < LI; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float m = kNone;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const float y = __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q];
+                if (vis[q] >> (2 * (j0 + j) + e) & 1) m = fmaxf(m, y);
+              }
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              if (g == 0) sh.part[quarter][c0 + 8 * (j0 + j) + 2 * t4 + e] = m;
+            }
           }
-        }
-        named_bar_sync(bar, 128);
-        if (wt < NC) {
-          const int r = c0 + wt;
-          const float old = -sh.nref[r];
-          const float m = fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
-          sh.nref[r] = -m;
-          sh.nsub[r] = m == -INFINITY ? 0.f : -m;
-          sh.alpha[r] = m == -INFINITY ? 1.f : exp2_fast(old - m);
         }
         if (started)  // the weights of tile i - 1 have been multiplied
           failed |= !tc_wait(&sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
+        tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < NC; ++j) l[j] *= sh.alpha[c0 + j];
-        if (started) {
-          tc_fence_after();
-#pragma unroll 1
-          for (int j0 = 0; j0 < T::NO * NC; j0 += 8) {
-            uint32_t x[8];
-            const int col = j0 % NC;
-            const uint32_t at_o = tm + lanes + T::COLS_O + (j0 / NC) * NR + c0 + col;
-            tc_ld<8>(x, at_o);
+        for (int j0 = 0; j0 < NI; j0 += LI) {
+          float al[LI][2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * sh.alpha[c0 + col + j]);
-            tc_st8(at_o, x);
+          for (int j = 0; j < LI; ++j) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = c0 + 8 * (j0 + j) + 2 * t4 + e;
+              const float old = -nref[j0 + j][e];
+              const float m =
+                  fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
+              al[j][e] = exp2_fast(old - m);
+              nref[j0 + j][e] = -m;
+              l[j0 + j][e] *= al[j][e];
+            }
           }
+          if (started) {
+#pragma unroll 1
+            for (int o = 0; o < T::NO; ++o) {
+              const uint32_t at_o = tm + lanes + T::COLS_O + o * NR + c0 + 8 * j0;
+              uint32_t x[2][4 * LI];
+              tc_ld_frag(x[0], x[1], at_o);
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int k = 0; k < 4 * LI; ++k) x[q][k] = __float_as_uint(__uint_as_float(x[q][k]) * al[k / 4][k % 2]);
+                tc_st_frag(at_o + ((uint32_t)(16 * q) << 16), x[q]);
+              }
+            }
+          }
+        }
+        if (started) {
           tc_wait_st();
           tc_fence_before();
         }
       }
       // pass 2: weights
       failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP + 1) & 1, a.status);
-      char* prow = smem + T::P_OFF + pb * T::P + tok * 128;
+      char* prow = smem + T::P_OFF + pb * T::P + (quarter * 32 + g) * 128 + 4 * t4;
 #pragma unroll
-      for (int j0 = 0; j0 < NC; j0 += LD) {
-        uint32_t x[LD], h[LD / 2];
-        tc_ld<LD>(x, s_addr + j0);
+      for (int j0 = 0; j0 < NI; j0 += LI) {
+        uint32_t x[2][4 * LI];
+        tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
 #pragma unroll
-        for (int j = 0; j < LD; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(&sh.nsub[c0 + j0 + j]);
-          float e[4];
-          fma2(e[0], e[1], __uint_as_float(x[j]), __uint_as_float(x[j + 1]), f, f, m.x, m.y);
-          fma2(e[2], e[3], __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]), f, f, m.z, m.w);
+        for (int j = 0; j < LI; ++j) {
+          const int col = c0 + 8 * (j0 + j);
+          char* at = prow + (col / 64) * (kTile * 128) + (((col / 8) % 8 ^ g) << 4);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) e[q] = exp2_fast(e[q]);
-          if (masked) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (!(vis >> (j0 + j + q) & 1)) e[q] = 0.f;
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t* xx = &x[q / 2][4 * j + 2 * (q % 2)];
+            float y0, y1;
+            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
+            y0 = exp2_fast(y0);
+            y1 = exp2_fast(y1);
+            if (masked) {
+              if (!(vis[q] >> (2 * (j0 + j)) & 1)) y0 = 0.f;
+              if (!(vis[q] >> (2 * (j0 + j) + 1) & 1)) y1 = 0.f;
+            }
+            add2_rn(l[j0 + j][0], l[j0 + j][1], l[j0 + j][0], l[j0 + j][1], y0, y1);
+            *reinterpret_cast<uint32_t*>(at + q * 8 * 128) = pack16<VK>(y0, y1);
           }
-          add2_rn(l[j0 + j], l[j0 + j + 1], l[j0 + j], l[j0 + j + 1], e[0], e[1]);
-          add2_rn(l[j0 + j + 2], l[j0 + j + 3], l[j0 + j + 2], l[j0 + j + 3], e[2], e[3]);
-          h[j / 2] = pack16<VK>(e[0], e[1]);
-          h[j / 2 + 1] = pack16<VK>(e[2], e[3]);
-        }
-#pragma unroll
-        for (int j = 0; j < LD; j += 8) {
-          const int col = c0 + j0 + j;
-          *reinterpret_cast<uint4*>(prow + (col / 64) * (kTile * 128) + (((col / 8) % 8 ^ (tok & 7)) << 4)) =
-              make_uint4(h[j / 2], h[j / 2 + 1], h[j / 2 + 2], h[j / 2 + 3]);
         }
       }
       // Values that no row sees must not reach the product (0 * NaN): cleared.
       // A drafted value that is not finite is taken out too and added for the
       // rows that see it when the stream ends.
-      if (masked && wg == 0 && tok < pages * kMqPage && (!real || draft)) {
-        Ring u = v;
+      if (masked && wg == 0 && tok < pages * kMqPage) {
+        const int at = d.at[tok / kMqPage] + tok % kMqPage;
+        bool real = d.at[tok / kMqPage] >= 0 && at < (draft ? d.drafts : d.len);
+        if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
+        if (!real || draft) {
+          Ring u = v;
 #pragma unroll 1
-        for (int k = tok / (kMqPage * T::PPU); k > 0; --k) u.next<T::NV>();
-        failed |= !tc_wait(&sh.v_full[u.s], u.ph, a.status);
-        char* row = smem + T::V_OFF + u.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
-        bool bad = false;
+          for (int k = tok / (kMqPage * T::PPU); k > 0; --k) u.next<T::NV>();
+          failed |= !tc_wait(&sh.v_full[u.s], u.ph, a.status);
+          char* row = smem + T::V_OFF + u.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+          bool bad = false;
 #pragma unroll 1
-        for (int q = 0; q < 8 * T::CH; ++q) {
-          uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
-          uint4 y = make_uint4(0, 0, 0, 0);
-          bool hit = !real;
-          if (real) {
-            y = *at16;
-            uint32_t e[4] = {y.x, y.y, y.z, y.w};
-            constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
+          for (int q = 0; q < 8 * T::CH; ++q) {
+            uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
+            uint4 y = make_uint4(0, 0, 0, 0);
+            bool hit = !real;
+            if (real) {
+              y = *at16;
+              uint32_t e[4] = {y.x, y.y, y.z, y.w};
+              constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-              if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
+              for (int k = 0; k < 4; ++k) {
+                if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
+                if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
+              }
+              bad |= hit;
+              y = make_uint4(e[0], e[1], e[2], e[3]);
             }
-            bad |= hit;
-            y = make_uint4(e[0], e[1], e[2], e[3]);
+            if (hit) *at16 = y;
           }
-          if (hit) *at16 = y;
+          if (bad) atomicOr(&sh.odd[sg], 1ull << (at & 63));
         }
-        if (bad) atomicOr(&sh.odd[sg], 1ull << (at & 63));
       }
-      if (masked) {
 #pragma unroll 1
-        for (int g = 0; g < pages; g += T::PPU) v.next<T::NV>();
-      } else {
-        v.s += kTilePages / T::PPU;
-        if (v.s >= T::NV) { v.s -= T::NV; v.ph ^= 1; }
-      }
+      for (int k = 0; k < pages; k += T::PPU) v.next<T::NV>();
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
@@ -959,34 +1069,37 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       started = true;
       if (last) {
         // ---- epilogue: O^T, a lane a channel, over the sums of the weights ----
-        // Each step of the butterfly halves the rows a lane holds: it ends with
-        // the sum over the warp's tokens of row NC k / 32.
 #pragma unroll
-        for (int st = 0; st < 5; ++st) {
-          const int o = 16 >> st, half = (NC >> st) / 2;
-          if (half >= 1) {
+        for (int j = 0; j < NI; ++j) {
 #pragma unroll
-            for (int j = 0; j < half; ++j) {
-              const bool up = lane & o;
-              const float send = up ? l[j] : l[j + half], keep = up ? l[j + half] : l[j];
-              l[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+          for (int e = 0; e < 2; ++e) {
+            float x = l[j][e];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const int r = c0 + 8 * j + 2 * t4 + e;
+            if (g == 0) {
+              sh.part[quarter][r] = x;
+              if (quarter == 0) sh.ref[r] = -nref[j][e];
             }
-          } else {
-            l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
           }
         }
-        sh.part[quarter][c0 + lane * NC / 32] = l[0];
         // (the product waited for every warp's weights: the list of odd values is complete)
         failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
+        const bool whole = flags & kWhole;
+        float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
         if (wt < NC) {
           const int r = c0 + wt;
-          sh.alpha[r] = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+          const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+          sh.sum[r] = 1.f / fmaxf(sum, 1e-10f);
+          if (!whole) {
+            rec[r] = sh.ref[r] > kNone ? sh.ref[r] * 0.6931471805599453f : (sh.ref[r] == kNone ? -INFINITY : sh.ref[r]);
+            rec[NR + r] = sum;
+          }
         }
         named_bar_sync(bar, 128);
         tc_fence_after();
-        const bool whole = flags & kWhole;
-        float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
         const unsigned long long odd = sh.odd[sg];
 #pragma unroll 1
         for (int j0 = 0; j0 < NC; j0 += 8) {
@@ -995,7 +1108,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           for (int o = 0; o < T::NO; ++o) {
             const int ch = o * 128 + tok;
             uint32_t x[8];
-            tc_ld<8>(x, tm + lanes + T::COLS_O + o * NR + col);
+            tc_ld8(x, tm + lanes + T::COLS_O + o * NR + col);
             if (ch >= D) continue;
 #pragma unroll 1
             for (unsigned long long left = odd; left; left &= left - 1) {
@@ -1017,18 +1130,13 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             for (int j = 0; j < 8; ++j) {
               const int r = col + j, rr = d.first_row + r;
               if (rr >= d.rows) continue;
-              const float y = __uint_as_float(x[j]), sum = sh.alpha[r];
+              const float y = __uint_as_float(x[j]);
               if (whole) {
                 const size_t to = out_row(a, d.row0, d.head, sh.draft[sg][r], rr) * D + ch;
-                const float q = y * (1.f / fmaxf(sum, 1e-10f));
-                if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(q);
-                else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(q);
+                if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.sum[r]);
+                else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.sum[r]);
               } else {
                 rec[2 * NR + r * D + ch] = y;
-                if (ch == 0) {
-                  rec[r] = -sh.nref[r] * 0.6931471805599453f;
-                  rec[NR + r] = sum;
-                }
               }
             }
           }
