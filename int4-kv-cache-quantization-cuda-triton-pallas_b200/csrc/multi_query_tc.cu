@@ -302,6 +302,433 @@ I4KV_DEVINL size_t out_row(const MultiQueryArgs& a, int row0, int head, int t, i
   return ((size_t)(row0 + t) * a.kv_heads + head) * a.group_q + (rr - t * a.group_q);
 }
 
+// ---- What runs once per stream, or rarely: kept out of the roles' loops, whose
+// code has to fit the instruction caches side by side (with all of it in line the
+// warps spent half of their time waiting for instructions). ----
+
+// A stream's drafts and rows, for one warp; returns the deepest draft's ancestors.
+template <int NR>
+__device__ __noinline__ int describe_rows(const MultiQueryArgs& a, TcShared<NR>& sh, const SeqWork& w, int chunk, int sg,
+                                          int lane) {
+  int top = 0;
+#pragma unroll 1
+  for (int t = lane; t < max(w.drafts, 1); t += 32) {
+    const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
+    const int dp = a.mask ? draft_depth(word, t, w.drafts) : 0;
+    sh.word[sg][t] = word;
+    sh.depth[sg][t] = dp;
+    top = max(top, dp);
+  }
+#pragma unroll 1
+  for (int r = lane; r < NR; r += 32) sh.draft[sg][r] = (uint8_t)(min(chunk * NR + r, w.rows - 1) / a.group_q);
+  return __reduce_max_sync(0xffffffffu, top);
+}
+
+// A stream's queries to shared memory, by a conversion group: as they are, for a
+// magnitude below float16's range loses nothing that a logit could show. Only one
+// above it (a bfloat16 input) takes the second pass, with a common power of two. A
+// thread takes 8 channels of a row.
+template <int D, int NR, int VK>
+__device__ __noinline__ void load_queries(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, char* q_smem, int ct,
+                                          int grp, int bar) {
+  float top = 0.f, down = 1.f, up = 1.f;
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+#pragma unroll 4
+    for (int k = ct; k < NR * (D / 8); k += 128) {
+      const int r = k / (D / 8), c8 = k % (D / 8), rr = d.first_row + r;
+      uint32_t h[4] = {0, 0, 0, 0};
+      if (rr < d.rows) {
+        float x[8];
+        load8<VK>(a.q, out_row(a, d.row0, d.head, sh.draft[d.seg][r], rr) * D + 8 * c8, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (VK == INT4KV_VALUES_BF16) top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+          h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+        }
+      }
+      // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
+      char* row = q_smem + (c8 / 8) * (NR * 128) + r * 128;
+      const int q = c8 % 8 / 2, j = c8 % 2 * 2;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const int at = 32 * (j + o) + 8 * q;  // byte of the row
+        *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
+      }
+    }
+    if (VK == INT4KV_VALUES_F16 || pass == 1) break;
+    if (!named_bar_or(bar, 128, top > kHalfRoom)) break;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (ct % 32 == 0) sh.qmax[grp][ct / 32] = top;
+    named_bar_sync(bar, 128);
+    top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
+    named_bar_sync(bar, 128);  // qmax is free again
+    unit_scale(top, down, up);
+  }
+  if (ct == 0) sh.qscale[d.seg] = up;
+  fence_proxy_async_smem();
+}
+
+// Keys, by a conversion group: thread (g, t) of a warp takes tokens g, g + 8 of each
+// of the warp's two pages and 16 channels 64 b + 16 t of each block b of 64: its
+// parameters stay in registers over the tokens, and the fragments go to tensor
+// memory as they are. Rows of codes are swizzled by 16 bytes, as the threads of a
+// warp read 8 rows at a time.
+template <int D>
+I4KV_DEVINL int code_swizzle(int t) {
+  return D == 64 ? (t >> 2 & 1) : (D == 128 ? (t >> 1 & 3) : (t & 7));
+}
+template <int D, bool SCALED>
+I4KV_DEVINL void convert_keys(const TileDesc& d, const char* codes, const float* scales, uint32_t keys, int ct, float down_a,
+                              float down_b) {
+  const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
+  const int slot_a = d.sz[page0], slot_b = d.sz[page0 + 1];  // (uniform in the warp)
+#pragma unroll 1
+  for (int blk = 0; blk < D / 64; ++blk) {
+    float e[16], z[16];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (p == 0 || slot_b != slot_a || SCALED) {
+        const float* sz = scales + (p ? slot_b : slot_a) * (2 * D) + 64 * blk + 16 * t4;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(sz + j);
+          const float4 y = *reinterpret_cast<const float4*>(sz + D + j);
+          e[j] = x.x; e[j + 1] = x.y; e[j + 2] = x.z; e[j + 3] = x.w;
+          z[j] = y.x; z[j + 1] = y.y; z[j + 2] = y.z; z[j + 3] = y.w;
+        }
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            e[j] *= p ? down_b : down_a;
+            z[j] *= p ? down_b : down_a;
+          }
+        }
+      }
+      uint32_t h[16];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int t = (page0 + p) * kMqPage + g + 8 * r;
+        // 16 channels: 8 bytes, half of the row's 16-byte piece 2 blk + t4 / 2
+        const uint2 wd = *reinterpret_cast<const uint2*>(codes + t * (D / 2) + 8 * (t4 & 1) +
+                                                         (((2 * blk + (t4 >> 1)) ^ code_swizzle<D>(t)) << 4));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t w4 = k ? wd.y : wd.x;
+          const uint32_t lo = (w4 & 0x0F0F0F0Fu) | 0x80808080u, hi = ((w4 >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = 8 * k + 2 * j;
+            float x0, x1;
+            fma2(x0, x1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
+                 __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), e[c], e[c + 1], z[c], z[c + 1]);
+            h[4 * (2 * k + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x0, x1);
+          }
+        }
+      }
+      tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
+    }
+  }
+}
+
+// The same with a power of two per group, for keys beyond float16's range.
+template <int D, int NR>
+__device__ __noinline__ void convert_scaled(TcShared<NR>& sh, const TileDesc& d, int ds, const char* codes, const float* scales,
+                                            uint32_t keys, int ct) {
+  const int lane = ct & 31, page0 = (ct >> 5) * 2;
+  float down[2];
+#pragma unroll 1
+  for (int p = 0; p < 2; ++p) {
+    const float* sz = scales + d.sz[page0 + p] * (2 * D);
+    float top = 0.f, dn, up;
+#pragma unroll 1
+    for (int ch = lane; ch < D; ch += 32) {
+      const float e = sz[ch], z = sz[D + ch];  // code 0: e + z; 15: 143/128 e + z
+      top = fmaxf(top, fmaxf(finite_abs(e + z), finite_abs(fmaf(143.f / 128.f, e, z))));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    unit_scale(top, dn, up);
+    if (p == 0) down[0] = dn; else down[1] = dn;
+    if (lane < kMqPage) sh.kscale[ds][(page0 + p) * kMqPage + lane] = up;
+  }
+  convert_keys<D, true>(d, codes, scales, keys, ct, down[0], down[1]);
+}
+
+// Drafted keys, with a power of two each.
+template <int D, int NR, int VK>
+__device__ __noinline__ void draft_keys(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, int ds, uint32_t keys,
+                                        int ct) {
+  const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
+#pragma unroll 1
+  for (int p = 0; p < 2; ++p) {
+    const int ta = (page0 + p) * kMqPage + g, tb = ta + 8;
+    float top[2] = {0.f, 0.f}, down[2] = {1.f, 1.f}, up[2] = {1.f, 1.f};
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // the rows' scales, then their keys
+#pragma unroll 1
+      for (int blk = 0; blk < D / 64; ++blk) {
+        uint32_t h[16];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int t = r ? tb : ta;
+          const size_t row = ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 64 * blk + 16 * t4;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (t < d.drafts) load8<VK>(a.kd, row + 8 * e, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              top[r] = fmaxf(top[r], fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+              // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
+              h[4 * (2 * e + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
+            }
+          }
+        }
+        __syncwarp();
+        if (pass) tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
+      }
+      if (!pass) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          unit_scale(top[r], down[r], up[r]);
+        }
+      }
+    }
+    if (t4 == 0) {
+      sh.kscale[ds][ta] = up[0];
+      sh.kscale[ds][tb] = up[1];
+    }
+  }
+}
+
+// Whether some row sees the token `at` of a tile at all (a cached one).
+I4KV_DEVINL bool token_real(const MultiQueryArgs& a, const TileDesc& d, int page, int at) {
+  const bool draft = d.flags & kDraftTile;
+  const bool here = page < d.pages && d.at[page] >= 0 && at < (draft ? d.drafts : d.len);
+  return here && (draft || a.window == 0 || at > d.low_edge || at < a.sinks);
+}
+
+// Rows that see a thread's tokens, a bit each: tokens g, g + 8 of the warp's first
+// page and of its second; bit j is row c0 + 8 (j / 2) + 2 t + j % 2.
+template <int NR>
+__device__ __noinline__ uint4 visible_rows(const MultiQueryArgs& a, const TcShared<NR>& sh, const TileDesc& d, int c0,
+                                           int quarter, int lane, int pairs) {
+  const int g = lane >> 2, t4 = lane & 3, sg = d.seg;
+  const bool draft = d.flags & kDraftTile;
+  uint32_t vis[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int page = 2 * quarter + q / 2, at = d.at[page] + g + 8 * (q % 2);
+    const bool real = token_real(a, d, page, at);
+    uint32_t bits = real ? ~0u : 0u;
+    if (real && (draft || a.window > 0)) {
+      const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
+      const bool edge = a.window > 0 && behind >= a.sinks;
+#pragma unroll 1
+      for (int j = 0; j < 2 * pairs; ++j) {
+        const int t = sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2];
+        const bool sees =
+            (!draft || (sh.word[sg][t] >> (at & 63) & 1)) && (!edge || behind > d.low_edge + sh.depth[sg][t]);
+        bits &= ~((uint32_t)!sees << j);
+      }
+    }
+    vis[q] = bits;
+  }
+  __syncwarp();
+  return make_uint4(vis[0], vis[1], vis[2], vis[3]);
+}
+
+// A softmax thread's rows: minus the references, and the sums.
+template <int NI>
+struct RowState {
+  float nref[NI][2], l[NI][2];
+  bool failed;
+};
+constexpr float kNoRef = -1e30f;  // the reference of a row that has seen nothing
+
+// Raise the references to the true maxima of the tile, rescale sums and outputs.
+// `prev`: the barrier of the last tile's weights (0: O^T holds nothing yet).
+template <int D, int NR>
+__device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const MultiQueryArgs& a, TcShared<NR>& sh,
+                                                                     RowState<Tc<D, NR>::NC / 8> s, uint4 vis4, float4 f4,
+                                                                     uint32_t s_addr, uint32_t o_addr, int c0, int quarter,
+                                                                     int lane, uint64_t* prev, uint32_t parity, int bar) {
+  using T = Tc<D, NR>;
+  constexpr int NI = T::NC / 8, LI = NI < 4 ? NI : 4;
+  const int g = lane >> 2, t4 = lane & 3;
+  const uint32_t vis[4] = {vis4.x, vis4.y, vis4.z, vis4.w};
+  const float f[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+  for (int j0 = 0; j0 < NI; j0 += LI) {
+    uint32_t x[2][4 * LI];
+    tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
+#pragma unroll
+    for (int j = 0; j < LI; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float m = kNoRef;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float y = __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q];
+          if (vis[q] >> (2 * (j0 + j) + e) & 1) m = fmaxf(m, y);
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        if (g == 0) sh.part[quarter][c0 + 8 * (j0 + j) + 2 * t4 + e] = m;
+      }
+    }
+  }
+  s.failed = prev && !tc_wait(prev, parity, a.status);  // the weights of tile i - 1 have been multiplied
+  named_bar_sync(bar, 128);
+  tc_fence_after();
+#pragma unroll
+  for (int j0 = 0; j0 < NI; j0 += LI) {
+    float al[LI][2];
+#pragma unroll
+    for (int j = 0; j < LI; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = c0 + 8 * (j0 + j) + 2 * t4 + e;
+        const float old = -s.nref[j0 + j][e];
+        const float m = fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
+        al[j][e] = exp2_fast(old - m);
+        s.nref[j0 + j][e] = -m;
+        s.l[j0 + j][e] *= al[j][e];
+      }
+    }
+    if (prev) {
+#pragma unroll 1
+      for (int o = 0; o < T::NO; ++o) {
+        const uint32_t at_o = o_addr + o * NR + 8 * j0;
+        uint32_t x[2][4 * LI];
+        tc_ld_frag(x[0], x[1], at_o);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+          for (int k = 0; k < 4 * LI; ++k) x[q][k] = __float_as_uint(__uint_as_float(x[q][k]) * al[k / 4][k % 2]);
+          tc_st_frag(at_o + ((uint32_t)(16 * q) << 16), x[q]);
+        }
+      }
+    }
+  }
+  if (prev) {
+    tc_wait_st();
+    tc_fence_before();
+  }
+  return s;
+}
+
+// Values that no row sees must not reach the product (0 * NaN): cleared. A drafted
+// value that is not finite is taken out too and added for the rows that see it when
+// the stream ends. One thread a token; `v` is the tile's first value unit.
+template <int D, int NR, int VK>
+__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, char* v_smem, Ring v,
+                                          int tok) {
+  using T = Tc<D, NR>;
+  bool ok = true;
+  const int at = d.at[tok / kMqPage] + tok % kMqPage;
+  const bool draft = d.flags & kDraftTile, real = token_real(a, d, tok / kMqPage, at);
+  if (tok < d.pages * kMqPage && (!real || draft)) {
+#pragma unroll 1
+    for (int k = tok / (kMqPage * T::PPU); k > 0; --k) v.next<T::NV>();
+    ok = tc_wait(&sh.v_full[v.s], v.ph, a.status);
+    char* row = v_smem + v.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+    bool bad = false;
+#pragma unroll 1
+    for (int q = 0; q < 8 * T::CH; ++q) {
+      uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
+      uint4 y = make_uint4(0, 0, 0, 0);
+      bool hit = !real;
+      if (real) {
+        y = *at16;
+        uint32_t e[4] = {y.x, y.y, y.z, y.w};
+        constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
+          if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
+        }
+        bad |= hit;
+        y = make_uint4(e[0], e[1], e[2], e[3]);
+      }
+      if (hit) *at16 = y;
+    }
+    if (bad) atomicOr(&sh.odd[d.seg], 1ull << (at & 63));
+  }
+  __syncwarp();
+  return ok;
+}
+
+// A stream's (or a run's share of it) end, by one softmax warpgroup: the sums of its
+// warps are in sh.part, its products are done. O^T, a lane a channel, over the sums,
+// or as a record.
+template <int D, int NR, int VK>
+__device__ __noinline__ void finish_stream(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, uint32_t tm, int c0,
+                                           int tok, int bar) {
+  using T = Tc<D, NR>;
+  const bool whole = d.flags & kWhole;
+  const int sg = d.seg;
+  float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
+  if (tok < T::NC) {
+    const int r = c0 + tok;
+    const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
+    sh.sum[r] = 1.f / fmaxf(sum, 1e-10f);
+    if (!whole) {
+      rec[r] = sh.ref[r] == kNoRef ? -INFINITY : sh.ref[r] * 0.6931471805599453f;
+      rec[NR + r] = sum;
+    }
+  }
+  named_bar_sync(bar, 128);
+  tc_fence_after();
+  const unsigned long long odd = sh.odd[sg];
+#pragma unroll 1
+  for (int j0 = 0; j0 < T::NC; j0 += 8) {
+    const int col = c0 + j0;
+#pragma unroll 1
+    for (int o = 0; o < T::NO; ++o) {
+      const int ch = o * 128 + tok;
+      uint32_t x[8];
+      tc_ld8(x, tm + T::COLS_O + o * NR + col);
+      if (ch >= D) continue;
+#pragma unroll 1
+      for (unsigned long long left = odd; left; left &= left - 1) {
+        const int u = __ffsll(left) - 1;
+        float y2[2];
+        load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
+        const float y = ch & 1 ? y2[1] : y2[0];
+        if (fabsf(y) <= 3.4e38f) continue;
+        const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int t = sh.draft[sg][col + j];
+          if ((sh.word[sg][t] >> u & 1) && (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
+            x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = col + j, rr = d.first_row + r;
+        if (rr >= d.rows) continue;
+        const float y = __uint_as_float(x[j]);
+        if (whole) {
+          const size_t to = out_row(a, d.row0, d.head, sh.draft[sg][r], rr) * D + ch;
+          if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.sum[r]);
+          else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.sum[r]);
+        } else {
+          rec[2 * NR + r * D + ch] = y;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+}
+
 template <int D, int NR, int VK>
 __global__ void __launch_bounds__(Tc<D, NR>::THREADS, 1)
 multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_constant__ CUtensorMap vmap,
@@ -392,21 +819,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         const bool first = i == 0 || p.tile == 0;
         if (first) {
           ++seg;
-          const int sg = seg % kDesc;
-          int top = 0;
-#pragma unroll 1
-          for (int t = lane; t < max(w.drafts, 1); t += 32) {
-            const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
-            const int dp = a.mask ? draft_depth(word, t, w.drafts) : 0;
-            sh.word[sg][t] = word;
-            sh.depth[sg][t] = dp;
-            top = max(top, dp);
-          }
-          top = __reduce_max_sync(0xffffffffu, top);
-          high_edge = w.pos0 + top - a.window;
-#pragma unroll 1
-          for (int r = lane; r < NR; r += 32)
-            sh.draft[sg][r] = (uint8_t)(min(p.chunk * NR + r, w.rows - 1) / a.group_q);
+          high_edge = w.pos0 + describe_rows(a, sh, w, p.chunk, seg % kDesc, lane) - a.window;
         }
         int at = -1;
         bool clean = lane >= here;  // every row sees all of the page
@@ -584,7 +997,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // the threads of a warp read 8 rows at a time.
     constexpr int kRow = D / 2;  // bytes of a row of codes
     auto codes_of = [&](int i) { return smem + T::KC_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::KC; };
-    auto swizzle = [](int t) { return D == 64 ? (t >> 2 & 1) : (D == 128 ? (t >> 1 & 3) : (t & 7)); };
     auto scales_of = [&](int i) {
       return reinterpret_cast<float*>(smem + T::SZ_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::SZ);
     };
@@ -594,7 +1006,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         const uint8_t* src = a.k_pool + ((size_t)slab * kMqPage + ct % kMqPage) * (D / 2);
 #pragma unroll
         for (int q = 0; q < D / 32; ++q)
-          cp_async16(codes_of(i) + ct * kRow + ((q ^ swizzle(ct)) << 4), src + 16 * q);
+          cp_async16(codes_of(i) + ct * kRow + ((q ^ code_swizzle<D>(ct)) << 4), src + 16 * q);
       }
       float* sz = scales_of(i);
 #pragma unroll 1
@@ -660,163 +1072,15 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         ahead = true;
       }
       if (flags & kFirst) {
-        // The stream's queries, as they are: a magnitude below float16's range
-        // loses nothing that a logit could show. Only one above it (a bfloat16
-        // input) takes the second pass, with a common power of two. A thread
-        // takes 8 channels of a row.
-        float top = 0.f, down = 1.f, up = 1.f;
-#pragma unroll 1
-        for (int pass = 0;; ++pass) {
-#pragma unroll 4
-          for (int k = ct; k < NR * (D / 8); k += 128) {
-            const int r = k / (D / 8), c8 = k % (D / 8), rr = d.first_row + r;
-            uint32_t h[4] = {0, 0, 0, 0};
-            if (rr < d.rows) {
-              float x[8];
-              load8<VK>(a.q, out_row(a, d.row0, d.head, sh.draft[d.seg][r], rr) * D + 8 * c8, x);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (VK == INT4KV_VALUES_BF16) top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-                h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
-              }
-            }
-            // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
-            char* row = smem + T::Q_OFF + (c8 / 8) * (NR * 128) + r * 128;
-            const int q = c8 % 8 / 2, j = c8 % 2 * 2;
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-              const int at = 32 * (j + o) + 8 * q;  // byte of the row
-              *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
-            }
-          }
-          if (VK == INT4KV_VALUES_F16 || pass == 1) break;
-          if (!named_bar_or(bar, 128, top > kHalfRoom)) break;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (lane == 0) sh.qmax[grp][ct / 32] = top;
-          named_bar_sync(bar, 128);
-          top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
-          named_bar_sync(bar, 128);  // qmax is free again
-          unit_scale(top, down, up);
-        }
-        if (ct == 0) sh.qscale[d.seg] = up;
-        fence_proxy_async_smem();
+        load_queries<D, NR, VK>(a, sh, d, smem + T::Q_OFF, ct, grp, bar);
       }
-      // Keys: thread (g, t) of a warp takes tokens g, g + 8 of each of the warp's two
-      // pages and 16 channels 64 b + 16 t of each block b of 64: its parameters stay
-      // in registers over the tokens, and the fragments go to tensor memory as they are.
       const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
-      const int g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
       if (draft) {
-#pragma unroll 1
-        for (int p = 0; p < 2; ++p) {
-          const int ta = (page0 + p) * kMqPage + g, tb = ta + 8;
-          float top[2] = {0.f, 0.f}, down[2] = {1.f, 1.f}, up[2] = {1.f, 1.f};
-#pragma unroll 1
-          for (int pass = 0; pass < 2; ++pass) {  // the rows' scales, then their keys
-#pragma unroll 1
-            for (int blk = 0; blk < D / 64; ++blk) {
-              uint32_t h[16];
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const int t = r ? tb : ta;
-                const size_t row = ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 64 * blk + 16 * t4;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                  if (t < d.drafts) load8<VK>(a.kd, row + 8 * e, x);
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    top[r] = fmaxf(top[r], fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-                    // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
-                    h[4 * (2 * e + j / 2) + 2 * r + j % 2] =
-                        pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
-                  }
-                }
-              }
-              __syncwarp();
-              if (pass) tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
-            }
-            if (!pass) {
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                unit_scale(top[r], down[r], up[r]);
-              }
-            }
-          }
-          if (t4 == 0) {
-            sh.kscale[ds][ta] = up[0];
-            sh.kscale[ds][tb] = up[1];
-          }
-        }
+        draft_keys<D, NR, VK>(a, sh, d, ds, keys, ct);
       } else {
-        const char* codes = codes_of(i) + 8 * (t4 & 1);
-        const int slot_a = d.sz[page0], slot_b = d.sz[page0 + 1];  // (uniform in the warp)
-        float down[2] = {1.f, 1.f};
-        if (scaled) {
-#pragma unroll 1
-          for (int p = 0; p < 2; ++p) {
-            const float* sz = scales + (p ? slot_b : slot_a) * (2 * D);
-            float top = 0.f, up;
-#pragma unroll 1
-            for (int ch = lane; ch < D; ch += 32) {
-              const float e = sz[ch], z = sz[D + ch];  // code 0: e + z; 15: 143/128 e + z
-              top = fmaxf(top, fmaxf(finite_abs(e + z), finite_abs(fmaf(143.f / 128.f, e, z))));
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            unit_scale(top, down[p], up);
-            if (lane < kMqPage) sh.kscale[ds][(page0 + p) * kMqPage + lane] = up;
-          }
-        }
-#pragma unroll 1
-        for (int blk = 0; blk < D / 64; ++blk) {
-          float e[16], z[16];
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            if (p == 0 || slot_b != slot_a || scaled) {
-              const float* sz = scales + (p ? slot_b : slot_a) * (2 * D) + 64 * blk + 16 * t4;
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(sz + j);
-                const float4 y = *reinterpret_cast<const float4*>(sz + D + j);
-                e[j] = x.x; e[j + 1] = x.y; e[j + 2] = x.z; e[j + 3] = x.w;
-                z[j] = y.x; z[j + 1] = y.y; z[j + 2] = y.z; z[j + 3] = y.w;
-              }
-              if (scaled) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  e[j] *= down[p];
-                  z[j] *= down[p];
-                }
-              }
-            }
-            uint32_t h[16];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int t = (page0 + p) * kMqPage + g + 8 * r;
-              // 16 channels: 8 bytes, half of the row's 16-byte piece 2 blk + t4 / 2
-              const uint2 wd =
-                  *reinterpret_cast<const uint2*>(codes + t * kRow + (((2 * blk + (t4 >> 1)) ^ swizzle(t)) << 4));
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const uint32_t w4 = k ? wd.y : wd.x;
-                const uint32_t lo = (w4 & 0x0F0F0F0Fu) | 0x80808080u, hi = ((w4 >> 4) & 0x0F0F0F0Fu) | 0x80808080u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const int c = 8 * k + 2 * j;
-                  float x0, x1;
-                  fma2(x0, x1, __uint_as_float(__byte_perm(lo, 0x3F000000u, 0x7044u | (j << 8))),
-                       __uint_as_float(__byte_perm(hi, 0x3F000000u, 0x7044u | (j << 8))), e[c], e[c + 1], z[c], z[c + 1]);
-                  h[4 * (2 * k + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x0, x1);
-                }
-              }
-            }
-            tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
-          }
-        }
+        const char* codes = codes_of(i);
+        if (scaled) convert_scaled<D, NR>(sh, d, ds, codes, scales, keys, ct);
+        else convert_keys<D, false>(d, codes, scales, keys, ct, 1.f, 1.f);
       }
       if (ct == 0) sh.scaled[ds] = scaled || draft;
       tc_wait_st();
@@ -845,13 +1109,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
-    constexpr float kNone = -1e30f;            // the reference of a row that has seen nothing
     float nref[NI][2], l[NI][2];               // minus the references; sums
     Ring v;                                    // first value unit of the tile
     bool failed = false, started = false;      // a wait ran out; O^T of the segment holds something
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
-      nref[j][0] = nref[j][1] = -kNone;
+      nref[j][0] = nref[j][1] = -kNoRef;
       l[j][0] = l[j][1] = 0.f;
     }
 #pragma unroll 1
@@ -869,25 +1132,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       // of the second
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (masked) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int page = 2 * quarter + q / 2, at = d.at[page] + g + 8 * (q % 2);
-          bool real = page < pages && d.at[page] >= 0 && at < (draft ? d.drafts : d.len);
-          if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
-          uint32_t bits = real ? ~0u : 0u;
-          if (real && (draft || a.window > 0)) {
-            const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
-            const bool edge = a.window > 0 && behind >= a.sinks;
-#pragma unroll 1
-            for (int j = 0; j < 2 * NI; ++j) {
-              const int t = sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2];
-              const bool sees = (!draft || (sh.word[sg][t] >> (at & 63) & 1)) &&
-                                (!edge || behind > d.low_edge + sh.depth[sg][t]);
-              bits &= ~((uint32_t)!sees << j);
-            }
-          }
-          vis[q] = bits;
-        }
+        const uint4 m = visible_rows(a, sh, d, c0, quarter, lane, NI);
+        vis[0] = m.x; vis[1] = m.y; vis[2] = m.z; vis[3] = m.w;
       }
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
       if (named_bar_or(bar, 128, failed)) break;
@@ -896,7 +1142,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         started = false;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-          nref[j][0] = nref[j][1] = -kNone;
+          nref[j][0] = nref[j][1] = -kNoRef;
           l[j][0] = l[j][1] = 0.f;
         }
       }
@@ -930,66 +1176,26 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
       }
       if (named_bar_or(bar, 128, over > kLazy)) {
-        // raise the references to the true maxima, rescale sums and outputs
+        RowState<NI> rows;
 #pragma unroll
-        for (int j0 = 0; j0 < NI; j0 += LI) {
-          uint32_t x[2][4 * LI];
-          tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
+        for (int j = 0; j < NI; ++j) {
 #pragma unroll
-          for (int j = 0; j < LI; ++j) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float m = kNone;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float y = __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q];
-                if (vis[q] >> (2 * (j0 + j) + e) & 1) m = fmaxf(m, y);
-              }
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-              if (g == 0) sh.part[quarter][c0 + 8 * (j0 + j) + 2 * t4 + e] = m;
-            }
+          for (int e = 0; e < 2; ++e) {
+            rows.nref[j][e] = nref[j][e];
+            rows.l[j][e] = l[j][e];
           }
         }
-        if (started)  // the weights of tile i - 1 have been multiplied
-          failed |= !tc_wait(&sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status);
-        named_bar_sync(bar, 128);
-        tc_fence_after();
+        rows = raise_references<D, NR>(a, sh, rows, make_uint4(vis[0], vis[1], vis[2], vis[3]),
+                                       make_float4(f[0], f[1], f[2], f[3]), s_addr, tm + lanes + T::COLS_O + c0, c0, quarter,
+                                       lane, started ? &sh.p_empty[(i - 1) % T::NP] : nullptr, ((i - 1) / T::NP) & 1, bar);
+        failed |= rows.failed;
 #pragma unroll
-        for (int j0 = 0; j0 < NI; j0 += LI) {
-          float al[LI][2];
+        for (int j = 0; j < NI; ++j) {
 #pragma unroll
-          for (int j = 0; j < LI; ++j) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = c0 + 8 * (j0 + j) + 2 * t4 + e;
-              const float old = -nref[j0 + j][e];
-              const float m =
-                  fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
-              al[j][e] = exp2_fast(old - m);
-              nref[j0 + j][e] = -m;
-              l[j0 + j][e] *= al[j][e];
-            }
+          for (int e = 0; e < 2; ++e) {
+            nref[j][e] = rows.nref[j][e];
+            l[j][e] = rows.l[j][e];
           }
-          if (started) {
-#pragma unroll 1
-            for (int o = 0; o < T::NO; ++o) {
-              const uint32_t at_o = tm + lanes + T::COLS_O + o * NR + c0 + 8 * j0;
-              uint32_t x[2][4 * LI];
-              tc_ld_frag(x[0], x[1], at_o);
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-#pragma unroll
-                for (int k = 0; k < 4 * LI; ++k) x[q][k] = __float_as_uint(__uint_as_float(x[q][k]) * al[k / 4][k % 2]);
-                tc_st_frag(at_o + ((uint32_t)(16 * q) << 16), x[q]);
-              }
-            }
-          }
-        }
-        if (started) {
-          tc_wait_st();
-          tc_fence_before();
         }
       }
       // pass 2: weights
@@ -1019,42 +1225,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
       }
-      // Values that no row sees must not reach the product (0 * NaN): cleared.
-      // A drafted value that is not finite is taken out too and added for the
-      // rows that see it when the stream ends.
-      if (masked && wg == 0 && tok < pages * kMqPage) {
-        const int at = d.at[tok / kMqPage] + tok % kMqPage;
-        bool real = d.at[tok / kMqPage] >= 0 && at < (draft ? d.drafts : d.len);
-        if (!draft && a.window > 0 && at <= d.low_edge && at >= a.sinks) real = false;
-        if (!real || draft) {
-          Ring u = v;
-#pragma unroll 1
-          for (int k = tok / (kMqPage * T::PPU); k > 0; --k) u.next<T::NV>();
-          failed |= !tc_wait(&sh.v_full[u.s], u.ph, a.status);
-          char* row = smem + T::V_OFF + u.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
-          bool bad = false;
-#pragma unroll 1
-          for (int q = 0; q < 8 * T::CH; ++q) {
-            uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
-            uint4 y = make_uint4(0, 0, 0, 0);
-            bool hit = !real;
-            if (real) {
-              y = *at16;
-              uint32_t e[4] = {y.x, y.y, y.z, y.w};
-              constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-                if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
-              }
-              bad |= hit;
-              y = make_uint4(e[0], e[1], e[2], e[3]);
-            }
-            if (hit) *at16 = y;
-          }
-          if (bad) atomicOr(&sh.odd[sg], 1ull << (at & 63));
-        }
-      }
+      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, sh, d, smem + T::V_OFF, v, tok);
 #pragma unroll 1
       for (int k = 0; k < pages; k += T::PPU) v.next<T::NV>();
       fence_proxy_async_smem();
@@ -1087,62 +1258,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         // (the product waited for every warp's weights: the list of odd values is complete)
         failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
-        const bool whole = flags & kWhole;
-        float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
-        if (wt < NC) {
-          const int r = c0 + wt;
-          const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
-          sh.sum[r] = 1.f / fmaxf(sum, 1e-10f);
-          if (!whole) {
-            rec[r] = sh.ref[r] > kNone ? sh.ref[r] * 0.6931471805599453f : (sh.ref[r] == kNone ? -INFINITY : sh.ref[r]);
-            rec[NR + r] = sum;
-          }
-        }
-        named_bar_sync(bar, 128);
-        tc_fence_after();
-        const unsigned long long odd = sh.odd[sg];
-#pragma unroll 1
-        for (int j0 = 0; j0 < NC; j0 += 8) {
-          const int col = c0 + j0;
-#pragma unroll 1
-          for (int o = 0; o < T::NO; ++o) {
-            const int ch = o * 128 + tok;
-            uint32_t x[8];
-            tc_ld8(x, tm + lanes + T::COLS_O + o * NR + col);
-            if (ch >= D) continue;
-#pragma unroll 1
-            for (unsigned long long left = odd; left; left &= left - 1) {
-              const int u = __ffsll(left) - 1;
-              float y2[2];
-              load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
-              const float y = y2[ch & 1];
-              if (fabsf(y) <= 3.4e38f) continue;
-              const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int t = sh.draft[sg][col + j];
-                if ((sh.word[sg][t] >> u & 1) &&
-                    (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
-                  x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = col + j, rr = d.first_row + r;
-              if (rr >= d.rows) continue;
-              const float y = __uint_as_float(x[j]);
-              if (whole) {
-                const size_t to = out_row(a, d.row0, d.head, sh.draft[sg][r], rr) * D + ch;
-                if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.sum[r]);
-                else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.sum[r]);
-              } else {
-                rec[2 * NR + r * D + ch] = y;
-              }
-            }
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
+        finish_stream<D, NR, VK>(a, sh, d, tm + lanes, c0, tok, bar);
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
       }
     }
