@@ -8,10 +8,10 @@ using namespace i4kv;
 
 namespace i4kv {
 size_t multi_query_f32_workspace(int dim, int sms);
-cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, size_t ws_bytes,
+cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, void* ws, size_t ws_bytes,
                             cudaStream_t stream);
 size_t multi_query_tc_workspace(int dim, long long rows, int sms);
-cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, size_t ws_bytes, cudaStream_t stream);
+cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, void* ws, size_t ws_bytes, cudaStream_t stream);
 }  // namespace i4kv
 
 namespace {
@@ -36,15 +36,14 @@ bool sizes_ok(int batch, int hq, int hkv, int dim, int page, int group, int max_
   return max_drafts >= 0 && max_drafts <= INT4KV_MAX_DRAFTS && (long long)hq * dim <= (1 << 24);
 }
 
-cudaError_t run(MultiQueryArgs a, int dim, int vk, void* workspace, size_t bytes, cudaStream_t stream) {
+cudaError_t run(const MultiQueryArgs& a, int dim, int vk, void* workspace, size_t bytes, cudaStream_t stream) {
   if (!aligned16(workspace) || !workspace) return cudaErrorInvalidValue;
   int sms = 0;
   if ((long long)a.total_rows * a.kv_heads * a.group_q > 0x7fffffffll) return cudaErrorInvalidValue;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
-  a.recs = static_cast<float*>(workspace);
-  if (a.qk != INT4KV_VALUES_F32) return multi_query_tc(a, dim, sms, bytes, stream);
-  return multi_query_f32(a, dim, vk, sms, bytes, stream);
+  if (a.qk != INT4KV_VALUES_F32) return multi_query_tc(a, dim, sms, workspace, bytes, stream);
+  return multi_query_f32(a, dim, vk, sms, workspace, bytes, stream);
 }
 
 }  // namespace
@@ -85,7 +84,7 @@ cudaError_t int4kv_paged_tree_decode(const void* query, const void* k_draft, con
   for (const void* p : {query, k_draft, v_draft, (const void*)k_pool, v_pool, (const void*)sz_pool, (const void*)out})
     if (!aligned16(p)) return cudaErrorInvalidValue;
   MultiQueryArgs a{query, k_draft, v_draft, tree_mask, draft_offsets, k_pool, v_pool, sz_pool,
-                   block_table, seq_lens, out, nullptr, status, qkv_dtype, batch, num_kv_heads,
+                   block_table, seq_lens, out, nullptr, nullptr, status, qkv_dtype, batch, num_kv_heads,
                    num_q_heads / num_kv_heads, num_rows, max_drafts, max_pages, num_pages,
                    group_tokens / kMqPage, window, sinks};
   return run(a, head_dim, value_dtype, workspace, workspace_bytes, stream);
@@ -109,7 +108,7 @@ cudaError_t int4kv_paged_window_decode(const void* query, int query_dtype, const
   for (const void* p : {query, (const void*)k_pool, v_pool, (const void*)sz_pool, (const void*)out})
     if (!aligned16(p)) return cudaErrorInvalidValue;
   MultiQueryArgs a{query, nullptr, nullptr, nullptr, nullptr, k_pool, v_pool, sz_pool,
-                   block_table, seq_lens, out, nullptr, status, query_dtype, batch, num_kv_heads,
+                   block_table, seq_lens, out, nullptr, nullptr, status, query_dtype, batch, num_kv_heads,
                    num_q_heads / num_kv_heads, batch, 1, max_pages, num_pages,
                    group_tokens / kMqPage, window, sinks};
   return run(a, head_dim, value_dtype, workspace, workspace_bytes, stream);

@@ -9,10 +9,11 @@
 // tokens. The streams' tiles are laid end to end and
 // every CTA takes one contiguous run of equal length, so the CTAs do the same
 // number of tiles whatever the lengths are. A stream inside one run is finished
-// by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per row,
-// and merge_records_kernel, one block per run boundary, combines them. The
-// records need no counters, so the workspace carries nothing between launches,
-// and their order of combination is fixed: equal inputs give equal bits.
+// by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per
+// row, and the first of them a note of who shares it (RunTail), by which
+// merge_records_kernel, one block per run, combines them. Records and notes need
+// no counters, so the workspace carries nothing between launches, and their order
+// of combination is fixed: equal inputs give equal bits.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -43,11 +44,20 @@ struct MultiQueryArgs {
   const int32_t* block_table;
   const int32_t* seq_lens;
   void* out;                   // [rows, Hq, D] of kind qk
+  struct RunTail* tails;       // one per CTA
   float* recs;                 // two records per CTA
   uint32_t* status;
   int qk, batch, kv_heads, group_q, total_rows, max_drafts;
   int max_pages, num_pages, group_pages;
   int window, sinks;           // window 0: the whole cache
+};
+
+// The stream at the end of a run that began in it and goes on in later runs, up to
+// run `last` (rows 0: there is none): what the merge has to know.
+struct RunTail {
+  int rows, row0, head, first_row;  // rows of the sequence, its first row; the chunk's
+  int slot, last;                   // this run's record of it; the last run that shares it
+  int pad[2];
 };
 
 // What one sequence asks for.
@@ -132,61 +142,6 @@ I4KV_DEVINL long long seq_units(const MultiQueryArgs& a, int b, bool report) {
   return (long long)w.tiles * w.chunks * a.kv_heads;
 }
 
-// Block-wide: total number of tiles, and the sequence that holds tile
-// pick(total) with the tiles before that sequence. `s_tmp`: 3 + warps int64 of
-// shared memory. Every thread of the block calls it.
-template <int NR, int TP, typename Pick>
-__device__ long long locate_sequence(const MultiQueryArgs& a, long long* s_tmp, Pick pick, int& b_out,
-                                     long long& before_out) {
-  const int nt = blockDim.x, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int per = (a.batch + nt - 1) / nt;
-  const int lo = min(a.batch, t * per), hi = min(a.batch, lo + per);
-  long long local = 0;
-#pragma unroll 1
-  for (int b = lo; b < hi; ++b) local += seq_units<NR, TP>(a, b, blockIdx.x == 0);
-  long long incl = local;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) s_tmp[3 + warp] = incl;
-  __syncthreads();
-  if (t == 0) {
-    long long run = 0;
-#pragma unroll 1
-    for (int i = 0; i < nt / 32; ++i) {
-      const long long v = s_tmp[3 + i];
-      s_tmp[3 + i] = run;
-      run += v;
-    }
-    s_tmp[0] = run;
-    s_tmp[1] = 0;
-    s_tmp[2] = 0;
-  }
-  __syncthreads();
-  const long long total = s_tmp[0];
-  const long long u = pick(total);
-  long long base = s_tmp[3 + warp] + incl - local;
-  if (u >= base && u < base + local) {
-#pragma unroll 1
-    for (int b = lo; b < hi; ++b) {
-      const long long n = seq_units<NR, TP>(a, b, false);
-      if (u < base + n) {
-        s_tmp[1] = b;
-        s_tmp[2] = base;
-        break;
-      }
-      base += n;
-    }
-  }
-  __syncthreads();
-  b_out = (int)s_tmp[1];
-  before_out = s_tmp[2];
-  __syncthreads();
-  return total;
-}
-
 // First tile of CTA c of n (n <= total): contiguous runs of equal length.
 static __device__ __noinline__ long long tile_div(long long x, long long n) { return floor_div_s52(x, n); }
 I4KV_DEVINL long long run_start(long long c, long long total, long long n) { return tile_div(c * total, n); }
@@ -201,6 +156,73 @@ I4KV_DEVINL TileAt tile_at(const MultiQueryArgs& a, const SeqWork& w, int b, lon
   p.chunk = r / w.tiles;
   p.tile = r - p.chunk * w.tiles;
   return p;
+}
+
+// A CTA's run: its tiles u0 .. u0 + tiles - 1 of all, of which the first lies in
+// sequence b, rem tiles after that sequence's first.
+struct RunPlan {
+  long long total, runs, u0, rem;
+  int tiles, b;
+};
+
+// ... by one converged warp, from the lengths alone (every CTA finds its own).
+template <int NR, int TP>
+__device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int ctas) {
+  const int lane = threadIdx.x & 31;
+  long long first = 0, total = 0;
+#pragma unroll 1
+  for (int base = 0; base < a.batch; base += 32) {
+    long long n = 0;
+    if (base + lane < a.batch) n = seq_units<NR, TP>(a, base + lane, cta == 0);
+    if (base == 0) first = n;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    total += n;
+  }
+  RunPlan p;
+  p.total = total;
+  p.runs = min((long long)ctas, total);
+  p.u0 = p.rem = 0;
+  p.tiles = p.b = 0;
+  if (cta >= p.runs) return p;
+  p.u0 = run_start(cta, total, p.runs);
+  p.tiles = (int)(run_start(cta + 1, total, p.runs) - p.u0);
+  long long before = 0;
+#pragma unroll 1
+  for (int base = 0; base < a.batch; base += 32) {
+    long long n = first;
+    if (base > 0) n = base + lane < a.batch ? seq_units<NR, TP>(a, base + lane, false) : 0;
+    long long incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > p.u0);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      p.b = base + l;
+      p.rem = p.u0 - before - __shfl_sync(0xffffffffu, incl - n, l);
+      return p;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return p;
+}
+
+// The note of a run's last stream (tile `t` of it is the run's last).
+I4KV_DEVINL void note_tail(const MultiQueryArgs& a, int cta, const RunPlan& p, const SeqWork& w, const TileAt& t, int nr) {
+  RunTail n = {};
+  const long long end = p.u0 + p.tiles, first = end - 1 - t.tile;  // the stream's first tile
+  if (t.tile + 1 < w.tiles && first >= p.u0) {
+    n.rows = w.rows;
+    n.row0 = w.row0;
+    n.head = t.head;
+    n.first_row = t.chunk * nr;
+    n.slot = 2 * cta + (first > p.u0 ? 1 : 0);
+    n.last = (int)run_of(first + w.tiles - 1, p.total, p.runs);
+  }
+  a.tails[cta] = n;
 }
 
 // Step to the next stream; `w` follows the sequence. False past the last one.
@@ -293,40 +315,36 @@ I4KV_DEVINL float exp2_fast(float x) {
   return r;
 }
 
+// Workspace of `runs` runs: their notes, then two records each.
+inline size_t mq_workspace_bytes(int runs, int record_floats) {
+  return (size_t)runs * sizeof(RunTail) + (size_t)runs * 2 * record_floats * 4;
+}
+inline bool mq_workspace(MultiQueryArgs& a, void* ws, size_t bytes, int runs, int record_floats) {
+  if (bytes < mq_workspace_bytes(runs, record_floats)) return false;
+  a.tails = static_cast<RunTail*>(ws);
+  a.recs = reinterpret_cast<float*>(a.tails + runs);
+  return true;
+}
+
 constexpr int kMergeWarps = 8;
 
-// Combine the records of the streams that lie across run boundaries: block x
-// looks at the boundary between runs x and x + 1, and merges the stream there if
-// it is the stream's first boundary; blocks y take kMergeWarps rows each, one
-// warp a row. Plain float32 with weights e^(m_i - M): a handful of terms.
-template <int NR, int TP, int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQueryArgs a, int runs) {
-  __shared__ long long s_tmp[3 + kMergeWarps];
+// Combine the records of the streams that lie across runs: block x the one that run
+// x began and did not end (if any), blocks y kMergeWarps rows each, one warp a row.
+// Plain float32 with weights e^(m_i - M): a handful of terms.
+template <int NR, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQueryArgs a) {
   grid_dependency_wait();
-  int b;
-  long long before;
-  const long long c = blockIdx.x;
-  const long long total = locate_sequence<NR, TP>(
-      a, s_tmp, [&](long long n) { return run_start(c + 1, n, min((long long)runs, n)) - 1; }, b, before);
-  const long long n = min((long long)runs, total);
-  if (c + 1 >= n) return;
-  const SeqWork w = seq_work<NR, TP>(a, b, false);
-  const long long edge = run_start(c + 1, total, n);
-  const TileAt p = tile_at(a, w, b, edge - 1 - before);
-  const long long s0 = edge - 1 - p.tile, s1 = s0 + w.tiles;
-  if (s1 == edge || s0 < run_start(c, total, n)) return;
-  const int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int rr = p.chunk * NR + r;
-  if (rr >= w.rows) return;
-  const long long last = run_of(s1 - 1, total, n);
+  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  const int4 n0 = __ldcg(reinterpret_cast<const int4*>(a.tails + c));
+  const int2 n1 = __ldcg(reinterpret_cast<const int2*>(a.tails + c) + 2);
+  const int rows = n0.x, row0 = n0.y, head = n0.z, r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);
+  const int rr = n0.w + r, slot = n1.x, last = n1.y;
+  if (rr >= rows) return;
   constexpr int kRec = Record<NR, D>::kFloats;
-  auto record = [&](long long i) {
-    const bool tail = i == c && run_start(c, total, n) != s0;  // the stream begins inside run c
-    return a.recs + (2 * i + (tail ? 1 : 0)) * (size_t)kRec;
-  };
+  auto record = [&](int i) { return a.recs + (size_t)(i == c ? slot : 2 * i) * kRec; };
   float M = -INFINITY;
 #pragma unroll 1
-  for (long long i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(record(i) + r));
+  for (int i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(record(i) + r));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   float L = 0.f, o[D / 32];
@@ -334,7 +352,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQu
   for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
   if (M != -INFINITY) {
 #pragma unroll 2
-    for (long long i = c; i <= last; ++i) {
+    for (int i = c; i <= last; ++i) {
       const float* rec = record(i);
       const float e = exp2_fast((__ldcg(rec + r) - M) * kLog2e);
       L = fmaf(__ldcg(rec + NR + r), e, L);
@@ -348,7 +366,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQu
     }
   }
   const float inv = 1.f / fmaxf(L, 1e-10f);
-  const size_t to = row_offset(a, w, p.head, rr, D);
+  const int t = rr / a.group_q;
+  const size_t to = (((size_t)(row0 + t) * a.kv_heads + head) * a.group_q + (rr - t * a.group_q)) * D;
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) store2(a.out, a.qk, to + 64 * k + 2 * lane, o[2 * k] * inv, o[2 * k + 1] * inv);
 }

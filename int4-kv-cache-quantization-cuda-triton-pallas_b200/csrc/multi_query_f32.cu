@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   extern __shared__ __align__(128) char smem[];
   __shared__ uint64_t s_full[2];
   __shared__ uint32_t s_pages[2];
-  __shared__ long long s_tmp[3 + kThreads / 32];
+  __shared__ RunPlan s_plan;
   __shared__ float s_alpha[NR], s_m[NR], s_l[NR];
   __shared__ int s_edge[NR], s_depth[kMqMaxDrafts];
   __shared__ uint64_t s_word[NR];
@@ -76,17 +76,21 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     fence_barrier_init();
   }
   zero_idle_rows<NR, TP, D>(a);
-  int b0;
-  long long before;
-  const long long cta = blockIdx.x, ctas = gridDim.x;
-  const long long total = locate_sequence<NR, TP>(
-      a, s_tmp, [&](long long n) { return n > cta ? run_start(cta, n, min(ctas, n)) : 0ll; }, b0, before);
-  const long long runs = min(ctas, total);
-  if (cta >= runs) return;
-  const long long u0 = run_start(cta, total, runs), u1 = run_start(cta + 1, total, runs);
+  const int cta = blockIdx.x;
+  if (warp == 0) {
+    const RunPlan mine = plan_run<NR, TP>(a, cta, gridDim.x);
+    if (lane == 0) s_plan = mine;
+  }
+  __syncthreads();
+  const RunPlan plan = s_plan;
+  if (plan.tiles == 0) {
+    if (tid == 0) a.tails[cta] = RunTail{};
+    return;
+  }
+  const long long u0 = plan.u0, u1 = u0 + plan.tiles;
 
-  SeqWork w = seq_work<NR, TP>(a, b0, false), nw = w;  // of the current tile, of the next copied one
-  TileAt p = tile_at(a, w, b0, u0 - before), np = p;
+  SeqWork w = seq_work<NR, TP>(a, plan.b, false), nw = w;  // of the current tile, of the next copied one
+  TileAt p = tile_at(a, w, plan.b, plan.rem), np = p;
 
   // Copies of tile `np` into stage st (lanes < TP of warp 0, a page each).
   auto issue = [&](int st) {
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
       }
       const long long first = u - p.tile;  // the stream's first tile
       const bool whole = ends && first >= u0;
-      float* rec = a.recs + (2 * cta + (first > u0 ? 1 : 0)) * (size_t)Record<NR, D>::kFloats;
+      float* rec = a.recs + (size_t)(2 * cta + (first > u0 ? 1 : 0)) *Record<NR, D>::kFloats;
       for (int i = 2 * tid; i < NR * D; i += 2 * kThreads) {
         const int r = i / D, c = i - r * D, rr = p.chunk * NR + r;
         if (rr >= w.rows) continue;
@@ -392,13 +396,14 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         }
       }
       fresh = true;
+      if (u + 1 == u1 && tid == 0) note_tail(a, cta, plan, w, p, NR);
     }
     step(w, p);
   }
 }
 
 template <int D, int NR, int VK>
-cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream_t stream) {
+cudaError_t launch(const MultiQueryArgs& args, int sms, void* ws, size_t ws_bytes, cudaStream_t stream) {
   using S = Shape<D, NR, VK>;
   constexpr auto kern = multi_query_f32_kernel<D, NR, VK>;
   static_assert(S::BYTES <= 225 * 1024, "shared memory");
@@ -406,25 +411,26 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   cudaError_t e = mq_occupancy<kern>(kThreads, S::BYTES, &per_sm);
   if (e != cudaSuccess) return e;
   const int runs = sms * std::min(per_sm, kMaxPerSm);
-  if (ws_bytes < (size_t)runs * 2 * Record<NR, D>::kFloats * 4) return cudaErrorInvalidValue;
+  MultiQueryArgs a = args;
+  if (!mq_workspace(a, ws, ws_bytes, runs, Record<NR, D>::kFloats)) return cudaErrorInvalidValue;
   e = mq_launch_pdl(kern, dim3(runs), dim3(kThreads), S::BYTES, stream, a);
   if (e != cudaSuccess) return e;
-  return mq_launch_pdl(merge_records_kernel<NR, S::TP, D>, dim3(runs - 1, (NR + kMergeWarps - 1) / kMergeWarps),
-                       dim3(kMergeWarps * 32), 0, stream, a, runs);
+  return mq_launch_pdl(merge_records_kernel<NR, D>, dim3(runs - 1, (NR + kMergeWarps - 1) / kMergeWarps),
+                       dim3(kMergeWarps * 32), 0, stream, a);
 }
 
 template <int D, int NR>
-cudaError_t launch_vk(int vk, const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
-  if (vk == INT4KV_VALUES_F32) return launch<D, NR, INT4KV_VALUES_F32>(a, sms, ws, st);
-  if (vk == INT4KV_VALUES_F16) return launch<D, NR, INT4KV_VALUES_F16>(a, sms, ws, st);
-  return launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, st);
+cudaError_t launch_vk(int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  if (vk == INT4KV_VALUES_F32) return launch<D, NR, INT4KV_VALUES_F32>(a, sms, ws, n, st);
+  if (vk == INT4KV_VALUES_F16) return launch<D, NR, INT4KV_VALUES_F16>(a, sms, ws, n, st);
+  return launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, n, st);
 }
 
 template <int D>
-cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
-  if (rows <= 4) return launch_vk<D, 4>(vk, a, sms, ws, st);
-  if (rows <= 8) return launch_vk<D, 8>(vk, a, sms, ws, st);
-  return launch_vk<D, 16>(vk, a, sms, ws, st);
+cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  if (rows <= 4) return launch_vk<D, 4>(vk, a, sms, ws, n, st);
+  if (rows <= 8) return launch_vk<D, 8>(vk, a, sms, ws, n, st);
+  return launch_vk<D, 16>(vk, a, sms, ws, n, st);
 }
 
 }  // namespace
@@ -432,16 +438,16 @@ cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, size
 namespace i4kv {
 
 size_t multi_query_f32_workspace(int dim, int sms) {
-  return (size_t)sms * kMaxPerSm * 2 * (2 * 16 + 16 * (size_t)dim) * 4;
+  return mq_workspace_bytes(sms * kMaxPerSm, 2 * 16 + 16 * dim);
 }
 
-cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, size_t ws_bytes,
+cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, void* ws, size_t ws_bytes,
                             cudaStream_t stream) {
   const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
   const int r = (int)std::min<long long>(rows, 1 << 20);
-  if (dim == 64) return launch_rows<64>(r, vk, a, sms, ws_bytes, stream);
-  if (dim == 128) return launch_rows<128>(r, vk, a, sms, ws_bytes, stream);
-  return launch_rows<256>(r, vk, a, sms, ws_bytes, stream);
+  if (dim == 64) return launch_rows<64>(r, vk, a, sms, ws, ws_bytes, stream);
+  if (dim == 128) return launch_rows<128>(r, vk, a, sms, ws, ws_bytes, stream);
+  return launch_rows<256>(r, vk, a, sms, ws, ws_bytes, stream);
 }
 
 }  // namespace i4kv

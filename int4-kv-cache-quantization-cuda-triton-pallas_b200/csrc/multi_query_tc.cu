@@ -232,12 +232,13 @@ struct TcShared {
   float qscale[kDesc];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
-  float ref[NR], sum[NR];       // a finished stream's references and sums
+  float ref[NR], inv[NR];       // a finished stream's references, inverse sums,
+  int row[NR];                  // and rows of the outputs [rows * heads]
   float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
   float qmax[2][4];
   unsigned long long odd[kDesc];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
-  long long scan[3 + 32];
+  RunPlan plan;
 };
 
 // Bounded wait: false (and a status bit) when its limit passes.
@@ -271,8 +272,7 @@ I4KV_DEVINL void fma2(float& d0, float& d1, float a0, float a1, float b0, float 
 
 // 8 consecutive 16-bit inputs widened to float32.
 template <int VK>
-I4KV_DEVINL void load8(const void* base, size_t i, float (&x)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i));
+I4KV_DEVINL void widen8(const uint4& u, float (&x)[8]) {
   const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -285,6 +285,10 @@ I4KV_DEVINL void load8(const void* base, size_t i, float (&x)[8]) {
       x[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
     }
   }
+}
+template <int VK>
+I4KV_DEVINL void load8(const void* base, size_t i, float (&x)[8]) {
+  widen8<VK>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + i)), x);
 }
 
 // Power of two that brings |x| <= top to [1, 2) (1 for 0), and its inverse.
@@ -310,18 +314,35 @@ I4KV_DEVINL size_t out_row(const MultiQueryArgs& a, int row0, int head, int t, i
 template <int NR>
 __device__ __noinline__ int describe_rows(const MultiQueryArgs& a, TcShared<NR>& sh, const SeqWork& w, int chunk, int sg,
                                           int lane) {
-  int top = 0;
-#pragma unroll 1
-  for (int t = lane; t < max(w.drafts, 1); t += 32) {
-    const uint64_t word = a.mask ? (uint64_t)a.mask[w.row0 + t] : 0ull;
-    const int dp = a.mask ? draft_depth(word, t, w.drafts) : 0;
-    sh.word[sg][t] = word;
-    sh.depth[sg][t] = dp;
-    top = max(top, dp);
+  uint64_t word[2] = {0, 0};
+  int depth[2] = {0, 0};
+  if (a.mask) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int t = lane + 32 * k;
+      if (t < w.drafts) {
+        word[k] = (uint64_t)a.mask[w.row0 + t];
+        depth[k] = draft_depth(word[k], t, w.drafts);
+      }
+    }
   }
+  sh.depth[sg][lane] = depth[0];
+  sh.depth[sg][lane + 32] = depth[1];
+  if (a.mask && a.window > 0) {  // drafts behind the window are not seen either
+    __syncwarp();
+#pragma unroll 1
+    for (int u = 0; u < w.drafts; ++u) {
+      const int at = w.len + sh.depth[sg][u];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (at <= w.pos0 + depth[k] - a.window && at >= a.sinks) word[k] &= ~(1ull << u);
+    }
+  }
+  sh.word[sg][lane] = word[0];
+  sh.word[sg][lane + 32] = word[1];
 #pragma unroll 1
   for (int r = lane; r < NR; r += 32) sh.draft[sg][r] = (uint8_t)(min(chunk * NR + r, w.rows - 1) / a.group_q);
-  return __reduce_max_sync(0xffffffffu, top);
+  return __reduce_max_sync(0xffffffffu, max(depth[0], depth[1]));
 }
 
 // A stream's queries to shared memory, by a conversion group: as they are, for a
@@ -334,7 +355,7 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, TcShared<NR>&
   float top = 0.f, down = 1.f, up = 1.f;
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = ct; k < NR * (D / 8); k += 128) {
       const int r = k / (D / 8), c8 = k % (D / 8), rr = d.first_row + r;
       uint32_t h[4] = {0, 0, 0, 0};
@@ -460,47 +481,59 @@ __device__ __noinline__ void convert_scaled(TcShared<NR>& sh, const TileDesc& d,
 template <int D, int NR, int VK>
 __device__ __noinline__ void draft_keys(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, int ds, uint32_t keys,
                                         int ct) {
+  constexpr int NB = D / 64;
   const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
 #pragma unroll 1
   for (int p = 0; p < 2; ++p) {
-    const int ta = (page0 + p) * kMqPage + g, tb = ta + 8;
-    float top[2] = {0.f, 0.f}, down[2] = {1.f, 1.f}, up[2] = {1.f, 1.f};
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {  // the rows' scales, then their keys
-#pragma unroll 1
-      for (int blk = 0; blk < D / 64; ++blk) {
-        uint32_t h[16];
+    if (page0 + p >= d.pages) break;  // (nothing there is seen)
+    uint4 raw[2][NB][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int t = r ? tb : ta;
-          const size_t row = ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 64 * blk + 16 * t4;
+    for (int r = 0; r < 2; ++r) {
+      const int t = (page0 + p) * kMqPage + g + 8 * r;
+      const uint16_t* src = static_cast<const uint16_t*>(a.kd) + ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 16 * t4;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (t < d.drafts) load8<VK>(a.kd, row + 8 * e, x);
+      for (int blk = 0; blk < NB; ++blk) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              top[r] = fmaxf(top[r], fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-              // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
-              h[4 * (2 * e + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
-            }
-          }
-        }
-        __syncwarp();
-        if (pass) tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
-      }
-      if (!pass) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-          unit_scale(top[r], down[r], up[r]);
+        for (int e = 0; e < 2; ++e) {
+          raw[r][blk][e] = make_uint4(0, 0, 0, 0);
+          if (t < d.drafts) raw[r][blk][e] = __ldg(reinterpret_cast<const uint4*>(src + 64 * blk + 8 * e));
         }
       }
     }
-    if (t4 == 0) {
-      sh.kscale[ds][ta] = up[0];
-      sh.kscale[ds][tb] = up[1];
+    float down[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float top = 0.f, up;
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x[8];
+          widen8<VK>(raw[r][blk][e], x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      unit_scale(top, down[r], up);
+      if (t4 == 0) sh.kscale[ds][(page0 + p) * kMqPage + g + 8 * r] = up;
+    }
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk) {
+      uint32_t h[16];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x[8];
+          widen8<VK>(raw[r][blk][e], x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
+            h[4 * (2 * e + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
+        }
+      }
+      tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
     }
   }
 }
@@ -514,29 +547,33 @@ I4KV_DEVINL bool token_real(const MultiQueryArgs& a, const TileDesc& d, int page
 
 // Rows that see a thread's tokens, a bit each: tokens g, g + 8 of the warp's first
 // page and of its second; bit j is row c0 + 8 (j / 2) + 2 t + j % 2.
-template <int NR>
+template <int NR, int ROWS>
 __device__ __noinline__ uint4 visible_rows(const MultiQueryArgs& a, const TcShared<NR>& sh, const TileDesc& d, int c0,
-                                           int quarter, int lane, int pairs) {
+                                           int quarter, int lane) {
   const int g = lane >> 2, t4 = lane & 3, sg = d.seg;
   const bool draft = d.flags & kDraftTile;
   uint32_t vis[4];
+  int at[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int page = 2 * quarter + q / 2, at = d.at[page] + g + 8 * (q % 2);
-    const bool real = token_real(a, d, page, at);
-    uint32_t bits = real ? ~0u : 0u;
-    if (real && (draft || a.window > 0)) {
-      const int behind = draft ? d.len + sh.depth[sg][at & 63] : at;
-      const bool edge = a.window > 0 && behind >= a.sinks;
-#pragma unroll 1
-      for (int j = 0; j < 2 * pairs; ++j) {
-        const int t = sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2];
-        const bool sees =
-            (!draft || (sh.word[sg][t] >> (at & 63) & 1)) && (!edge || behind > d.low_edge + sh.depth[sg][t]);
-        bits &= ~((uint32_t)!sees << j);
-      }
+    const int page = 2 * quarter + q / 2;
+    at[q] = d.at[page] + g + 8 * (q % 2);
+    vis[q] = token_real(a, d, page, at[q]) ? ~0u : 0u;
+  }
+  if (draft) {
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const uint64_t word = sh.word[sg][sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2]];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vis[q] &= ~((uint32_t)(~(word >> (at[q] & 63)) & 1) << j);
     }
-    vis[q] = bits;
+  } else if (a.window > 0) {
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const int edge = d.low_edge + sh.depth[sg][sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2]];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vis[q] &= ~((uint32_t)(at[q] <= edge && at[q] >= a.sinks) << j);
+    }
   }
   __syncwarp();
   return make_uint4(vis[0], vis[1], vis[2], vis[3]);
@@ -638,25 +675,33 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, TcShared<NR>&
     for (int k = tok / (kMqPage * T::PPU); k > 0; --k) v.next<T::NV>();
     ok = tc_wait(&sh.v_full[v.s], v.ph, a.status);
     char* row = v_smem + v.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+    // (the order of a thread's 16-byte pieces spreads a warp's over the banks)
+    auto piece = [&](int q) {
+      return reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
+    };
     bool bad = false;
-#pragma unroll 1
-    for (int q = 0; q < 8 * T::CH; ++q) {
-      uint4* at16 = reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
-      uint4 y = make_uint4(0, 0, 0, 0);
-      bool hit = !real;
-      if (real) {
-        y = *at16;
-        uint32_t e[4] = {y.x, y.y, y.z, y.w};
-        constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C00u : 0x7F80u;
+    if (!real) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if ((e[k] & kExp) == kExp) { e[k] &= 0xFFFF0000u; hit = true; }
-          if ((e[k] >> 16 & kExp) == kExp) { e[k] &= 0x0000FFFFu; hit = true; }
-        }
-        bad |= hit;
-        y = make_uint4(e[0], e[1], e[2], e[3]);
+      for (int q = 0; q < 8 * T::CH; ++q) *piece(q) = make_uint4(0, 0, 0, 0);
+    } else {
+      // an exponent of all ones carries into the sign's place
+      constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C007C00u : 0x7F807F80u;
+      constexpr uint32_t kOne = VK == INT4KV_VALUES_F16 ? 0x04000400u : 0x00800080u;
+      uint32_t any = 0;
+#pragma unroll 8
+      for (int q = 0; q < 8 * T::CH; ++q) {
+        const uint4 y = *piece(q);
+        any |= ((y.x & kExp) + kOne) | ((y.y & kExp) + kOne) | ((y.z & kExp) + kOne) | ((y.w & kExp) + kOne);
       }
-      if (hit) *at16 = y;
+      bad = any & 0x80008000u;
+      if (bad) {
+#pragma unroll 1
+        for (int q = 0; q < 32 * T::CH; ++q) {
+          uint32_t* y = reinterpret_cast<uint32_t*>(piece(q / 4)) + q % 4;
+          const uint32_t m = ((*y & kExp) + kOne) & 0x80008000u;
+          if (m) *y &= (m & 0x8000u ? 0u : 0x0000FFFFu) | (m >> 31 ? 0u : 0xFFFF0000u);
+        }
+      }
     }
     if (bad) atomicOr(&sh.odd[d.seg], 1ull << (at & 63));
   }
@@ -675,9 +720,10 @@ __device__ __noinline__ void finish_stream(const MultiQueryArgs& a, TcShared<NR>
   const int sg = d.seg;
   float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
   if (tok < T::NC) {
-    const int r = c0 + tok;
+    const int r = c0 + tok, rr = d.first_row + r;
     const float sum = (sh.part[0][r] + sh.part[1][r]) + (sh.part[2][r] + sh.part[3][r]);
-    sh.sum[r] = 1.f / fmaxf(sum, 1e-10f);
+    sh.inv[r] = 1.f / fmaxf(sum, 1e-10f);
+    sh.row[r] = (int)out_row(a, d.row0, d.head, sh.draft[sg][r], rr);
     if (!whole) {
       rec[r] = sh.ref[r] == kNoRef ? -INFINITY : sh.ref[r] * 0.6931471805599453f;
       rec[NR + r] = sum;
@@ -686,42 +732,47 @@ __device__ __noinline__ void finish_stream(const MultiQueryArgs& a, TcShared<NR>
   named_bar_sync(bar, 128);
   tc_fence_after();
   const unsigned long long odd = sh.odd[sg];
+  const int cols = min(T::NC, d.rows - d.first_row - c0);  // rows that are there
 #pragma unroll 1
-  for (int j0 = 0; j0 < T::NC; j0 += 8) {
-    const int col = c0 + j0;
+  for (int o = 0; o < T::NO; ++o) {
+    const int ch = o * 128 + tok;
+    if (o * 128 + (tok & 96) >= D) break;  // (a warp's channels are all there or none is)
 #pragma unroll 1
-    for (int o = 0; o < T::NO; ++o) {
-      const int ch = o * 128 + tok;
+    for (int j0 = 0; j0 < cols; j0 += 8) {
+      const int col = c0 + j0;
       uint32_t x[8];
       tc_ld8(x, tm + T::COLS_O + o * NR + col);
-      if (ch >= D) continue;
+      if (odd) {
 #pragma unroll 1
-      for (unsigned long long left = odd; left; left &= left - 1) {
-        const int u = __ffsll(left) - 1;
-        float y2[2];
-        load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
-        const float y = ch & 1 ? y2[1] : y2[0];
-        if (fabsf(y) <= 3.4e38f) continue;
-        const int pos = a.window > 0 ? d.len + sh.depth[sg][u] : 0;
+        for (unsigned long long left = odd; left; left &= left - 1) {
+          const int u = __ffsll(left) - 1;
+          float y2[2];
+          load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
+          const float y = ch & 1 ? y2[1] : y2[0];
+          if (fabsf(y) <= 3.4e38f) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (sh.word[sg][sh.draft[sg][col + j]] >> u & 1) x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+        }
+        __syncwarp();
+      }
+      if (whole) {
+        const float4 i0 = *reinterpret_cast<const float4*>(&sh.inv[col]), i1 = *reinterpret_cast<const float4*>(&sh.inv[col + 4]);
+        const int4 r0 = *reinterpret_cast<const int4*>(&sh.row[col]), r1 = *reinterpret_cast<const int4*>(&sh.row[col + 4]);
+        const float inv[8] = {i0.x, i0.y, i0.z, i0.w, i1.x, i1.y, i1.z, i1.w};
+        const int row[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int t = sh.draft[sg][col + j];
-          if ((sh.word[sg][t] >> u & 1) && (a.window == 0 || pos > d.low_edge + sh.depth[sg][t] || pos < a.sinks))
-            x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
+          if (j0 + j >= cols) break;
+          const float y = __uint_as_float(x[j]) * inv[j];
+          const size_t to = (size_t)row[j] * D + ch;
+          if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y);
+          else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y);
         }
-      }
+      } else {
+        float* to = rec + 2 * NR + (size_t)col * D + ch;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = col + j, rr = d.first_row + r;
-        if (rr >= d.rows) continue;
-        const float y = __uint_as_float(x[j]);
-        if (whole) {
-          const size_t to = out_row(a, d.row0, d.head, sh.draft[sg][r], rr) * D + ch;
-          if constexpr (VK == INT4KV_VALUES_F16) static_cast<__half*>(a.out)[to] = __float2half_rn(y * sh.sum[r]);
-          else static_cast<__nv_bfloat16*>(a.out)[to] = __float2bfloat16_rn(y * sh.sum[r]);
-        } else {
-          rec[2 * NR + r * D + ch] = y;
-        }
+        for (int j = 0; j < 8; ++j) to[j * D] = __uint_as_float(x[j]);
       }
     }
   }
@@ -770,15 +821,17 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   grid_dependency_wait();
   allow_dependent_launch();
   if (!a.offs) zero_idle_rows<NR, kTilePages, D>(a);
-  int b0;
-  long long before;
-  const long long cta = blockIdx.x, ctas = gridDim.x;
-  const long long total = locate_sequence<NR, kTilePages>(
-      a, sh.scan, [&](long long n) { return n > cta ? run_start(cta, n, min(ctas, n)) : 0ll; }, b0, before);
-  const long long runs = min(ctas, total);
-  const long long u0 = cta < runs ? run_start(cta, total, runs) : 0;
-  const int n_tiles = cta < runs ? (int)(run_start(cta + 1, total, runs) - u0) : 0;
+  const int cta = blockIdx.x;
+  if (warp == kCopyWarp) {
+    const RunPlan mine = plan_run<NR, kTilePages>(a, cta, gridDim.x);
+    if (lane == 0) {
+      sh.plan = mine;
+      if (mine.tiles == 0) a.tails[cta] = RunTail{};
+    }
+  }
+  __syncthreads();
   tc_fence_after();
+  const int n_tiles = sh.plan.tiles;
   const uint32_t tm = sh.tmem;
 
   if (n_tiles == 0) {
@@ -787,8 +840,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // Both warps walk the tiles; the first publishes their descriptors, the second
     // copies the values.
     const bool values = warp > kCopyWarp;
-    SeqWork w = seq_work<NR, kTilePages>(a, b0, false);
-    TileAt p = tile_at(a, w, b0, u0 - before);
+    const RunPlan plan = sh.plan;
+    const long long u0 = plan.u0;
+    SeqWork w = seq_work<NR, kTilePages>(a, plan.b, false);
+    TileAt p = tile_at(a, w, plan.b, plan.rem);
     int seg = -1, high_edge = 0;
     Ring v;
     bool ok = true;
@@ -859,10 +914,11 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.rows = w.rows;
           d.first_row = p.chunk * NR;
           d.seg = seg % kDesc;
-          d.slot = 2 * (int)cta + (first_u > u0 ? 1 : 0);
+          d.slot = 2 * cta + (first_u > u0 ? 1 : 0);
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
           d.slots = draft ? 0 : starts;
           if (first) sh.odd[seg % kDesc] = 0;
+          if (i + 1 == n_tiles) note_tail(a, cta, plan, w, p, NR);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
@@ -1132,7 +1188,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       // of the second
       uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
       if (masked) {
-        const uint4 m = visible_rows(a, sh, d, c0, quarter, lane, NI);
+        const uint4 m = visible_rows<NR, 2 * NI>(a, sh, d, c0, quarter, lane);
         vis[0] = m.x; vis[1] = m.y; vis[2] = m.z; vis[3] = m.w;
       }
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
@@ -1305,7 +1361,7 @@ cudaError_t value_map(CUtensorMap* map, const void* base, int vk, int dim, uint6
 }
 
 template <int D, int NR, int VK>
-cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream_t stream) {
+cudaError_t launch(const MultiQueryArgs& args, int sms, void* ws, size_t ws_bytes, cudaStream_t stream) {
   using T = Tc<D, NR>;
   constexpr size_t kBytes = T::END + sizeof(TcShared<NR>);
   static_assert(T::END + sizeof(TcShared<NR>) <= 227 * 1024, "shared memory");
@@ -1313,7 +1369,8 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   int per_sm = 0;
   cudaError_t e = mq_occupancy<kern>(T::THREADS, kBytes, &per_sm);
   if (e != cudaSuccess) return e;
-  if (ws_bytes < (size_t)sms * 2 * Record<NR, D>::kFloats * 4) return cudaErrorInvalidValue;
+  MultiQueryArgs a = args;
+  if (!mq_workspace(a, ws, ws_bytes, sms, Record<NR, D>::kFloats)) return cudaErrorInvalidValue;
   CUtensorMap vmap, dmap;
   const uint64_t row = (uint64_t)D * 2;
   if ((long long)a.num_pages * a.kv_heads > 0x7fffffffll) return cudaErrorInvalidValue;  // a TMA coordinate
@@ -1324,8 +1381,8 @@ cudaError_t launch(const MultiQueryArgs& a, int sms, size_t ws_bytes, cudaStream
   if (e != cudaSuccess) return e;
   e = mq_launch_pdl(kern, dim3(sms), dim3(T::THREADS), kBytes, stream, a, vmap, dmap);
   if (e != cudaSuccess) return e;
-  return mq_launch_pdl(merge_records_kernel<NR, kTilePages, D>, dim3(sms - 1, (NR + kMergeWarps - 1) / kMergeWarps),
-                       dim3(kMergeWarps * 32), 0, stream, a, sms);
+  return mq_launch_pdl(merge_records_kernel<NR, D>, dim3(sms - 1, (NR + kMergeWarps - 1) / kMergeWarps),
+                       dim3(kMergeWarps * 32), 0, stream, a);
 }
 
 // Rows of one kv head's chunk: the smallest of 16, 32, 64, 128 that holds them
@@ -1337,19 +1394,19 @@ int rows_of(long long rows, int dim) {
 }
 
 template <int D, int NR>
-cudaError_t launch_kind(const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
-  return a.qk == INT4KV_VALUES_F16 ? launch<D, NR, INT4KV_VALUES_F16>(a, sms, ws, st)
-                                   : launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, st);
+cudaError_t launch_kind(const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  return a.qk == INT4KV_VALUES_F16 ? launch<D, NR, INT4KV_VALUES_F16>(a, sms, ws, n, st)
+                                   : launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, n, st);
 }
 
 template <int D>
-cudaError_t launch_rows(int nr, const MultiQueryArgs& a, int sms, size_t ws, cudaStream_t st) {
-  if (nr == 16) return launch_kind<D, 16>(a, sms, ws, st);
-  if (nr == 32) return launch_kind<D, 32>(a, sms, ws, st);
+cudaError_t launch_rows(int nr, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  if (nr == 16) return launch_kind<D, 16>(a, sms, ws, n, st);
+  if (nr == 32) return launch_kind<D, 32>(a, sms, ws, n, st);
   if constexpr (D < 256) {
-    if (nr == 128) return launch_kind<D, 128>(a, sms, ws, st);
+    if (nr == 128) return launch_kind<D, 128>(a, sms, ws, n, st);
   }
-  return launch_kind<D, 64>(a, sms, ws, st);
+  return launch_kind<D, 64>(a, sms, ws, n, st);
 }
 
 }  // namespace
@@ -1358,14 +1415,14 @@ namespace i4kv {
 
 size_t multi_query_tc_workspace(int dim, long long rows, int sms) {
   const int nr = rows_of(rows, dim);
-  return (size_t)sms * 2 * (2 * nr + (size_t)nr * dim) * 4;
+  return mq_workspace_bytes(sms, 2 * nr + nr * dim);
 }
 
-cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, size_t ws_bytes, cudaStream_t stream) {
+cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, void* ws, size_t ws_bytes, cudaStream_t stream) {
   const int nr = rows_of((long long)std::max(1, a.max_drafts) * a.group_q, dim);
-  if (dim == 64) return launch_rows<64>(nr, a, sms, ws_bytes, stream);
-  if (dim == 128) return launch_rows<128>(nr, a, sms, ws_bytes, stream);
-  return launch_rows<256>(nr, a, sms, ws_bytes, stream);
+  if (dim == 64) return launch_rows<64>(nr, a, sms, ws, ws_bytes, stream);
+  if (dim == 128) return launch_rows<128>(nr, a, sms, ws, ws_bytes, stream);
+  return launch_rows<256>(nr, a, sms, ws, ws_bytes, stream);
 }
 
 }  // namespace i4kv
