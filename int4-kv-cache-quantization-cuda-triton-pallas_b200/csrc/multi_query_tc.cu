@@ -87,6 +87,11 @@ I4KV_DEVINL void tc_ld8(uint32_t (&r)[8], uint32_t addr) {
       : "r"(addr)
       : "memory");
 }
+I4KV_DEVINL void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
 // 16 lanes x 8 N columns in the layout of mma fragments: thread (g, t) = (lane / 4,
 // lane % 4) holds columns 8 j + 2 t, + 1 of lane g in r[4 j], r[4 j + 1] and of lane
 // g + 8 in r[4 j + 2], r[4 j + 3].
@@ -310,10 +315,18 @@ I4KV_DEVINL size_t out_row(const MultiQueryArgs& a, int row0, int head, int t, i
 // code has to fit the instruction caches side by side (with all of it in line the
 // warps spent half of their time waiting for instructions). ----
 
+// (They name the shared memory themselves: through a reference parameter its
+// accesses would be generic ones.)
+extern __shared__ __align__(1024) char tc_smem[];
+template <int D, int NR>
+I4KV_DEVINL TcShared<NR>& tc_shared() {
+  return *reinterpret_cast<TcShared<NR>*>(tc_smem + Tc<D, NR>::END);
+}
+
 // A stream's drafts and rows, for one warp; returns the deepest draft's ancestors.
-template <int NR>
-__device__ __noinline__ int describe_rows(const MultiQueryArgs& a, TcShared<NR>& sh, const SeqWork& w, int chunk, int sg,
-                                          int lane) {
+template <int D, int NR>
+__device__ __noinline__ int describe_rows(const MultiQueryArgs& a, const SeqWork w, int chunk, int sg, int lane) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
   uint64_t word[2] = {0, 0};
   int depth[2] = {0, 0};
   if (a.mask) {
@@ -350,31 +363,48 @@ __device__ __noinline__ int describe_rows(const MultiQueryArgs& a, TcShared<NR>&
 // above it (a bfloat16 input) takes the second pass, with a common power of two. A
 // thread takes 8 channels of a row.
 template <int D, int NR, int VK>
-__device__ __noinline__ void load_queries(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, char* q_smem, int ct,
-                                          int grp, int bar) {
+__device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int ct, int grp, int bar) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  char* const q_smem = tc_smem + Tc<D, NR>::Q_OFF;
+  constexpr int kAll = NR * (D / 8) / 128, kBatch = kAll < 8 ? kAll : 8;  // pieces of a thread, in flight
+  const TileDesc& d = sh.desc[ds];
+  const int rows = d.rows, first = d.first_row, row0 = d.row0, head = d.head, seg = d.seg;
+  const int c8 = ct % (D / 8), r0 = ct / (D / 8);
   float top = 0.f, down = 1.f, up = 1.f;
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
-#pragma unroll 8
-    for (int k = ct; k < NR * (D / 8); k += 128) {
-      const int r = k / (D / 8), c8 = k % (D / 8), rr = d.first_row + r;
-      uint32_t h[4] = {0, 0, 0, 0};
-      if (rr < d.rows) {
-        float x[8];
-        load8<VK>(a.q, out_row(a, d.row0, d.head, sh.draft[d.seg][r], rr) * D + 8 * c8, x);
+#pragma unroll 1
+    for (int k0 = 0; k0 < kAll; k0 += kBatch) {
+      uint4 raw[kBatch];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (VK == INT4KV_VALUES_BF16) top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-          h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
-        }
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (k0 + k) * (128 / (D / 8)), rr = first + r;
+        raw[k] = make_uint4(0, 0, 0, 0);
+        if (rr < rows)
+          raw[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                        out_row(a, row0, head, sh.draft[seg][r], rr) * D + 8 * c8));
       }
-      // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
-      char* row = q_smem + (c8 / 8) * (NR * 128) + r * 128;
-      const int q = c8 % 8 / 2, j = c8 % 2 * 2;
 #pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int at = 32 * (j + o) + 8 * q;  // byte of the row
-        *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (k0 + k) * (128 / (D / 8));
+        uint32_t h[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        if constexpr (VK == INT4KV_VALUES_BF16) {
+          float x[8];
+          widen8<VK>(raw[k], x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
+            h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
+          }
+        }
+        // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
+        char* row = q_smem + (c8 / 8) * (NR * 128) + r * 128;
+        const int q = c8 % 8 / 2, j = c8 % 2 * 2;
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          const int at = 32 * (j + o) + 8 * q;  // byte of the row
+          *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
+        }
       }
     }
     if (VK == INT4KV_VALUES_F16 || pass == 1) break;
@@ -387,7 +417,7 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, TcShared<NR>&
     named_bar_sync(bar, 128);  // qmax is free again
     unit_scale(top, down, up);
   }
-  if (ct == 0) sh.qscale[d.seg] = up;
+  if (ct == 0) sh.qscale[seg] = up;
   fence_proxy_async_smem();
 }
 
@@ -455,8 +485,9 @@ I4KV_DEVINL void convert_keys(const TileDesc& d, const char* codes, const float*
 
 // The same with a power of two per group, for keys beyond float16's range.
 template <int D, int NR>
-__device__ __noinline__ void convert_scaled(TcShared<NR>& sh, const TileDesc& d, int ds, const char* codes, const float* scales,
-                                            uint32_t keys, int ct) {
+__device__ __noinline__ void convert_scaled(int ds, const char* codes, const float* scales, uint32_t keys, int ct) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
   const int lane = ct & 31, page0 = (ct >> 5) * 2;
   float down[2];
 #pragma unroll 1
@@ -479,8 +510,9 @@ __device__ __noinline__ void convert_scaled(TcShared<NR>& sh, const TileDesc& d,
 
 // Drafted keys, with a power of two each.
 template <int D, int NR, int VK>
-__device__ __noinline__ void draft_keys(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, int ds, uint32_t keys,
-                                        int ct) {
+__device__ __noinline__ void draft_keys(const MultiQueryArgs& a, int ds, uint32_t keys, int ct) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
   constexpr int NB = D / 64;
   const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
 #pragma unroll 1
@@ -545,38 +577,32 @@ I4KV_DEVINL bool token_real(const MultiQueryArgs& a, const TileDesc& d, int page
   return here && (draft || a.window == 0 || at > d.low_edge || at < a.sinks);
 }
 
-// Rows that see a thread's tokens, a bit each: tokens g, g + 8 of the warp's first
-// page and of its second; bit j is row c0 + 8 (j / 2) + 2 t + j % 2.
-template <int NR, int ROWS>
-__device__ __noinline__ uint4 visible_rows(const MultiQueryArgs& a, const TcShared<NR>& sh, const TileDesc& d, int c0,
-                                           int quarter, int lane) {
-  const int g = lane >> 2, t4 = lane & 3, sg = d.seg;
-  const bool draft = d.flags & kDraftTile;
-  uint32_t vis[4];
-  int at[4];
+// A tile that some row does not see all of: the logits it must not see become -inf
+// in tensor memory, so nothing else has to know. A thread takes one token; whether
+// row r sees it hangs on the row's draft, the same for the whole warp.
+template <int D, int NR>
+__device__ __noinline__ void mask_tile(const MultiQueryArgs& a, int ds, uint32_t s_addr, int c0, int tok) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
+  const int sg = d.seg, page = tok / kMqPage, at = d.at[page] + tok % kMqPage, low = d.low_edge;
+  const bool draft = d.flags & kDraftTile, real = token_real(a, d, page, at);
+  const bool edge = !draft && a.window > 0 && at >= a.sinks;
+#pragma unroll 1
+  for (int j0 = 0; j0 < Tc<D, NR>::NC; j0 += 8) {
+    uint32_t x[8];
+    tc_ld8(x, s_addr + j0);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int page = 2 * quarter + q / 2;
-    at[q] = d.at[page] + g + 8 * (q % 2);
-    vis[q] = token_real(a, d, page, at[q]) ? ~0u : 0u;
-  }
-  if (draft) {
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      const uint64_t word = sh.word[sg][sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2]];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) vis[q] &= ~((uint32_t)(~(word >> (at[q] & 63)) & 1) << j);
+    for (int j = 0; j < 8; ++j) {
+      const int t = sh.draft[sg][c0 + j0 + j];
+      bool sees = real;
+      if (draft) sees = sees && (sh.word[sg][t] >> (at & 63) & 1);
+      if (edge) sees = sees && at > low + sh.depth[sg][t];
+      if (!sees) x[j] = 0xFF800000u;
     }
-  } else if (a.window > 0) {
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-      const int edge = d.low_edge + sh.depth[sg][sh.draft[sg][c0 + 8 * (j / 2) + 2 * t4 + j % 2]];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) vis[q] &= ~((uint32_t)(at[q] <= edge && at[q] >= a.sinks) << j);
-    }
+    __syncwarp();
+    tc_st8(s_addr + j0, x);
   }
-  __syncwarp();
-  return make_uint4(vis[0], vis[1], vis[2], vis[3]);
+  tc_wait_st();
 }
 
 // A softmax thread's rows: minus the references, and the sums.
@@ -588,16 +614,16 @@ struct RowState {
 constexpr float kNoRef = -1e30f;  // the reference of a row that has seen nothing
 
 // Raise the references to the true maxima of the tile, rescale sums and outputs.
-// `prev`: the barrier of the last tile's weights (0: O^T holds nothing yet).
+// `prev`: the buffer of the last tile's weights (-1: O^T holds nothing yet).
 template <int D, int NR>
-__device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const MultiQueryArgs& a, TcShared<NR>& sh,
-                                                                     RowState<Tc<D, NR>::NC / 8> s, uint4 vis4, float4 f4,
-                                                                     uint32_t s_addr, uint32_t o_addr, int c0, int quarter,
-                                                                     int lane, uint64_t* prev, uint32_t parity, int bar) {
+__device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const MultiQueryArgs& a, RowState<Tc<D, NR>::NC / 8> s,
+                                                                     float4 f4, uint32_t s_addr, uint32_t o_addr, int c0,
+                                                                     int quarter, int lane, int prev, uint32_t parity,
+                                                                     int bar) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
   using T = Tc<D, NR>;
   constexpr int NI = T::NC / 8, LI = NI < 4 ? NI : 4;
   const int g = lane >> 2, t4 = lane & 3;
-  const uint32_t vis[4] = {vis4.x, vis4.y, vis4.z, vis4.w};
   const float f[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
   for (int j0 = 0; j0 < NI; j0 += LI) {
@@ -610,8 +636,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
         float m = kNoRef;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float y = __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q];
-          if (vis[q] >> (2 * (j0 + j) + e) & 1) m = fmaxf(m, y);
+          m = fmaxf(m, __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q]);
         }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
@@ -620,7 +645,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
       }
     }
   }
-  s.failed = prev && !tc_wait(prev, parity, a.status);  // the weights of tile i - 1 have been multiplied
+  s.failed = prev >= 0 && !tc_wait(&sh.p_empty[prev & 1], parity, a.status);  // the weights of tile i - 1 have been multiplied
   named_bar_sync(bar, 128);
   tc_fence_after();
 #pragma unroll
@@ -638,7 +663,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
         s.l[j0 + j][e] *= al[j][e];
       }
     }
-    if (prev) {
+    if (prev >= 0) {
 #pragma unroll 1
       for (int o = 0; o < T::NO; ++o) {
         const uint32_t at_o = o_addr + o * NR + 8 * j0;
@@ -653,7 +678,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
       }
     }
   }
-  if (prev) {
+  if (prev >= 0) {
     tc_wait_st();
     tc_fence_before();
   }
@@ -664,9 +689,10 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
 // value that is not finite is taken out too and added for the rows that see it when
 // the stream ends. One thread a token; `v` is the tile's first value unit.
 template <int D, int NR, int VK>
-__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, char* v_smem, Ring v,
-                                          int tok) {
+__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, Ring v, int tok) {
   using T = Tc<D, NR>;
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
   bool ok = true;
   const int at = d.at[tok / kMqPage] + tok % kMqPage;
   const bool draft = d.flags & kDraftTile, real = token_real(a, d, tok / kMqPage, at);
@@ -674,7 +700,7 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, TcShared<NR>&
 #pragma unroll 1
     for (int k = tok / (kMqPage * T::PPU); k > 0; --k) v.next<T::NV>();
     ok = tc_wait(&sh.v_full[v.s], v.ph, a.status);
-    char* row = v_smem + v.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+    char* row = tc_smem + T::V_OFF + v.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
     // (the order of a thread's 16-byte pieces spreads a warp's over the banks)
     auto piece = [&](int q) {
       return reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
@@ -713,9 +739,10 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, TcShared<NR>&
 // warps are in sh.part, its products are done. O^T, a lane a channel, over the sums,
 // or as a record.
 template <int D, int NR, int VK>
-__device__ __noinline__ void finish_stream(const MultiQueryArgs& a, TcShared<NR>& sh, const TileDesc& d, uint32_t tm, int c0,
-                                           int tok, int bar) {
+__device__ __noinline__ void finish_stream(const MultiQueryArgs& a, int ds, uint32_t tm, int c0, int tok, int bar) {
   using T = Tc<D, NR>;
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
   const bool whole = d.flags & kWhole;
   const int sg = d.seg;
   float* rec = a.recs + (size_t)d.slot * Record<NR, D>::kFloats;
@@ -788,8 +815,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   constexpr int kSoftWarps = T::SOFT, kConvWarps = T::CONV;
   constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;  // two copy warps
   constexpr int kBarConv = 1, kBarGroup = 3;  // named barriers: one per conversion group, one per softmax warpgroup
-  extern __shared__ __align__(1024) char smem[];  // (no static shared memory: it starts on a 1024-byte boundary)
-  TcShared<NR>& sh = *reinterpret_cast<TcShared<NR>*>(smem + T::END);
+  char* const smem = tc_smem;  // (no static shared memory: it starts on a 1024-byte boundary)
+  TcShared<NR>& sh = tc_shared<D, NR>();
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
   if (warp == kMmaWarp) {
@@ -874,7 +901,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         const bool first = i == 0 || p.tile == 0;
         if (first) {
           ++seg;
-          high_edge = w.pos0 + describe_rows(a, sh, w, p.chunk, seg % kDesc, lane) - a.window;
+          high_edge = w.pos0 + describe_rows<D, NR>(a, w, p.chunk, seg % kDesc, lane) - a.window;
         }
         int at = -1;
         bool clean = lane >= here;  // every row sees all of the page
@@ -1128,14 +1155,14 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         ahead = true;
       }
       if (flags & kFirst) {
-        load_queries<D, NR, VK>(a, sh, d, smem + T::Q_OFF, ct, grp, bar);
+        load_queries<D, NR, VK>(a, ds, ct, grp, bar);
       }
       const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
       if (draft) {
-        draft_keys<D, NR, VK>(a, sh, d, ds, keys, ct);
+        draft_keys<D, NR, VK>(a, ds, keys, ct);
       } else {
         const char* codes = codes_of(i);
-        if (scaled) convert_scaled<D, NR>(sh, d, ds, codes, scales, keys, ct);
+        if (scaled) convert_scaled<D, NR>(ds, codes, scales, keys, ct);
         else convert_keys<D, false>(d, codes, scales, keys, ct, 1.f, 1.f);
       }
       if (ct == 0) sh.scaled[ds] = scaled || draft;
@@ -1161,7 +1188,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // would cost a cycle per row and warp, as many as the exponentials do).
     constexpr int NC = T::NC, NI = NC / 8;     // rows of the warpgroup; pairs of rows of a thread
     constexpr int LI = NI < 4 ? NI : 4;        // pairs per load
-    const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC, wt = tid % 128;
+    const int wg = warp / 4, quarter = warp % 4, tok = quarter * 32 + lane, c0 = wg * NC;
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
@@ -1183,14 +1210,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       failed |= !ok;
       const TileDesc& d = sh.desc[ds];
       const int flags = ok ? d.flags : 0, pages = ok ? d.pages : 0, sg = ok ? d.seg : 0;
-      const bool draft = flags & kDraftTile, masked = flags & kMasked;
-      // rows that see a token: a bit each, for tokens g, g + 8 of the first page and
-      // of the second
-      uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-      if (masked) {
-        const uint4 m = visible_rows<NR, 2 * NI>(a, sh, d, c0, quarter, lane);
-        vis[0] = m.x; vis[1] = m.y; vis[2] = m.z; vis[3] = m.w;
-      }
+      const bool masked = flags & kMasked;
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
       if (named_bar_or(bar, 128, failed)) break;
       tc_fence_after();
@@ -1202,13 +1222,17 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           l[j][0] = l[j][1] = 0.f;
         }
       }
+      const uint32_t s_addr = tm + lanes + sb * NR + c0;
+      if (masked) mask_tile<D, NR>(a, ds, s_addr, c0, tok);
       float f[4];
       f[0] = f[1] = f[2] = f[3] = sh.qscale[sg] * kLog2e;
       if (sh.scaled[ds]) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) f[q] *= sh.kscale[ds][quarter * 32 + 8 * q + g];
+        for (int q = 0; q < 4; ++q) {  // (a token that is not there: any finite scale, its logits are -inf)
+          const float k = sh.kscale[ds][quarter * 32 + 8 * q + g];
+          f[q] *= k > 0.f && k < 3e38f ? k : 1.f;
+        }
       }
-      const uint32_t s_addr = tm + lanes + sb * NR + c0;
 
       // pass 1: does some logit exceed its row's reference by more than kLazy?
       float over = -INFINITY;
@@ -1223,10 +1247,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             const uint32_t* xx = &x[q / 2][4 * j + 2 * (q % 2)];
             float y0, y1;
             fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
-            if (masked) {
-              if (!(vis[q] >> (2 * (j0 + j)) & 1)) y0 = -INFINITY;
-              if (!(vis[q] >> (2 * (j0 + j) + 1) & 1)) y1 = -INFINITY;
-            }
             over = fmax3f(over, y0, y1);
           }
         }
@@ -1241,9 +1261,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             rows.l[j][e] = l[j][e];
           }
         }
-        rows = raise_references<D, NR>(a, sh, rows, make_uint4(vis[0], vis[1], vis[2], vis[3]),
-                                       make_float4(f[0], f[1], f[2], f[3]), s_addr, tm + lanes + T::COLS_O + c0, c0, quarter,
-                                       lane, started ? &sh.p_empty[(i - 1) % T::NP] : nullptr, ((i - 1) / T::NP) & 1, bar);
+        rows = raise_references<D, NR>(a, rows, make_float4(f[0], f[1], f[2], f[3]), s_addr, tm + lanes + T::COLS_O + c0, c0,
+                                       quarter, lane, started ? (i - 1) % T::NP : -1, ((i - 1) / T::NP) & 1, bar);
         failed |= rows.failed;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
@@ -1272,16 +1291,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
             y0 = exp2_fast(y0);
             y1 = exp2_fast(y1);
-            if (masked) {
-              if (!(vis[q] >> (2 * (j0 + j)) & 1)) y0 = 0.f;
-              if (!(vis[q] >> (2 * (j0 + j) + 1) & 1)) y1 = 0.f;
-            }
             add2_rn(l[j0 + j][0], l[j0 + j][1], l[j0 + j][0], l[j0 + j][1], y0, y1);
             *reinterpret_cast<uint32_t*>(at + q * 8 * 128) = pack16<VK>(y0, y1);
           }
         }
       }
-      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, sh, d, smem + T::V_OFF, v, tok);
+      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, ds, v, tok);
 #pragma unroll 1
       for (int k = 0; k < pages; k += T::PPU) v.next<T::NV>();
       fence_proxy_async_smem();
@@ -1314,7 +1329,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         // (the product waited for every warp's weights: the list of odd values is complete)
         failed |= !tc_wait(&sh.p_empty[pb], (i / T::NP) & 1, a.status);
         named_bar_sync(bar, 128);
-        finish_stream<D, NR, VK>(a, sh, d, tm + lanes, c0, tok, bar);
+        finish_stream<D, NR, VK>(a, ds, tm + lanes, c0, tok, bar);
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
       }
     }
