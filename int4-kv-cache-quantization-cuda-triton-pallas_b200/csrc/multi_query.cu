@@ -40,6 +40,9 @@ cudaError_t run(const MultiQueryArgs& a, int dim, int vk, void* workspace, size_
   if (!aligned16(workspace) || !workspace) return cudaErrorInvalidValue;
   int sms = 0;
   if ((long long)a.total_rows * a.kv_heads * a.group_q > 0x7fffffffll) return cudaErrorInvalidValue;
+  // the kernels count tiles of at least 32 tokens and chunks of at least 4 rows in 31 bits
+  const double tiles = (a.max_pages / 2 + 4.0) * ((double)std::max(1, a.max_drafts) * a.group_q / 4 + 1);
+  if (tiles * a.batch * a.kv_heads > 2e9) return cudaErrorInvalidValue;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   if (a.qk != INT4KV_VALUES_F32) return multi_query_tc(a, dim, sms, workspace, bytes, stream);

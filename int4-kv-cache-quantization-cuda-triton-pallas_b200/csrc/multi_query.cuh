@@ -136,23 +136,23 @@ struct TileAt {
   int b, head, chunk, tile;
 };
 
+// (Counts of tiles fit 31 bits: checked on the host for the largest lengths.)
 template <int NR, int TP>
-I4KV_DEVINL long long seq_units(const MultiQueryArgs& a, int b, bool report) {
+I4KV_DEVINL int seq_units(const MultiQueryArgs& a, int b, bool report) {
   const SeqWork w = seq_work<NR, TP>(a, b, report);
-  return (long long)w.tiles * w.chunks * a.kv_heads;
+  return w.tiles * w.chunks * a.kv_heads;
 }
 
 // First tile of CTA c of n (n <= total): contiguous runs of equal length.
-static __device__ __noinline__ long long tile_div(long long x, long long n) { return floor_div_s52(x, n); }
-I4KV_DEVINL long long run_start(long long c, long long total, long long n) { return tile_div(c * total, n); }
-I4KV_DEVINL long long run_of(long long u, long long total, long long n) { return tile_div((u + 1) * n - 1, total); }
+I4KV_DEVINL int run_start(int c, int total, int n) { return (int)((long long)c * total / n); }
+I4KV_DEVINL int run_of(int u, int total, int n) { return (int)((((long long)u + 1) * n - 1) / total); }
 
-I4KV_DEVINL TileAt tile_at(const MultiQueryArgs& a, const SeqWork& w, int b, long long rem) {
+static __device__ __noinline__ TileAt tile_at(const MultiQueryArgs& a, const SeqWork w, int b, int rem) {
   TileAt p;
   const int per_head = w.tiles * w.chunks;
   p.b = b;
-  p.head = (int)tile_div(rem, per_head);
-  const int r = (int)(rem - (long long)p.head * per_head);
+  p.head = rem / per_head;
+  const int r = rem - p.head * per_head;
   p.chunk = r / w.tiles;
   p.tile = r - p.chunk * w.tiles;
   return p;
@@ -161,41 +161,34 @@ I4KV_DEVINL TileAt tile_at(const MultiQueryArgs& a, const SeqWork& w, int b, lon
 // A CTA's run: its tiles u0 .. u0 + tiles - 1 of all, of which the first lies in
 // sequence b, rem tiles after that sequence's first.
 struct RunPlan {
-  long long total, runs, u0, rem;
-  int tiles, b;
+  int total, runs, u0, rem, tiles, b;
 };
 
 // ... by one converged warp, from the lengths alone (every CTA finds its own).
 template <int NR, int TP>
 __device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int ctas) {
   const int lane = threadIdx.x & 31;
-  long long first = 0, total = 0;
+  RunPlan p = {};
+  int first = 0;
 #pragma unroll 1
   for (int base = 0; base < a.batch; base += 32) {
-    long long n = 0;
-    if (base + lane < a.batch) n = seq_units<NR, TP>(a, base + lane, cta == 0);
+    const int n = base + lane < a.batch ? seq_units<NR, TP>(a, base + lane, cta == 0) : 0;
     if (base == 0) first = n;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
+    p.total += __reduce_add_sync(0xffffffffu, n);
   }
-  RunPlan p;
-  p.total = total;
-  p.runs = min((long long)ctas, total);
-  p.u0 = p.rem = 0;
-  p.tiles = p.b = 0;
+  p.runs = min(ctas, p.total);
   if (cta >= p.runs) return p;
-  p.u0 = run_start(cta, total, p.runs);
-  p.tiles = (int)(run_start(cta + 1, total, p.runs) - p.u0);
-  long long before = 0;
+  p.u0 = run_start(cta, p.total, p.runs);
+  p.tiles = run_start(cta + 1, p.total, p.runs) - p.u0;
+  int before = 0;
 #pragma unroll 1
   for (int base = 0; base < a.batch; base += 32) {
-    long long n = first;
+    int n = first;
     if (base > 0) n = base + lane < a.batch ? seq_units<NR, TP>(a, base + lane, false) : 0;
-    long long incl = n;
+    int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
     const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > p.u0);
@@ -203,7 +196,7 @@ __device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int c
       const int l = __ffs(hit) - 1;
       p.b = base + l;
       p.rem = p.u0 - before - __shfl_sync(0xffffffffu, incl - n, l);
-      return p;
+      break;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
@@ -211,16 +204,17 @@ __device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int c
 }
 
 // The note of a run's last stream (tile `t` of it is the run's last).
-I4KV_DEVINL void note_tail(const MultiQueryArgs& a, int cta, const RunPlan& p, const SeqWork& w, const TileAt& t, int nr) {
+static __device__ __noinline__ void note_tail(const MultiQueryArgs& a, int cta, const RunPlan p, const SeqWork w, const TileAt t,
+                                              int nr) {
   RunTail n = {};
-  const long long end = p.u0 + p.tiles, first = end - 1 - t.tile;  // the stream's first tile
+  const int end = p.u0 + p.tiles, first = end - 1 - t.tile;  // the stream's first tile
   if (t.tile + 1 < w.tiles && first >= p.u0) {
     n.rows = w.rows;
     n.row0 = w.row0;
     n.head = t.head;
     n.first_row = t.chunk * nr;
     n.slot = 2 * cta + (first > p.u0 ? 1 : 0);
-    n.last = (int)run_of(first + w.tiles - 1, p.total, p.runs);
+    n.last = run_of(first + w.tiles - 1, p.total, p.runs);
   }
   a.tails[cta] = n;
 }
@@ -297,7 +291,7 @@ struct Record {
 
 // Rows of sequences that see nothing (a window over an empty cache) are zeros.
 template <int NR, int TP, int D>
-__device__ void zero_idle_rows(const MultiQueryArgs& a) {
+__device__ __noinline__ void zero_idle_rows(const MultiQueryArgs& a) {
 #pragma unroll 1
   for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
     const SeqWork w = seq_work<NR, TP>(a, b, false);

@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     if (tid == 0) a.tails[cta] = RunTail{};
     return;
   }
-  const long long u0 = plan.u0, u1 = u0 + plan.tiles;
+  const int u0 = plan.u0, u1 = u0 + plan.tiles;
 
   SeqWork w = seq_work<NR, TP>(a, plan.b, false), nw = w;  // of the current tile, of the next copied one
   TileAt p = tile_at(a, w, plan.b, plan.rem), np = p;
@@ -136,12 +136,12 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
 
   if (warp == 0) issue(0);
   step(nw, np);
-  long long copied = u0 + 1;
+  int copied = u0 + 1;
   int max_edge = -1;
   bool fresh = true;
 
-  for (long long u = u0; u < u1; ++u) {
-    const int st = (int)((u - u0) & 1);
+  for (int u = u0; u < u1; ++u) {
+    const int st = (u - u0) & 1;
     const uint32_t parity = (uint32_t)(((u - u0) >> 1) & 1);
     __syncthreads();  // everyone is done with the previous tile
     if (copied < u1) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         }
         __syncthreads();
       }
-      const long long first = u - p.tile;  // the stream's first tile
+      const int first = u - p.tile;  // the stream's first tile
       const bool whole = ends && first >= u0;
       float* rec = a.recs + (size_t)(2 * cta + (first > u0 ? 1 : 0)) *Record<NR, D>::kFloats;
       for (int i = 2 * tid; i < NR * D; i += 2 * kThreads) {

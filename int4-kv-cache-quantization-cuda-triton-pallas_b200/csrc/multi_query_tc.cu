@@ -233,7 +233,7 @@ struct TcShared {
   TileDesc desc[kDesc];
   uint64_t word[kDesc][kMqMaxDrafts];  // per segment: the drafts each draft sees,
   int depth[kDesc][kMqMaxDrafts];      // its ancestors,
-  uint8_t draft[kDesc][NR];            // and each row's draft
+  alignas(8) uint8_t draft[kDesc][NR];  // and each row's draft
   float qscale[kDesc];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
@@ -358,64 +358,82 @@ __device__ __noinline__ int describe_rows(const MultiQueryArgs& a, const SeqWork
   return __reduce_max_sync(0xffffffffu, max(depth[0], depth[1]));
 }
 
+// Largest finite magnitude of 8 16-bit values; and whether any exceeds float16's room.
+template <int VK>
+I4KV_DEVINL float top8(const uint4& u, float top) {
+  float x[8];
+  widen8<VK>(u, x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
+  return top;
+}
+I4KV_DEVINL uint32_t beyond_half(const uint4& u) {  // of bfloat16: magnitude bits >= 2^15's
+  const uint32_t m = 0x7FFF7FFFu, k = 0x7FFF7FFFu - 0x46FF46FFu;  // (| x | + k carries into the sign's place)
+  return (((u.x & m) + k) | ((u.y & m) + k) | ((u.z & m) + k) | ((u.w & m) + k)) & 0x80008000u;
+}
+// 8 16-bit values as float16, times a power of two.
+template <int VK>
+I4KV_DEVINL uint4 to_half8(const uint4& u, float down) {
+  if (VK == INT4KV_VALUES_F16) return u;
+  float x[8];
+  widen8<VK>(u, x);
+  return make_uint4(pack16<INT4KV_VALUES_F16>(x[0] * down, x[1] * down), pack16<INT4KV_VALUES_F16>(x[2] * down, x[3] * down),
+                    pack16<INT4KV_VALUES_F16>(x[4] * down, x[5] * down), pack16<INT4KV_VALUES_F16>(x[6] * down, x[7] * down));
+}
+
+// A common power of two for a stream's queries, where some are beyond float16's
+// range (a bfloat16 input): a conversion group finds it.
+template <int D, int NR, int VK>
+__device__ __noinline__ float query_scale(float top, int ct, int grp, int bar) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (ct % 32 == 0) sh.qmax[grp][ct / 32] = top;
+  named_bar_sync(bar, 128);
+  top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
+  named_bar_sync(bar, 128);  // qmax is free again
+  return top;
+}
+
 // A stream's queries to shared memory, by a conversion group: as they are, for a
 // magnitude below float16's range loses nothing that a logit could show. Only one
-// above it (a bfloat16 input) takes the second pass, with a common power of two. A
-// thread takes 8 channels of a row.
+// above it takes more passes, to find and apply a common power of two. 128 / NR
+// threads take a row together.
 template <int D, int NR, int VK>
 __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int ct, int grp, int bar) {
   TcShared<NR>& sh = tc_shared<D, NR>();
-  char* const q_smem = tc_smem + Tc<D, NR>::Q_OFF;
-  constexpr int kAll = NR * (D / 8) / 128, kBatch = kAll < 8 ? kAll : 8;  // pieces of a thread, in flight
+  constexpr int kShare = 128 / NR, kPieces = D / 8 / kShare > 0 ? D / 8 / kShare : 1;
   const TileDesc& d = sh.desc[ds];
-  const int rows = d.rows, first = d.first_row, row0 = d.row0, head = d.head, seg = d.seg;
-  const int c8 = ct % (D / 8), r0 = ct / (D / 8);
-  float top = 0.f, down = 1.f, up = 1.f;
+  const int r = ct / kShare, rr = d.first_row + r, c0 = ct % kShare * kPieces, seg = d.seg;
+  const bool real = rr < d.rows && c0 < D / 8;
+  const uint4* src = reinterpret_cast<const uint4*>(
+      static_cast<const uint16_t*>(a.q) + (real ? out_row(a, d.row0, d.head, sh.draft[seg][r], rr) : 0) * D);
+  char* const row = tc_smem + Tc<D, NR>::Q_OFF + r * 128;
+  float down = 1.f, up = 1.f, top = 0.f;
 #pragma unroll 1
-  for (int pass = 0;; ++pass) {
-#pragma unroll 1
-    for (int k0 = 0; k0 < kAll; k0 += kBatch) {
-      uint4 raw[kBatch];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int r = r0 + (k0 + k) * (128 / (D / 8)), rr = first + r;
-        raw[k] = make_uint4(0, 0, 0, 0);
-        if (rr < rows)
-          raw[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                        out_row(a, row0, head, sh.draft[seg][r], rr) * D + 8 * c8));
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int r = r0 + (k0 + k) * (128 / (D / 8));
-        uint32_t h[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-        if constexpr (VK == INT4KV_VALUES_BF16) {
-          float x[8];
-          widen8<VK>(raw[k], x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            top = fmaxf(top, fmaxf(finite_abs(x[2 * j]), finite_abs(x[2 * j + 1])));
-            h[j] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down, x[2 * j + 1] * down);
-          }
-        }
-        // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
-        char* row = q_smem + (c8 / 8) * (NR * 128) + r * 128;
-        const int q = c8 % 8 / 2, j = c8 % 2 * 2;
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          const int at = 32 * (j + o) + 8 * q;  // byte of the row
-          *reinterpret_cast<uint2*>(row + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)) = make_uint2(h[2 * o], h[2 * o + 1]);
+  for (int pass = 0; pass < 3; ++pass) {  // as they are; (their maximum; scaled)
+    uint32_t big = 0;
+    if (c0 < D / 8) {
+#pragma unroll 4
+      for (int k = 0; k < kPieces; ++k) {
+        const int c8 = c0 + k;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (real) u = __ldg(src + c8);
+        big |= beyond_half(u);
+        if (pass == 1) {
+          top = top8<VK>(u, top);
+        } else {
+          // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
+          const uint4 h = to_half8<VK>(u, down);
+          char* at = row + (c8 / 8) * (NR * 128) + (c8 & 2 ? 8 : 0);
+          const int p16 = (c8 % 2) * 4 + (c8 % 8) / 4;  // 16-byte piece of the row; the next words' is 2 on
+          *reinterpret_cast<uint2*>(at + ((p16 ^ (r & 7)) << 4)) = make_uint2(h.x, h.y);
+          *reinterpret_cast<uint2*>(at + (((p16 + 2) ^ (r & 7)) << 4)) = make_uint2(h.z, h.w);
         }
       }
     }
-    if (VK == INT4KV_VALUES_F16 || pass == 1) break;
-    if (!named_bar_or(bar, 128, top > kHalfRoom)) break;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (ct % 32 == 0) sh.qmax[grp][ct / 32] = top;
-    named_bar_sync(bar, 128);
-    top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
-    named_bar_sync(bar, 128);  // qmax is free again
-    unit_scale(top, down, up);
+    if (VK == INT4KV_VALUES_F16 || (pass == 0 && !named_bar_or(bar, 128, big))) break;
+    if (pass == 1) unit_scale(query_scale<D, NR, VK>(top, ct, grp, bar), down, up);
   }
   if (ct == 0) sh.qscale[seg] = up;
   fence_proxy_async_smem();
@@ -508,66 +526,70 @@ __device__ __noinline__ void convert_scaled(int ds, const char* codes, const flo
   convert_keys<D, true>(d, codes, scales, keys, ct, down[0], down[1]);
 }
 
-// Drafted keys, with a power of two each.
+// Drafted keys, as they are, or (true) with a power of two each where one of them is
+// beyond float16's range.
 template <int D, int NR, int VK>
-__device__ __noinline__ void draft_keys(const MultiQueryArgs& a, int ds, uint32_t keys, int ct) {
+__device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_t keys, int ct, int bar) {
   TcShared<NR>& sh = tc_shared<D, NR>();
   const TileDesc& d = sh.desc[ds];
-  constexpr int NB = D / 64;
-  const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2;
+  const int lane = ct & 31, g = lane >> 2, t4 = lane & 3, page0 = (ct >> 5) * 2, drafts = d.drafts, pages = d.pages;
+  const uint16_t* const base = static_cast<const uint16_t*>(a.kd) + ((size_t)d.row0 * a.kv_heads + d.head) * D + 16 * t4;
+  const size_t step = (size_t)a.kv_heads * D;
+  bool scaled = false;
 #pragma unroll 1
-  for (int p = 0; p < 2; ++p) {
-    if (page0 + p >= d.pages) break;  // (nothing there is seen)
-    uint4 raw[2][NB][2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int t = (page0 + p) * kMqPage + g + 8 * r;
-      const uint16_t* src = static_cast<const uint16_t*>(a.kd) + ((size_t)(d.row0 + t) * a.kv_heads + d.head) * D + 16 * t4;
-#pragma unroll
-      for (int blk = 0; blk < NB; ++blk) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          raw[r][blk][e] = make_uint4(0, 0, 0, 0);
-          if (t < d.drafts) raw[r][blk][e] = __ldg(reinterpret_cast<const uint4*>(src + 64 * blk + 8 * e));
+  for (int pass = 0; pass < 2; ++pass) {
+    uint32_t big = 0;
+#pragma unroll 1
+    for (int p = 0; p < 2; ++p) {
+      if (page0 + p >= pages) break;  // (nothing there is seen)
+      const int ta = (page0 + p) * kMqPage + g, tb = ta + 8;
+      const uint16_t *sa = base + ta * step, *sb = base + tb * step;
+      float down[2] = {1.f, 1.f};
+      if (scaled) {
+#pragma unroll 1
+        for (int r = 0; r < 2; ++r) {
+          float top = 0.f, up, dn;
+#pragma unroll 1
+          for (int blk = 0; blk < D / 64; ++blk)
+#pragma unroll 1
+            for (int e = 0; e < 2; ++e)
+              if ((r ? tb : ta) < drafts)
+                top = top8<VK>(__ldg(reinterpret_cast<const uint4*>((r ? sb : sa) + 64 * blk + 8 * e)), top);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          unit_scale(top, dn, up);
+          if (r) down[1] = dn; else down[0] = dn;
+          if (t4 == 0) sh.kscale[ds][r ? tb : ta] = up;
         }
       }
-    }
-    float down[2];
+#pragma unroll 1
+      for (int blk = 0; blk < D / 64; ++blk) {
+        uint4 u[4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float top = 0.f, up;
-#pragma unroll
-      for (int blk = 0; blk < NB; ++blk) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x[8];
-          widen8<VK>(raw[r][blk][e], x);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
+        for (int k = 0; k < 4; ++k) {  // token k / 2, half k % 2 of the channels
+          u[k] = make_uint4(0, 0, 0, 0);
+          if ((k / 2 ? tb : ta) < drafts)
+            u[k] = __ldg(reinterpret_cast<const uint4*>((k / 2 ? sb : sa) + 64 * blk + 8 * (k % 2)));
         }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      unit_scale(top, down[r], up);
-      if (t4 == 0) sh.kscale[ds][(page0 + p) * kMqPage + g + 8 * r] = up;
-    }
+        uint32_t h[16];
 #pragma unroll
-    for (int blk = 0; blk < NB; ++blk) {
-      uint32_t h[16];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x[8];
-          widen8<VK>(raw[r][blk][e], x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
-            h[4 * (2 * e + j / 2) + 2 * r + j % 2] = pack16<INT4KV_VALUES_F16>(x[2 * j] * down[r], x[2 * j + 1] * down[r]);
+        for (int k = 0; k < 4; ++k) {
+          big |= beyond_half(u[k]);
+          const uint4 v = to_half8<VK>(u[k], down[k / 2]);
+          // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
+          h[8 * (k % 2) + 2 * (k / 2)] = v.x;
+          h[8 * (k % 2) + 2 * (k / 2) + 1] = v.y;
+          h[8 * (k % 2) + 4 + 2 * (k / 2)] = v.z;
+          h[8 * (k % 2) + 4 + 2 * (k / 2) + 1] = v.w;
         }
+        __syncwarp();
+        tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
       }
-      tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
     }
+    if (VK == INT4KV_VALUES_F16 || scaled || !named_bar_or(bar, 128, big)) break;
+    scaled = true;
   }
+  return scaled;
 }
 
 // Whether some row sees the token `at` of a tile at all (a cached one).
@@ -584,20 +606,20 @@ template <int D, int NR>
 __device__ __noinline__ void mask_tile(const MultiQueryArgs& a, int ds, uint32_t s_addr, int c0, int tok) {
   TcShared<NR>& sh = tc_shared<D, NR>();
   const TileDesc& d = sh.desc[ds];
-  const int sg = d.seg, page = tok / kMqPage, at = d.at[page] + tok % kMqPage, low = d.low_edge;
+  const int sg = d.seg, page = tok / kMqPage, at = d.at[page] + tok % kMqPage;
   const bool draft = d.flags & kDraftTile, real = token_real(a, d, page, at);
-  const bool edge = !draft && a.window > 0 && at >= a.sinks;
+  // a cached token is seen by row r iff at > low + its draft's depth
+  const int low = a.window > 0 && at >= a.sinks ? d.low_edge : -(1 << 30);
 #pragma unroll 1
   for (int j0 = 0; j0 < Tc<D, NR>::NC; j0 += 8) {
     uint32_t x[8];
     tc_ld8(x, s_addr + j0);
+    const uint2 rows = *reinterpret_cast<const uint2*>(&sh.draft[sg][c0 + j0]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int t = sh.draft[sg][c0 + j0 + j];
-      bool sees = real;
-      if (draft) sees = sees && (sh.word[sg][t] >> (at & 63) & 1);
-      if (edge) sees = sees && at > low + sh.depth[sg][t];
-      if (!sees) x[j] = 0xFF800000u;
+      const int t = (j < 4 ? rows.x >> (8 * j) : rows.y >> (8 * j - 32)) & 63;
+      const bool in_tree = sh.word[sg][t] >> (at & 63) & 1, in_cache = at > low + sh.depth[sg][t];
+      if (!(real && (draft ? in_tree : in_cache))) x[j] = 0xFF800000u;
     }
     __syncwarp();
     tc_st8(s_addr + j0, x);
@@ -707,14 +729,14 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, Ring 
     };
     bool bad = false;
     if (!real) {
-#pragma unroll
+#pragma unroll 4
       for (int q = 0; q < 8 * T::CH; ++q) *piece(q) = make_uint4(0, 0, 0, 0);
     } else {
       // an exponent of all ones carries into the sign's place
       constexpr uint32_t kExp = VK == INT4KV_VALUES_F16 ? 0x7C007C00u : 0x7F807F80u;
       constexpr uint32_t kOne = VK == INT4KV_VALUES_F16 ? 0x04000400u : 0x00800080u;
       uint32_t any = 0;
-#pragma unroll 8
+#pragma unroll 4
       for (int q = 0; q < 8 * T::CH; ++q) {
         const uint4 y = *piece(q);
         any |= ((y.x & kExp) + kOne) | ((y.y & kExp) + kOne) | ((y.z & kExp) + kOne) | ((y.w & kExp) + kOne);
@@ -733,6 +755,30 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, Ring 
   }
   __syncwarp();
   return ok;
+}
+
+// Drafted values that are not finite, for the rows that see them (8 rows from `col`).
+struct Eight {
+  uint32_t x[8];
+};
+template <int D, int NR, int VK>
+__device__ __noinline__ Eight add_odd_values(const MultiQueryArgs& a, int ds, unsigned long long odd, int ch, int col,
+                                             Eight e) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const TileDesc& d = sh.desc[ds];
+#pragma unroll 1
+  for (unsigned long long left = odd; left; left &= left - 1) {
+    const int u = __ffsll(left) - 1;
+    float y2[2];
+    load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
+    const float y = ch & 1 ? y2[1] : y2[0];
+    if (fabsf(y) <= 3.4e38f) continue;
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j)
+      if (sh.word[d.seg][sh.draft[d.seg][col + j]] >> u & 1) e.x[j] = __float_as_uint(__uint_as_float(e.x[j]) + y);
+  }
+  __syncwarp();
+  return e;
 }
 
 // A stream's (or a run's share of it) end, by one softmax warpgroup: the sums of its
@@ -770,18 +816,12 @@ __device__ __noinline__ void finish_stream(const MultiQueryArgs& a, int ds, uint
       uint32_t x[8];
       tc_ld8(x, tm + T::COLS_O + o * NR + col);
       if (odd) {
-#pragma unroll 1
-        for (unsigned long long left = odd; left; left &= left - 1) {
-          const int u = __ffsll(left) - 1;
-          float y2[2];
-          load_f32<2>(a.vd, VK, ((size_t)(d.row0 + u) * a.kv_heads + d.head) * D + (ch & ~1), y2);
-          const float y = ch & 1 ? y2[1] : y2[0];
-          if (fabsf(y) <= 3.4e38f) continue;
+        Eight e;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (sh.word[sg][sh.draft[sg][col + j]] >> u & 1) x[j] = __float_as_uint(__uint_as_float(x[j]) + y);
-        }
-        __syncwarp();
+        for (int j = 0; j < 8; ++j) e.x[j] = x[j];
+        e = add_odd_values<D, NR, VK>(a, ds, odd, ch, col, e);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = e.x[j];
       }
       if (whole) {
         const float4 i0 = *reinterpret_cast<const float4*>(&sh.inv[col]), i1 = *reinterpret_cast<const float4*>(&sh.inv[col + 4]);
@@ -868,7 +908,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // copies the values.
     const bool values = warp > kCopyWarp;
     const RunPlan plan = sh.plan;
-    const long long u0 = plan.u0;
+    const int u0 = plan.u0;
     SeqWork w = seq_work<NR, kTilePages>(a, plan.b, false);
     TileAt p = tile_at(a, w, plan.b, plan.rem);
     int seg = -1, high_edge = 0;
@@ -929,7 +969,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
         if (lane == 0) {
           TileDesc& d = sh.desc[ds];
-          const long long first_u = u0 + i - p.tile;  // the stream's first tile
+          const int first_u = u0 + i - p.tile;  // the stream's first tile
           const bool ends = p.tile + 1 == w.tiles;
           d.flags = (draft ? kDraftTile : 0) | (masked ? kMasked : 0) | (first ? kFirst : 0) |
                     ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= u0) ? kWhole : 0);
@@ -952,26 +992,19 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       } else {
         const CUtensorMap* map = draft ? &dmap : &vmap;
         const int row = draft ? w.row0 + lane * kMqPage : 0, slab = draft ? p.head : phys * a.kv_heads + p.head;
-        int rows[kTilePages], slabs[kTilePages];
-#pragma unroll
-        for (int g = 0; g < kTilePages; ++g) {
-          rows[g] = __shfl_sync(0xffffffffu, row, g);
-          slabs[g] = __shfl_sync(0xffffffffu, slab, g);
-        }
-#pragma unroll
-        for (int g0 = 0; g0 < kTilePages; g0 += T::PPU) {
-          if (g0 >= here) break;
+#pragma unroll 1
+        for (int g0 = 0; g0 < here; g0 += T::PPU) {
           ok = ok && tc_wait(&sh.v_empty[v.s], v.ph ^ 1, a.status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          if (elect_one()) {
-            uint64_t* bar = &sh.v_full[v.s];
-            const uint32_t unit = lives >> g0 & ((1u << T::PPU) - 1);
-            mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
-            char* dst = smem + T::V_OFF + v.s * T::UNIT;
-#pragma unroll
-            for (int q = 0; q < T::PPU; ++q)
-              if (unit >> q & 1) tma_page(dst + q * T::PAGE_V, map, rows[g0 + q], slabs[g0 + q], bar);
+          uint64_t* bar = &sh.v_full[v.s];
+          const uint32_t unit = lives >> g0 & ((1u << T::PPU) - 1);
+          char* dst = smem + T::V_OFF + v.s * T::UNIT;
+          if (elect_one()) mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
+#pragma unroll 1
+          for (int q = 0; q < T::PPU; ++q) {
+            const int y = __shfl_sync(0xffffffffu, row, g0 + q), z = __shfl_sync(0xffffffffu, slab, g0 + q);
+            if ((unit >> q & 1) && elect_one()) tma_page(dst + q * T::PAGE_V, map, y, z, bar);
           }
           __syncwarp();
           v.next<T::NV>();
@@ -995,29 +1028,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     int pages = 0;       // of tile i - 1
     bool fresh = true;   // tile i - 1 starts its segment
     bool ok = true;
-    auto logits = [&](int i) {  // S^T of tile i
-      const int hb = i & 1;
-      ok = ok && tc_wait(&sh.kh_full[hb], (i / 2) & 1, a.status) &&
-           tc_wait(&sh.s_empty[i & 1], (i / 2 + 1) & 1, a.status);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) return;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t keys = tm + T::COLS_K + hb * (D / 2);
-        const uint64_t qd = mat_desc(base + T::Q_OFF, 16, 1024);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma_ts(tm + (i & 1) * NR, keys + k * 8,
-                    qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
-        tc_commit(&sh.s_full[i & 1]);
-        tc_commit(&sh.kh_empty[hb]);
-      }
-      __syncwarp();
-    };
 #pragma unroll 1
     for (int i = 0; i <= n_tiles && ok; ++i) {
       int next_pages = 0;
-      bool next_fresh = false, waiting = i < n_tiles;  // the logits of tile i are still to be issued
+      bool next_fresh = false, keys_first = false;
       if (i < n_tiles) {
         const int ds = i % kDesc;
         ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
@@ -1026,42 +1040,61 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
         // the outputs of tile i - 1 go first where the keys of tile i are not there yet
-        if (i == 0 || __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i & 1], (i / 2) & 1))) {
-          logits(i);
-          waiting = false;
-        }
+        keys_first = __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i & 1], (i / 2) & 1));
       }
-      if (i > 0 && ok) {
-        const int j = i - 1, pb = j % T::NP;
-        ok = __all_sync(0xffffffffu, tc_wait(&sh.p_full[pb], (j / T::NP) & 1, a.status));
-        if (!ok) break;
-        const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P, kTile * 128, 1024);
 #pragma unroll 1
-        for (int g0 = 0; g0 < pages; g0 += T::PPU) {
-          ok = __all_sync(0xffffffffu, tc_wait(&sh.v_full[v.s], v.ph, a.status));
+      for (int turn = 0; turn < 2; ++turn) {
+        if ((turn == 0) == keys_first) {
+          if (i == n_tiles) continue;
+          // S^T of tile i
+          const int hb = i & 1;
+          ok = ok && tc_wait(&sh.kh_full[hb], (i / 2) & 1, a.status) &&
+               tc_wait(&sh.s_empty[hb], (i / 2 + 1) & 1, a.status);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t vd = mat_desc(base + T::V_OFF + v.s * T::UNIT, 2048, 1024);
+            const uint32_t keys = tm + T::COLS_K + hb * (D / 2);
+            const uint64_t qd = mat_desc(base + T::Q_OFF, 16, 1024);
 #pragma unroll
-            for (int q = 0; q < T::PPU; ++q) {
-              if (g0 + q < pages) {
-#pragma unroll
-                for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
-                  tc_mma(tm + T::COLS_O + o * NR, vd + (q * T::PAGE_V + o * 4096) / 16, pd + (g0 + q) * (2048 / 16),
-                         kPv, !(fresh && g0 + q == 0));
-              }
-            }
-            tc_commit(&sh.v_empty[v.s]);
+            for (int k = 0; k < D / 16; ++k)
+              tc_mma_ts(tm + hb * NR, keys + k * 8, qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
+            tc_commit(&sh.s_full[hb]);
+            tc_commit(&sh.kh_empty[hb]);
           }
           __syncwarp();
-          v.next<T::NV>();
+        } else if (i > 0) {
+          // O^T of tile i - 1
+          const int j = i - 1, pb = j % T::NP;
+          ok = ok && tc_wait(&sh.p_full[pb], (j / T::NP) & 1, a.status);
+          const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P, kTile * 128, 1024);
+#pragma unroll 1
+          for (int g0 = 0; g0 < pages; g0 += T::PPU) {
+            ok = ok && tc_wait(&sh.v_full[v.s], v.ph, a.status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vd = mat_desc(base + T::V_OFF + v.s * T::UNIT, 2048, 1024);
+#pragma unroll
+              for (int q = 0; q < T::PPU; ++q) {
+                if (g0 + q < pages) {
+#pragma unroll
+                  for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
+                    tc_mma(tm + T::COLS_O + o * NR, vd + (q * T::PAGE_V + o * 4096) / 16, pd + (g0 + q) * (2048 / 16),
+                           kPv, !(fresh && g0 + q == 0));
+                }
+              }
+              tc_commit(&sh.v_empty[v.s]);
+            }
+            __syncwarp();
+            v.next<T::NV>();
+          }
+          if (!ok) break;
+          if (elect_one()) tc_commit(&sh.p_empty[pb]);
+          __syncwarp();
         }
-        if (!ok) break;
-        if (elect_one()) tc_commit(&sh.p_empty[pb]);
-        __syncwarp();
       }
-      if (waiting && ok) logits(i);
       pages = next_pages;
       fresh = next_fresh;
     }
@@ -1107,65 +1140,67 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       cp_async_commit();
     };
     bool ok = true;
-    if (grp < n_tiles) {
-      ok = tc_wait(&sh.desc_full[grp], 0, a.status);
-      if (ok) prefetch(sh.desc[grp], grp);
-    }
+    // (the first turn, before the group's first tile, only starts that tile's copies)
 #pragma unroll 1
-    for (int i = grp; i < n_tiles; i += 2) {
-      const int ds = i % kDesc;
+    for (int i = grp - 2; i < n_tiles; i += 2) {
+      const int ds = i & (kDesc - 1), next = i + 2;
       const TileDesc& d = sh.desc[ds];
-      const int flags = d.flags;
+      const int flags = i >= 0 ? d.flags : 0;
       const bool draft = flags & kDraftTile;
-      // Scale and zero point, in place: a code c enters as 1 + c / 128 (its bits in
-      // the mantissa), so a key is (1 + c / 128) e + z with e = 128 s, z = -zp s - e.
       float* scales = scales_of(i);
-      float key_top = 0.f;
-      cp_async_wait<0>();
+      bool scaled = false;
+      if (i >= 0) {
+        // Scale and zero point, in place: a code c enters as 1 + c / 128 (its bits in
+        // the mantissa), so a key is (1 + c / 128) e + z with e = 128 s, z = -zp s - e.
+        float key_top = 0.f;
+        cp_async_wait<0>();
 #pragma unroll 1
-      for (uint32_t left = ok ? d.slots : 0u; left; left &= left - 1) {
-        float* sz = scales + (__ffs(left) - 1) * (2 * D) + ct;
+        for (uint32_t left = ok ? d.slots : 0u; left; left &= left - 1) {
+          float* sz = scales + (__ffs(left) - 1) * (2 * D) + ct;
 #pragma unroll
-        for (int ch = 0; ch < D; ch += 128) {
-          if (D >= 128 || ct < D) {
-            const float s = sz[ch], z = -sz[D + ch] * s;
-            key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
-            sz[ch] = 128.f * s;
-            sz[D + ch] = fmaf(-128.f, s, z);
+          for (int ch = 0; ch < D; ch += 128) {
+            if (D >= 128 || ct < D) {
+              const float s = sz[ch], z = -sz[D + ch] * s;
+              key_top = fmaxf(key_top, fmaxf(finite_abs(z), finite_abs(fmaf(15.f, s, z))));
+              sz[ch] = 128.f * s;
+              sz[D + ch] = fmaf(-128.f, s, z);
+            }
           }
         }
+        // A new stream's queries replace the last one's: every product with those
+        // is done. Otherwise the keys of tile i - 2 have been multiplied.
+        if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
+        ok = ok && tc_wait(&sh.kh_empty[i & 1], (i / 2 + 1) & 1, a.status);
+        // Keys beyond float16's range take a power of two per group.
+        if (named_bar_or(bar, 128, !ok || key_top > kHalfRoom)) {
+          // (uniform over the group: its warps meet in named barriers)
+          if (named_bar_or(bar, 128, !ok)) break;
+          scaled = true;
+        }
+        tc_fence_after();
       }
-      // A new stream's queries replace the last one's: every product with those
-      // is done. Otherwise the keys of tile i - 2 have been multiplied.
-      if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
-      ok = ok && tc_wait(&sh.kh_empty[i & 1], (i / 2 + 1) & 1, a.status);
-      // Keys beyond float16's range take a power of two per group.
-      bool scaled = false;
-      if (named_bar_or(bar, 128, !ok || key_top > kHalfRoom)) {
-        // (uniform over the group: its warps meet in named barriers)
-        if (named_bar_or(bar, 128, !ok)) break;
-        scaled = true;
+      if (T::NB > 1 && next < n_tiles) {
+        ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+        if (ok) prefetch(sh.desc[next % kDesc], next);
       }
-      tc_fence_after();
-      // the next tile's copies, now if its descriptor is there (else at the end)
-      const int next = i + 2;
-      bool ahead = false;
-      if (T::NB > 1 && next < n_tiles && mbar_test(&sh.desc_full[next % kDesc], (next / kDesc) & 1)) {
-        prefetch(sh.desc[next % kDesc], next);
-        ahead = true;
+      if (i < 0) {
+        if (T::NB > 1) continue;
+        if (next < n_tiles) {
+          ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+          if (ok) prefetch(sh.desc[next % kDesc], next);
+        }
+        continue;
       }
-      if (flags & kFirst) {
-        load_queries<D, NR, VK>(a, ds, ct, grp, bar);
-      }
+      if (flags & kFirst) load_queries<D, NR, VK>(a, ds, ct, grp, bar);
       const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
       if (draft) {
-        draft_keys<D, NR, VK>(a, ds, keys, ct);
+        scaled = draft_keys<D, NR, VK>(a, ds, keys, ct, bar);
       } else {
         const char* codes = codes_of(i);
         if (scaled) convert_scaled<D, NR>(ds, codes, scales, keys, ct);
         else convert_keys<D, false>(d, codes, scales, keys, ct, 1.f, 1.f);
       }
-      if (ct == 0) sh.scaled[ds] = scaled || draft;
+      if (ct == 0) sh.scaled[ds] = scaled;
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -1173,10 +1208,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         mbar_arrive(&sh.kh_full[i & 1]);
         mbar_arrive(&sh.desc_empty[ds]);
       }
-      if (T::NB == 1) named_bar_sync(bar, 128);
-      if (next < n_tiles && !ahead) {
-        ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
-        if (ok) prefetch(sh.desc[next % kDesc], next);
+      if (T::NB == 1) {
+        named_bar_sync(bar, 128);
+        if (next < n_tiles) {
+          ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+          if (ok) prefetch(sh.desc[next % kDesc], next);
+        }
       }
     }
     cp_async_wait<0>();
