@@ -41,7 +41,7 @@ cudaError_t run(const MultiQueryArgs& a, int dim, int vk, void* workspace, size_
   int sms = 0;
   if ((long long)a.total_rows * a.kv_heads * a.group_q > 0x7fffffffll) return cudaErrorInvalidValue;
   // the kernels count tiles of at least 32 tokens and chunks of at least 4 rows in 31 bits
-  const double tiles = (a.max_pages / 2 + 4.0) * ((double)std::max(1, a.max_drafts) * a.group_q / 4 + 1);
+  const double tiles = (a.max_pages / 2 + 12.0) * ((double)std::max(1, a.max_drafts) * a.group_q / 4 + 1);
   if (tiles * a.batch * a.kv_heads > 2e9) return cudaErrorInvalidValue;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;

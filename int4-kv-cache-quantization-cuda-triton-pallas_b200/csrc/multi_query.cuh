@@ -7,8 +7,9 @@
 // block lies in one quantization group wherever groups are that long) that hold
 // visible pages, those of the sinks and those of the window, then the drafted
 // tokens. The streams' tiles are laid end to end and
-// every CTA takes one contiguous run of equal length, so the CTAs do the same
-// number of tiles whatever the lengths are. A stream inside one run is finished
+// every CTA takes one contiguous run of equal cost, whatever the lengths are: a
+// tile costs one unit, and what a stream costs besides (its queries, its end, and
+// drafts' masks) is counted as a few units before its first tile. A stream inside one run is finished
 // by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per
 // row, and the first of them a note of who shares it (RunTail), by which
 // merge_records_kernel, one block per run, combines them. Records and notes need
@@ -136,14 +137,8 @@ struct TileAt {
   int b, head, chunk, tile;
 };
 
-// (Counts of tiles fit 31 bits: checked on the host for the largest lengths.)
-template <int NR, int TP>
-I4KV_DEVINL int seq_units(const MultiQueryArgs& a, int b, bool report) {
-  const SeqWork w = seq_work<NR, TP>(a, b, report);
-  return w.tiles * w.chunks * a.kv_heads;
-}
-
-// First tile of CTA c of n (n <= total): contiguous runs of equal length.
+// Unit at which run c of n begins, and the run of a unit. (Counts of units fit 31
+// bits: checked on the host for the largest lengths.)
 I4KV_DEVINL int run_start(int c, int total, int n) { return (int)((long long)c * total / n); }
 I4KV_DEVINL int run_of(int u, int total, int n) { return (int)((((long long)u + 1) * n - 1) / total); }
 
@@ -158,48 +153,79 @@ static __device__ __noinline__ TileAt tile_at(const MultiQueryArgs& a, const Seq
   return p;
 }
 
-// A CTA's run: its tiles u0 .. u0 + tiles - 1 of all, of which the first lies in
-// sequence b, rem tiles after that sequence's first.
+// A CTA's run: `tiles` tiles, the first of them tile `rem` of sequence b; all runs
+// together have `total` units, and this one's end before unit `end`.
 struct RunPlan {
-  int total, runs, u0, rem, tiles, b;
+  int total, runs, end, tiles, b, rem;
 };
 
-// ... by one converged warp, from the lengths alone (every CTA finds its own).
-template <int NR, int TP>
+// ... by one converged warp, from the lengths alone (every CTA finds its own). A
+// stream costs EXTRA units besides its tiles, DRAFT more with drafts.
+template <int NR, int TP, int EXTRA, int DRAFT>
 __device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int ctas) {
   const int lane = threadIdx.x & 31;
   RunPlan p = {};
-  int first = 0;
+  // units and tiles of this lane's sequence of the 32 from `base` on
+  int tiles = 0, units = 0, extra = 0, streams = 0;
+  auto of_sequence = [&](int base, bool report) {
+    tiles = units = streams = extra = 0;
+    if (base + lane < a.batch) {
+      const SeqWork w = seq_work<NR, TP>(a, base + lane, report);
+      if (w.tiles > 0) {
+        tiles = w.tiles;
+        extra = EXTRA + (w.drafts > 0 ? DRAFT : 0);
+        streams = w.chunks * a.kv_heads;
+        units = streams * (tiles + extra);
+      }
+    }
+  };
 #pragma unroll 1
   for (int base = 0; base < a.batch; base += 32) {
-    const int n = base + lane < a.batch ? seq_units<NR, TP>(a, base + lane, cta == 0) : 0;
-    if (base == 0) first = n;
-    p.total += __reduce_add_sync(0xffffffffu, n);
+    of_sequence(base, cta == 0);
+    p.total += __reduce_add_sync(0xffffffffu, units);
   }
   p.runs = min(ctas, p.total);
   if (cta >= p.runs) return p;
-  p.u0 = run_start(cta, p.total, p.runs);
-  p.tiles = run_start(cta + 1, p.total, p.runs) - p.u0;
-  int before = 0;
+  const int begin = run_start(cta, p.total, p.runs);
+  p.end = run_start(cta + 1, p.total, p.runs);
+  // tiles before the run's first unit and before its end
+  int before = 0, tiles_before = 0, first_tile = 0, last_tile = -1;
 #pragma unroll 1
-  for (int base = 0; base < a.batch; base += 32) {
-    int n = first;
-    if (base > 0) n = base + lane < a.batch ? seq_units<NR, TP>(a, base + lane, false) : 0;
-    int incl = n;
+  for (int base = 0; base < a.batch && last_tile < 0; base += 32) {
+    if (a.batch > 32) of_sequence(base, false);
+    int iu = units, it = streams * tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const int u = __shfl_up_sync(0xffffffffu, iu, o), t = __shfl_up_sync(0xffffffffu, it, o);
+      if (lane >= o) {
+        iu += u;
+        it += t;
+      }
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > p.u0);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      p.b = base + l;
-      p.rem = p.u0 - before - __shfl_sync(0xffffffffu, incl - n, l);
-      break;
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      const int u = k ? p.end : begin;
+      // the sequence of unit u; for the run's end, of the unit before it
+      const uint32_t hit = __ballot_sync(0xffffffffu, before + iu > (k ? u - 1 : u) && before + iu - units <= (k ? u - 1 : u));
+      if (!hit) continue;
+      const int l = __ffs(hit) - 1, off = u - before - (iu - units), per = tiles + extra;
+      // (lane l's own numbers) whole streams before u, then tiles of the one u lies in
+      const int whole = per > 0 ? off / per : 0;
+      const int in_seq = whole * tiles + max(0, off - whole * per - extra);
+      const int at = __shfl_sync(0xffffffffu, in_seq, l);
+      const int all = tiles_before + __shfl_sync(0xffffffffu, it - streams * tiles, l) + at;
+      if (k) {
+        last_tile = all;
+      } else {
+        first_tile = all;
+        p.b = base + l;
+        p.rem = at;
+      }
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    before += __shfl_sync(0xffffffffu, iu, 31);
+    tiles_before += __shfl_sync(0xffffffffu, it, 31);
   }
+  p.tiles = last_tile - first_tile;
   return p;
 }
 
@@ -207,14 +233,14 @@ __device__ __noinline__ RunPlan plan_run(const MultiQueryArgs& a, int cta, int c
 static __device__ __noinline__ void note_tail(const MultiQueryArgs& a, int cta, const RunPlan p, const SeqWork w, const TileAt t,
                                               int nr) {
   RunTail n = {};
-  const int end = p.u0 + p.tiles, first = end - 1 - t.tile;  // the stream's first tile
-  if (t.tile + 1 < w.tiles && first >= p.u0) {
+  const int first = p.tiles - 1 - t.tile;  // the stream's first tile, of the run's
+  if (t.tile + 1 < w.tiles && first >= 0) {
     n.rows = w.rows;
     n.row0 = w.row0;
     n.head = t.head;
     n.first_row = t.chunk * nr;
-    n.slot = 2 * cta + (first > p.u0 ? 1 : 0);
-    n.last = run_of(first + w.tiles - 1, p.total, p.runs);
+    n.slot = 2 * cta + (first > 0 ? 1 : 0);
+    n.last = run_of(p.end + w.tiles - 2 - t.tile, p.total, p.runs);  // (the units from here on are its tiles)
   }
   a.tails[cta] = n;
 }

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   zero_idle_rows<NR, TP, D>(a);
   const int cta = blockIdx.x;
   if (warp == 0) {
-    const RunPlan mine = plan_run<NR, TP>(a, cta, gridDim.x);
+    const RunPlan mine = plan_run<NR, TP, 1, 1>(a, cta, gridDim.x);
     if (lane == 0) s_plan = mine;
   }
   __syncthreads();
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     if (tid == 0) a.tails[cta] = RunTail{};
     return;
   }
-  const int u0 = plan.u0, u1 = u0 + plan.tiles;
+  const int u1 = plan.tiles;
 
   SeqWork w = seq_work<NR, TP>(a, plan.b, false), nw = w;  // of the current tile, of the next copied one
   TileAt p = tile_at(a, w, plan.b, plan.rem), np = p;
@@ -136,13 +136,12 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
 
   if (warp == 0) issue(0);
   step(nw, np);
-  int copied = u0 + 1;
-  int max_edge = -1;
+  int copied = 1;
   bool fresh = true;
 
-  for (int u = u0; u < u1; ++u) {
-    const int st = (u - u0) & 1;
-    const uint32_t parity = (uint32_t)(((u - u0) >> 1) & 1);
+  for (int u = 0; u < u1; ++u) {
+    const int st = u & 1;
+    const uint32_t parity = (uint32_t)((u >> 1) & 1);
     __syncthreads();  // everyone is done with the previous tile
     if (copied < u1) {
       if (warp == 0) issue(st ^ 1);
@@ -378,8 +377,8 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         __syncthreads();
       }
       const int first = u - p.tile;  // the stream's first tile
-      const bool whole = ends && first >= u0;
-      float* rec = a.recs + (size_t)(2 * cta + (first > u0 ? 1 : 0)) *Record<NR, D>::kFloats;
+      const bool whole = ends && first >= 0;
+      float* rec = a.recs + (size_t)(2 * cta + (first > 0 ? 1 : 0)) *Record<NR, D>::kFloats;
       for (int i = 2 * tid; i < NR * D; i += 2 * kThreads) {
         const int r = i / D, c = i - r * D, rr = p.chunk * NR + r;
         if (rr >= w.rows) continue;

@@ -51,7 +51,10 @@ using namespace i4kv;
 namespace {
 
 constexpr int kTile = 128, kTilePages = kTile / kMqPage;
-constexpr int kDesc = 4;                        // tiles in flight between the roles
+constexpr int kDesc = 8, kSeg = 4;              // tiles, and streams, in flight between the roles
+// What a stream costs besides its tiles, in tiles: its queries and its end; the
+// masks of its drafts (measured: 6 and 6 us of 1.5 to 3 us a tile).
+constexpr int kStreamUnits = 2, kDraftUnits = 2;
 constexpr uint64_t kTcWaitNs = 2000000000ull;   // bounded waits: 2 s
 constexpr float kLazy = 8.f;                    // weights reach 2^8 before a rescale
 
@@ -231,17 +234,17 @@ struct TcShared {
   uint64_t desc_full[kDesc], desc_empty[kDesc], v_full[8], v_empty[8];
   uint64_t kh_full[2], kh_empty[2], s_full[2], s_empty[2], p_full[2], p_empty[2];
   TileDesc desc[kDesc];
-  uint64_t word[kDesc][kMqMaxDrafts];  // per segment: the drafts each draft sees,
-  int depth[kDesc][kMqMaxDrafts];      // its ancestors,
-  alignas(8) uint8_t draft[kDesc][NR];  // and each row's draft
-  float qscale[kDesc];
+  uint64_t word[kSeg][kMqMaxDrafts];  // per segment: the drafts each draft sees,
+  int depth[kSeg][kMqMaxDrafts];      // its ancestors,
+  alignas(8) uint8_t draft[kSeg][NR];  // and each row's draft
+  float qscale[kSeg];
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
   float ref[NR], inv[NR];       // a finished stream's references, inverse sums,
   int row[NR];                  // and rows of the outputs [rows * heads]
   float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
   float qmax[2][4];
-  unsigned long long odd[kDesc];  // per segment: drafts whose values are not all finite
+  unsigned long long odd[kSeg];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
   RunPlan plan;
 };
@@ -890,7 +893,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
   if (!a.offs) zero_idle_rows<NR, kTilePages, D>(a);
   const int cta = blockIdx.x;
   if (warp == kCopyWarp) {
-    const RunPlan mine = plan_run<NR, kTilePages>(a, cta, gridDim.x);
+    const RunPlan mine = plan_run<NR, kTilePages, kStreamUnits, kDraftUnits>(a, cta, gridDim.x);
     if (lane == 0) {
       sh.plan = mine;
       if (mine.tiles == 0) a.tails[cta] = RunTail{};
@@ -908,10 +911,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // copies the values.
     const bool values = warp > kCopyWarp;
     const RunPlan plan = sh.plan;
-    const int u0 = plan.u0;
     SeqWork w = seq_work<NR, kTilePages>(a, plan.b, false);
     TileAt p = tile_at(a, w, plan.b, plan.rem);
     int seg = -1, high_edge = 0;
+    int end1 = -1, end2 = -1, end3 = -1;  // last tiles of the streams before the last one, ..
     Ring v;
     bool ok = true;
     // this lane's page of tile p: loaded one tile ahead of its use
@@ -940,8 +943,14 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         if (!ok) break;
         const bool first = i == 0 || p.tile == 0;
         if (first) {
-          ++seg;
-          high_edge = w.pos0 + describe_rows<D, NR>(a, w, p.chunk, seg % kDesc, lane) - a.window;
+          // (the stream kSeg before this one has left its ring entry)
+          if (++seg >= kSeg && end3 > i - kDesc)
+            ok = __all_sync(0xffffffffu, tc_wait(&sh.desc_empty[end3 % kDesc], (end3 / kDesc) & 1, a.status));
+          if (!ok) break;
+          end3 = end2;
+          end2 = end1;
+          end1 = i - 1;
+          high_edge = w.pos0 + describe_rows<D, NR>(a, w, p.chunk, seg % kSeg, lane) - a.window;
         }
         int at = -1;
         bool clean = lane >= here;  // every row sees all of the page
@@ -969,10 +978,10 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
         if (lane == 0) {
           TileDesc& d = sh.desc[ds];
-          const int first_u = u0 + i - p.tile;  // the stream's first tile
+          const int first_u = i - p.tile;  // the stream's first tile, of the run's
           const bool ends = p.tile + 1 == w.tiles;
           d.flags = (draft ? kDraftTile : 0) | (masked ? kMasked : 0) | (first ? kFirst : 0) |
-                    ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= u0) ? kWhole : 0);
+                    ((ends || i + 1 == n_tiles) ? kLast : 0) | ((ends && first_u >= 0) ? kWhole : 0);
           d.pages = here;
           d.len = w.len;
           d.drafts = w.drafts;
@@ -980,11 +989,11 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.head = p.head;
           d.rows = w.rows;
           d.first_row = p.chunk * NR;
-          d.seg = seg % kDesc;
-          d.slot = 2 * cta + (first_u > u0 ? 1 : 0);
+          d.seg = seg % kSeg;
+          d.slot = 2 * cta + (first_u > 0 ? 1 : 0);
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
           d.slots = draft ? 0 : starts;
-          if (first) sh.odd[seg % kDesc] = 0;
+          if (first) sh.odd[seg % kSeg] = 0;
           if (i + 1 == n_tiles) note_tail(a, cta, plan, w, p, NR);
         }
         __syncwarp();
@@ -1112,9 +1121,9 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     // meets again before the next copies.) Rows of codes are swizzled by 16 bytes, as
     // the threads of a warp read 8 rows at a time.
     constexpr int kRow = D / 2;  // bytes of a row of codes
-    auto codes_of = [&](int i) { return smem + T::KC_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::KC; };
+    auto codes_of = [&](int i) { return smem + T::KC_OFF + (T::NB * grp + (i >> 1 & (T::NB - 1))) * T::KC; };
     auto scales_of = [&](int i) {
-      return reinterpret_cast<float*>(smem + T::SZ_OFF + (T::NB * grp + (i >> 1) % T::NB) * T::SZ);
+      return reinterpret_cast<float*>(smem + T::SZ_OFF + (T::NB * grp + (i >> 1 & (T::NB - 1))) * T::SZ);
     };
     auto prefetch = [&](const TileDesc& d, int i) {
       const int slab = d.slab[ct / kMqPage];
