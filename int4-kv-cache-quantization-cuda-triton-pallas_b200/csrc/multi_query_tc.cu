@@ -417,7 +417,7 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int c
   for (int pass = 0; pass < 3; ++pass) {  // as they are; (their maximum; scaled)
     uint32_t big = 0;
     if (c0 < D / 8) {
-#pragma unroll 4
+#pragma unroll 8
       for (int k = 0; k < kPieces; ++k) {
         const int c8 = c0 + k;
         uint4 u = make_uint4(0, 0, 0, 0);
@@ -611,8 +611,24 @@ __device__ __noinline__ void mask_tile(const MultiQueryArgs& a, int ds, uint32_t
   const TileDesc& d = sh.desc[ds];
   const int sg = d.seg, page = tok / kMqPage, at = d.at[page] + tok % kMqPage;
   const bool draft = d.flags & kDraftTile, real = token_real(a, d, page, at);
-  // a cached token is seen by row r iff at > low + its draft's depth
-  const int low = a.window > 0 && at >= a.sinks ? d.low_edge : -(1 << 30);
+  // the drafts that see the token: of the cached ones all, but for the window's edge
+  uint32_t seen[2] = {0, 0};
+  if (real) {
+    const bool edge = !draft && a.window > 0 && at >= a.sinks;
+    if (draft || edge) {
+      const int drafts = max(1, d.drafts);  // (a window's one query counts as draft 0)
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t s = 0;
+#pragma unroll 4
+        for (int t = 0; t < min(32, drafts - 32 * h); ++t)
+          s |= (uint32_t)(draft ? sh.word[sg][32 * h + t] >> (at & 63) & 1 : at > d.low_edge + sh.depth[sg][32 * h + t]) << t;
+        if (h) seen[1] = s; else seen[0] = s;
+      }
+    } else {
+      seen[0] = seen[1] = 0xFFFFFFFFu;
+    }
+  }
 #pragma unroll 1
   for (int j0 = 0; j0 < Tc<D, NR>::NC; j0 += 8) {
     uint32_t x[8];
@@ -621,8 +637,7 @@ __device__ __noinline__ void mask_tile(const MultiQueryArgs& a, int ds, uint32_t
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int t = (j < 4 ? rows.x >> (8 * j) : rows.y >> (8 * j - 32)) & 63;
-      const bool in_tree = sh.word[sg][t] >> (at & 63) & 1, in_cache = at > low + sh.depth[sg][t];
-      if (!(real && (draft ? in_tree : in_cache))) x[j] = 0xFF800000u;
+      if (!((t < 32 ? seen[0] : seen[1]) >> (t & 31) & 1)) x[j] = 0xFF800000u;
     }
     __syncwarp();
     tc_st8(s_addr + j0, x);

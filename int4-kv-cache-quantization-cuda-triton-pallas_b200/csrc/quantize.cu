@@ -32,6 +32,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include <mutex>
 
 #include "common.cuh"
@@ -617,8 +619,10 @@ append_quant_kernel(AppendArgs ap, int C, int R, OutPaged op) {
 // staged rows of the old open group are read by the y = 0 CTA alone, and the
 // same CTA writes those of the new one after the barrier that follows its
 // reads: when the rows cross a group boundary the slot is reused in place.
-// Bound by HBM bytes for long chunks, by launch and two dependent loads
-// (metadata, rows) for a few tokens.
+// Where each row comes from and goes to is looked up once, by the lanes of a warp
+// side by side, and its values are loaded with its keys: every load of a CTA is in
+// flight before the first is used. Bound by HBM bytes for long chunks, by launch
+// and three dependent loads (metadata, page and row, data) for a few tokens.
 struct ExtendArgs {
   const void* k;             // [num_src, C] keys of the kernel's input type
   const void* v;             // [num_src, C] (nullable)
@@ -664,7 +668,8 @@ __device__ __forceinline__ void store_value4(const OutPaged& op, size_t vi, cons
   }
 }
 
-template <int KIND>
+// ROWS: rows of a warp, 8 for groups of up to 64 tokens (half of the registers), else 16.
+template <int KIND, int ROWS>
 __global__ void __launch_bounds__(kQuantThreads)
 extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   __shared__ __align__(16) float s_min[kQuantWarps * kSlab];
@@ -693,34 +698,48 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   const int rows = min(R, end - gpos);
   const bool lane_ok = c0 < C;
   float* stage = ea.stage + (size_t)sl * R * C;
-  auto source = [&](int pos) -> long long {  // input row of the new token at `pos`, -1 if malformed
+  const int32_t* row_bt = op.block_table + (size_t)b * op.max_pages;
+  auto source = [&](int pos) {  // input row of the new token at `pos`, -1 if malformed
     const int i = off + pos - start;
     const int r = ea.rows ? __ldg(ea.rows + i) : i;
-    return (r >= 0 && r < ea.num_src) ? (long long)r : -1;
+    return r >= 0 && r < ea.num_src ? r : -1;
   };
 
-  float4 vals[kMaxRowsPerWarp];
-  float4 mn = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
-  float4 mx = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-  bool lost = false;
+  // Lane i: the warp's row i, its page and its input row (kStaged: a staged row).
+  constexpr int kStaged = -2;
+  int my_page = -1, my_src = kStaged;
+  const int my_r = warp + lane * kQuantWarps;
+  if (lane < ROWS && my_r < rows) {
+    const int pos = gpos + my_r;
+    if (pos >= start) my_src = source(pos);
+    my_page = row_bt[pos / op.page];
+    const bool bad_page = my_page < 0 || my_page >= op.num_pages;
+    if (bad_page) my_page = -1;
+    if (op.status && (bad_page || my_src == -1))
+      atomicOr(op.status, (bad_page ? kStatusBadPage : 0u) | (my_src == -1 ? kStatusBadLength : 0u));
+  }
+  int gslot = row_bt[gpos / op.page];  // (0 <= gpos < end: in the table)
+  if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
+
+  float4 vals[ROWS], vv[ROWS];
 #pragma unroll
-  for (int i = 0; i < kMaxRowsPerWarp; ++i) {
-    const int r = warp + i * kQuantWarps;
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = warp + i * kQuantWarps, src = __shfl_sync(0xffffffffu, my_src, i);
+    vals[i] = vv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < rows && lane_ok) {
-      if (gpos + r < start) {
+      if (src == kStaged) {
         vals[i] = *reinterpret_cast<const float4*>(stage + (size_t)r * C + c0);
-      } else {
-        const long long src = source(gpos + r);
-        lost |= src < 0;
-        vals[i] = src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
+      } else if (src >= 0) {
+        vals[i] = load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
+        if (ea.v) vv[i] = load4_as_f32<KIND>(ea.v, (size_t)src * C + c0);
       }
-      minmax4(vals[i], mn, mx);
     }
   }
-  if (lost && op.status) atomicOr(op.status, kStatusBadLength);
-  const int32_t* row_bt = op.block_table + (size_t)b * op.max_pages;
-  int gslot = row_bt[gpos / op.page];
-  if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
+  float4 mn = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
+  float4 mx = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i)
+    if (warp + i * kQuantWarps < rows && lane_ok) minmax4(vals[i], mn, mx);
   // (its barriers also order this CTA's reads of the staged rows before the
   // writes of the new open group's below)
   reduce_params(mn, mx, s_min, s_max, s_lo, s_sc, s_rc, slab_c0, C, [&](int ch, float sc, float zp) {
@@ -731,12 +750,11 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
     dst[op.head_dim + d] = zp;
   });
   if (gslot < 0 && threadIdx.x == 0 && op.status) atomicOr(op.status, kStatusBadPage);
-  if (!lane_ok) return;
   const int open0 = end - end % R;  // first token of the group left open (== end: none)
-  if (blockIdx.y == 0 && open0 >= gpos + R) {
+  if (blockIdx.y == 0 && open0 >= gpos + R && lane_ok) {
     // the rows crossed into another open group: its rows go over the old ones
     for (int pos = open0 + warp; pos < end; pos += kQuantWarps) {
-      const long long src = source(pos);
+      const int src = source(pos);
       *reinterpret_cast<float4*>(stage + (size_t)(pos - open0) * C + c0) =
           src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
     }
@@ -745,26 +763,19 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   const float4 sc = reinterpret_cast<const float4*>(s_sc)[lane];
   const float4 rc = reinterpret_cast<const float4*>(s_rc)[lane];
   const int h = c0 / op.head_dim, d = c0 - h * op.head_dim;
+  const bool keep = blockIdx.y == 0 && open0 == gpos;  // the group stays open: its new rows are staged
+  const int my_t = (gpos + my_r) % op.page;
 #pragma unroll
-  for (int i = 0; i < kMaxRowsPerWarp; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     const int r = warp + i * kQuantWarps;
-    if (r < rows) {
-      const int pos = gpos + r;
-      const bool fresh = pos >= start;
-      if (blockIdx.y == 0 && fresh && open0 == gpos)
-        *reinterpret_cast<float4*>(stage + (size_t)r * C + c0) = vals[i];
-      const int pg = pos / op.page, t = pos - pg * op.page;
-      const int phys = row_bt[pg];
-      if (phys < 0 || phys >= op.num_pages) {
-        if (op.status) atomicOr(op.status, kStatusBadPage);
-        continue;
-      }
-      const size_t ph = ((size_t)phys * op.heads + h) * op.page + t;
-      *reinterpret_cast<uint16_t*>(op.k_pool + ph * (op.head_dim / 2) + d / 2) = pack4(vals[i], lo, sc, rc);
-      if (fresh && ea.v) {
-        const long long src = source(pos);
-        store_value4(op, ph * op.head_dim + d,
-                     src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.v, (size_t)src * C + c0));
+    const int page = __shfl_sync(0xffffffffu, my_page, i), t = __shfl_sync(0xffffffffu, my_t, i);
+    const bool fresh = __shfl_sync(0xffffffffu, my_src, i) != kStaged;
+    if (r < rows && lane_ok) {
+      if (keep && fresh) *reinterpret_cast<float4*>(stage + (size_t)r * C + c0) = vals[i];
+      if (page >= 0) {
+        const size_t ph = ((size_t)page * op.heads + h) * op.page + t;
+        *reinterpret_cast<uint16_t*>(op.k_pool + ph * (op.head_dim / 2) + d / 2) = pack4(vals[i], lo, sc, rc);
+        if (fresh && ea.v) store_value4(op, ph * op.head_dim + d, vv[i]);
       }
     }
   }
@@ -1335,9 +1346,13 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
                 stage_slots, k_stage, num_slots, max_rows_per_seq};
   OutPaged op{nullptr, nullptr, nullptr, block_table, max_pages, page_tokens, num_pages,
               num_heads, head_dim, k_pool, v_pool, value_dtype, sz_pool, status};
-  auto kern = kv_dtype == INT4KV_VALUES_F32   ? extend_quant_kernel<INT4KV_VALUES_F32>
-              : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16>
-                                              : extend_quant_kernel<INT4KV_VALUES_BF16>;
+  auto pick = [&](auto rows_of_warp) {
+    constexpr int kRows = decltype(rows_of_warp)::value;
+    return kv_dtype == INT4KV_VALUES_F32   ? extend_quant_kernel<INT4KV_VALUES_F32, kRows>
+           : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16, kRows>
+                                           : extend_quant_kernel<INT4KV_VALUES_BF16, kRows>;
+  };
+  auto kern = group_tokens <= 8 * kQuantWarps ? pick(std::integral_constant<int, 8>()) : pick(std::integral_constant<int, 16>());
   kern<<<grid, kQuantThreads, 0, stream>>>(ea, (int)C, group_tokens, op);
   return cudaGetLastError();
 }
