@@ -32,7 +32,8 @@
 //       ahead, to float16 keys, a thread a token; a stream's queries; drafted
 //       keys. A tile's way through a group is a chain of waits, loads and
 //       arithmetic; two chains side by side keep the arithmetic busy.
-//   MMA issue (1): S^T of tile i and O^T of tile i - 1, the one that can go first
+//   MMA issue (2): S^T, and O^T. Each product waits for its own operands: one warp
+//       that issued both in turn was what a tile of 64 or 128 rows waited for.
 //   copies (2): the tiles' descriptors; values by tensor copies, in the swizzled
 //       layout the MMA reads (V is stored token-major, which is the transposed
 //       operand's contiguous side, so nothing is rearranged)
@@ -146,16 +147,6 @@ I4KV_DEVINL bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
-// Whether a phase is over, without waiting.
-I4KV_DEVINL bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_addr(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
 I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -199,7 +190,7 @@ struct Tc {
   static constexpr int NC = NR > 64 ? 64 : (NR < 32 ? NR : 32);  // rows of a softmax warpgroup
   static constexpr int WG = NR / NC, SOFT = 4 * WG;        // softmax warpgroups, warps
   static constexpr int CONV = 8;                           // two conversion groups of four warps
-  static constexpr int WARPS = SOFT + CONV + 3, THREADS = 32 * WARPS;
+  static constexpr int WARPS = SOFT + CONV + 4, THREADS = 32 * WARPS;
   // Stages, as shared memory allows.
   static constexpr int NV = D == 256 ? (NR > 32 ? 4 : 5) : (NR > 64 ? 3 : (NR > 32 ? 6 : 7));  // value units
   static constexpr int NP = 2;                             // weights
@@ -400,36 +391,44 @@ __device__ __noinline__ float query_scale(float top, int ct, int grp, int bar) {
 
 // A stream's queries to shared memory, by a conversion group: as they are, for a
 // magnitude below float16's range loses nothing that a logit could show. Only one
-// above it takes more passes, to find and apply a common power of two. 128 / NR
-// threads take a row together.
+// above it takes more passes, to find and apply a common power of two. D / 8 threads
+// take a row together.
 template <int D, int NR, int VK>
 __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int ct, int grp, int bar) {
   TcShared<NR>& sh = tc_shared<D, NR>();
-  constexpr int kShare = 128 / NR, kPieces = D / 8 / kShare > 0 ? D / 8 / kShare : 1;
+  constexpr int kRowThreads = D / 8, kStep = 128 / kRowThreads, kPieces = NR / kStep > 0 ? NR / kStep : 1;
   const TileDesc& d = sh.desc[ds];
-  const int r = ct / kShare, rr = d.first_row + r, c0 = ct % kShare * kPieces, seg = d.seg;
-  const bool real = rr < d.rows && c0 < D / 8;
-  const uint4* src = reinterpret_cast<const uint4*>(
-      static_cast<const uint16_t*>(a.q) + (real ? out_row(a, d.row0, d.head, sh.draft[seg][r], rr) : 0) * D);
-  char* const row = tc_smem + Tc<D, NR>::Q_OFF + r * 128;
+  const int c8 = ct % kRowThreads, r0 = ct / kRowThreads, seg = d.seg;
+  const int p16 = (c8 % 2) * 4 + (c8 % 8) / 4;  // first 16-byte piece of a row's (the next words' is 2 on)
+  // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
+  char* const to = tc_smem + Tc<D, NR>::Q_OFF + (c8 / 8) * (NR * 128) + (c8 & 2 ? 8 : 0);
+  const int real = min(NR, d.rows - d.first_row), first_row = d.first_row, row0 = d.row0, head = d.head;
   float down = 1.f, up = 1.f, top = 0.f;
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {  // as they are; (their maximum; scaled)
     uint32_t big = 0;
-    if (c0 < D / 8) {
-#pragma unroll 8
-      for (int k = 0; k < kPieces; ++k) {
-        const int c8 = c0 + k;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (real) u = __ldg(src + c8);
-        big |= beyond_half(u);
+    constexpr int kBatch = kPieces < 8 ? kPieces : 8;  // loads in flight
+#pragma unroll 1
+    for (int k0 = 0; k0 < kPieces; k0 += kBatch) {
+      uint4 u[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (k0 + k) * kStep;
+        u[k] = make_uint4(0, 0, 0, 0);
+        if (r < real)
+          u[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                      out_row(a, row0, head, sh.draft[seg][r], first_row + r) * D) + c8);
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + (k0 + k) * kStep;
+        if (kStep > NR && r >= NR) break;
+        big |= beyond_half(u[k]);
         if (pass == 1) {
-          top = top8<VK>(u, top);
+          top = top8<VK>(u[k], top);
         } else {
-          // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
-          const uint4 h = to_half8<VK>(u, down);
-          char* at = row + (c8 / 8) * (NR * 128) + (c8 & 2 ? 8 : 0);
-          const int p16 = (c8 % 2) * 4 + (c8 % 8) / 4;  // 16-byte piece of the row; the next words' is 2 on
+          const uint4 h = to_half8<VK>(u[k], down);
+          char* at = to + r * 128;
           *reinterpret_cast<uint2*>(at + ((p16 ^ (r & 7)) << 4)) = make_uint2(h.x, h.y);
           *reinterpret_cast<uint2*>(at + (((p16 + 2) ^ (r & 7)) << 4)) = make_uint2(h.z, h.w);
         }
@@ -871,7 +870,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
                       const __grid_constant__ CUtensorMap dmap) {
   using T = Tc<D, NR>;
   constexpr int kSoftWarps = T::SOFT, kConvWarps = T::CONV;
-  constexpr int kMmaWarp = kSoftWarps + kConvWarps, kCopyWarp = kMmaWarp + 1;  // two copy warps
+  constexpr int kMmaWarp = kSoftWarps + kConvWarps, kOutWarp = kMmaWarp + 1, kCopyWarp = kMmaWarp + 2;  // two copy warps
   constexpr int kBarConv = 1, kBarGroup = 3;  // named barriers: one per conversion group, one per softmax warpgroup
   char* const smem = tc_smem;  // (no static shared memory: it starts on a 1024-byte boundary)
   TcShared<NR>& sh = tc_shared<D, NR>();
@@ -932,22 +931,36 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     int end1 = -1, end2 = -1, end3 = -1;  // last tiles of the streams before the last one, ..
     Ring v;
     bool ok = true;
-    // this lane's page of tile p: loaded one tile ahead of its use
-    int pg = 0, phys = -1, home = -1;
-    auto fetch = [&]() {
-      phys = home = -1;
-      pg = tile_page<kTilePages>(w, p.tile, lane);
-      if (lane < kTilePages && p.tile < w.cache_tiles && page_visible(w, pg)) {
+    // Lane 8 k + j: page j of tile set + k (and the page its scales are kept with),
+    // and of the four tiles behind those, loaded while these four are in work.
+    static_assert(kTilePages == 8, "four tiles a warp");
+    int set = 0, phys4 = -1, home4 = -1, phys_next = -1, home_next = -1;
+    auto load_set = [&](int tile, int& ph, int& hm) {
+      ph = hm = -1;
+      tile += lane >> 3;
+      const int pg = tile_page<kTilePages>(w, tile, lane & 7);
+      if (tile < w.cache_tiles && page_visible(w, pg)) {
         const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
-        phys = __ldg(bt + pg);
-        home = __ldg(bt + pg / a.group_pages * a.group_pages);
+        ph = __ldg(bt + pg);
+        hm = __ldg(bt + pg / a.group_pages * a.group_pages);
       }
     };
-    fetch();
+    bool turn = true;  // a new stream
 #pragma unroll 1
     for (int i = 0; i < n_tiles && ok; ++i) {
       const int ds = i % kDesc;
       const bool draft = p.tile >= w.cache_tiles;
+      if (turn || p.tile == set + 4) {
+        set = p.tile;
+        phys4 = phys_next;
+        home4 = home_next;
+        if (turn) load_set(set, phys4, home4);
+        load_set(set + 4, phys_next, home_next);
+        turn = false;
+      }
+      const int from = 8 * (p.tile - set) + (lane & 7), pg = tile_page<kTilePages>(w, p.tile, lane & 7);
+      const int phys = __shfl_sync(0xffffffffu, phys4, from);
+      int home = __shfl_sync(0xffffffffu, home4, from);
       const int here = draft ? (w.drafts + kMqPage - 1) / kMqPage
                              : min(kTilePages, w.pages - tile_page<kTilePages>(w, p.tile, 0));
       const bool mine = lane < here && (draft || page_visible(w, pg));
@@ -1025,18 +1038,17 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           const uint32_t unit = lives >> g0 & ((1u << T::PPU) - 1);
           char* dst = smem + T::V_OFF + v.s * T::UNIT;
           if (elect_one()) mbar_arrive_expect_tx(bar, __popc(unit) * T::PAGE_V);
-#pragma unroll 1
-          for (int q = 0; q < T::PPU; ++q) {
-            const int y = __shfl_sync(0xffffffffu, row, g0 + q), z = __shfl_sync(0xffffffffu, slab, g0 + q);
-            if ((unit >> q & 1) && elect_one()) tma_page(dst + q * T::PAGE_V, map, y, z, bar);
-          }
+          __syncwarp();
+          if (lane >= g0 && lane < g0 + T::PPU && live) tma_page(dst + (lane - g0) * T::PAGE_V, map, row, slab, bar);
           __syncwarp();
           v.next<T::NV>();
         }
         if (!ok) break;
       }
-      if (++p.tile >= w.tiles) next_stream<NR, kTilePages>(a, w, p);
-      if (i + 1 < n_tiles) fetch();
+      if (++p.tile >= w.tiles) {
+        next_stream<NR, kTilePages>(a, w, p);
+        turn = true;
+      }
     }
     // after a timeout: the copies issued so far land (or a bound passes) before the CTA ends
     if (!ok && lane == 0) {
@@ -1044,83 +1056,66 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issue
+    // ------------------------------------------------------------ S^T = K^ Q^T
     constexpr uint32_t kQk = mma_desc(128, NR, 0, false);
+    const uint32_t base = smem_addr(smem);
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; ++i) {
+      const int hb = i & 1;
+      ok = tc_wait(&sh.kh_full[hb], (i / 2) & 1, a.status) && tc_wait(&sh.s_empty[hb], (i / 2 + 1) & 1, a.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t keys = tm + T::COLS_K + hb * (D / 2);
+        const uint64_t qd = mat_desc(base + T::Q_OFF, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_ts(tm + hb * NR, keys + k * 8, qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
+        tc_commit(&sh.s_full[hb]);
+        tc_commit(&sh.kh_empty[hb]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == kOutWarp) {
+    // ------------------------------------------------------------ O^T += V^T P^T
     constexpr uint32_t kPv = mma_desc(128, NR, VK == INT4KV_VALUES_BF16 ? 1 : 0, true);
     const uint32_t base = smem_addr(smem);
     Ring v;
-    int pages = 0;       // of tile i - 1
-    bool fresh = true;   // tile i - 1 starts its segment
-    bool ok = true;
 #pragma unroll 1
-    for (int i = 0; i <= n_tiles && ok; ++i) {
-      int next_pages = 0;
-      bool next_fresh = false, keys_first = false;
-      if (i < n_tiles) {
-        const int ds = i % kDesc;
-        ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
-        next_pages = sh.desc[ds].pages;
-        next_fresh = sh.desc[ds].flags & kFirst;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
-        // the outputs of tile i - 1 go first where the keys of tile i are not there yet
-        keys_first = __all_sync(0xffffffffu, mbar_test(&sh.kh_full[i & 1], (i / 2) & 1));
-      }
+    for (int i = 0; i < n_tiles; ++i) {
+      const int ds = i % kDesc, pb = i % T::NP;
+      bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
+      const int pages = ok ? sh.desc[ds].pages : 0;
+      const bool fresh = sh.desc[ds].flags & kFirst;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.desc_empty[ds]);
+      ok = ok && tc_wait(&sh.p_full[pb], (i / T::NP) & 1, a.status);
+      const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P, kTile * 128, 1024);
 #pragma unroll 1
-      for (int turn = 0; turn < 2; ++turn) {
-        if ((turn == 0) == keys_first) {
-          if (i == n_tiles) continue;
-          // S^T of tile i
-          const int hb = i & 1;
-          ok = ok && tc_wait(&sh.kh_full[hb], (i / 2) & 1, a.status) &&
-               tc_wait(&sh.s_empty[hb], (i / 2 + 1) & 1, a.status);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t keys = tm + T::COLS_K + hb * (D / 2);
-            const uint64_t qd = mat_desc(base + T::Q_OFF, 16, 1024);
+      for (int g0 = 0; g0 < pages; g0 += T::PPU) {
+        ok = ok && tc_wait(&sh.v_full[v.s], v.ph, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = mat_desc(base + T::V_OFF + v.s * T::UNIT, 2048, 1024);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              tc_mma_ts(tm + hb * NR, keys + k * 8, qd + (k / 4) * (NR * 128 / 16) + (k % 4) * 2, kQk, k > 0);
-            tc_commit(&sh.s_full[hb]);
-            tc_commit(&sh.kh_empty[hb]);
-          }
-          __syncwarp();
-        } else if (i > 0) {
-          // O^T of tile i - 1
-          const int j = i - 1, pb = j % T::NP;
-          ok = ok && tc_wait(&sh.p_full[pb], (j / T::NP) & 1, a.status);
-          const uint64_t pd = mat_desc(base + T::P_OFF + pb * T::P, kTile * 128, 1024);
-#pragma unroll 1
-          for (int g0 = 0; g0 < pages; g0 += T::PPU) {
-            ok = ok && tc_wait(&sh.v_full[v.s], v.ph, a.status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vd = mat_desc(base + T::V_OFF + v.s * T::UNIT, 2048, 1024);
+          for (int q = 0; q < T::PPU; ++q) {
+            if (g0 + q < pages) {
 #pragma unroll
-              for (int q = 0; q < T::PPU; ++q) {
-                if (g0 + q < pages) {
-#pragma unroll
-                  for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
-                    tc_mma(tm + T::COLS_O + o * NR, vd + (q * T::PAGE_V + o * 4096) / 16, pd + (g0 + q) * (2048 / 16),
-                           kPv, !(fresh && g0 + q == 0));
-                }
-              }
-              tc_commit(&sh.v_empty[v.s]);
+              for (int o = 0; o < T::NO; ++o)  // (head_dim 64: lanes 64-127 take what follows, and are not read)
+                tc_mma(tm + T::COLS_O + o * NR, vd + (q * T::PAGE_V + o * 4096) / 16, pd + (g0 + q) * (2048 / 16), kPv,
+                       !(fresh && g0 + q == 0));
             }
-            __syncwarp();
-            v.next<T::NV>();
           }
-          if (!ok) break;
-          if (elect_one()) tc_commit(&sh.p_empty[pb]);
-          __syncwarp();
+          tc_commit(&sh.v_empty[v.s]);
+          if (g0 + T::PPU >= pages) tc_commit(&sh.p_empty[pb]);
         }
+        __syncwarp();
+        v.next<T::NV>();
       }
-      pages = next_pages;
-      fresh = next_fresh;
+      if (!__all_sync(0xffffffffu, ok)) break;
     }
   } else if (warp >= kSoftWarps) {
     // ------------------------------------------------------------ conversion
