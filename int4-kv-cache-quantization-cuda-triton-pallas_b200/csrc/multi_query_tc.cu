@@ -13,7 +13,7 @@
 // of the softmax holds one token and up to 32 rows, so a row's sum of weights
 // stays in one register per thread until the stream ends. The running maximum is
 // kept lazily: weights are 2^(x - ref) against a reference that is raised to the
-// true maximum only when some logit exceeds it by more than 8 (in log2), so the
+// true maximum only when some logit exceeds it by more than 14 (in log2), so the
 // outputs are rescaled a few times per stream instead of every tile; sums and
 // outputs are float32 in registers and tensor memory.
 //
@@ -57,7 +57,7 @@ constexpr int kDesc = 8, kSeg = 4;              // tiles, and streams, in flight
 // masks of its drafts (measured: 6 and 6 us of 1.5 to 3 us a tile).
 constexpr int kStreamUnits = 2, kDraftUnits = 2;
 constexpr uint64_t kTcWaitNs = 2000000000ull;   // bounded waits: 2 s
-constexpr float kLazy = 8.f;                    // weights reach 2^8 before a rescale
+constexpr float kLazy = 14.f;                   // weights reach 2^14 (float16's range) before a rescale
 
 // ---- tcgen05 ----
 I4KV_DEVINL void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -217,6 +217,7 @@ struct TileDesc {
   int sz[kTilePages];           // its scale slot (the first page here of its group),
   int home[kTilePages];         // and a slot's slab in the scale pool
   uint32_t slots;               // slots in use (a bit each)
+  int unit;                     // units of values before it
 };
 enum : int { kDraftTile = 1, kMasked = 2, kFirst = 4, kLast = 8, kWhole = 16 };
 
@@ -726,9 +727,9 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
 
 // Values that no row sees must not reach the product (0 * NaN): cleared. A drafted
 // value that is not finite is taken out too and added for the rows that see it when
-// the stream ends. One thread a token; `v` is the tile's first value unit.
+// the stream ends. One thread a token.
 template <int D, int NR, int VK>
-__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, Ring v, int tok) {
+__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, int tok) {
   using T = Tc<D, NR>;
   TcShared<NR>& sh = tc_shared<D, NR>();
   const TileDesc& d = sh.desc[ds];
@@ -736,10 +737,9 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, Ring 
   const int at = d.at[tok / kMqPage] + tok % kMqPage;
   const bool draft = d.flags & kDraftTile, real = token_real(a, d, tok / kMqPage, at);
   if (tok < d.pages * kMqPage && (!real || draft)) {
-#pragma unroll 1
-    for (int k = tok / (kMqPage * T::PPU); k > 0; --k) v.next<T::NV>();
-    ok = tc_wait(&sh.v_full[v.s], v.ph, a.status);
-    char* row = tc_smem + T::V_OFF + v.s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
+    const int u = d.unit + tok / (kMqPage * T::PPU), s = u % T::NV;
+    ok = tc_wait(&sh.v_full[s], (u / T::NV) & 1, a.status);
+    char* row = tc_smem + T::V_OFF + s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
     // (the order of a thread's 16-byte pieces spreads a warp's over the banks)
     auto piece = [&](int q) {
       return reinterpret_cast<uint4*>(row + (q / 8) * (kMqPage * 128) + 16 * (q % 8 ^ (tok & 7)));
@@ -946,6 +946,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       }
     };
     bool turn = true;  // a new stream
+    int units = 0;
 #pragma unroll 1
     for (int i = 0; i < n_tiles && ok; ++i) {
       const int ds = i % kDesc;
@@ -1021,9 +1022,11 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.slot = 2 * cta + (first_u > 0 ? 1 : 0);
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
           d.slots = draft ? 0 : starts;
+          d.unit = units;
           if (first) sh.odd[seg % kSeg] = 0;
           if (i + 1 == n_tiles) note_tail(a, cta, plan, w, p, NR);
         }
+        units += (here + T::PPU - 1) / T::PPU;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.desc_full[ds]);
       } else {
@@ -1249,7 +1252,6 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int bar = kBarGroup + wg;
     float nref[NI][2], l[NI][2];               // minus the references; sums
-    Ring v;                                    // first value unit of the tile
     bool failed = false, started = false;      // a wait ran out; O^T of the segment holds something
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -1259,16 +1261,15 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       const int ds = i % kDesc, sb = i & 1, pb = i % T::NP;
-      // Every thread waits. A timeout is made uniform over the warpgroup here
-      // alone: until then the tile goes on with what it has, so no barrier of the
-      // warpgroup (they share none) ever waits for a warp that has left.
+      // Every thread waits. A timeout is made uniform over the warpgroup with the
+      // tile's vote alone: until then the tile goes on with what it has, so no barrier
+      // of the warpgroup (they share none) ever waits for a warp that has left.
       const bool ok = tc_wait(&sh.desc_full[ds], (i / kDesc) & 1, a.status);
       failed |= !ok;
       const TileDesc& d = sh.desc[ds];
-      const int flags = ok ? d.flags : 0, pages = ok ? d.pages : 0, sg = ok ? d.seg : 0;
+      const int flags = ok ? d.flags : 0, sg = ok ? d.seg : 0;
       const bool masked = flags & kMasked;
       failed |= !tc_wait(&sh.s_full[sb], (i / 2) & 1, a.status);
-      if (named_bar_or(bar, 128, failed)) break;
       tc_fence_after();
       if (flags & kFirst) {
         started = false;
@@ -1290,11 +1291,13 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
       }
 
-      // pass 1: does some logit exceed its row's reference by more than kLazy?
+      // pass 1: does some logit exceed its row's reference by more than kLazy? (Up to
+      // 32 rows' logits stay in registers for pass 2.)
+      constexpr bool kHeld = LI == NI;
+      uint32_t x[2][4 * LI];
       float over = -INFINITY;
 #pragma unroll
       for (int j0 = 0; j0 < NI; j0 += LI) {
-        uint32_t x[2][4 * LI];
         tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
 #pragma unroll
         for (int j = 0; j < LI; ++j) {
@@ -1307,7 +1310,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
       }
-      if (named_bar_or(bar, 128, over > kLazy)) {
+      if (named_bar_or(bar, 128, over > kLazy || failed)) {
+        if (named_bar_or(bar, 128, failed)) break;
         RowState<NI> rows;
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
@@ -1334,8 +1338,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       char* prow = smem + T::P_OFF + pb * T::P + (quarter * 32 + g) * 128 + 4 * t4;
 #pragma unroll
       for (int j0 = 0; j0 < NI; j0 += LI) {
-        uint32_t x[2][4 * LI];
-        tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
+        if (!kHeld) tc_ld_frag(x[0], x[1], s_addr + 8 * j0);
 #pragma unroll
         for (int j = 0; j < LI; ++j) {
           const int col = c0 + 8 * (j0 + j);
@@ -1352,9 +1355,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
       }
-      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, ds, v, tok);
-#pragma unroll 1
-      for (int k = 0; k < pages; k += T::PPU) v.next<T::NV>();
+      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, ds, tok);
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();
