@@ -22,7 +22,7 @@
 // Pages arrive by bulk copies into a two-stage ring, the next tile's while the
 // current one is computed. Which of bytes and arithmetic bounds it depends on
 // NR: a tile costs NR * 2 * D * TOK fused multiply-adds whatever the rows'
-// count, so NR is the smallest of 4, 8, 16 that holds the rows of one kv head.
+// count, so NR is the smallest of 1, 4, 8, 16 that holds the rows of one kv head.
 #include <algorithm>
 
 #include "multi_query.cuh"
@@ -42,11 +42,11 @@ struct Shape {
   static constexpr int VB = VK == INT4KV_VALUES_F32 ? 4 : 2;
   static constexpr int V_BYTES = TOK * D * VB, K_BYTES = TOK * D / 2, SZ_BYTES = TP * 2 * D * 4;
   static constexpr int STAGE = V_BYTES + K_BYTES + SZ_BYTES;
-  static constexpr int P_STRIDE = NR + 4;
+  static constexpr int P_STRIDE = NR == 1 ? 1 : NR + 4;
   static constexpr int Q_OFF = 2 * STAGE;
   static constexpr int O_OFF = Q_OFF + NR * D * 4;
   static constexpr int S_OFF = O_OFF + NR * D * 4;
-  static constexpr int P_OFF = S_OFF + NR * (TOK + 4) * 4;
+  static constexpr int P_OFF = S_OFF + NR * (TOK + 4) * 4;  // (16-byte aligned: TOK is a multiple of 4)
   static constexpr int BYTES = P_OFF + TOK * P_STRIDE * 4;
   static constexpr int PAIRS = D / 2, TG = kThreads / PAIRS, TPG = TOK / TG;
 };
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
             }
           }
         }
-        float mine[NR / 4];
+        float mine[(NR + 3) / 4] = {};
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           float x = s2[r][0] + s2[r][1];
@@ -260,8 +260,9 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         }
         const int behind = in_cache ? at : (real && a.window > 0 ? w.pos0 + s_depth[at] : 0);
 #pragma unroll
-        for (int j = 0; j < NR / 4; ++j) {
+        for (int j = 0; j < (NR + 3) / 4; ++j) {
           const int r = 4 * j + qd;
+          if (NR == 1 && qd != 0) break;
           bool sees = real;
           if (!in_cache) sees = sees && (s_word[r] >> (at & 63) & 1);
           if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
@@ -324,8 +325,9 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         for (int t = t0; t < t0 + S::TPG; ++t) {
           float v[2];
           value(t, v);
+          if (NR == 1) fma2_rn(ps[0][0], ps[0][1], v[0], v[1], s_p[t]);
 #pragma unroll
-          for (int r = 0; r < NR; r += 4) {
+          for (int r = 0; r + 4 <= NR; r += 4) {
             const float4 e = *reinterpret_cast<const float4*>(s_p + t * S::P_STRIDE + r);
             fma2_rn(ps[r][0], ps[r][1], v[0], v[1], e.x);
             fma2_rn(ps[r + 1][0], ps[r + 1][1], v[0], v[1], e.y);
@@ -334,14 +336,19 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
           }
         }
       } else {  // some row does not see some token: what stands there, even NaN, adds nothing
-        for (int t = t0; t < t0 + S::TPG; ++t) {
-          float v[2];
-          value(t, v);
+        static_assert(S::TPG % 4 == 0, "four tokens a turn");
+#pragma unroll 1
+        for (int t4 = t0; t4 < t0 + S::TPG; t4 += 4) {
+          float v[4][2];
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const float e = s_p[t * S::P_STRIDE + r];
-            if (e != 0.f) fma2_rn(ps[r][0], ps[r][1], v[0], v[1], e);
-          }
+          for (int t = 0; t < 4; ++t) value(t4 + t, v[t]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              const float e = s_p[(t4 + t) * S::P_STRIDE + r];
+              if (e != 0.f) fma2_rn(ps[r][0], ps[r][1], v[t][0], v[t][1], e);
+            }
         }
       }
 #pragma unroll
@@ -427,6 +434,7 @@ cudaError_t launch_vk(int vk, const MultiQueryArgs& a, int sms, void* ws, size_t
 
 template <int D>
 cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  if (rows == 1) return launch_vk<D, 1>(vk, a, sms, ws, n, st);
   if (rows <= 4) return launch_vk<D, 4>(vk, a, sms, ws, n, st);
   if (rows <= 8) return launch_vk<D, 8>(vk, a, sms, ws, n, st);
   return launch_vk<D, 16>(vk, a, sms, ws, n, st);
