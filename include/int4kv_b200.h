@@ -495,10 +495,14 @@ cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, in
  * or float16 / bfloat16 with a value pool of the same type (keys and softmax
  * weights are then rounded to 16 bits for the tensor cores, sums stay
  * float32). head_dim 64, 128 or 256, pages of 16 tokens, tensors 16-byte
- * aligned. Cached values that some row of the sequence sees must be finite for
- * the other rows' results to be. Bad pages are not read (their tokens are not seen); offsets outside
- * [0, num_rows], too many drafts or bad lengths set INT4KV_STATUS_BAD_LENGTH
- * and the sequence's drafts are skipped (a length is clamped). */
+ * aligned, `out` apart from the inputs. What stands behind a sequence's length,
+ * outside every window or in drafts nobody sees is never part of a result, even
+ * NaN; a 16-bit cached value that some row of a sequence sees must be finite for
+ * the results of its other rows to be. Pages outside the pool are not read: their
+ * tokens are not seen (INT4KV_STATUS_BAD_PAGE). Offsets outside [0, num_rows] or
+ * too many drafts skip the sequence's drafts, a bad length is clamped to the
+ * table (INT4KV_STATUS_BAD_LENGTH). Results do not depend on the order of any
+ * atomics: equal calls on equal devices give equal bits. */
 cudaError_t int4kv_paged_tree_decode(const void* query, const void* k_draft, const void* v_draft,
                                      int qkv_dtype, const int64_t* tree_mask,
                                      const int32_t* draft_offsets, int num_rows, int max_drafts,

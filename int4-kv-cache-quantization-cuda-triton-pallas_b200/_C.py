@@ -14,6 +14,8 @@ The paged entry points (``quantize_int4_grouped``, ``cache_write``,
 Nothing here computes on the CPU: a missing library raises.
 """
 
+import functools
+
 import torch
 
 from . import _lib
@@ -723,17 +725,24 @@ def cache_read(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, num
     return k_out, v_out
 
 
-def paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_drafts=1, device=None):
-    """Workspace bytes of ``paged_tree_decode`` (``max_drafts`` per sequence) and
-    ``paged_window_decode`` (``max_drafts=1``); needs no initialisation."""
+@functools.lru_cache(maxsize=1024)
+def _attention_need(batch, q_heads, kv_heads, head_dim, max_drafts, device):
     import ctypes
     lib = _lib.load()
     need = ctypes.c_size_t(0)
-    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+    with torch.cuda.device(device):
         _lib.check(lib.int4kv_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim,
                                                              max_drafts, ctypes.byref(need)),
                    "paged_attention_workspace_size")
     return need.value
+
+
+def paged_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, max_drafts=1, device=None):
+    """Workspace bytes of ``paged_tree_decode`` (``max_drafts`` per sequence) and
+    ``paged_window_decode`` (``max_drafts=1``); needs no initialisation."""
+    index = torch.device(device).index if device is not None else None
+    return _attention_need(int(batch), int(q_heads), int(kv_heads), int(head_dim), int(max_drafts),
+                           torch.cuda.current_device() if index is None else index)
 
 
 def _check_attention(query, hkv, d, page, v_pool, group_tokens, sinks):
@@ -760,9 +769,11 @@ def _check_attention(query, hkv, d, page, v_pool, group_tokens, sinks):
     return rows, hq
 
 
-def _attention_buffers(query, out, workspace, need):
+def _attention_buffers(query, out, workspace, need, inputs=()):
     if out is None:
         out = torch.empty_like(query)
+    elif any(out.data_ptr() == t.data_ptr() for t in (query, *inputs) if t.numel()):
+        raise RuntimeError("out must not be one of the inputs")
     elif out.dtype != query.dtype or out.shape != query.shape or not out.is_contiguous():
         raise RuntimeError("out must be contiguous with the type and shape of query")
     if workspace is None:
@@ -783,8 +794,8 @@ def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool,
     ``tree_mask[row]`` (int64; ``paged.tree_mask``) lets a draft see draft u of its sequence. With
     ``window`` a query at position p sees positions above p - window and the first ``sinks`` only.
     float32 with any value pool, or float16 / bfloat16 with a value pool of the same type. Rows
-    past the last sequence's are left as ``out`` held them. A ``workspace`` belongs to one call at
-    a time; None allocates one.
+    past the last sequence's are left as ``out`` (not one of the inputs) held them. A ``workspace``
+    belongs to one call at a time; None allocates one.
     """
     lib = _lib.load()
     num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)
@@ -808,8 +819,8 @@ def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool,
     _same_device(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool, v_pool, sz_pool,
                  block_table, seq_lens, out, workspace, status)
     with torch.cuda.device(query.device):
-        need = paged_attention_workspace_bytes(b, hq, hkv, d, max_drafts, query.device)
-        out, workspace = _attention_buffers(query, out, workspace, need)
+        need = _attention_need(b, hq, hkv, d, int(max_drafts), query.device.index)
+        out, workspace = _attention_buffers(query, out, workspace, need, (k_draft, v_draft))
         _lib.check(lib.int4kv_paged_tree_decode(
             _p(query), _p(k_draft), _p(v_draft), VALUE_KINDS[query.dtype], _p(tree_mask),
             _p(draft_offsets), rows, int(max_drafts), _p(k_pool), _p(v_pool),
@@ -838,7 +849,7 @@ def paged_window_decode(query, k_pool, v_pool, sz_pool, block_table, seq_lens, w
     _check_status(status)
     _same_device(query, k_pool, v_pool, sz_pool, block_table, seq_lens, out, workspace, status)
     with torch.cuda.device(query.device):
-        need = paged_attention_workspace_bytes(b, hq, hkv, d, 1, query.device)
+        need = _attention_need(b, hq, hkv, d, 1, query.device.index)
         out, workspace = _attention_buffers(query, out, workspace, need)
         _lib.check(lib.int4kv_paged_window_decode(
             _p(query), VALUE_KINDS[query.dtype], _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype],

@@ -17,13 +17,14 @@
 // outputs are rescaled a few times per stream instead of every tile; sums and
 // outputs are float32 in registers and tensor memory.
 //
-// Numerics: keys are dequantized as code * s - zp * s in float32, scaled by a
-// power of two that brings the largest channel of their group to [1, 2), and
-// rounded once to float16 (relative step 2^-11; bfloat16 would lose 3 bits of
-// the logits); queries (exact in float16 after their own power of two) likewise;
-// the scales return in the float32 logits. Weights are rounded to the value
-// pool's type, which the tensor cores multiply with the stored values as they
-// are.
+// Numerics: keys are dequantized as code * s - zp * s in float32 and rounded once to
+// float16 (relative step 2^-11; bfloat16 would lose 3 bits of the logits); queries
+// and drafted keys are exact there. What lies outside float16's range is scaled by
+// a power of two first, cached keys by group, drafted ones and queries each by its
+// own, where the largest magnitude is not in [2^-8, 2^15): inside it what is lost to
+// float16's smallest step is 2^-17 of that magnitude at most. The scales return in
+// the float32 logits. Weights are rounded to the value pool's type, which the
+// tensor cores multiply with the stored values as they are.
 //
 // A tile is 128 cached tokens (8 pages) or the drafts. Roles of the warps:
 //   softmax (a warpgroup for up to 32 rows): S^T from tensor memory, mask, weights
@@ -229,13 +230,13 @@ struct TcShared {
   uint64_t word[kSeg][kMqMaxDrafts];  // per segment: the drafts each draft sees,
   int depth[kSeg][kMqMaxDrafts];      // its ancestors,
   alignas(8) uint8_t draft[kSeg][NR];  // and each row's draft
-  float qscale[kSeg];
+  float qscale[kSeg][NR];       // the rows' scales,
+  int qscaled[kSeg];            // where any is not 1
   int scaled[kDesc];            // the tile's keys carry scales of their own
   float kscale[kDesc][kTile];
   float ref[NR], inv[NR];       // a finished stream's references, inverse sums,
   int row[NR];                  // and rows of the outputs [rows * heads]
   float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
-  float qmax[2][4];
   unsigned long long odd[kSeg];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
   RunPlan plan;
@@ -298,7 +299,8 @@ I4KV_DEVINL void unit_scale(float top, float& down, float& up) {
   down = __uint_as_float((uint32_t)(254 - c) << 23);
   up = __uint_as_float((uint32_t)c << 23);
 }
-constexpr float kHalfRoom = 32768.f;  // magnitudes up to here are kept as float16 unscaled
+// A largest magnitude in [kHalfLow, kHalfRoom) is kept as float16 unscaled.
+constexpr float kHalfLow = 1.f / 256, kHalfRoom = 32768.f;
 I4KV_DEVINL float finite_abs(float x) { return fabsf(x) <= 3.4e38f ? fabsf(x) : 0.f; }
 
 // Row of the outputs [rows * heads] of a sequence's row rr, one of draft t's.
@@ -362,10 +364,13 @@ I4KV_DEVINL float top8(const uint4& u, float top) {
   for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
   return top;
 }
-I4KV_DEVINL uint32_t beyond_half(const uint4& u) {  // of bfloat16: magnitude bits >= 2^15's
-  const uint32_t m = 0x7FFF7FFFu, k = 0x7FFF7FFFu - 0x46FF46FFu;  // (| x | + k carries into the sign's place)
+// Whether any of 8 bfloat16 magnitudes reaches the one whose bits are B.
+template <uint32_t B>
+I4KV_DEVINL uint32_t reaches(const uint4& u) {
+  const uint32_t m = 0x7FFF7FFFu, k = (0x8000u - B) * 0x10001u;  // (|x| + k carries into the sign's place)
   return (((u.x & m) + k) | ((u.y & m) + k) | ((u.z & m) + k) | ((u.w & m) + k)) & 0x80008000u;
 }
+constexpr uint32_t kBfRoom = 0x4700u, kBfLow = 0x3B80u;  // bfloat16's 2^15, 2^-8
 // 8 16-bit values as float16, times a power of two.
 template <int VK>
 I4KV_DEVINL uint4 to_half8(const uint4& u, float down) {
@@ -376,26 +381,25 @@ I4KV_DEVINL uint4 to_half8(const uint4& u, float down) {
                     pack16<INT4KV_VALUES_F16>(x[4] * down, x[5] * down), pack16<INT4KV_VALUES_F16>(x[6] * down, x[7] * down));
 }
 
-// A common power of two for a stream's queries, where some are beyond float16's
-// range (a bfloat16 input): a conversion group finds it.
-template <int D, int NR, int VK>
-__device__ __noinline__ float query_scale(float top, int ct, int grp, int bar) {
-  TcShared<NR>& sh = tc_shared<D, NR>();
+// Powers of two of a batch of rows' queries (bfloat16), where some row is outside
+// float16's range: KT neighbouring threads hold a row.
+struct Pow2 {
+  float down, up;
+};
+template <int VK, int KT>
+__device__ __noinline__ Pow2 row_scale(uint4 u, bool scaled) {
+  float top = top8<VK>(u, 0.f);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (ct % 32 == 0) sh.qmax[grp][ct / 32] = top;
-  named_bar_sync(bar, 128);
-  top = fmaxf(fmaxf(sh.qmax[grp][0], sh.qmax[grp][1]), fmaxf(sh.qmax[grp][2], sh.qmax[grp][3]));
-  named_bar_sync(bar, 128);  // qmax is free again
-  return top;
+  for (int o = KT / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  Pow2 p = {1.f, 1.f};
+  if (scaled) unit_scale(top, p.down, p.up);
+  return p;
 }
 
-// A stream's queries to shared memory, by a conversion group: as they are, for a
-// magnitude below float16's range loses nothing that a logit could show. Only one
-// above it takes more passes, to find and apply a common power of two. D / 8 threads
-// take a row together.
+// A stream's queries to shared memory, by a conversion group; D / 8 threads take a
+// row together.
 template <int D, int NR, int VK>
-__device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int ct, int grp, int bar) {
+__device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int ct) {
   TcShared<NR>& sh = tc_shared<D, NR>();
   constexpr int kRowThreads = D / 8, kStep = 128 / kRowThreads, kPieces = NR / kStep > 0 ? NR / kStep : 1;
   const TileDesc& d = sh.desc[ds];
@@ -404,41 +408,40 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int c
   // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
   char* const to = tc_smem + Tc<D, NR>::Q_OFF + (c8 / 8) * (NR * 128) + (c8 & 2 ? 8 : 0);
   const int real = min(NR, d.rows - d.first_row), first_row = d.first_row, row0 = d.row0, head = d.head;
-  float down = 1.f, up = 1.f, top = 0.f;
+  const uint32_t mates = (kRowThreads == 32 ? 0xffffffffu : (1u << (kRowThreads & 31)) - 1) << (ct % 32 / kRowThreads * kRowThreads);
+  constexpr int kBatch = kPieces < 8 ? kPieces : 8;  // loads in flight
+  static_assert(kStep <= NR, "every thread has a row");
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {  // as they are; (their maximum; scaled)
-    uint32_t big = 0;
-    constexpr int kBatch = kPieces < 8 ? kPieces : 8;  // loads in flight
-#pragma unroll 1
-    for (int k0 = 0; k0 < kPieces; k0 += kBatch) {
-      uint4 u[kBatch];
+  for (int k0 = 0; k0 < kPieces; k0 += kBatch) {
+    uint4 u[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int r = r0 + (k0 + k) * kStep;
-        u[k] = make_uint4(0, 0, 0, 0);
-        if (r < real)
-          u[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                      out_row(a, row0, head, sh.draft[seg][r], first_row + r) * D) + c8);
-      }
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + (k0 + k) * kStep;
+      u[k] = make_uint4(0, 0, 0, 0);
+      if (r < real)
+        u[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                    out_row(a, row0, head, sh.draft[seg][r], first_row + r) * D) + c8);
+    }
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int r = r0 + (k0 + k) * kStep;
-        if (kStep > NR && r >= NR) break;
-        big |= beyond_half(u[k]);
-        if (pass == 1) {
-          top = top8<VK>(u[k], top);
-        } else {
-          const uint4 h = to_half8<VK>(u[k], down);
-          char* at = to + r * 128;
-          *reinterpret_cast<uint2*>(at + ((p16 ^ (r & 7)) << 4)) = make_uint2(h.x, h.y);
-          *reinterpret_cast<uint2*>(at + (((p16 + 2) ^ (r & 7)) << 4)) = make_uint2(h.z, h.w);
+    for (int k = 0; k < kBatch; ++k) {
+      const int r = r0 + (k0 + k) * kStep;
+      Pow2 p = {1.f, 1.f};
+      if (VK == INT4KV_VALUES_BF16) {
+        const uint32_t high = __ballot_sync(0xffffffffu, reaches<kBfRoom>(u[k]));
+        const uint32_t some = __ballot_sync(0xffffffffu, reaches<kBfLow>(u[k]));
+        const bool scaled = r < real && ((high & mates) || !(some & mates));
+        if (__any_sync(0xffffffffu, scaled)) p = row_scale<VK, kRowThreads>(u[k], scaled);
+        if (c8 == 0) {
+          sh.qscale[seg][r] = p.up;
+          if (p.up != 1.f) sh.qscaled[seg] = 1;
         }
       }
+      const uint4 h = to_half8<VK>(u[k], p.down);
+      char* at = to + r * 128;
+      *reinterpret_cast<uint2*>(at + ((p16 ^ (r & 7)) << 4)) = make_uint2(h.x, h.y);
+      *reinterpret_cast<uint2*>(at + (((p16 + 2) ^ (r & 7)) << 4)) = make_uint2(h.z, h.w);
     }
-    if (VK == INT4KV_VALUES_F16 || (pass == 0 && !named_bar_or(bar, 128, big))) break;
-    if (pass == 1) unit_scale(query_scale<D, NR, VK>(top, ct, grp, bar), down, up);
   }
-  if (ct == 0) sh.qscale[seg] = up;
   fence_proxy_async_smem();
 }
 
@@ -504,7 +507,7 @@ I4KV_DEVINL void convert_keys(const TileDesc& d, const char* codes, const float*
   }
 }
 
-// The same with a power of two per group, for keys beyond float16's range.
+// The same with a power of two per group, for keys outside float16's range.
 template <int D, int NR>
 __device__ __noinline__ void convert_scaled(int ds, const char* codes, const float* scales, uint32_t keys, int ct) {
   TcShared<NR>& sh = tc_shared<D, NR>();
@@ -529,8 +532,8 @@ __device__ __noinline__ void convert_scaled(int ds, const char* codes, const flo
   convert_keys<D, true>(d, codes, scales, keys, ct, down[0], down[1]);
 }
 
-// Drafted keys, as they are, or (true) with a power of two each where one of them is
-// beyond float16's range.
+// Drafted keys, as they are, or (true) with a power of two each where one of them
+// (or a thread's share of it) is outside float16's range.
 template <int D, int NR, int VK>
 __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_t keys, int ct, int bar) {
   TcShared<NR>& sh = tc_shared<D, NR>();
@@ -565,6 +568,7 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
           if (t4 == 0) sh.kscale[ds][r ? tb : ta] = up;
         }
       }
+      uint32_t some[2] = {0, 0};
 #pragma unroll 1
       for (int blk = 0; blk < D / 64; ++blk) {
         uint4 u[4];
@@ -577,7 +581,8 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
         uint32_t h[16];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          big |= beyond_half(u[k]);
+          big |= reaches<kBfRoom>(u[k]);
+          some[k / 2] |= reaches<kBfLow>(u[k]);
           const uint4 v = to_half8<VK>(u[k], down[k / 2]);
           // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
           h[8 * (k % 2) + 2 * (k / 2)] = v.x;
@@ -588,6 +593,7 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
         __syncwarp();
         tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
       }
+      if ((ta < drafts && !some[0]) || (tb < drafts && !some[1])) big = 1;
     }
     if (VK == INT4KV_VALUES_F16 || scaled || !named_bar_or(bar, 128, big)) break;
     scaled = true;
@@ -600,6 +606,27 @@ I4KV_DEVINL bool token_real(const MultiQueryArgs& a, const TileDesc& d, int page
   const bool draft = d.flags & kDraftTile;
   const bool here = page < d.pages && d.at[page] >= 0 && at < (draft ? d.drafts : d.len);
   return here && (draft || a.window == 0 || at > d.low_edge || at < a.sinks);
+}
+
+// Logits of scaled keys or queries, brought back in tensor memory, so nothing else
+// has to know. A thread takes one token. (What is not there is masked afterwards.)
+template <int D, int NR>
+__device__ __noinline__ void scale_tile(int ds, uint32_t s_addr, int c0, int tok) {
+  TcShared<NR>& sh = tc_shared<D, NR>();
+  const int sg = sh.desc[ds].seg;
+  const float ks = sh.scaled[ds] ? sh.kscale[ds][tok] : 1.f;
+  const bool rows = sh.qscaled[sg];
+#pragma unroll 1
+  for (int j0 = 0; j0 < Tc<D, NR>::NC; j0 += 8) {
+    uint32_t x[8];
+    tc_ld8(x, s_addr + j0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = __float_as_uint(__uint_as_float(x[j]) * (ks * (rows ? sh.qscale[sg][c0 + j0 + j] : 1.f)));
+    __syncwarp();
+    tc_st8(s_addr + j0, x);
+  }
+  tc_wait_st();
 }
 
 // A tile that some row does not see all of: the logits it must not see become -inf
@@ -657,14 +684,13 @@ constexpr float kNoRef = -1e30f;  // the reference of a row that has seen nothin
 // `prev`: the buffer of the last tile's weights (-1: O^T holds nothing yet).
 template <int D, int NR>
 __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const MultiQueryArgs& a, RowState<Tc<D, NR>::NC / 8> s,
-                                                                     float4 f4, uint32_t s_addr, uint32_t o_addr, int c0,
+                                                                     uint32_t s_addr, uint32_t o_addr, int c0,
                                                                      int quarter, int lane, int prev, uint32_t parity,
                                                                      int bar) {
   TcShared<NR>& sh = tc_shared<D, NR>();
   using T = Tc<D, NR>;
   constexpr int NI = T::NC / 8, LI = NI < 4 ? NI : 4;
   const int g = lane >> 2, t4 = lane & 3;
-  const float f[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
   for (int j0 = 0; j0 < NI; j0 += LI) {
     uint32_t x[2][4 * LI];
@@ -676,7 +702,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
         float m = kNoRef;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          m = fmaxf(m, __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * f[q]);
+          m = fmaxf(m, __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * kLog2e);
         }
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
@@ -1023,7 +1049,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           d.low_edge = a.window > 0 ? w.pos0 - a.window : -1;
           d.slots = draft ? 0 : starts;
           d.unit = units;
-          if (first) sh.odd[seg % kSeg] = 0;
+          if (first) sh.odd[seg % kSeg] = sh.qscaled[seg % kSeg] = 0;
           if (i + 1 == n_tiles) note_tail(a, cta, plan, w, p, NR);
         }
         units += (here + T::PPU - 1) / T::PPU;
@@ -1174,11 +1200,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       if (i >= 0) {
         // Scale and zero point, in place: a code c enters as 1 + c / 128 (its bits in
         // the mantissa), so a key is (1 + c / 128) e + z with e = 128 s, z = -zp s - e.
-        float key_top = 0.f;
+        bool odd = false;  // a group outside float16's range
         cp_async_wait<0>();
 #pragma unroll 1
         for (uint32_t left = ok ? d.slots : 0u; left; left &= left - 1) {
           float* sz = scales + (__ffs(left) - 1) * (2 * D) + ct;
+          float key_top = 0.f;
 #pragma unroll
           for (int ch = 0; ch < D; ch += 128) {
             if (D >= 128 || ct < D) {
@@ -1188,13 +1215,15 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
               sz[D + ch] = fmaf(-128.f, s, z);
             }
           }
+          // (a warp judges its own channels: too small there alone costs time, no more)
+          odd |= key_top >= kHalfRoom || ((D >= 128 || ct < D) && !__any_sync(0xffffffffu, key_top >= kHalfLow));
         }
         // A new stream's queries replace the last one's: every product with those
         // is done. Otherwise the keys of tile i - 2 have been multiplied.
         if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
         ok = ok && tc_wait(&sh.kh_empty[i & 1], (i / 2 + 1) & 1, a.status);
-        // Keys beyond float16's range take a power of two per group.
-        if (named_bar_or(bar, 128, !ok || key_top > kHalfRoom)) {
+        // Keys outside float16's range take a power of two per group.
+        if (named_bar_or(bar, 128, !ok || odd)) {
           // (uniform over the group: its warps meet in named barriers)
           if (named_bar_or(bar, 128, !ok)) break;
           scaled = true;
@@ -1202,18 +1231,18 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         tc_fence_after();
       }
       if (T::NB > 1 && next < n_tiles) {
-        ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+        ok = __all_sync(0xffffffffu, tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status));
         if (ok) prefetch(sh.desc[next % kDesc], next);
       }
       if (i < 0) {
         if (T::NB > 1) continue;
         if (next < n_tiles) {
-          ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status));
           if (ok) prefetch(sh.desc[next % kDesc], next);
         }
         continue;
       }
-      if (flags & kFirst) load_queries<D, NR, VK>(a, ds, ct, grp, bar);
+      if (flags & kFirst) load_queries<D, NR, VK>(a, ds, ct);
       const uint32_t keys = tm + lanes + T::COLS_K + (i & 1) * (D / 2);
       if (draft) {
         scaled = draft_keys<D, NR, VK>(a, ds, keys, ct, bar);
@@ -1233,7 +1262,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       if (T::NB == 1) {
         named_bar_sync(bar, 128);
         if (next < n_tiles) {
-          ok = tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status);
+          ok = __all_sync(0xffffffffu, tc_wait(&sh.desc_full[next % kDesc], (next / kDesc) & 1, a.status));
           if (ok) prefetch(sh.desc[next % kDesc], next);
         }
       }
@@ -1280,17 +1309,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
         }
       }
       const uint32_t s_addr = tm + lanes + sb * NR + c0;
+      if (sh.scaled[ds] | sh.qscaled[sg]) scale_tile<D, NR>(ds, s_addr, c0, tok);
       if (masked) mask_tile<D, NR>(a, ds, s_addr, c0, tok);
-      float f[4];
-      f[0] = f[1] = f[2] = f[3] = sh.qscale[sg] * kLog2e;
-      if (sh.scaled[ds]) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // (a token that is not there: any finite scale, its logits are -inf)
-          const float k = sh.kscale[ds][quarter * 32 + 8 * q + g];
-          f[q] *= k > 0.f && k < 3e38f ? k : 1.f;
-        }
-      }
-
       // pass 1: does some logit exceed its row's reference by more than kLazy? (Up to
       // 32 rows' logits stay in registers for pass 2.)
       constexpr bool kHeld = LI == NI;
@@ -1305,7 +1325,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           for (int q = 0; q < 4; ++q) {
             const uint32_t* xx = &x[q / 2][4 * j + 2 * (q % 2)];
             float y0, y1;
-            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
+            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), kLog2e, kLog2e, nref[j0 + j][0], nref[j0 + j][1]);
             over = fmax3f(over, y0, y1);
           }
         }
@@ -1321,7 +1341,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             rows.l[j][e] = l[j][e];
           }
         }
-        rows = raise_references<D, NR>(a, rows, make_float4(f[0], f[1], f[2], f[3]), s_addr, tm + lanes + T::COLS_O + c0, c0,
+        rows = raise_references<D, NR>(a, rows, s_addr, tm + lanes + T::COLS_O + c0, c0,
                                        quarter, lane, started ? (i - 1) % T::NP : -1, ((i - 1) / T::NP) & 1, bar);
         failed |= rows.failed;
 #pragma unroll
@@ -1347,7 +1367,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           for (int q = 0; q < 4; ++q) {
             const uint32_t* xx = &x[q / 2][4 * j + 2 * (q % 2)];
             float y0, y1;
-            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), f[q], f[q], nref[j0 + j][0], nref[j0 + j][1]);
+            fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), kLog2e, kLog2e, nref[j0 + j][0], nref[j0 + j][1]);
             y0 = exp2_fast(y0);
             y1 = exp2_fast(y1);
             add2_rn(l[j0 + j][0], l[j0 + j][1], l[j0 + j][0], l[j0 + j][1], y0, y1);
