@@ -329,6 +329,10 @@ __device__ __noinline__ void zero_idle_rows(const MultiQueryArgs& a) {
   }
 }
 
+I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
 I4KV_DEVINL float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

@@ -11,18 +11,18 @@
 // long cache costs two short sums instead of one long one: the error stays
 // near 2^-24 sqrt(tokens / TOK) instead of 2^-24 sqrt(tokens).
 //
-// Layout of the work in a CTA of eight warps over a tile of TOK tokens:
-//   logits: a lane holds one token and 8 of every 32 channels (word lane & 3 of
-//     each 16 bytes of the packed row), so code words, scales and queries are
-//     read from shared memory without bank conflicts, and two shuffles finish a
-//     logit; every row reuses the dequantized channels from registers.
-//   softmax: a warp a row, lanes over the tokens.
-//   values: a thread holds two channels of all NR rows and a share of the tile's
-//     tokens; the shares meet in shared memory when the stream ends.
-// Pages arrive by bulk copies into a two-stage ring, the next tile's while the
-// current one is computed. Which of bytes and arithmetic bounds it depends on
-// NR: a tile costs NR * 2 * D * TOK fused multiply-adds whatever the rows'
-// count, so NR is the smallest of 1, 4, 8, 16 that holds the rows of one kv head.
+// A tile is 64 tokens. A warp takes 8 of them from the logits to the values by
+// itself, with its own running maxima, sums and outputs, and the eight warps meet
+// only when the stream ends: nothing in a tile waits for another warp but the
+// copies do (a ninth warp issues them, two stages, as soon as all have left one).
+//   logits: 8 lanes share a token, a lane holds two tokens and 8 of every 64
+//     channels, so a scale or query read from shared memory serves both; a
+//     reduce-scatter leaves each lane one token's logits of NR / 4 rows.
+//   values: a lane holds D / 32 channels of all NR rows; the weights come as
+//     broadcasts from shared memory.
+// Which of bytes and arithmetic bounds it depends on NR: a tile costs NR * 2 * D *
+// 64 fused multiply-adds whatever the rows' count, so NR is the smallest of 1, 4, 8,
+// 16 that holds the rows of one kv head.
 #include <algorithm>
 
 #include "multi_query.cuh"
@@ -31,48 +31,71 @@ using namespace i4kv;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 8, kConsumers = 32 * kWarps, kThreads = kConsumers + 32;
 constexpr int kMaxPerSm = 4;                  // CTAs per SM the workspace is sized for
 constexpr uint64_t kWaitNs = 2000000000ull;  // bounded waits: 2 s
 
 template <int D, int NR, int VK>
 struct Shape {
-  static constexpr int TOK = D == 256 ? 32 : 64;
-  static constexpr int TP = TOK / kMqPage;
+  static constexpr int TOK = 64, TP = TOK / kMqPage;
   static constexpr int VB = VK == INT4KV_VALUES_F32 ? 4 : 2;
   static constexpr int V_BYTES = TOK * D * VB, K_BYTES = TOK * D / 2, SZ_BYTES = TP * 2 * D * 4;
   static constexpr int STAGE = V_BYTES + K_BYTES + SZ_BYTES;
-  static constexpr int P_STRIDE = NR == 1 ? 1 : NR + 4;
+  static constexpr int KB = NR <= 4 ? kWarps : 1;  // copies of the outputs the warps' sums meet in
   static constexpr int Q_OFF = 2 * STAGE;
   static constexpr int O_OFF = Q_OFF + NR * D * 4;
-  static constexpr int S_OFF = O_OFF + NR * D * 4;
-  static constexpr int P_OFF = S_OFF + NR * (TOK + 4) * 4;  // (16-byte aligned: TOK is a multiple of 4)
-  static constexpr int BYTES = P_OFF + TOK * P_STRIDE * 4;
-  static constexpr int PAIRS = D / 2, TG = kThreads / PAIRS, TPG = TOK / TG;
+  static constexpr int P_OFF = O_OFF + KB * NR * D * 4;      // weights [warps][8 tokens][NR]
+  static constexpr int A_OFF = P_OFF + kWarps * 8 * NR * 4;  // rescales [warps][NR]
+  static constexpr int BYTES = A_OFF + kWarps * NR * 4;
+  // Rows whose logits are taken together (registers), and a lane's share of them.
+  static constexpr int RH = D == 256 && NR == 16 ? 8 : NR, H = NR / RH, RPL = RH < 4 ? 1 : RH / 4;
+  static constexpr int CPL = D / 32, CV = CPL < 4 ? CPL : 4;  // a lane's channels, CV side by side
 };
+
+// N = 2 or 4 consecutive stored values as float32.
+template <int VK, int N>
+I4KV_DEVINL void load_values(const void* base, size_t i, float (&x)[N]) {
+  if constexpr (VK == INT4KV_VALUES_F32 && N == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    load_f32<N>(base, VK, i, x);
+  }
+}
+
+// (s0, s1) += (a0 b0, a1 b1), each rounded once.
+I4KV_DEVINL void dot2(float (&s)[2], float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tfma.rn.f32x2 s, x, y, s;\n\t"
+      "mov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(s[0]), "+f"(s[1])
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
 
 template <int D, int NR, int VK>
 __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArgs a) {
   using S = Shape<D, NR, VK>;
-  constexpr int TOK = S::TOK, TP = S::TP;
+  constexpr int TOK = S::TOK, TP = S::TP, RH = S::RH, H = S::H, RPL = S::RPL, CPL = S::CPL, CV = S::CV;
   extern __shared__ __align__(128) char smem[];
-  __shared__ uint64_t s_full[2];
+  __shared__ uint64_t s_full[2], s_empty[2];
   __shared__ uint32_t s_pages[2];
   __shared__ RunPlan s_plan;
-  __shared__ float s_alpha[NR], s_m[NR], s_l[NR];
+  __shared__ float s_m[kWarps][NR], s_l[kWarps][NR];
   __shared__ int s_edge[NR], s_depth[kMqMaxDrafts];
   __shared__ uint64_t s_word[NR];
+  __shared__ volatile int s_failed;  // a wait ran out: nobody waits any more
   float* s_q = reinterpret_cast<float*>(smem + S::Q_OFF);
   float* s_o = reinterpret_cast<float*>(smem + S::O_OFF);
-  float* s_s = reinterpret_cast<float*>(smem + S::S_OFF);
-  float* s_p = reinterpret_cast<float*>(smem + S::P_OFF);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   grid_dependency_wait();
   allow_dependent_launch();
   if (tid == 0) {
-    mbar_init(&s_full[0], TP);
-    mbar_init(&s_full[1], TP);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], TP);
+      mbar_init(&s_empty[i], kWarps);
+    }
+    s_failed = 0;
     fence_barrier_init();
   }
   zero_idle_rows<NR, TP, D>(a);
@@ -88,75 +111,90 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     return;
   }
   const int u1 = plan.tiles;
-
-  SeqWork w = seq_work<NR, TP>(a, plan.b, false), nw = w;  // of the current tile, of the next copied one
-  TileAt p = tile_at(a, w, plan.b, plan.rem), np = p;
-
-  // Copies of tile `np` into stage st (lanes < TP of warp 0, a page each).
-  auto issue = [&](int st) {
-    if (lane < TP) {
-      uint32_t bytes = 0;
-      int phys = 0, home = 0, rows = 0;
-      bool ok = false;
-      const int pg = tile_page<TP>(nw, np.tile, lane);
-      if (np.tile < nw.cache_tiles && page_visible(nw, pg)) {
-        const int32_t* bt = a.block_table + (size_t)np.b * a.max_pages;
-        phys = __ldg(bt + pg);
-        home = __ldg(bt + pg / a.group_pages * a.group_pages);
-        rows = min(kMqPage, nw.len - pg * kMqPage);
-        ok = phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages;
-        if (!ok) mq_status(a.status, kStatusBadPage);
-        if (ok) bytes = (uint32_t)rows * (D * S::VB + D / 2) + 2 * D * 4;
-      }
-      const uint32_t live = __ballot_sync((1u << TP) - 1, ok);
-      if (lane == 0) s_pages[st] = live;
-      __syncwarp((1u << TP) - 1);
-      fence_proxy_async_smem();
-      mbar_arrive_expect_tx(&s_full[st], bytes);
-      if (ok) {
-        char* base = smem + st * S::STAGE;
-        const size_t slab = ((size_t)phys * a.kv_heads + np.head) * kMqPage;
-        bulk_g2s(base + lane * kMqPage * D * S::VB, static_cast<const char*>(a.v_pool) + slab * D * S::VB,
-                 (uint32_t)rows * D * S::VB, &s_full[st]);
-        bulk_g2s(base + S::V_BYTES + lane * kMqPage * D / 2, a.k_pool + slab * (D / 2),
-                 (uint32_t)rows * (D / 2), &s_full[st]);
-        bulk_g2s(base + S::V_BYTES + S::K_BYTES + lane * 2 * D * 4,
-                 a.sz_pool + ((size_t)home * a.kv_heads + np.head) * 2 * D, 2 * D * 4, &s_full[st]);
-      }
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_try_wait(bar, parity) && !s_failed && !mbar_wait_bounded(bar, parity, kWaitNs)) {
+      s_failed = 1;
+      mq_status(a.status, kStatusWaitTimeout);
     }
   };
-  auto step = [&](SeqWork& sw, TileAt& t) {
-    if (++t.tile >= sw.tiles) next_stream<NR, TP>(a, sw, t);
+
+  SeqWork w = seq_work<NR, TP>(a, plan.b, false);
+  TileAt p = tile_at(a, w, plan.b, plan.rem);
+  auto step = [&]() {
+    if (++p.tile >= w.tiles) next_stream<NR, TP>(a, w, p);
   };
 
-  constexpr int RPW = (NR + 7) / 8;  // softmax rows of a warp: warp, warp + 8
-  float m_run[RPW], l_run[RPW];
-  float acc[NR][2];
-  const int pair = tid % S::PAIRS, group = tid / S::PAIRS;
+  if (warp == kWarps) {
+    // ---- copies: lanes < TP, a page each ----
+#pragma unroll 1
+    for (int u = 0; u < u1; ++u) {
+      const int st = u & 1;
+      wait(&s_empty[st], (uint32_t)((u >> 1) + 1) & 1);
+      __syncwarp();
+      if (s_failed) {  // the copies issued so far land, or a bound passes
+        for (int v = max(0, u - 2); v < u; ++v) mbar_wait_bounded(&s_full[v & 1], (uint32_t)(v >> 1) & 1, 10000000ull);
+        break;
+      }
+      if (lane < TP) {
+        uint32_t bytes = 0;
+        int phys = 0, home = 0, rows = 0;
+        bool ok = false;
+        const int pg = tile_page<TP>(w, p.tile, lane);
+        if (p.tile < w.cache_tiles && page_visible(w, pg)) {
+          const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
+          phys = __ldg(bt + pg);
+          home = __ldg(bt + pg / a.group_pages * a.group_pages);
+          rows = min(kMqPage, w.len - pg * kMqPage);
+          ok = phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages;
+          if (!ok) mq_status(a.status, kStatusBadPage);
+          if (ok) bytes = (uint32_t)rows * (D * S::VB + D / 2) + 2 * D * 4;
+        }
+        const uint32_t live = __ballot_sync((1u << TP) - 1, ok);
+        if (lane == 0) s_pages[st] = live;
+        __syncwarp((1u << TP) - 1);
+        mbar_arrive_expect_tx(&s_full[st], bytes);
+        if (ok) {
+          char* base = smem + st * S::STAGE;
+          const size_t slab = ((size_t)phys * a.kv_heads + p.head) * kMqPage;
+          bulk_g2s(base + S::V_BYTES + lane * kMqPage * D / 2, a.k_pool + slab * (D / 2),
+                   (uint32_t)rows * (D / 2), &s_full[st]);
+          bulk_g2s(base + S::V_BYTES + S::K_BYTES + lane * 2 * D * 4,
+                   a.sz_pool + ((size_t)home * a.kv_heads + p.head) * 2 * D, 2 * D * 4, &s_full[st]);
+          bulk_g2s(base + lane * kMqPage * D * S::VB, static_cast<const char*>(a.v_pool) + slab * D * S::VB,
+                   (uint32_t)rows * D * S::VB, &s_full[st]);
+        }
+      }
+      step();
+    }
+    return;
+  }
 
-  if (warp == 0) issue(0);
-  step(nw, np);
-  int copied = 1;
+  const int ql = lane & 7, tl = lane >> 3;        // logits: channels 8 ql + 64 i of tokens tl, tl + 4
+  const int my_tok = tl + 4 * (ql >> 2);          // after the reduction: this token of the warp's 8,
+  const int my_row = (ql & 3) * (NR < 4 ? 0 : RPL);  // rows my_row + RH h + j
+  float* s_p = reinterpret_cast<float*>(smem + S::P_OFF) + warp * 8 * NR;
+  float* s_al = reinterpret_cast<float*>(smem + S::A_OFF) + warp * NR;
+  float m_run[H][RPL], l_run[H][RPL];  // maxima; this lane's share of the sums
+  float acc[NR][CPL];
   bool fresh = true;
 
+#pragma unroll 1
   for (int u = 0; u < u1; ++u) {
     const int st = u & 1;
-    const uint32_t parity = (uint32_t)((u >> 1) & 1);
-    __syncthreads();  // everyone is done with the previous tile
-    if (copied < u1) {
-      if (warp == 0) issue(st ^ 1);
-      if (++copied < u1) step(nw, np);
-    }
-    if (fresh) {  // a stream begins: its queries and what they see
+    if (fresh) {  // a stream begins (no warp is in another tile): its queries and what they see
       fresh = false;
 #pragma unroll
-      for (int j = 0; j < RPW; ++j) {
-        m_run[j] = -INFINITY;
-        l_run[j] = 0.f;
-      }
+      for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int r = 0; r < NR; ++r) acc[r][0] = acc[r][1] = 0.f;
-      for (int i = 2 * tid; i < NR * D; i += 2 * kThreads) {
+        for (int j = 0; j < RPL; ++j) {
+          m_run[h][j] = -INFINITY;
+          l_run[h][j] = 0.f;
+        }
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) acc[r][c] = 0.f;
+      for (int i = 2 * tid; i < NR * D; i += 2 * kConsumers) {
         const int r = i / D, rr = p.chunk * NR + r;
         float x[2] = {0.f, 0.f};
         if (rr < w.rows) load_f32<2>(a.q, a.qk, row_offset(a, w, p.head, rr, D) + (i - r * D), x);
@@ -171,240 +209,263 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         s_edge[tid] = a.window > 0 ? w.pos0 + (a.mask ? draft_depth(word, t, w.drafts) : 0) - a.window : -1;
       }
       if (a.mask && tid < w.drafts) s_depth[tid] = draft_depth((uint64_t)a.mask[w.row0 + tid], tid, w.drafts);
-      __syncthreads();
+      named_bar_sync(1, kConsumers);
     }
     const bool in_cache = p.tile < w.cache_tiles;
-    if (in_cache) {
-      if (!mbar_wait_bounded(&s_full[st], parity, kWaitNs)) mq_status(a.status, kStatusWaitTimeout);
-    } else {
-      mbar_wait_bounded(&s_full[st], parity, kWaitNs);  // an empty phase
-    }
+    wait(&s_full[st], (uint32_t)(u >> 1) & 1);
     const char* base = smem + st * S::STAGE;
-
-    // ---- logits ----
-    constexpr int kPasses = TOK / 64 == 0 ? 1 : TOK / 64;  // 8 warps x 8 tokens
-    bool all_seen = true;
+    const int tok0 = warp * 8;  // the warp's tokens: half a page
+    const int pos0 = in_cache ? tile_page<TP>(w, p.tile, tok0 / kMqPage) * kMqPage + tok0 % kMqPage
+                              : (p.tile - w.cache_tiles) * TOK + tok0;  // position, or draft, of the first
+    const int there = in_cache ? ((s_pages[st] >> (tok0 / kMqPage) & 1) ? min(8, w.len - pos0) : 0)
+                               : min(8, w.drafts - pos0);
+    if (there > 0) {
+      // ---- logits ----
+      float x[H][RPL];
 #pragma unroll
-    for (int ps = 0; ps < kPasses; ++ps) {
-      const int tok = ps * 64 + warp * 8 + (lane >> 2), qd = lane & 3;
-      if (tok < TOK) {
-        float s2[NR][2];
+      for (int h = 0; h < H; ++h) {
+        float s2[2][RH][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) s2[r][0] = s2[r][1] = 0.f;
-        auto rows_add = [&](const float (&k)[8], int c) {
+        for (int r = 0; r < RH; ++r) s2[0][r][0] = s2[0][r][1] = s2[1][r][0] = s2[1][r][1] = 0.f;
+#pragma unroll 1
+        for (int c = 8 * ql; c < D; c += 64) {
+          float k[2][8];
+          if (in_cache) {  // (rows behind the length hold what the stage held: never used)
+            const char* krow = base + S::V_BYTES + (tok0 + tl) * (D / 2) + c / 2;
+            const float* sz = reinterpret_cast<const float*>(base + S::V_BYTES + S::K_BYTES) + tok0 / kMqPage * 2 * D + c;
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(krow), w1 = *reinterpret_cast<const uint32_t*>(krow + 2 * D);
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            const float4 x = *reinterpret_cast<const float4*>(s_q + r * D + c);
-            const float4 y = *reinterpret_cast<const float4*>(s_q + r * D + c + 4);
-            asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
-                "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tfma.rn.f32x2 s, x, y, s;\n\t"
-                "mov.b64 {%0, %1}, s;\n\t}"
-                : "+f"(s2[r][0]), "+f"(s2[r][1]) : "f"(k[0]), "f"(k[1]), "f"(x.x), "f"(x.y));
-            asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
-                "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tfma.rn.f32x2 s, x, y, s;\n\t"
-                "mov.b64 {%0, %1}, s;\n\t}"
-                : "+f"(s2[r][0]), "+f"(s2[r][1]) : "f"(k[2]), "f"(k[3]), "f"(x.z), "f"(x.w));
-            asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
-                "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tfma.rn.f32x2 s, x, y, s;\n\t"
-                "mov.b64 {%0, %1}, s;\n\t}"
-                : "+f"(s2[r][0]), "+f"(s2[r][1]) : "f"(k[4]), "f"(k[5]), "f"(y.x), "f"(y.y));
-            asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
-                "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tfma.rn.f32x2 s, x, y, s;\n\t"
-                "mov.b64 {%0, %1}, s;\n\t}"
-                : "+f"(s2[r][0]), "+f"(s2[r][1]) : "f"(k[6]), "f"(k[7]), "f"(y.z), "f"(y.w));
-          }
-        };
-        int at;        // position of the token (cache), or index of the draft
-        bool real;
-        if (in_cache) {
-          at = tile_page<TP>(w, p.tile, tok / kMqPage) * kMqPage + tok % kMqPage;
-          real = at < w.len && (s_pages[st] >> (tok / kMqPage) & 1);
-          const char* krow = base + S::V_BYTES + tok * (D / 2);
-          const float* sz = reinterpret_cast<const float*>(base + S::V_BYTES + S::K_BYTES) + tok / kMqPage * 2 * D;
-          if (real) {
-#pragma unroll 2
-            for (int c = 8 * qd; c < D; c += 32) {
-              const uint32_t wd = *reinterpret_cast<const uint32_t*>(krow + c / 2);
-              float k[8];
+            for (int j = 0; j < 8; j += 4) {
+              const float4 sc = *reinterpret_cast<const float4*>(sz + j);
+              const float4 zp = *reinterpret_cast<const float4*>(sz + D + j);
 #pragma unroll
-              for (int j = 0; j < 8; j += 4) {
-                const float4 sc = *reinterpret_cast<const float4*>(sz + c + j);
-                const float4 zp = *reinterpret_cast<const float4*>(sz + D + c + j);
-                k[j] = ((float)((wd >> (4 * j)) & 15u) - zp.x) * sc.x;
-                k[j + 1] = ((float)((wd >> (4 * j + 4)) & 15u) - zp.y) * sc.y;
-                k[j + 2] = ((float)((wd >> (4 * j + 8)) & 15u) - zp.z) * sc.z;
-                k[j + 3] = ((float)((wd >> (4 * j + 12)) & 15u) - zp.w) * sc.w;
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t wd = e ? w1 : w0;
+                k[e][j] = ((float)((wd >> (4 * j)) & 15u) - zp.x) * sc.x;
+                k[e][j + 1] = ((float)((wd >> (4 * j + 4)) & 15u) - zp.y) * sc.y;
+                k[e][j + 2] = ((float)((wd >> (4 * j + 8)) & 15u) - zp.z) * sc.z;
+                k[e][j + 3] = ((float)((wd >> (4 * j + 12)) & 15u) - zp.w) * sc.w;
               }
-              rows_add(k, c);
             }
-          }
-        } else {
-          at = (p.tile - w.cache_tiles) * TOK + tok;
-          real = at < w.drafts;
-          if (real) {
-            const size_t row = ((size_t)(w.row0 + at) * a.kv_heads + p.head) * D;
-            for (int c = 8 * qd; c < D; c += 32) {
-              float k[8];
-              load_f32<8>(a.kd, a.qk, row + c, k);
-              rows_add(k, c);
-            }
-          }
-        }
-        float mine[(NR + 3) / 4] = {};
+          } else {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float x = s2[r][0] + s2[r][1];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if ((r & 3) == qd) mine[r >> 2] = x;
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) k[e][j] = 0.f;
+              if (tl + 4 * e < there)
+                load_f32<8>(a.kd, a.qk, ((size_t)(w.row0 + pos0 + tl + 4 * e) * a.kv_heads + p.head) * D + c, k[e]);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < RH; ++r) {
+            const float4 y0 = *reinterpret_cast<const float4*>(s_q + (h * RH + r) * D + c);
+            const float4 y1 = *reinterpret_cast<const float4*>(s_q + (h * RH + r) * D + c + 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              dot2(s2[e][r], k[e][0], k[e][1], y0.x, y0.y);
+              dot2(s2[e][r], k[e][2], k[e][3], y0.z, y0.w);
+              dot2(s2[e][r], k[e][4], k[e][5], y1.x, y1.y);
+              dot2(s2[e][r], k[e][6], k[e][7], y1.z, y1.w);
+            }
+          }
         }
+        // reduce-scatter over the 8 lanes of a token: token tl + 4 to the upper four,
+        // then quarters of the rows
+        float v[RH];
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          const float x0 = s2[0][r][0] + s2[0][r][1], x1 = s2[1][r][0] + s2[1][r][1];
+          const float give = ql & 4 ? x0 : x1, keep = ql & 4 ? x1 : x0;
+          v[r] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
+        }
+        if constexpr (RH == 1) {
+          v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
+          v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+          x[h][0] = v[0];
+        } else {
+          float v2[RH / 2];
+#pragma unroll
+          for (int r = 0; r < RH / 2; ++r) {
+            const float give = ql & 2 ? v[r] : v[r + RH / 2], keep = ql & 2 ? v[r + RH / 2] : v[r];
+            v2[r] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+          }
+#pragma unroll
+          for (int r = 0; r < RPL; ++r) {
+            const float give = ql & 1 ? v2[r] : v2[r + RPL], keep = ql & 1 ? v2[r + RPL] : v2[r];
+            x[h][r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+          }
+        }
+      }
+      // ---- what the rows see ----
+      const int at = pos0 + my_tok;
+      const bool real = my_tok < there;
+      bool guard = !real;
+      if (!in_cache || a.window > 0) {
         const int behind = in_cache ? at : (real && a.window > 0 ? w.pos0 + s_depth[at] : 0);
 #pragma unroll
-        for (int j = 0; j < (NR + 3) / 4; ++j) {
-          const int r = 4 * j + qd;
-          if (NR == 1 && qd != 0) break;
-          bool sees = real;
-          if (!in_cache) sees = sees && (s_word[r] >> (at & 63) & 1);
-          if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
-          all_seen = all_seen && sees;
-          s_s[r * (TOK + 4) + tok] = sees ? mine[j] : -INFINITY;
-        }
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int j = 0; j < RPL; ++j) {
+            const int r = RH * h + my_row + j;
+            bool sees = in_cache || (s_word[r] >> (at & 63) & 1);
+            if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
+            guard = guard || !sees;
+            if (!sees) x[h][j] = -INFINITY;
+          }
       }
-    }
-    const bool guard = !__syncthreads_and(all_seen);
-
-    // ---- softmax: warp w has rows w, w + 8 ----
+      if (!real) {
 #pragma unroll
-    for (int j = 0; j < RPW; ++j) {
-      const int r = warp + 8 * j;
-      if (r < NR) {
-        float x[TOK / 32];
-        float mx = m_run[j];
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < TOK / 32; ++i) {
-          x[i] = s_s[r * (TOK + 4) + 32 * i + lane];
-          mx = fmaxf(mx, x[i]);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[j] - mx) * kLog2e);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < TOK / 32; ++i) {
-          const float e = x[i] == -INFINITY ? 0.f : exp2_fast((x[i] - mx) * kLog2e);
-          s_p[(32 * i + lane) * S::P_STRIDE + r] = e;
-          sum += e;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l_run[j] = fmaf(l_run[j], al, sum);
-        m_run[j] = mx;
-        if (lane == 0) s_alpha[r] = al;
+          for (int j = 0; j < RPL; ++j) x[h][j] = -INFINITY;
       }
-    }
-    __syncthreads();
-
-    // ---- values ----
-    {
-      float ps[NR][2];
+      guard = __any_sync(0xffffffffu, guard);
+      // ---- softmax over the warp's 8 tokens ----
 #pragma unroll
-      for (int r = 0; r < NR; ++r) ps[r][0] = ps[r][1] = 0.f;
-      const int t0 = group * S::TPG;
-      auto value = [&](int t, float (&v)[2]) {
-        if (in_cache) {
-          load_f32<2>(base, VK, (size_t)t * D + 2 * pair, v);
-        } else {
-          const int at = (p.tile - w.cache_tiles) * TOK + t;
-          v[0] = v[1] = 0.f;
-          if (at < w.drafts)
-            load_f32<2>(a.vd, a.qk, ((size_t)(w.row0 + at) * a.kv_heads + p.head) * D + 2 * pair, v);
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int j = 0; j < RPL; ++j) {
+          float mx = fmaxf(m_run[h][j], x[h][j]);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[h][j] - mx) * kLog2e);
+          const float e = x[h][j] == -INFINITY ? 0.f : exp2_fast((x[h][j] - mx) * kLog2e);
+          l_run[h][j] = fmaf(l_run[h][j], al, e);
+          m_run[h][j] = mx;
+          const int r = RH * h + my_row + j;
+          if (NR >= 4 || (ql & 3) == 0) s_p[my_tok * NR + r] = e;
+          if (lane < 4 && (NR >= 4 || lane == 0)) s_al[r] = al;
         }
+      __syncwarp();
+      // ---- values: the tile's sum from zero, then added to the running one ----
+      float ps[NR][CPL];
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) ps[r][c] = 0.f;
+      auto value = [&](int t, int c0, float (&v)[CV]) {
+        const int ch = c0 / CV * 32 * CV + lane * CV;
+        if (in_cache) load_values<VK, CV>(base, (size_t)(tok0 + t) * D + ch, v);
+        else load_f32<CV>(a.vd, a.qk, ((size_t)(w.row0 + pos0 + t) * a.kv_heads + p.head) * D + ch, v);
       };
       if (!guard) {
 #pragma unroll 4
-        for (int t = t0; t < t0 + S::TPG; ++t) {
-          float v[2];
-          value(t, v);
-          if (NR == 1) fma2_rn(ps[0][0], ps[0][1], v[0], v[1], s_p[t]);
+        for (int t = 0; t < 8; ++t) {
 #pragma unroll
-          for (int r = 0; r + 4 <= NR; r += 4) {
-            const float4 e = *reinterpret_cast<const float4*>(s_p + t * S::P_STRIDE + r);
-            fma2_rn(ps[r][0], ps[r][1], v[0], v[1], e.x);
-            fma2_rn(ps[r + 1][0], ps[r + 1][1], v[0], v[1], e.y);
-            fma2_rn(ps[r + 2][0], ps[r + 2][1], v[0], v[1], e.z);
-            fma2_rn(ps[r + 3][0], ps[r + 3][1], v[0], v[1], e.w);
+          for (int c0 = 0; c0 < CPL; c0 += CV) {
+            float v[CV];
+            value(t, c0, v);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+              const float e = s_p[t * NR + r];
+#pragma unroll
+              for (int c = 0; c < CV; c += 2) fma2_rn(ps[r][c0 + c], ps[r][c0 + c + 1], v[c], v[c + 1], e);
+            }
           }
         }
       } else {  // some row does not see some token: what stands there, even NaN, adds nothing
-        static_assert(S::TPG % 4 == 0, "four tokens a turn");
 #pragma unroll 1
-        for (int t4 = t0; t4 < t0 + S::TPG; t4 += 4) {
-          float v[4][2];
+        for (int t = 0; t < there; ++t) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) value(t4 + t, v[t]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
+          for (int c0 = 0; c0 < CPL; c0 += CV) {
+            float v[CV];
+            value(t, c0, v);
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-              const float e = s_p[(t4 + t) * S::P_STRIDE + r];
-              if (e != 0.f) fma2_rn(ps[r][0], ps[r][1], v[t][0], v[t][1], e);
+              const float e = s_p[t * NR + r];
+              if (e != 0.f) {
+#pragma unroll
+                for (int c = 0; c < CV; c += 2) fma2_rn(ps[r][c0 + c], ps[r][c0 + c + 1], v[c], v[c + 1], e);
+              }
             }
+          }
         }
       }
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        const float al = s_alpha[r];
-        acc[r][0] = fmaf(acc[r][0], al, ps[r][0]);
-        acc[r][1] = fmaf(acc[r][1], al, ps[r][1]);
+        const float al = s_al[r];
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) acc[r][c] = fmaf(acc[r][c], al, ps[r][c]);
       }
     }
+    __syncwarp();  // (the weights and the stage are free)
+    if (lane == 0) mbar_arrive(&s_empty[st]);
 
-    // ---- the stream, or this run's share of it, ends ----
+    // ---- the stream, or this run's share of it, ends: the warps meet ----
     const bool ends = p.tile + 1 >= w.tiles;
     if (ends || u + 1 == u1) {
 #pragma unroll
-      for (int j = 0; j < RPW; ++j) {
-        const int r = warp + 8 * j;
-        if (r < NR && lane == 0) {
-          s_m[r] = m_run[j];
-          s_l[r] = l_run[j];
-        }
-      }
-      for (int g = 0; g < S::TG; ++g) {
-        if (group == g) {
+      for (int h = 0; h < H; ++h)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            float2* o = reinterpret_cast<float2*>(s_o + r * D + 2 * pair);
-            float2 x = g == 0 ? make_float2(0.f, 0.f) : *o;
-            x.x += acc[r][0];
-            x.y += acc[r][1];
-            *o = x;
+        for (int j = 0; j < RPL; ++j) {
+          float l = l_run[h][j];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          if (lane < 4 && (NR >= 4 || lane == 0)) {
+            s_m[warp][RH * h + my_row + j] = m_run[h][j];
+            s_l[warp][RH * h + my_row + j] = l;
           }
         }
-        __syncthreads();
+      named_bar_sync(1, kConsumers);
+      auto top_of = [&](int r) {
+        float m = s_m[0][r];
+#pragma unroll
+        for (int i = 1; i < kWarps; ++i) m = fmaxf(m, s_m[i][r]);
+        return m;
+      };
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float m = top_of(r), al = m == -INFINITY ? 1.f : exp2_fast((s_m[warp][r] - m) * kLog2e);
+#pragma unroll
+        for (int c = 0; c < CPL; ++c) acc[r][c] *= al;
+      }
+#pragma unroll 1
+      for (int turn = 0; turn < kWarps / S::KB; ++turn) {
+        if (warp / S::KB == turn) {
+          float* o = s_o + warp % S::KB * (NR * D);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int c = 0; c < CPL; ++c) {
+              float* at = o + r * D + c / CV * 32 * CV + lane * CV + c % CV;
+              *at = turn == 0 ? acc[r][c] : *at + acc[r][c];
+            }
+        }
+        named_bar_sync(1, kConsumers);
       }
       const int first = u - p.tile;  // the stream's first tile
       const bool whole = ends && first >= 0;
-      float* rec = a.recs + (size_t)(2 * cta + (first > 0 ? 1 : 0)) *Record<NR, D>::kFloats;
-      for (int i = 2 * tid; i < NR * D; i += 2 * kThreads) {
+      float* rec = a.recs + (size_t)(2 * cta + (first > 0 ? 1 : 0)) * Record<NR, D>::kFloats;
+      for (int i = 2 * tid; i < NR * D; i += 2 * kConsumers) {
         const int r = i / D, c = i - r * D, rr = p.chunk * NR + r;
         if (rr >= w.rows) continue;
-        const float2 x = *reinterpret_cast<const float2*>(s_o + i);
+        float2 y = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < S::KB; ++k) {
+          const float2 z = *reinterpret_cast<const float2*>(s_o + k * (NR * D) + i);
+          y.x += z.x;
+          y.y += z.y;
+        }
+        const float m = top_of(r);
+        float l = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) l += m == -INFINITY ? 0.f : s_l[k][r] * exp2_fast((s_m[k][r] - m) * kLog2e);
         if (whole) {
-          const float inv = 1.f / fmaxf(s_l[r], 1e-10f);
-          store2(a.out, a.qk, row_offset(a, w, p.head, rr, D) + c, x.x * inv, x.y * inv);
+          const float inv = 1.f / fmaxf(l, 1e-10f);
+          store2(a.out, a.qk, row_offset(a, w, p.head, rr, D) + c, y.x * inv, y.y * inv);
         } else {
-          *reinterpret_cast<float2*>(rec + 2 * NR + i) = x;
+          *reinterpret_cast<float2*>(rec + 2 * NR + i) = y;
           if (c == 0) {
-            rec[r] = s_m[r];
-            rec[NR + r] = s_l[r];
+            rec[r] = m;
+            rec[NR + r] = l;
           }
         }
       }
       fresh = true;
       if (u + 1 == u1 && tid == 0) note_tail(a, cta, plan, w, p, NR);
+      named_bar_sync(1, kConsumers);  // (s_o, s_m and s_l are free)
     }
-    step(w, p);
+    step();
   }
 }
 

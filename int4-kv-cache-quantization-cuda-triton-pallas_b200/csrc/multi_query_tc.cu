@@ -148,9 +148,6 @@ I4KV_DEVINL bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
   return p != 0;
 }
-I4KV_DEVINL void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
 
 // One page of values: box of 64 channels x 16 rows x D / 64 chunks at the pool's
 // page-head slab `slab` (or, of the drafts, 16 rows from `row` of head `slab`).
