@@ -6,23 +6,26 @@
 // visible cached tokens and q . k over the visible drafts, one pass with the
 // running maximum m and sum l, out = sum_j 2^((x_j - m) log2 e) v_j / l. Keys
 // are dequantized in registers, once for the NR rows of a CTA; products and
-// sums are float32 in paired instructions (two lanes of work per issue). A
-// tile's values are summed from zero and then added to the running sum, so a
-// long cache costs two short sums instead of one long one: the error stays
-// near 2^-24 sqrt(tokens / TOK) instead of 2^-24 sqrt(tokens).
+// sums are float32 in paired instructions (two lanes of work per issue). Each of
+// eight warps sums its share of the tokens, where registers allow a tile's values
+// from zero first, so a long cache costs several short sums instead of one long
+// one: the error stays near 2^-24 sqrt(tokens / 64), not 2^-24 sqrt(tokens).
 //
 // A tile is 64 tokens. A warp takes 8 of them from the logits to the values by
 // itself, with its own running maxima, sums and outputs, and the eight warps meet
 // only when the stream ends: nothing in a tile waits for another warp but the
 // copies do (a ninth warp issues them, two stages, as soon as all have left one).
 //   logits: 8 lanes share a token, a lane holds two tokens and 8 of every 64
-//     channels, so a scale or query read from shared memory serves both; a
-//     reduce-scatter leaves each lane one token's logits of NR / 4 rows.
+//     channels, so a scale or query read from shared memory serves both (the upper
+//     four lanes take their second four channels first: the eight 16-byte reads of
+//     a token's lanes then hit different banks); a reduce-scatter leaves each lane one
+//     token's logits of NR / 4 rows.
 //   values: a lane holds D / 32 channels of all NR rows; the weights come as
 //     broadcasts from shared memory.
 // Which of bytes and arithmetic bounds it depends on NR: a tile costs NR * 2 * D *
 // 64 fused multiply-adds whatever the rows' count, so NR is the smallest of 1, 4, 8,
-// 16 that holds the rows of one kv head.
+// 16 that holds the rows of one kv head (head_dim 256: at most 8, what its
+// accumulators leave of the registers).
 #include <algorithm>
 
 #include "multi_query.cuh"
@@ -47,8 +50,7 @@ struct Shape {
   static constexpr int P_OFF = O_OFF + KB * NR * D * 4;      // weights [warps][8 tokens][NR]
   static constexpr int A_OFF = P_OFF + kWarps * 8 * NR * 4;  // rescales [warps][NR]
   static constexpr int BYTES = A_OFF + kWarps * NR * 4;
-  // Rows whose logits are taken together (registers), and a lane's share of them.
-  static constexpr int RH = D == 256 && NR == 16 ? 8 : NR, H = NR / RH, RPL = RH < 4 ? 1 : RH / 4;
+  static constexpr int RPL = NR < 4 ? 1 : NR / 4;             // rows of a lane, once reduced
   static constexpr int CPL = D / 32, CV = CPL < 4 ? CPL : 4;  // a lane's channels, CV side by side
 };
 
@@ -63,6 +65,12 @@ I4KV_DEVINL void load_values(const void* base, size_t i, float (&x)[N]) {
   }
 }
 
+template <bool FIRST, class A, class B>
+I4KV_DEVINL auto& pick(A& a, B& b) {
+  if constexpr (FIRST) return a;
+  else return b;
+}
+
 // (s0, s1) += (a0 b0, a1 b1), each rounded once.
 I4KV_DEVINL void dot2(float (&s)[2], float a0, float a1, float b0, float b1) {
   asm("{\n\t.reg .b64 s, x, y;\n\tmov.b64 s, {%0, %1};\n\t"
@@ -75,7 +83,7 @@ I4KV_DEVINL void dot2(float (&s)[2], float a0, float a1, float b0, float b1) {
 template <int D, int NR, int VK>
 __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArgs a) {
   using S = Shape<D, NR, VK>;
-  constexpr int TOK = S::TOK, TP = S::TP, RH = S::RH, H = S::H, RPL = S::RPL, CPL = S::CPL, CV = S::CV;
+  constexpr int TOK = S::TOK, TP = S::TP, RPL = S::RPL, CPL = S::CPL, CV = S::CV;
   extern __shared__ __align__(128) char smem[];
   __shared__ uint64_t s_full[2], s_empty[2];
   __shared__ uint32_t s_pages[2];
@@ -170,11 +178,12 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   }
 
   const int ql = lane & 7, tl = lane >> 3;        // logits: channels 8 ql + 64 i of tokens tl, tl + 4
+  const int swap = ql & 4;                        // these lanes' second quad of channels comes first
   const int my_tok = tl + 4 * (ql >> 2);          // after the reduction: this token of the warp's 8,
-  const int my_row = (ql & 3) * (NR < 4 ? 0 : RPL);  // rows my_row + RH h + j
+  const int my_row = (ql & 3) * (NR < 4 ? 0 : RPL);  // rows my_row + j
   float* s_p = reinterpret_cast<float*>(smem + S::P_OFF) + warp * 8 * NR;
   float* s_al = reinterpret_cast<float*>(smem + S::A_OFF) + warp * NR;
-  float m_run[H][RPL], l_run[H][RPL];  // maxima; this lane's share of the sums
+  float m_run[RPL], l_run[RPL];  // maxima; this lane's share of the sums
   float acc[NR][CPL];
   bool fresh = true;
 
@@ -184,11 +193,9 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     if (fresh) {  // a stream begins (no warp is in another tile): its queries and what they see
       fresh = false;
 #pragma unroll
-      for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) {
-          m_run[h][j] = -INFINITY;
-          l_run[h][j] = 0.f;
+      for (int j = 0; j < RPL; ++j) {
+          m_run[j] = -INFINITY;
+          l_run[j] = 0.f;
         }
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -221,23 +228,24 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
                                : min(8, w.drafts - pos0);
     if (there > 0) {
       // ---- logits ----
-      float x[H][RPL];
+      float x[RPL];
+      {
+        float s2[2][NR][2];
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        float s2[2][RH][2];
-#pragma unroll
-        for (int r = 0; r < RH; ++r) s2[0][r][0] = s2[0][r][1] = s2[1][r][0] = s2[1][r][1] = 0.f;
-#pragma unroll 1
+        for (int r = 0; r < NR; ++r) s2[0][r][0] = s2[0][r][1] = s2[1][r][0] = s2[1][r][1] = 0.f;
+#pragma unroll(NR <= 4 ? 2 : 1)
         for (int c = 8 * ql; c < D; c += 64) {
           float k[2][8];
           if (in_cache) {  // (rows behind the length hold what the stage held: never used)
             const char* krow = base + S::V_BYTES + (tok0 + tl) * (D / 2) + c / 2;
             const float* sz = reinterpret_cast<const float*>(base + S::V_BYTES + S::K_BYTES) + tok0 / kMqPage * 2 * D + c;
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(krow), w1 = *reinterpret_cast<const uint32_t*>(krow + 2 * D);
+            uint32_t w0 = *reinterpret_cast<const uint32_t*>(krow), w1 = *reinterpret_cast<const uint32_t*>(krow + 2 * D);
+            w0 = __funnelshift_r(w0, w0, 4 * swap);
+            w1 = __funnelshift_r(w1, w1, 4 * swap);
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
-              const float4 sc = *reinterpret_cast<const float4*>(sz + j);
-              const float4 zp = *reinterpret_cast<const float4*>(sz + D + j);
+              const float4 sc = *reinterpret_cast<const float4*>(sz + (j ^ swap));
+              const float4 zp = *reinterpret_cast<const float4*>(sz + D + (j ^ swap));
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const uint32_t wd = e ? w1 : w0;
@@ -252,14 +260,21 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) k[e][j] = 0.f;
-              if (tl + 4 * e < there)
-                load_f32<8>(a.kd, a.qk, ((size_t)(w.row0 + pos0 + tl + 4 * e) * a.kv_heads + p.head) * D + c, k[e]);
+              if (tl + 4 * e < there) {
+                const size_t row = ((size_t)(w.row0 + pos0 + tl + 4 * e) * a.kv_heads + p.head) * D + c;
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                  load_f32<4>(a.kd, a.qk, row + (j ^ swap), y);
+                  k[e][j] = y[0]; k[e][j + 1] = y[1]; k[e][j + 2] = y[2]; k[e][j + 3] = y[3];
+                }
+              }
             }
           }
 #pragma unroll
-          for (int r = 0; r < RH; ++r) {
-            const float4 y0 = *reinterpret_cast<const float4*>(s_q + (h * RH + r) * D + c);
-            const float4 y1 = *reinterpret_cast<const float4*>(s_q + (h * RH + r) * D + c + 4);
+          for (int r = 0; r < NR; ++r) {
+            const float4 y0 = *reinterpret_cast<const float4*>(s_q + r * D + c + swap);
+            const float4 y1 = *reinterpret_cast<const float4*>(s_q + r * D + c + (4 ^ swap));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               dot2(s2[e][r], k[e][0], k[e][1], y0.x, y0.y);
@@ -271,28 +286,28 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         }
         // reduce-scatter over the 8 lanes of a token: token tl + 4 to the upper four,
         // then quarters of the rows
-        float v[RH];
+        float v[NR];
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
+        for (int r = 0; r < NR; ++r) {
           const float x0 = s2[0][r][0] + s2[0][r][1], x1 = s2[1][r][0] + s2[1][r][1];
           const float give = ql & 4 ? x0 : x1, keep = ql & 4 ? x1 : x0;
           v[r] = keep + __shfl_xor_sync(0xffffffffu, give, 4);
         }
-        if constexpr (RH == 1) {
+        if constexpr (NR == 1) {
           v[0] += __shfl_xor_sync(0xffffffffu, v[0], 2);
           v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
-          x[h][0] = v[0];
+          x[0] = v[0];
         } else {
-          float v2[RH / 2];
+          float v2[NR / 2];
 #pragma unroll
-          for (int r = 0; r < RH / 2; ++r) {
-            const float give = ql & 2 ? v[r] : v[r + RH / 2], keep = ql & 2 ? v[r + RH / 2] : v[r];
+          for (int r = 0; r < NR / 2; ++r) {
+            const float give = ql & 2 ? v[r] : v[r + NR / 2], keep = ql & 2 ? v[r + NR / 2] : v[r];
             v2[r] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
           }
 #pragma unroll
           for (int r = 0; r < RPL; ++r) {
             const float give = ql & 1 ? v2[r] : v2[r + RPL], keep = ql & 1 ? v2[r + RPL] : v2[r];
-            x[h][r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+            x[r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
           }
         }
       }
@@ -303,46 +318,45 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
       if (!in_cache || a.window > 0) {
         const int behind = in_cache ? at : (real && a.window > 0 ? w.pos0 + s_depth[at] : 0);
 #pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-          for (int j = 0; j < RPL; ++j) {
-            const int r = RH * h + my_row + j;
+        for (int j = 0; j < RPL; ++j) {
+            const int r = my_row + j;
             bool sees = in_cache || (s_word[r] >> (at & 63) & 1);
             if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
             guard = guard || !sees;
-            if (!sees) x[h][j] = -INFINITY;
+            if (!sees) x[j] = -INFINITY;
           }
       }
       if (!real) {
 #pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-          for (int j = 0; j < RPL; ++j) x[h][j] = -INFINITY;
+        for (int j = 0; j < RPL; ++j) x[j] = -INFINITY;
       }
       guard = __any_sync(0xffffffffu, guard);
       // ---- softmax over the warp's 8 tokens ----
 #pragma unroll
-      for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) {
-          float mx = fmaxf(m_run[h][j], x[h][j]);
+      for (int j = 0; j < RPL; ++j) {
+          float mx = fmaxf(m_run[j], x[j]);
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[h][j] - mx) * kLog2e);
-          const float e = x[h][j] == -INFINITY ? 0.f : exp2_fast((x[h][j] - mx) * kLog2e);
-          l_run[h][j] = fmaf(l_run[h][j], al, e);
-          m_run[h][j] = mx;
-          const int r = RH * h + my_row + j;
+          const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[j] - mx) * kLog2e);
+          const float e = x[j] == -INFINITY ? 0.f : exp2_fast((x[j] - mx) * kLog2e);
+          l_run[j] = fmaf(l_run[j], al, e);
+          m_run[j] = mx;
+          const int r = my_row + j;
           if (NR >= 4 || (ql & 3) == 0) s_p[my_tok * NR + r] = e;
           if (lane < 4 && (NR >= 4 || lane == 0)) s_al[r] = al;
         }
       __syncwarp();
-      // ---- values: the tile's sum from zero, then added to the running one ----
-      float ps[NR][CPL];
+      // ---- values: the tile's sum from zero, then added to the running one (a
+      // shorter chain of roundings); with many sums straight into those ----
+      constexpr bool kApart = NR * CPL < 64;
+      float sum[kApart ? NR : 1][kApart ? CPL : 1];
+      auto& ps = pick<kApart>(sum, acc);
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
+      for (int r = 0; r < NR; ++r) {
+        const float al = kApart ? 0.f : s_al[r];
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) ps[r][c] = 0.f;
+        for (int c = 0; c < CPL; ++c) ps[r][c] = kApart ? 0.f : ps[r][c] * al;
+      }
       auto value = [&](int t, int c0, float (&v)[CV]) {
         const int ch = c0 / CV * 32 * CV + lane * CV;
         if (in_cache) load_values<VK, CV>(base, (size_t)(tok0 + t) * D + ch, v);
@@ -355,11 +369,19 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
           for (int c0 = 0; c0 < CPL; c0 += CV) {
             float v[CV];
             value(t, c0, v);
+            if constexpr (NR == 1) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-              const float e = s_p[t * NR + r];
+              for (int c = 0; c < CV; c += 2) fma2_rn(ps[0][c0 + c], ps[0][c0 + c + 1], v[c], v[c + 1], s_p[t]);
+            } else {  // pairs of rows
 #pragma unroll
-              for (int c = 0; c < CV; c += 2) fma2_rn(ps[r][c0 + c], ps[r][c0 + c + 1], v[c], v[c + 1], e);
+              for (int r = 0; r < NR; r += 4) {
+                const float4 e = *reinterpret_cast<const float4*>(s_p + t * NR + r);
+#pragma unroll
+                for (int c = 0; c < CV; ++c) {
+                  fma2_rn(ps[r][c0 + c], ps[r + 1][c0 + c], e.x, e.y, v[c]);
+                  fma2_rn(ps[r + 2][c0 + c], ps[r + 3][c0 + c], e.z, e.w, v[c]);
+                }
+              }
             }
           }
         }
@@ -381,11 +403,13 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
           }
         }
       }
+      if constexpr (kApart) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const float al = s_al[r];
+        for (int r = 0; r < NR; ++r) {
+          const float al = s_al[r];
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) acc[r][c] = fmaf(acc[r][c], al, ps[r][c]);
+          for (int c = 0; c < CPL; ++c) acc[r][c] = fmaf(acc[r][c], al, sum[r][c]);
+        }
       }
     }
     __syncwarp();  // (the weights and the stage are free)
@@ -395,15 +419,13 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     const bool ends = p.tile + 1 >= w.tiles;
     if (ends || u + 1 == u1) {
 #pragma unroll
-      for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int j = 0; j < RPL; ++j) {
-          float l = l_run[h][j];
+      for (int j = 0; j < RPL; ++j) {
+          float l = l_run[j];
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
           if (lane < 4 && (NR >= 4 || lane == 0)) {
-            s_m[warp][RH * h + my_row + j] = m_run[h][j];
-            s_l[warp][RH * h + my_row + j] = l;
+            s_m[warp][my_row + j] = m_run[j];
+            s_l[warp][my_row + j] = l;
           }
         }
       named_bar_sync(1, kConsumers);
@@ -497,8 +519,10 @@ template <int D>
 cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
   if (rows == 1) return launch_vk<D, 1>(vk, a, sms, ws, n, st);
   if (rows <= 4) return launch_vk<D, 4>(vk, a, sms, ws, n, st);
-  if (rows <= 8) return launch_vk<D, 8>(vk, a, sms, ws, n, st);
-  return launch_vk<D, 16>(vk, a, sms, ws, n, st);
+  if constexpr (D < 256) {
+    if (rows > 8) return launch_vk<D, 16>(vk, a, sms, ws, n, st);
+  }
+  return launch_vk<D, 8>(vk, a, sms, ws, n, st);
 }
 
 }  // namespace
