@@ -750,9 +750,11 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
 
 // Values that no row sees must not reach the product (0 * NaN): cleared. A drafted
 // value that is not finite is taken out too and added for the rows that see it when
-// the stream ends. One thread a token.
+// the stream ends. One thread a token. (The values of tile i - 1 have been multiplied
+// before those of tile i are waited for: a short ring reuses their units, and a wait
+// tells a phase from its neighbours only.)
 template <int D, int NR, int VK>
-__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, int tok) {
+__device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, int i, int tok) {
   using T = Tc<D, NR>;
   TcShared<NR>& sh = tc_shared<D, NR>();
   const TileDesc& d = sh.desc[ds];
@@ -761,7 +763,8 @@ __device__ __noinline__ bool clear_values(const MultiQueryArgs& a, int ds, int t
   const bool draft = d.flags & kDraftTile, real = token_real(a, d, tok / kMqPage, at);
   if (tok < d.pages * kMqPage && (!real || draft)) {
     const int u = d.unit + tok / (kMqPage * T::PPU), s = u % T::NV;
-    ok = tc_wait(&sh.v_full[s], (u / T::NV) & 1, a.status);
+    ok = (i == 0 || tc_wait(&sh.p_empty[(i - 1) % T::NP], ((i - 1) / T::NP) & 1, a.status)) &&
+         tc_wait(&sh.v_full[s], (u / T::NV) & 1, a.status);
     char* row = tc_smem + T::V_OFF + s * T::UNIT + (tok / kMqPage % T::PPU) * T::PAGE_V + (tok % kMqPage) * 128;
     // (the order of a thread's 16-byte pieces spreads a warp's over the banks)
     auto piece = [&](int q) {
@@ -1215,10 +1218,12 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           // (a warp judges its own channels: too small there alone costs time, no more)
           odd |= key_top >= kHalfRoom || ((D >= 128 || ct < D) && !__any_sync(0xffffffffu, key_top >= kHalfLow));
         }
-        // A new stream's queries replace the last one's: every product with those
-        // is done. Otherwise the keys of tile i - 2 have been multiplied.
-        if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
+        // The keys of tile i - 2 have been multiplied. A new stream's queries replace
+        // the last one's: every product with those is done. (In this order: a wait
+        // tells a phase from its neighbours only, and tile i - 3's has to be over
+        // before tile i - 1's is asked for.)
         ok = ok && tc_wait(&sh.kh_empty[i & 1], (i / 2 + 1) & 1, a.status);
+        if (ok && (flags & kFirst) && i > 0) ok = tc_wait(&sh.kh_empty[(i - 1) & 1], ((i - 1) / 2) & 1, a.status);
         // Keys outside float16's range take a power of two per group.
         if (named_bar_or(bar, 128, !ok || odd)) {
           // (uniform over the group: its warps meet in named barriers)
@@ -1372,7 +1377,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
       }
-      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, ds, tok);
+      if (masked && wg == 0) failed |= !clear_values<D, NR, VK>(a, ds, i, tok);
       fence_proxy_async_smem();
       tc_fence_before();
       __syncwarp();

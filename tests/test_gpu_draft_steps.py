@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from helpers import pkg
-from test_gpu_drafts import (BF16, F16, F32, close, logical, make_cache, random_trees, tree64)
+from test_gpu_drafts import (BF16, F16, F32, close, logical, make_cache, random_trees, tokens64, tree64)
 
 pytestmark = pytest.mark.gpu
 
@@ -173,7 +173,6 @@ def test_bad_pages_and_lengths_are_reported(dtype, values):
     assert torch.equal(out[3:], clean[3:]) and torch.isfinite(out).all()
     # the same tokens, as if they were not there: the float64 form without pages 2 and 9
     keep = torch.cat([torch.arange(0, 32), torch.arange(48, 144), torch.arange(160, 200)]).cuda()
-    from test_gpu_drafts import tokens64
     kc, vc = tokens64((k_pool, v_pool, sz, bt), 0, 0, 200, 64)
     # (a page that is bad where its group's scales live hides its whole group: neither does here)
     for i in range(3):
@@ -224,6 +223,35 @@ def test_many_sequences(dtype, values):
     assert torch.isfinite(out).all()
     empty = torch.tensor([x == 0 for x in lens], device="cuda")
     assert (out[empty] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, BF16), (32, 8, 128, F32), (32, 8, 64, F16), (16, 4, 256, BF16),
+                                            (16, 4, 256, F32), (16, 16, 128, F16)])
+@pytest.mark.parametrize("tokens,drafts", [(20, 31), (148, 31), (148, 4), (256, 9), (257, 16), (390, 32), (0, 12)])
+def test_many_short_streams(hq, hkv, d, dtype, tokens, drafts):
+    """Several streams a CTA, each of a few tiles: one's queries, values and sums replace another's."""
+    s = Step([tokens] * 40, [drafts] * 40, hq, hkv, d, 128, dtype, dtype, seed=tokens)
+    first = s.run()
+    close(first, s.want(), dtype)
+    for _ in range(3):
+        assert torch.equal(s.run(), first)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_ragged_batch(dtype):
+    rng = np.random.default_rng(0)
+    s = Step([int(x) for x in rng.integers(0, 6000, 24)], [int(x) for x in rng.integers(0, 33, 24)], 32, 8, 128, 128,
+             dtype, dtype, seed=6)
+    close(s.run(), s.want(), dtype)
+    q = s.q[:24].contiguous()
+    out = C.paged_window_decode(q, *s.pools[:5], window=2000, sinks=20, group_tokens=128)
+    for b, n in enumerate(s.lens):
+        k, v = tokens64(s.pools, b, 0, n, 128)
+        pos = torch.arange(n, device="cuda")
+        sees = (pos > n - 1 - 2000) | (pos < 20)
+        x = torch.einsum("hgd,jhd->hgj", q[b].double().view(8, 4, 128), k[sees])
+        want = torch.einsum("hgj,jhd->hgd", torch.softmax(x, -1), v[sees]).reshape(-1, 128)
+        close(out[b], want, dtype)
 
 
 @pytest.mark.parametrize("group", [16, 48, 256, 4096])
