@@ -84,7 +84,7 @@ __device__ __forceinline__ uint16_t pack4(const float4& v, const float4& mn, con
 // Cross-warp reduction of per-lane [4-channel] min/max into per-channel
 // (min, scale, 1/scale) in shared memory; also emits scale/zp through
 // `emit(ch, s, z)`.
-template <class Emit>
+template <int WARPS = kQuantWarps, class Emit>
 __device__ __forceinline__ void reduce_params(float4 mn, float4 mx, float* s_min, float* s_max,
                                               float* s_lo, float* s_sc, float* s_rc, int slab_c0,
                                               int C, Emit emit) {
@@ -96,7 +96,7 @@ __device__ __forceinline__ void reduce_params(float4 mn, float4 mx, float* s_min
     const int ch = threadIdx.x;
     float lo = s_min[ch], hi = s_max[ch];
 #pragma unroll
-    for (int w = 1; w < kQuantWarps; ++w) {
+    for (int w = 1; w < WARPS; ++w) {
       lo = fminf(lo, s_min[w * kSlab + ch]);
       hi = fmaxf(hi, s_max[w * kSlab + ch]);
     }
@@ -619,9 +619,10 @@ append_quant_kernel(AppendArgs ap, int C, int R, OutPaged op) {
 // staged rows of the old open group are read by the y = 0 CTA alone, and the
 // same CTA writes those of the new one after the barrier that follows its
 // reads: when the rows cross a group boundary the slot is reused in place.
-// Where each row comes from and goes to is looked up once, by the lanes of a warp
-// side by side, and its values are loaded with its keys: every load of a CTA is in
-// flight before the first is used. Bound by HBM bytes for long chunks, by launch
+// Values are copied by CTAs of their own (x = slabs ..): they need no barrier, and
+// without their registers more CTAs share an SM, so one's loads meet another's
+// stores. Where each row comes from and goes to is looked up once, by the lanes of a
+// warp side by side, and every load of a CTA is in flight before the first is used. Bound by HBM bytes for long chunks, by launch
 // and three dependent loads (metadata, page and row, data) for a few tokens.
 struct ExtendArgs {
   const void* k;             // [num_src, C] keys of the kernel's input type
@@ -668,17 +669,22 @@ __device__ __forceinline__ void store_value4(const OutPaged& op, size_t vi, cons
   }
 }
 
-// ROWS: rows of a warp, 8 for groups of up to 64 tokens (half of the registers), else 16.
-template <int KIND, int ROWS>
-__global__ void __launch_bounds__(kQuantThreads)
-extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
-  __shared__ __align__(16) float s_min[kQuantWarps * kSlab];
-  __shared__ __align__(16) float s_max[kQuantWarps * kSlab];
+// WARPS: 8 for groups of up to 64 tokens, else 16, so that a thread never holds more
+// than 8 rows' keys: with 16 rows and their values a thread, one CTA of 8 warps
+// filled an SM's registers (8 x 1000 rows of 32 heads x 128 float32 in groups of 128:
+// 140 us, now 105 us = 3.9 TB/s; 64 x 8 rows of 8 heads bfloat16: 28 us).
+template <int KIND, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 2)
+extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
+  __shared__ __align__(16) float s_min[WARPS * kSlab];
+  __shared__ __align__(16) float s_max[WARPS * kSlab];
   __shared__ __align__(16) float s_lo[kSlab];
   __shared__ __align__(16) float s_sc[kSlab];
   __shared__ __align__(16) float s_rc[kSlab];
+  constexpr int ROWS = 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slab_c0 = blockIdx.x * kSlab;
+  const bool values = (int)blockIdx.x >= slabs;  // (uniform: this CTA copies values)
+  const int slab_c0 = ((int)blockIdx.x - (values ? slabs : 0)) * kSlab;
   const int c0 = slab_c0 + lane * 4;
   const int b = blockIdx.z;
   const int off = ea.tok_off[b], n = ea.tok_off[b + 1] - off, start = ea.start[b], sl = ea.slot[b];
@@ -708,7 +714,7 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   // Lane i: the warp's row i, its page and its input row (kStaged: a staged row).
   constexpr int kStaged = -2;
   int my_page = -1, my_src = kStaged;
-  const int my_r = warp + lane * kQuantWarps;
+  const int my_r = warp + lane * WARPS;
   if (lane < ROWS && my_r < rows) {
     const int pos = gpos + my_r;
     if (pos >= start) my_src = source(pos);
@@ -718,31 +724,39 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
     if (op.status && (bad_page || my_src == -1))
       atomicOr(op.status, (bad_page ? kStatusBadPage : 0u) | (my_src == -1 ? kStatusBadLength : 0u));
   }
-  int gslot = row_bt[gpos / op.page];  // (0 <= gpos < end: in the table)
-  if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
 
-  float4 vals[ROWS], vv[ROWS];
+  const int my_t = (gpos + my_r) % op.page;
+  const int h = c0 / op.head_dim, d = c0 - h * op.head_dim;
+  float4 vals[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = warp + i * kQuantWarps, src = __shfl_sync(0xffffffffu, my_src, i);
-    vals[i] = vv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int r = warp + i * WARPS, src = __shfl_sync(0xffffffffu, my_src, i);
+    vals[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < rows && lane_ok) {
-      if (src == kStaged) {
-        vals[i] = *reinterpret_cast<const float4*>(stage + (size_t)r * C + c0);
-      } else if (src >= 0) {
-        vals[i] = load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
-        if (ea.v) vv[i] = load4_as_f32<KIND>(ea.v, (size_t)src * C + c0);
-      }
+      if (src >= 0) vals[i] = load4_as_f32<KIND>(values ? ea.v : ea.k, (size_t)src * C + c0);
+      else if (src == kStaged && !values) vals[i] = *reinterpret_cast<const float4*>(stage + (size_t)r * C + c0);
     }
   }
+  if (values) {
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int page = __shfl_sync(0xffffffffu, my_page, i), t = __shfl_sync(0xffffffffu, my_t, i);
+      const bool fresh = __shfl_sync(0xffffffffu, my_src, i) != kStaged;
+      if (warp + i * WARPS < rows && lane_ok && page >= 0 && fresh)
+        store_value4(op, (((size_t)page * op.heads + h) * op.page + t) * op.head_dim + d, vals[i]);
+    }
+    return;
+  }
+  int gslot = row_bt[gpos / op.page];  // (0 <= gpos < end: in the table)
+  if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
   float4 mn = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
   float4 mx = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
 #pragma unroll
   for (int i = 0; i < ROWS; ++i)
-    if (warp + i * kQuantWarps < rows && lane_ok) minmax4(vals[i], mn, mx);
+    if (warp + i * WARPS < rows && lane_ok) minmax4(vals[i], mn, mx);
   // (its barriers also order this CTA's reads of the staged rows before the
   // writes of the new open group's below)
-  reduce_params(mn, mx, s_min, s_max, s_lo, s_sc, s_rc, slab_c0, C, [&](int ch, float sc, float zp) {
+  reduce_params<WARPS>(mn, mx, s_min, s_max, s_lo, s_sc, s_rc, slab_c0, C, [&](int ch, float sc, float zp) {
     if (gslot < 0) return;
     const int h = ch / op.head_dim, d = ch - h * op.head_dim;
     float* dst = op.sz_pool + ((size_t)gslot * op.heads + h) * 2 * op.head_dim;
@@ -753,7 +767,7 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   const int open0 = end - end % R;  // first token of the group left open (== end: none)
   if (blockIdx.y == 0 && open0 >= gpos + R && lane_ok) {
     // the rows crossed into another open group: its rows go over the old ones
-    for (int pos = open0 + warp; pos < end; pos += kQuantWarps) {
+    for (int pos = open0 + warp; pos < end; pos += WARPS) {
       const int src = source(pos);
       *reinterpret_cast<float4*>(stage + (size_t)(pos - open0) * C + c0) =
           src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.k, (size_t)src * C + c0);
@@ -762,12 +776,10 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
   const float4 lo = reinterpret_cast<const float4*>(s_lo)[lane];
   const float4 sc = reinterpret_cast<const float4*>(s_sc)[lane];
   const float4 rc = reinterpret_cast<const float4*>(s_rc)[lane];
-  const int h = c0 / op.head_dim, d = c0 - h * op.head_dim;
   const bool keep = blockIdx.y == 0 && open0 == gpos;  // the group stays open: its new rows are staged
-  const int my_t = (gpos + my_r) % op.page;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = warp + i * kQuantWarps;
+    const int r = warp + i * WARPS;
     const int page = __shfl_sync(0xffffffffu, my_page, i), t = __shfl_sync(0xffffffffu, my_t, i);
     const bool fresh = __shfl_sync(0xffffffffu, my_src, i) != kStaged;
     if (r < rows && lane_ok) {
@@ -775,7 +787,6 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, OutPaged op) {
       if (page >= 0) {
         const size_t ph = ((size_t)page * op.heads + h) * op.page + t;
         *reinterpret_cast<uint16_t*>(op.k_pool + ph * (op.head_dim / 2) + d / 2) = pack4(vals[i], lo, sc, rc);
-        if (fresh && ea.v) store_value4(op, ph * op.head_dim + d, vv[i]);
       }
     }
   }
@@ -1341,19 +1352,21 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
   // an open group's rows may come before the new ones: up to group_tokens - 1
   const long long groups = ((long long)max_rows_per_seq + 2 * group_tokens - 2) / group_tokens;
   if (groups > 65535) return cudaErrorInvalidValue;
-  dim3 grid((unsigned)((C + kSlab - 1) / kSlab), (unsigned)groups, batch);
+  const int slabs = (int)((C + kSlab - 1) / kSlab);
+  dim3 grid((unsigned)(v ? 2 * slabs : slabs), (unsigned)groups, batch);
   ExtendArgs ea{k, v, tok_offsets, start_pos, rows, num_src, rows ? num_rows : num_src,
                 stage_slots, k_stage, num_slots, max_rows_per_seq};
   OutPaged op{nullptr, nullptr, nullptr, block_table, max_pages, page_tokens, num_pages,
               num_heads, head_dim, k_pool, v_pool, value_dtype, sz_pool, status};
-  auto pick = [&](auto rows_of_warp) {
-    constexpr int kRows = decltype(rows_of_warp)::value;
-    return kv_dtype == INT4KV_VALUES_F32   ? extend_quant_kernel<INT4KV_VALUES_F32, kRows>
-           : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16, kRows>
-                                           : extend_quant_kernel<INT4KV_VALUES_BF16, kRows>;
+  auto pick = [&](auto warps) {
+    constexpr int kWarps = decltype(warps)::value;
+    return kv_dtype == INT4KV_VALUES_F32   ? extend_quant_kernel<INT4KV_VALUES_F32, kWarps>
+           : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16, kWarps>
+                                           : extend_quant_kernel<INT4KV_VALUES_BF16, kWarps>;
   };
-  auto kern = group_tokens <= 8 * kQuantWarps ? pick(std::integral_constant<int, 8>()) : pick(std::integral_constant<int, 16>());
-  kern<<<grid, kQuantThreads, 0, stream>>>(ea, (int)C, group_tokens, op);
+  const int warps = group_tokens <= 64 ? 8 : 16;
+  auto kern = warps == 8 ? pick(std::integral_constant<int, 8>()) : pick(std::integral_constant<int, 16>());
+  kern<<<grid, warps * 32, 0, stream>>>(ea, (int)C, group_tokens, slabs, op);
   return cudaGetLastError();
 }
 
