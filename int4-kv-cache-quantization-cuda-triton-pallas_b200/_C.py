@@ -14,6 +14,7 @@ The paged entry points (``quantize_int4_grouped``, ``cache_write``,
 Nothing here computes on the CPU: a missing library raises.
 """
 
+import contextlib
 import functools
 
 import torch
@@ -21,13 +22,20 @@ import torch
 from . import _lib
 
 MAX_HEAD_DIM = 256
+_HERE = contextlib.nullcontext()
 PAGE_TOKENS = 16
 
 #: value-pool dtypes of the paged path -> INT4KV_VALUES_* (include/int4kv_b200.h)
 VALUE_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+# (torch.cuda.current_stream builds an object around this number, several us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t):
+    if _raw_stream is not None:
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -45,9 +53,15 @@ def _check_input(t, name):
 
 
 def _same_device(ref, *ts):
+    index = ref.get_device()
     for t in ts:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != index:
             raise RuntimeError("all tensors must be on the same CUDA device")
+
+
+def _guard(index):
+    """``torch.cuda.device(index)``, without its cost (several us) where it is current already."""
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 # --------------------------------------------------------------------------
@@ -669,7 +683,7 @@ def cache_extend(k, v, tok_offsets, start_pos, stage_slots, k_stage, block_table
     _same_device(k, v, tok_offsets, start_pos, stage_slots, rows, k_stage, block_table, k_pool,
                  v_pool, sz_pool, status)
     vk = VALUE_KINDS[v_pool.dtype] if v_pool is not None else 0
-    with torch.cuda.device(k.device):
+    with _guard(k.get_device()):
         _lib.check(lib.int4kv_cache_extend(
             _p(k), _p(v), VALUE_KINDS[k.dtype], k.shape[0], _p(tok_offsets), _p(start_pos),
             _p(rows), rows.shape[0] if rows is not None else k.shape[0],
@@ -712,7 +726,7 @@ def cache_read(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, num
                 raise RuntimeError(f"{name} must be {dtype} {list(shape)}")
     _check_status(status)
     _same_device(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, k_out, v_out, status)
-    with torch.cuda.device(k_pool.device):
+    with _guard(k_pool.get_device()):
         if k_out is None:
             k_out = torch.empty(shape, dtype=dtype, device=k_pool.device)
         if v_pool is not None and v_out is None:
@@ -730,7 +744,7 @@ def _attention_need(batch, q_heads, kv_heads, head_dim, max_drafts, device):
     import ctypes
     lib = _lib.load()
     need = ctypes.c_size_t(0)
-    with torch.cuda.device(device):
+    with _guard(device):
         _lib.check(lib.int4kv_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim,
                                                              max_drafts, ctypes.byref(need)),
                    "paged_attention_workspace_size")
@@ -818,8 +832,8 @@ def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool,
     _check_status(status)
     _same_device(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool, v_pool, sz_pool,
                  block_table, seq_lens, out, workspace, status)
-    with torch.cuda.device(query.device):
-        need = _attention_need(b, hq, hkv, d, int(max_drafts), query.device.index)
+    with _guard(query.get_device()):
+        need = _attention_need(b, hq, hkv, d, int(max_drafts), query.get_device())
         out, workspace = _attention_buffers(query, out, workspace, need, (k_draft, v_draft))
         _lib.check(lib.int4kv_paged_tree_decode(
             _p(query), _p(k_draft), _p(v_draft), VALUE_KINDS[query.dtype], _p(tree_mask),
@@ -848,8 +862,8 @@ def paged_window_decode(query, k_pool, v_pool, sz_pool, block_table, seq_lens, w
         raise RuntimeError(f"window must be positive, got {window}")
     _check_status(status)
     _same_device(query, k_pool, v_pool, sz_pool, block_table, seq_lens, out, workspace, status)
-    with torch.cuda.device(query.device):
-        need = _attention_need(b, hq, hkv, d, 1, query.device.index)
+    with _guard(query.get_device()):
+        need = _attention_need(b, hq, hkv, d, 1, query.get_device())
         out, workspace = _attention_buffers(query, out, workspace, need)
         _lib.check(lib.int4kv_paged_window_decode(
             _p(query), VALUE_KINDS[query.dtype], _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype],
