@@ -233,7 +233,7 @@ struct TcShared {
   float kscale[kDesc][kTile];
   float ref[NR], inv[NR];       // a finished stream's references, inverse sums,
   int row[NR];                  // and rows of the outputs [rows * heads]
-  float part[4][NR];            // maxima, or sums, over the four quarters of a tile's tokens
+  alignas(8) float part[4][NR];  // maxima, or sums, over the four quarters of a tile's tokens
   unsigned long long odd[kSeg];  // per segment: drafts whose values are not all finite
   uint32_t tmem;
   RunPlan plan;
@@ -361,17 +361,24 @@ I4KV_DEVINL float top8(const uint4& u, float top) {
   for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_abs(x[j]));
   return top;
 }
-// Whether any of 8 bfloat16 magnitudes reaches the one whose bits are B.
-template <uint32_t B>
-I4KV_DEVINL uint32_t reaches(const uint4& u) {
-  const uint32_t m = 0x7FFF7FFFu, k = (0x8000u - B) * 0x10001u;  // (|x| + k carries into the sign's place)
-  return (((u.x & m) + k) | ((u.y & m) + k) | ((u.z & m) + k) | ((u.w & m) + k)) & 0x80008000u;
-}
 constexpr uint32_t kBfRoom = 0x4700u, kBfLow = 0x3B80u;  // bfloat16's 2^15, 2^-8
-// 8 16-bit values as float16, times a power of two.
+// The bits of the largest of 8 magnitudes.
+I4KV_DEVINL uint32_t top_bits(const uint4& u) {
+  const uint32_t m = 0x7FFF7FFFu;
+  const uint32_t t = __vmaxu2(__vmaxu2(u.x & m, u.y & m), __vmaxu2(u.z & m, u.w & m));
+  return max(t >> 16, t & 0xFFFFu);
+}
+// 8 16-bit values as float16; times a power of two.
 template <int VK>
-I4KV_DEVINL uint4 to_half8(const uint4& u, float down) {
+I4KV_DEVINL uint4 to_half8(const uint4& u) {
   if (VK == INT4KV_VALUES_F16) return u;
+  float x[8];
+  widen8<VK>(u, x);
+  return make_uint4(pack16<INT4KV_VALUES_F16>(x[0], x[1]), pack16<INT4KV_VALUES_F16>(x[2], x[3]),
+                    pack16<INT4KV_VALUES_F16>(x[4], x[5]), pack16<INT4KV_VALUES_F16>(x[6], x[7]));
+}
+template <int VK>
+__device__ __noinline__ uint4 scale_half8(uint4 u, float down) {
   float x[8];
   widen8<VK>(u, x);
   return make_uint4(pack16<INT4KV_VALUES_F16>(x[0] * down, x[1] * down), pack16<INT4KV_VALUES_F16>(x[2] * down, x[3] * down),
@@ -404,7 +411,11 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int c
   const int p16 = (c8 % 2) * 4 + (c8 % 8) / 4;  // first 16-byte piece of a row's (the next words' is 2 on)
   // channel 64 b + 16 q + 4 j + e stands at 64 b + 16 j + 4 q + e, as in the keys
   char* const to = tc_smem + Tc<D, NR>::Q_OFF + (c8 / 8) * (NR * 128) + (c8 & 2 ? 8 : 0);
-  const int real = min(NR, d.rows - d.first_row), first_row = d.first_row, row0 = d.row0, head = d.head;
+  const int real = min(NR, d.rows - d.first_row);
+  // row r's place: ((row0 + t) kv_heads + head) group_q + rr - t group_q, rr = first_row + r
+  // (31 bits: checked on the host)
+  const int place = (d.row0 * a.kv_heads + d.head) * a.group_q + d.first_row, per_draft = (a.kv_heads - 1) * a.group_q;
+  const uint16_t* const q = static_cast<const uint16_t*>(a.q) + c8 * 8;
   const uint32_t mates = (kRowThreads == 32 ? 0xffffffffu : (1u << (kRowThreads & 31)) - 1) << (ct % 32 / kRowThreads * kRowThreads);
   constexpr int kBatch = kPieces < 8 ? kPieces : 8;  // loads in flight
   static_assert(kStep <= NR, "every thread has a row");
@@ -416,24 +427,25 @@ __device__ __noinline__ void load_queries(const MultiQueryArgs& a, int ds, int c
       const int r = r0 + (k0 + k) * kStep;
       u[k] = make_uint4(0, 0, 0, 0);
       if (r < real)
-        u[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                    out_row(a, row0, head, sh.draft[seg][r], first_row + r) * D) + c8);
+        u[k] = __ldg(reinterpret_cast<const uint4*>(q + (size_t)(place + r + sh.draft[seg][r] * per_draft) * D));
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int r = r0 + (k0 + k) * kStep;
-      Pow2 p = {1.f, 1.f};
+      uint4 h = to_half8<VK>(u[k]);
       if (VK == INT4KV_VALUES_BF16) {
-        const uint32_t high = __ballot_sync(0xffffffffu, reaches<kBfRoom>(u[k]));
-        const uint32_t some = __ballot_sync(0xffffffffu, reaches<kBfLow>(u[k]));
+        const uint32_t top = top_bits(u[k]);
+        const uint32_t high = __ballot_sync(0xffffffffu, top >= kBfRoom), some = __ballot_sync(0xffffffffu, top >= kBfLow);
         const bool scaled = r < real && ((high & mates) || !(some & mates));
-        if (__any_sync(0xffffffffu, scaled)) p = row_scale<VK, kRowThreads>(u[k], scaled);
-        if (c8 == 0) {
-          sh.qscale[seg][r] = p.up;
-          if (p.up != 1.f) sh.qscaled[seg] = 1;
+        float up = 1.f;
+        if (__any_sync(0xffffffffu, scaled)) {
+          const Pow2 p = row_scale<VK, kRowThreads>(u[k], scaled);
+          if (scaled) h = scale_half8<VK>(u[k], p.down);
+          up = p.up;
+          if (up != 1.f) sh.qscaled[seg] = 1;
         }
+        if (c8 == 0) sh.qscale[seg][r] = up;
       }
-      const uint4 h = to_half8<VK>(u[k], p.down);
       char* at = to + r * 128;
       *reinterpret_cast<uint2*>(at + ((p16 ^ (r & 7)) << 4)) = make_uint2(h.x, h.y);
       *reinterpret_cast<uint2*>(at + (((p16 + 2) ^ (r & 7)) << 4)) = make_uint2(h.z, h.w);
@@ -565,7 +577,7 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
           if (t4 == 0) sh.kscale[ds][r ? tb : ta] = up;
         }
       }
-      uint32_t some[2] = {0, 0};
+      uint32_t top[2] = {0, 0};
 #pragma unroll 1
       for (int blk = 0; blk < D / 64; ++blk) {
         uint4 u[4];
@@ -578,9 +590,9 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
         uint32_t h[16];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          big |= reaches<kBfRoom>(u[k]);
-          some[k / 2] |= reaches<kBfLow>(u[k]);
-          const uint4 v = to_half8<VK>(u[k], down[k / 2]);
+          top[k / 2] = max(top[k / 2], top_bits(u[k]));
+          uint4 v = to_half8<VK>(u[k]);
+          if (scaled) v = scale_half8<VK>(u[k], down[k / 2]);
           // channels 8 e + 2 j, + 1: fragment column (2 e + j / 2), word j % 2
           h[8 * (k % 2) + 2 * (k / 2)] = v.x;
           h[8 * (k % 2) + 2 * (k / 2) + 1] = v.y;
@@ -590,7 +602,7 @@ __device__ __noinline__ bool draft_keys(const MultiQueryArgs& a, int ds, uint32_
         __syncwarp();
         tc_st_frag(keys + ((uint32_t)(16 * p) << 16) + 32 * blk, h);
       }
-      if ((ta < drafts && !some[0]) || (tb < drafts && !some[1])) big = 1;
+      big |= (ta < drafts && (top[0] < kBfLow || top[0] >= kBfRoom)) || (tb < drafts && (top[1] < kBfLow || top[1] >= kBfRoom));
     }
     if (VK == INT4KV_VALUES_F16 || scaled || !named_bar_or(bar, 128, big)) break;
     scaled = true;
@@ -688,6 +700,9 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
   using T = Tc<D, NR>;
   constexpr int NI = T::NC / 8, LI = NI < 4 ? NI : 4;
   const int g = lane >> 2, t4 = lane & 3;
+  // Maxima of 2 NI rows over a thread's four tokens, then over the 8 threads with the
+  // same t4: each gives half of its rows away and keeps the other, three times.
+  float m[2 * NI];
 #pragma unroll
   for (int j0 = 0; j0 < NI; j0 += LI) {
     uint32_t x[2][4 * LI];
@@ -695,19 +710,30 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
 #pragma unroll
     for (int j = 0; j < LI; ++j) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float m = kNoRef;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          m = fmaxf(m, __uint_as_float(x[q / 2][4 * j + 2 * (q % 2) + e]) * kLog2e);
-        }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-        if (g == 0) sh.part[quarter][c0 + 8 * (j0 + j) + 2 * t4 + e] = m;
-      }
+      for (int e = 0; e < 2; ++e)
+        m[2 * (j0 + j) + e] = fmaxf(fmaxf(__uint_as_float(x[0][4 * j + e]), __uint_as_float(x[0][4 * j + 2 + e])),
+                                    fmaxf(__uint_as_float(x[1][4 * j + e]), __uint_as_float(x[1][4 * j + 2 + e])));
     }
   }
+  int at = 0;  // first of the pairs of rows this thread keeps
+#pragma unroll
+  for (int o = 4, n = 2 * NI; o > 0; o >>= 1) {
+    if (n > 2) {  // (pairs stay together)
+      n /= 2;
+      const bool upper = g & o;
+      at += upper ? n / 2 : 0;
+#pragma unroll
+      for (int k = 0; k < n; ++k) {
+        const float give = upper ? m[k] : m[k + n], keep = upper ? m[k + n] : m[k];
+        m[k] = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, 4 * o));
+      }
+    } else {
+      m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], 4 * o));
+      m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], 4 * o));
+    }
+  }
+  *reinterpret_cast<float2*>(&sh.part[quarter][c0 + 8 * at + 2 * t4]) =
+      make_float2(fmaxf(m[0] * kLog2e, kNoRef), fmaxf(m[1] * kLog2e, kNoRef));
   s.failed = prev >= 0 && !tc_wait(&sh.p_empty[prev & 1], parity, a.status);  // the weights of tile i - 1 have been multiplied
   named_bar_sync(bar, 128);
   tc_fence_after();
@@ -716,12 +742,16 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
     float al[LI][2];
 #pragma unroll
     for (int j = 0; j < LI; ++j) {
+      float2 top = make_float2(-s.nref[j0 + j][0], -s.nref[j0 + j][1]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 p = *reinterpret_cast<const float2*>(&sh.part[q][c0 + 8 * (j0 + j) + 2 * t4]);
+        top = make_float2(fmaxf(top.x, p.x), fmaxf(top.y, p.y));
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = c0 + 8 * (j0 + j) + 2 * t4 + e;
-        const float old = -s.nref[j0 + j][e];
-        const float m = fmaxf(fmaxf(fmaxf(sh.part[0][r], sh.part[1][r]), fmaxf(sh.part[2][r], sh.part[3][r])), old);
-        al[j][e] = exp2_fast(old - m);
+        const float m = e ? top.y : top.x;
+        al[j][e] = exp2_fast(-s.nref[j0 + j][e] - m);
         s.nref[j0 + j][e] = -m;
         s.l[j0 + j][e] *= al[j][e];
       }
@@ -1332,7 +1362,8 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
           }
         }
       }
-      if (named_bar_or(bar, 128, over > kLazy || failed)) {
+      const bool raised = named_bar_or(bar, 128, over > kLazy || failed);  // (the warpgroup's answer)
+      if (raised) {
         if (named_bar_or(bar, 128, failed)) break;
         RowState<NI> rows;
 #pragma unroll
@@ -1390,6 +1421,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
       started = true;
       if (last) {
         // ---- epilogue: O^T, a lane a channel, over the sums of the weights ----
+        if (raised) named_bar_sync(bar, 128);  // (every warp has read the maxima where the sums go)
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
 #pragma unroll

@@ -237,6 +237,17 @@ def test_many_short_streams(hq, hkv, d, dtype, tokens, drafts):
         assert torch.equal(s.run(), first)
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, BF16), (8, 8, 64, F16), (16, 4, 256, BF16), (8, 2, 128, F32)])
+def test_logits_that_rise_late(hq, hkv, d, dtype):
+    """The largest logits in a stream's last tile: every sum and output before it shrinks."""
+    s = Step([300] * 30 + [100, 129], [20] * 32, hq, hkv, d, 128, dtype, dtype, seed=2)
+    s.k *= 8
+    first = s.run()
+    close(first, s.want(), dtype)
+    for _ in range(3):
+        assert torch.equal(s.run(), first)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_long_ragged_batch(dtype):
     rng = np.random.default_rng(0)
