@@ -499,7 +499,8 @@ cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, in
  * outside every window or in drafts nobody sees is never part of a result, even
  * NaN; a 16-bit cached value that some row of a sequence sees must be finite for
  * the results of its other rows to be. Pages outside the pool are not read: their
- * tokens are not seen (INT4KV_STATUS_BAD_PAGE). Offsets outside [0, num_rows] or
+ * tokens are not seen (INT4KV_STATUS_BAD_PAGE); nor are those of a group whose first
+ * page, which keeps its scales, is outside (with a window, that page may lie before it). Offsets outside [0, num_rows] or
  * too many drafts skip the sequence's drafts, a bad length is clamped to the
  * table (INT4KV_STATUS_BAD_LENGTH). Results do not depend on the order of any
  * atomics: equal calls on equal devices give equal bits. */

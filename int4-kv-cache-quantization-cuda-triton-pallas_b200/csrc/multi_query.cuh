@@ -9,9 +9,9 @@
 // tokens. The streams' tiles are laid end to end and
 // every CTA takes one contiguous run of equal cost, whatever the lengths are: a
 // tile costs one unit, and what a stream costs besides (its queries, its end, and
-// drafts' masks) is counted as a few units before its first tile. A stream inside one run is finished
-// by its CTA; of a shared stream each CTA leaves a record (m, l, acc) per
-// row, and the first of them a note of who shares it (RunTail), by which
+// drafts' masks) is counted as a few units before its first tile. A stream inside one
+// run is finished by its CTA; of a shared stream each CTA leaves a record (m, l, acc)
+// per row, and the first of them a note of who shares it (RunTail), by which
 // merge_records_kernel, one block per run, combines them. Records and notes need
 // no counters, so the workspace carries nothing between launches, and their order
 // of combination is fixed: equal inputs give equal bits.

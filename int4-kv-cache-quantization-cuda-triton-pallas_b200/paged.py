@@ -271,9 +271,11 @@ class PagedKVCache:
                       sinks: int = 0) -> torch.Tensor:
         """``decode`` over each sequence's last ``window`` and first ``sinks`` tokens only.
 
+        The pages before the window are not read, but for the first page of a group
+        that reaches into it, which keeps the group's scales.
         query [B, heads, head_dim] float32, or of the value pool's 16-bit type.
         """
-        bt, sl = self.block_table(seq_ids)
+        bt, sl = self.block_table(list(seq_ids))
         return _C.paged_window_decode(query.to(self.device).contiguous(), self.k_pool, self.v_pool,
                                       self.sz_pool, bt, sl, window=window, sinks=sinks,
                                       group_tokens=self.group_tokens)
@@ -287,10 +289,10 @@ class PagedKVCache:
         (rotated, not in the cache), ``mask`` from ``tree_mask``. float32, or of
         the value pool's 16-bit type. ``extend`` then writes the accepted path.
         """
-        n = [int(c) for c in counts]
-        if len(n) != len(list(seq_ids)) or any(c < 0 for c in n) or sum(n) > query.shape[0]:
+        ids, n = list(seq_ids), [int(c) for c in counts]
+        if not ids or len(n) != len(ids) or any(c < 0 for c in n) or sum(n) > query.shape[0]:
             raise ValueError("counts must give the number of drafts of each sequence")
-        bt, sl = self.block_table(seq_ids)
+        bt, sl = self.block_table(ids)
         offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n)]).astype(np.int32))
         return _C.paged_tree_decode(
             query.to(self.device).contiguous(), k_draft.to(self.device).contiguous(),
