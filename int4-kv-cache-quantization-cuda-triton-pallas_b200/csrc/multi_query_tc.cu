@@ -53,6 +53,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "multi_query.cuh"
 
@@ -1522,11 +1523,25 @@ cudaError_t launch(const MultiQueryArgs& args, int sms, void* ws, size_t ws_byte
 }
 
 // Rows of one kv head's chunk: the smallest of 16, 32, 64, 128 that holds them
-// (head_dim 256: at most 64, the most its shared memory holds).
-int rows_of(long long rows, int dim) {
+// (head_dim 256: at most 64, the most its shared memory holds). More than 64 rows go in
+// chunks of 64 all the same where a CTA has little to do (`units` of 128-row tiles, at
+// most): a tile of 64 is not half as dear, but a stream's start and end are. (drafts
+// over 8 sequences, 128 rows a kv head, 64 against 128: 5.6 units 43 and 47 us, 12 units
+// 66 and 74; 16 x 1000 tokens, 256 rows, 21 units 135 and 115; 8 x 8192, 30 units 113 and
+// 109; 32 x 8192 410 and 320.)
+constexpr double kFewUnits = 12;
+int rows_of(long long rows, int dim, double units) {
   if (rows <= 16) return 16;
   if (rows <= 32) return 32;
-  return rows <= 64 || dim == 256 ? 64 : 128;
+  return rows <= 64 || dim == 256 || units < kFewUnits ? 64 : 128;
+}
+// Units of a CTA in tiles of 128 rows, from the sizes that the host knows: the table's
+// width, or the window, for every sequence.
+double units_of(const MultiQueryArgs& a, long long rows, int sms) {
+  double pages = a.max_pages;
+  if (a.window > 0) pages = std::min(pages, ((double)a.window + a.sinks) / kMqPage + 2);
+  return (double)a.batch * a.kv_heads * (double)((rows + 127) / 128) *
+         (std::ceil(pages / kTilePages) + 1 + kStreamUnits + kDraftUnits) / sms;
 }
 
 template <int D, int NR>
@@ -1550,12 +1565,13 @@ cudaError_t launch_rows(int nr, const MultiQueryArgs& a, int sms, void* ws, size
 namespace i4kv {
 
 size_t multi_query_tc_workspace(int dim, long long rows, int sms) {
-  const int nr = rows_of(rows, dim);
+  const int nr = rows_of(rows, dim, kFewUnits);  // (the larger choice)
   return mq_workspace_bytes(sms, 2 * nr + nr * dim);
 }
 
 cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, void* ws, size_t ws_bytes, cudaStream_t stream) {
-  const int nr = rows_of((long long)std::max(1, a.max_drafts) * a.group_q, dim);
+  const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
+  const int nr = rows_of(rows, dim, units_of(a, rows, sms));
   if (dim == 64) return launch_rows<64>(nr, a, sms, ws, ws_bytes, stream);
   if (dim == 128) return launch_rows<128>(nr, a, sms, ws, ws_bytes, stream);
   return launch_rows<256>(nr, a, sms, ws, ws_bytes, stream);

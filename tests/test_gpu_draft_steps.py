@@ -248,6 +248,15 @@ def test_logits_that_rise_late(hq, hkv, d, dtype):
         assert torch.equal(s.run(), first)
 
 
+@pytest.mark.parametrize("batch,tokens", [(1, 300), (40, 300), (6, 2500)])
+@pytest.mark.parametrize("hq,hkv,d,drafts", [(32, 4, 128, 40), (28, 4, 64, 33), (16, 2, 256, 30)])
+def test_rows_in_chunks(batch, tokens, hq, hkv, d, drafts):
+    """More rows a kv head than a chunk holds, with little and with much to do a CTA."""
+    s = Step([tokens] * batch, [drafts] * batch, hq, hkv, d, 64, BF16, BF16, seed=batch)
+    close(s.run(), s.want(), BF16)
+    close(s.run(window=200, sinks=10), s.want(200, 10), BF16)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_long_ragged_batch(dtype):
     rng = np.random.default_rng(0)
