@@ -140,16 +140,11 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
 #pragma unroll 1
     for (int u = 0; u < u1; ++u) {
       const int st = u & 1;
-      wait(&s_empty[st], (uint32_t)((u >> 1) + 1) & 1);
-      __syncwarp();
-      if (s_failed) {  // the copies issued so far land, or a bound passes
-        for (int v = max(0, u - 2); v < u; ++v) mbar_wait_bounded(&s_full[v & 1], (uint32_t)(v >> 1) & 1, 10000000ull);
-        break;
-      }
+      // (the pages are looked up while the stage is still in use)
+      uint32_t bytes = 0;
+      int phys = 0, home = 0, rows = 0;
+      bool ok = false;
       if (lane < TP) {
-        uint32_t bytes = 0;
-        int phys = 0, home = 0, rows = 0;
-        bool ok = false;
         const int pg = tile_page<TP>(w, p.tile, lane);
         if (p.tile < w.cache_tiles && page_visible(w, pg)) {
           const int32_t* bt = a.block_table + (size_t)p.b * a.max_pages;
@@ -160,20 +155,26 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
           if (!ok) mq_status(a.status, kStatusBadPage);
           if (ok) bytes = (uint32_t)rows * (D * S::VB + D / 2) + 2 * D * 4;
         }
-        const uint32_t live = __ballot_sync((1u << TP) - 1, ok);
-        if (lane == 0) s_pages[st] = live;
-        __syncwarp((1u << TP) - 1);
-        mbar_arrive_expect_tx(&s_full[st], bytes);
-        if (ok) {
-          char* base = smem + st * S::STAGE;
-          const size_t slab = ((size_t)phys * a.kv_heads + p.head) * kMqPage;
-          bulk_g2s(base + S::V_BYTES + lane * kMqPage * D / 2, a.k_pool + slab * (D / 2),
-                   (uint32_t)rows * (D / 2), &s_full[st]);
-          bulk_g2s(base + S::V_BYTES + S::K_BYTES + lane * 2 * D * 4,
-                   a.sz_pool + ((size_t)home * a.kv_heads + p.head) * 2 * D, 2 * D * 4, &s_full[st]);
-          bulk_g2s(base + lane * kMqPage * D * S::VB, static_cast<const char*>(a.v_pool) + slab * D * S::VB,
-                   (uint32_t)rows * D * S::VB, &s_full[st]);
-        }
+      }
+      const uint32_t live = __ballot_sync(0xffffffffu, ok);
+      wait(&s_empty[st], (uint32_t)((u >> 1) + 1) & 1);
+      __syncwarp();
+      if (s_failed) {  // the copies issued so far land, or a bound passes
+        for (int v = max(0, u - 2); v < u; ++v) mbar_wait_bounded(&s_full[v & 1], (uint32_t)(v >> 1) & 1, 10000000ull);
+        break;
+      }
+      if (lane == 0) s_pages[st] = live;
+      __syncwarp();
+      if (lane < TP) mbar_arrive_expect_tx(&s_full[st], bytes);
+      if (ok) {
+        char* base = smem + st * S::STAGE;
+        const size_t slab = ((size_t)phys * a.kv_heads + p.head) * kMqPage;
+        bulk_g2s(base + S::V_BYTES + lane * kMqPage * D / 2, a.k_pool + slab * (D / 2), (uint32_t)rows * (D / 2),
+                 &s_full[st]);
+        bulk_g2s(base + S::V_BYTES + S::K_BYTES + lane * 2 * D * 4,
+                 a.sz_pool + ((size_t)home * a.kv_heads + p.head) * 2 * D, 2 * D * 4, &s_full[st]);
+        bulk_g2s(base + lane * kMqPage * D * S::VB, static_cast<const char*>(a.v_pool) + slab * D * S::VB,
+                 (uint32_t)rows * D * S::VB, &s_full[st]);
       }
       step();
     }
@@ -197,9 +198,9 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
       fresh = false;
 #pragma unroll
       for (int j = 0; j < RPL; ++j) {
-          m_run[j] = -INFINITY;
-          l_run[j] = 0.f;
-        }
+        m_run[j] = -INFINITY;
+        l_run[j] = 0.f;
+      }
 #pragma unroll
       for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -322,12 +323,12 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
         const int behind = in_cache ? at : (real && a.window > 0 ? w.pos0 + s_depth[at] : 0);
 #pragma unroll
         for (int j = 0; j < RPL; ++j) {
-            const int r = my_row + j;
-            bool sees = in_cache || (s_word[r] >> (at & 63) & 1);
-            if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
-            guard = guard || !sees;
-            if (!sees) x[j] = -INFINITY;
-          }
+          const int r = my_row + j;
+          bool sees = in_cache || (s_word[r] >> (at & 63) & 1);
+          if (a.window > 0) sees = sees && (behind > s_edge[r] || behind < a.sinks);
+          guard = guard || !sees;
+          if (!sees) x[j] = -INFINITY;
+        }
       }
       if (!real) {
 #pragma unroll
@@ -337,17 +338,17 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
       // ---- softmax over the warp's 8 tokens ----
 #pragma unroll
       for (int j = 0; j < RPL; ++j) {
-          float mx = fmaxf(m_run[j], x[j]);
+        float mx = fmaxf(m_run[j], x[j]);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[j] - mx) * kLog2e);
-          const float e = x[j] == -INFINITY ? 0.f : exp2_fast((x[j] - mx) * kLog2e);
-          l_run[j] = fmaf(l_run[j], al, e);
-          m_run[j] = mx;
-          const int r = my_row + j;
-          if (NR >= 4 || (ql & 3) == 0) s_p[my_tok * NR + r] = e;
-          if (lane < 4 && (NR >= 4 || lane == 0)) s_al[r] = al;
-        }
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float al = mx == -INFINITY ? 1.f : exp2_fast((m_run[j] - mx) * kLog2e);
+        const float e = x[j] == -INFINITY ? 0.f : exp2_fast((x[j] - mx) * kLog2e);
+        l_run[j] = fmaf(l_run[j], al, e);
+        m_run[j] = mx;
+        const int r = my_row + j;
+        if (NR >= 4 || (ql & 3) == 0) s_p[my_tok * NR + r] = e;
+        if (lane < 4 && (NR >= 4 || lane == 0)) s_al[r] = al;
+      }
       __syncwarp();
       // ---- values: the tile's sum from zero, then added to the running one (a
       // shorter chain of roundings); with many sums straight into those ----
@@ -423,14 +424,14 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
     if (ends || u + 1 == u1) {
 #pragma unroll
       for (int j = 0; j < RPL; ++j) {
-          float l = l_run[j];
+        float l = l_run[j];
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-          if (lane < 4 && (NR >= 4 || lane == 0)) {
-            s_m[warp][my_row + j] = m_run[j];
-            s_l[warp][my_row + j] = l;
-          }
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane < 4 && (NR >= 4 || lane == 0)) {
+          s_m[warp][my_row + j] = m_run[j];
+          s_l[warp][my_row + j] = l;
         }
+      }
       named_bar_sync(1, kConsumers);
       auto top_of = [&](int r) {
         float m = s_m[0][r];
