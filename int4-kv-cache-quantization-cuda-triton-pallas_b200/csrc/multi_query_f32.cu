@@ -27,7 +27,7 @@
 // 16 that holds the rows of one kv head (head_dim 256: at most 8, what its
 // accumulators leave of the registers).
 // Measured (B200, 32 heads, head_dim 128, float32 values): window of 2000 over 32 x
-// 4096 tokens 243 us (4.9 TB/s, HBM and the logits' arithmetic); 4 drafts over 8 x
+// 4096 tokens 220 us (5.5 TB/s, HBM and the logits' arithmetic); 4 drafts over 8 x
 // 2048 90 us (3.4 TB/s, issue and shared-memory reads).
 #include <algorithm>
 
