@@ -622,8 +622,9 @@ append_quant_kernel(AppendArgs ap, int C, int R, OutPaged op) {
 // Values are copied by CTAs of their own (x = slabs ..): they need no barrier, and
 // without their registers more CTAs share an SM, so one's loads meet another's
 // stores. Where each row comes from and goes to is looked up once, by the lanes of a
-// warp side by side, and every load of a CTA is in flight before the first is used. Bound by HBM bytes for long chunks, by launch
-// and three dependent loads (metadata, page and row, data) for a few tokens.
+// warp side by side, and every load of a CTA is in flight before the first is used.
+// Bound by HBM bytes for long chunks, by launch and three dependent loads (metadata,
+// page and row, data) for a few tokens.
 struct ExtendArgs {
   const void* k;             // [num_src, C] keys of the kernel's input type
   const void* v;             // [num_src, C] (nullable)
@@ -1343,7 +1344,7 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
     return cudaErrorInvalidValue;
   if (!tok_offsets || !start_pos || !stage_slots || !k_stage || !block_table || !k_pool || !sz_pool)
     return cudaErrorInvalidValue;
-  if (!aligned16(k_stage)) return cudaErrorInvalidValue;
+  if (!aligned16(k_stage) || !aligned16(k_pool)) return cudaErrorInvalidValue;
   const long long C = (long long)num_heads * head_dim;
   if (C > (1 << 30)) return cudaErrorInvalidValue;
   if (max_rows_per_seq == 0 || num_src == 0 || num_rows == 0) return cudaSuccess;

@@ -122,7 +122,7 @@ def test_extend_refuses(lib, bad):
 
 def test_extend_refuses_misaligned(lib):
     keep, p = aligned()
-    for name in ("k", "v", "vp", "stage"):
+    for name in ("k", "v", "kp", "vp", "stage"):
         assert extend(lib, p, **{name: p + 8}) == INVALID
     assert extend(lib, p, max_rows=0) == OK
 
@@ -147,6 +147,12 @@ def read(lib, p, **kw):
 def test_read_refuses(lib, bad):
     keep, p = aligned()
     assert read(lib, p, **bad) == INVALID
+
+
+@pytest.mark.parametrize("name", ["kp", "vp", "sz", "ko", "vo"])
+def test_read_refuses_misaligned(lib, name):
+    keep, p = aligned()
+    assert read(lib, p, **{name: p + 4}) == INVALID
 
 
 def test_tree_mask_words():
