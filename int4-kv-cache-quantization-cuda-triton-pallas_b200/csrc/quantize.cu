@@ -673,7 +673,7 @@ __device__ __forceinline__ void store_value4(const OutPaged& op, size_t vi, cons
 // WARPS: 8 for groups of up to 64 tokens, else 16, so that a thread never holds more
 // than 8 rows' keys: with 16 rows and their values a thread, one CTA of 8 warps
 // filled an SM's registers (8 x 1000 rows of 32 heads x 128 float32 in groups of 128:
-// 140 us, now 105 us = 3.9 TB/s; 64 x 8 rows of 8 heads bfloat16: 28 us).
+// 140 us, now 105 us = 3.9 TB/s).
 template <int KIND, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 2)
 extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
@@ -747,6 +747,15 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
         store_value4(op, (((size_t)page * op.heads + h) * op.page + t) * op.head_dim + d, vals[i]);
     }
     return;
+  }
+  if (ea.v && (int)gridDim.x == slabs) {  // few new rows: copied here, while the keys arrive
+#pragma unroll 1
+    for (int pos = max(start, gpos) + warp; pos < gpos + rows; pos += WARPS) {
+      const int page = row_bt[pos / op.page], src = source(pos);
+      if (lane_ok && page >= 0 && page < op.num_pages)
+        store_value4(op, (((size_t)page * op.heads + h) * op.page + pos % op.page) * op.head_dim + d,
+                     src < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : load4_as_f32<KIND>(ea.v, (size_t)src * C + c0));
+    }
   }
   int gslot = row_bt[gpos / op.page];  // (0 <= gpos < end: in the table)
   if (gslot < 0 || gslot >= op.num_pages) gslot = -1;
@@ -1354,7 +1363,11 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
   const long long groups = ((long long)max_rows_per_seq + 2 * group_tokens - 2) / group_tokens;
   if (groups > 65535) return cudaErrorInvalidValue;
   const int slabs = (int)((C + kSlab - 1) / kSlab);
-  dim3 grid((unsigned)(v ? 2 * slabs : slabs), (unsigned)groups, batch);
+  const int warps = group_tokens <= 64 ? 8 : 16;
+  // values by CTAs of their own, but for few new rows a sequence, where those CTAs would
+  // mostly look metadata up (64 x 8 rows and the read after them: 45 us with, 39 without)
+  const bool apart = v && max_rows_per_seq > 2 * warps;
+  dim3 grid((unsigned)(apart ? 2 * slabs : slabs), (unsigned)groups, batch);
   ExtendArgs ea{k, v, tok_offsets, start_pos, rows, num_src, rows ? num_rows : num_src,
                 stage_slots, k_stage, num_slots, max_rows_per_seq};
   OutPaged op{nullptr, nullptr, nullptr, block_table, max_pages, page_tokens, num_pages,
@@ -1365,7 +1378,6 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
            : kv_dtype == INT4KV_VALUES_F16 ? extend_quant_kernel<INT4KV_VALUES_F16, kWarps>
                                            : extend_quant_kernel<INT4KV_VALUES_BF16, kWarps>;
   };
-  const int warps = group_tokens <= 64 ? 8 : 16;
   auto kern = warps == 8 ? pick(std::integral_constant<int, 8>()) : pick(std::integral_constant<int, 16>());
   kern<<<grid, warps * 32, 0, stream>>>(ea, (int)C, group_tokens, slabs, op);
   return cudaGetLastError();

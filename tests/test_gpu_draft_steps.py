@@ -492,10 +492,11 @@ def test_same_row_taken_twice(dtype):
         assert all(torch.equal(x, y) for x, y in zip(a.read(s), b.read(s)))
 
 
-def test_extend_reports_malformed_metadata():
+@pytest.mark.parametrize("bound", [3, 300])  # values written with the keys, and by blocks of their own
+def test_extend_reports_malformed_metadata(bound):
     heads, d, group = 2, 64, 32
     k = torch.randn((6, heads, d), device="cuda")
-    base = dict(offs=[0, 3, 6], start=[0, 0], slots=[0, 1], rows=None, table=[[0, 1], [2, 3]], max_rows=3)
+    base = dict(offs=[0, 3, 6], start=[0, 0], slots=[0, 1], rows=None, table=[[0, 1], [2, 3]], max_rows=bound)
 
     def go(**kw):
         a = {**base, **kw}
