@@ -197,8 +197,8 @@ class PagedKVCache:
                values: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None) -> None:
         """Append ``counts[i]`` tokens to each sequence, quantized as they are written.
 
-        ``keys`` / ``values`` [n, heads, head_dim] (float32, float16 or bfloat16)
-        hold the sequences' new tokens one after another; with ``rows`` (int32
+        ``keys`` / ``values`` [n, heads, head_dim] (float32, float16 or bfloat16, not
+        necessarily the same) hold the sequences' new tokens one after another; with ``rows`` (int32
         [sum of counts]) the new tokens are those rows of ``keys`` in that order:
         the accepted paths out of all drafted rows. Sequences may be new. The
         cache equals a bulk write of the same tokens bit for bit.
@@ -231,7 +231,9 @@ class PagedKVCache:
         k = keys.to(self.device).contiguous()
         v = None
         if values is not None and self.v_pool is not None:
-            v = values.to(self.device, k.dtype).contiguous()
+            v = values.to(self.device).contiguous()
+            if v.dtype != k.dtype:  # float32 holds either: neither is rounded to the other's type
+                k, v = k.float(), v.float()
         offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n_new)]).astype(np.int32))
         _C.cache_extend(k, v, offs.to(self.device),
                         torch.tensor(start, dtype=torch.int32, device=self.device),
