@@ -271,6 +271,19 @@ I4KV_DEVINL uint32_t pack16(float x, float y) {
   }
 }
 
+// ... and back.
+template <int VK>
+I4KV_DEVINL void widen2(uint32_t w, float& x, float& y) {
+  if constexpr (VK == INT4KV_VALUES_F16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x = f.x;
+    y = f.y;
+  } else {
+    x = __uint_as_float(w << 16);
+    y = __uint_as_float(w & 0xFFFF0000u);
+  }
+}
+
 // (d0, d1) = (a0 b0 + c0, a1 b1 + c1), each rounded once.
 I4KV_DEVINL void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
@@ -284,16 +297,7 @@ template <int VK>
 I4KV_DEVINL void widen8(const uint4& u, float (&x)[8]) {
   const uint32_t wd[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if constexpr (VK == INT4KV_VALUES_F16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&wd[j]));
-      x[2 * j] = f.x;
-      x[2 * j + 1] = f.y;
-    } else {
-      x[2 * j] = __uint_as_float(wd[j] << 16);
-      x[2 * j + 1] = __uint_as_float(wd[j] & 0xFFFF0000u);
-    }
-  }
+  for (int j = 0; j < 4; ++j) widen2<VK>(wd[j], x[2 * j], x[2 * j + 1]);
 }
 template <int VK>
 I4KV_DEVINL void load8(const void* base, size_t i, float (&x)[8]) {
@@ -1414,8 +1418,11 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), kLog2e, kLog2e, nref[j0 + j][0], nref[j0 + j][1]);
             y0 = exp2_fast(y0);
             y1 = exp2_fast(y1);
+            const uint32_t w2 = pack16<VK>(y0, y1);
+            *reinterpret_cast<uint32_t*>(at + q * 8 * 128) = w2;
+            // (the sums take what the product takes: a row's weights sum to one)
+            widen2<VK>(w2, y0, y1);
             add2_rn(l[j0 + j][0], l[j0 + j][1], l[j0 + j][0], l[j0 + j][1], y0, y1);
-            *reinterpret_cast<uint32_t*>(at + q * 8 * 128) = pack16<VK>(y0, y1);
           }
         }
       }

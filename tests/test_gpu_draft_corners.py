@@ -1,10 +1,9 @@
-"""The draft operators in corners of what they allow: keys and values of different types."""
+"""The draft operators in corners of what they allow: mixed types, weights that sum to one."""
 
-
-import numpy as np
 import pytest
 
 from helpers import pkg
+from test_gpu_draft_steps import Step
 from test_gpu_drafts import BF16, F16, F32, logical
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +36,18 @@ def test_extend_of_mixed_types_equals_bulk_write(kd, vd, values):
     for s in ids:
         for x, y in zip(logical(caches[1], s), logical(caches[0], s)):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,hkv,d,drafts", [(8, 4, 128, 8), (8, 2, 128, 8), (16, 2, 64, 8), (32, 2, 128, 8), (8, 4, 256, 13)])
+def test_weights_sum_to_one(hq, hkv, d, drafts, dtype):
+    """Where every value is 1 every output is: the sum takes the weights as the product does,
+    rounded. (Exact: float32 sums are off by 2^-24 times the count of tokens at most, below
+    2^-12 here, and 1 is the nearest 16-bit value to all that is closer than that.)"""
+    s = Step([1000, 130, 0, 2000], [drafts] * 4, hq, hkv, d, 128, dtype, dtype, seed=d)
+    s.v.fill_(1)
+    s.pools[1].fill_(1)
+    s.q *= 12  # few tokens carry most of the weight
+    assert (s.run() == 1).all()
+    out = C.paged_window_decode(s.q[:4].contiguous(), *s.pools[:5], window=300, sinks=5, group_tokens=128)
+    assert (out[[0, 1, 3]] == 1).all()
