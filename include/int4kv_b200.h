@@ -494,8 +494,8 @@ cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, in
  * num_kv_heads, head_dim], all of type qkv_dtype: float32 with any value pool,
  * or float16 / bfloat16 with a value pool of the same type (keys and softmax
  * weights are then rounded to 16 bits for the tensor cores, sums stay
- * float32). head_dim 64, 128 or 256, pages of 16 tokens, tensors 16-byte
- * aligned, `out` apart from the inputs. What stands behind a sequence's length,
+ * float32; bfloat16 logits must stay within +- 2^29). head_dim 64, 128 or 256,
+ * pages of 16 tokens, tensors 16-byte aligned, `out` apart from the inputs. What stands behind a sequence's length,
  * outside every window or in drafts nobody sees is never part of a result, even
  * NaN; a 16-bit cached value that some row of a sequence sees must be finite for
  * the results of its other rows to be. Pages outside the pool are not read: their

@@ -271,7 +271,18 @@ I4KV_DEVINL uint32_t pack16(float x, float y) {
   }
 }
 
-// ... and back.
+// Two weights; float16 past its range as its largest value (bfloat16 has float32's).
+template <int VK>
+I4KV_DEVINL uint32_t pack_weights(float x, float y) {
+  if constexpr (VK == INT4KV_VALUES_F16) {
+    uint32_t w;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+    return w;
+  } else {
+    return pack16<VK>(x, y);
+  }
+}
+// Two 16-bit values as float32.
 template <int VK>
 I4KV_DEVINL void widen2(uint32_t w, float& x, float& y) {
   if constexpr (VK == INT4KV_VALUES_F16) {
@@ -702,9 +713,16 @@ struct RowState {
   float nref[NI][2], l[NI][2];
   bool failed;
 };
-constexpr float kNoRef = -1e30f;  // the reference of a row that has seen nothing
+// The reference of a row that has seen nothing: below every logit but those the factor
+// log2 e takes to (minus) infinity.
+constexpr float kNoRef = -3e38f;
 
-// Raise the references to the true maxima of the tile, rescale sums and outputs.
+// Raise the references to the true maxima of the tile, rescale sums and outputs. A
+// weight is 2^(x log2 e - ref), the product unrounded, so the references are rounded
+// down: a row's largest weight is then 1 or more whatever the logits' size (rounded to
+// nearest it came below float16's smallest for logits past 2^27). What it is above 1,
+// less than 2^(2^-23 |ref|), float16 cuts at its largest value; logits that large are
+// too far apart for a second one to come near.
 // `prev`: the buffer of the last tile's weights (-1: O^T holds nothing yet).
 template <int D, int NR>
 __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const MultiQueryArgs& a, RowState<Tc<D, NR>::NC / 8> s,
@@ -748,7 +766,7 @@ __device__ __noinline__ RowState<Tc<D, NR>::NC / 8> raise_references(const Multi
     }
   }
   *reinterpret_cast<float2*>(&sh.part[quarter][c0 + 8 * at + 2 * t4]) =
-      make_float2(fmaxf(m[0] * kLog2e, kNoRef), fmaxf(m[1] * kLog2e, kNoRef));
+      make_float2(fmaxf(__fmul_rd(m[0], kLog2e), kNoRef), fmaxf(__fmul_rd(m[1], kLog2e), kNoRef));
   s.failed = prev >= 0 && !tc_wait(&sh.p_empty[prev & 1], parity, a.status);  // the weights of tile i - 1 have been multiplied
   named_bar_sync(bar, 128);
   tc_fence_after();
@@ -1418,7 +1436,7 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
             fma2(y0, y1, __uint_as_float(xx[0]), __uint_as_float(xx[1]), kLog2e, kLog2e, nref[j0 + j][0], nref[j0 + j][1]);
             y0 = exp2_fast(y0);
             y1 = exp2_fast(y1);
-            const uint32_t w2 = pack16<VK>(y0, y1);
+            const uint32_t w2 = pack_weights<VK>(y0, y1);
             *reinterpret_cast<uint32_t*>(at + q * 8 * 128) = w2;
             // (the sums take what the product takes: a row's weights sum to one)
             widen2<VK>(w2, y0, y1);

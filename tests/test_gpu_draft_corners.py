@@ -1,4 +1,5 @@
-"""The draft operators in corners of what they allow: mixed types, weights that sum to one."""
+"""The draft operators in corners of what they allow: mixed types, weights that sum to one,
+logits of any size."""
 
 import pytest
 
@@ -51,3 +52,38 @@ def test_weights_sum_to_one(hq, hkv, d, drafts, dtype):
     assert (s.run() == 1).all()
     out = C.paged_window_decode(s.q[:4].contiguous(), *s.pools[:5], window=300, sinks=5, group_tokens=128)
     assert (out[[0, 1, 3]] == 1).all()
+
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 1e3), (BF16, 30.0), (F16, 1e4), (F16, 200.0), (F32, 1e16)])
+def test_logits_of_any_size(dtype, size):
+    """Logits from 10^5 to 10^34 (bfloat16: up to 2^29), above and below zero: a row's only token has
+    weight 1, the lower of two none, and two equal ones a half each."""
+    s = Step([0, 0, 0, 0, 40], [1, 3, 2, 300 // 6, 2], 8, 2, 128, 64, dtype, dtype)
+    words = s.words.copy()
+    words[:6] = [1, 1, 2, 4, 3, 3]
+    s.q.fill_(size)
+    s.q[:, 1::2].neg_()
+    s.k.fill_(-size)
+    s.k[5] = -2 * size
+    s.k[6:] = -2 * size
+    s.k[20] = -size
+    s.k[31] = -size
+    words[6:56] = (1 << 50) - 1
+    out = s.run(words=words)
+    v = s.v.double().repeat_interleave(4, dim=1)
+    for row in range(4):
+        assert torch.equal(out[row], v[row].to(dtype))
+    low = torch.tensor([False, True] * 4, device="cuda")[:, None]  # heads of negative queries: positive logits
+    # q > 0: the higher logit is that of draft 4, of the key nearer to zero; q < 0: draft 5's
+    for row in (4, 5):
+        assert torch.equal(out[row], torch.where(low, v[5], v[4]).to(dtype))
+    half = ((v[20] + v[31]) / 2).expand(50, 8, 128)
+    tol = torch.finfo(dtype).eps / 2 * half.abs() + 2.0 ** -22 * (v[20].abs() + v[31].abs())
+    assert ((out[6:56].double() - half).abs() <= tol)[:, 0::2].all()
+    # a cache of keys from -20 to -5 times 2^e, one of them seen
+    k_pool, v_pool, sz, bt, sl, _ = s.pools
+    scale = {1e16: 2.0 ** 60, 1e3: 2.0 ** 6, 30.0: 2.0 ** 4, 1e4: 2.0 ** 60, 200.0: 2.0 ** 5}[size]
+    sz[:, :, 0], sz[:, :, 1] = scale, 20
+    q = torch.full((5, 8, 128), size, device="cuda").to(dtype)
+    out = C.paged_window_decode(q, *s.pools[:5], window=1, group_tokens=64)
+    assert torch.equal(out[4].view(2, 4, 128), v_pool[bt[4, 39 // 16], :, 39 % 16][:, None].expand(2, 4, 128))
