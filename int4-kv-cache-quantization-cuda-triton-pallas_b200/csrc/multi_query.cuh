@@ -25,6 +25,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "run_tail.h"
 #include "../../include/int4kv_b200.h"
 
 namespace i4kv {
@@ -45,20 +46,12 @@ struct MultiQueryArgs {
   const int32_t* block_table;
   const int32_t* seq_lens;
   void* out;                   // [rows, Hq, D] of kind qk
-  struct RunTail* tails;       // one per CTA
+  RunTail* tails;              // one per CTA
   float* recs;                 // two records per CTA
   uint32_t* status;
   int qk, batch, kv_heads, group_q, total_rows, max_drafts;
   int max_pages, num_pages, group_pages;
   int window, sinks;           // window 0: the whole cache
-};
-
-// The stream at the end of a run that began in it and goes on in later runs, up to
-// run `last` (rows 0: there is none): what the merge has to know.
-struct RunTail {
-  int rows, row0, head, first_row;  // rows of the sequence, its first row; the chunk's
-  int slot, last;                   // this run's record of it; the last run that shares it
-  int pad[2];
 };
 
 // What one sequence asks for.
@@ -361,9 +354,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_records_kernel(MultiQu
   const int c = blockIdx.x, lane = threadIdx.x & 31;
   const int4 n0 = __ldcg(reinterpret_cast<const int4*>(a.tails + c));
   const int2 n1 = __ldcg(reinterpret_cast<const int2*>(a.tails + c) + 2);
-  const int rows = n0.x, row0 = n0.y, head = n0.z, r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);
-  const int rr = n0.w + r, slot = n1.x, last = n1.y;
-  if (rr >= rows) return;
+  const RunTail n = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, {}};
+  // (one block less than runs)
+  if (!tail_in_range(n, c, gridDim.x + 1, a.total_rows, a.kv_heads, a.group_q)) return;
+  const int row0 = n.row0, head = n.head, slot = n.slot, last = n.last;
+  const int r = blockIdx.y * kMergeWarps + (threadIdx.x >> 5), rr = n.first_row + r;
+  if (rr >= n.rows) return;
   constexpr int kRec = Record<NR, D>::kFloats;
   auto record = [&](int i) { return a.recs + (size_t)(i == c ? slot : 2 * i) * kRec; };
   float M = -INFINITY;

@@ -117,10 +117,8 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   }
   __syncthreads();
   const RunPlan plan = s_plan;
-  if (plan.tiles == 0) {
-    if (tid == 0) a.tails[cta] = RunTail{};
-    return;
-  }
+  if (tid == 0) a.tails[cta] = RunTail{};  // (overwritten by the same thread where the run shares its last stream)
+  if (plan.tiles == 0) return;
   const int u1 = plan.tiles;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!mbar_try_wait(bar, parity) && !s_failed && !mbar_wait_bounded(bar, parity, kWaitNs)) {

@@ -999,7 +999,9 @@ multi_query_tc_kernel(const __grid_constant__ MultiQueryArgs a, const __grid_con
     const RunPlan mine = plan_run<NR, kTilePages, kStreamUnits, kDraftUnits>(a, cta, gridDim.x);
     if (lane == 0) {
       sh.plan = mine;
-      if (mine.tiles == 0) a.tails[cta] = RunTail{};
+      // (the same thread writes the note of the run's last tile, which a wait that runs out
+      // keeps it from: until then, and then for good, this run shares no stream)
+      a.tails[cta] = RunTail{};
     }
   }
   __syncthreads();
