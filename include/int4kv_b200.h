@@ -426,6 +426,7 @@ cudaError_t int4kv_stage_inputs(void* dst, const void* src, size_t bytes, cudaSt
 /* ---------------------------------------------------------------------------
  * Serving with drafted tokens and sliding windows. No counterpart in the
  * reference, whose decode takes one query per sequence over its whole cache.
+ * Tables of at most 2^31 - 1025 tokens (max_pages * page_tokens).
  * ------------------------------------------------------------------------- */
 
 /* Most drafted tokens of one sequence (one bit of a mask word each). */

@@ -110,9 +110,10 @@ __global__ void __launch_bounds__(kReadWarps * 32) cache_read_kernel(ReadArgs a)
     if (a.status && lane == 0) atomicOr(a.status, kStatusBadLength);
     return;
   }
-  const int pg = start / a.page + (int)blockIdx.y;
-  const int t0 = max(start, pg * a.page), t1 = min(start + n, (pg + 1) * a.page);
-  if (t0 >= t1) return;
+  const int behind = (int)blockIdx.y * a.page;  // from the first page's first token
+  if (behind >= start % a.page + n) return;     // (a sum of both could pass 2^31)
+  const int pg = start / a.page + (int)blockIdx.y, p0 = pg * a.page;
+  const int t0 = max(start, p0), t1 = start + n - p0 < a.page ? start + n : p0 + a.page;
   const int32_t* row = a.block_table + (size_t)b * a.max_pages;
   const int phys = row[pg], home = row[pg * a.page / a.group_tokens * (a.group_tokens / a.page)];
   const bool ok = phys >= 0 && phys < a.num_pages && home >= 0 && home < a.num_pages;
@@ -196,7 +197,8 @@ extern "C" cudaError_t int4kv_cache_read(const uint8_t* k_pool, const void* v_po
       head_dim <= 0 || head_dim % 4 != 0 || max_pages <= 0 || num_pages <= 0)
     return cudaErrorInvalidValue;
   if (page_tokens <= 0 || group_tokens <= 0 || group_tokens % page_tokens != 0) return cudaErrorInvalidValue;
-  if ((long long)max_pages * page_tokens > 0x7fffffffll) return cudaErrorInvalidValue;
+  // (the kernel's loops step past the last token by less than 1024)
+  if ((long long)max_pages * page_tokens > 0x7fffffffll - 1024) return cudaErrorInvalidValue;
   for (int kind : {value_dtype, out_dtype})
     if (kind != INT4KV_VALUES_F32 && kind != INT4KV_VALUES_F16 && kind != INT4KV_VALUES_BF16)
       return cudaErrorInvalidValue;

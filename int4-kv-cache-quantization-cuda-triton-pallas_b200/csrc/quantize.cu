@@ -700,8 +700,9 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
     return;
   }
   const int end = start + n;
-  const int gpos = (start / R + (int)blockIdx.y) * R;  // the group's first token
-  if (gpos >= end) return;
+  const int behind = (int)blockIdx.y * R;  // from the first touched group's first token
+  if (behind >= end - (start - start % R)) return;  // (a sum of both could pass 2^31)
+  const int gpos = start - start % R + behind;      // the group's first token
   const int rows = min(R, end - gpos);
   const bool lane_ok = c0 < C;
   float* stage = ea.stage + (size_t)sl * R * C;
@@ -1349,7 +1350,8 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
   for (int kind : {kv_dtype, value_dtype})
     if (kind != INT4KV_VALUES_F32 && kind != INT4KV_VALUES_F16 && kind != INT4KV_VALUES_BF16)
       return cudaErrorInvalidValue;
-  if (max_pages <= 0 || num_pages <= 0 || (long long)max_pages * page_tokens > 0x7fffffffll)
+  // (the kernel's loops step past the last token by less than 1024)
+  if (max_pages <= 0 || num_pages <= 0 || (long long)max_pages * page_tokens > 0x7fffffffll - 1024)
     return cudaErrorInvalidValue;
   if (!tok_offsets || !start_pos || !stage_slots || !k_stage || !block_table || !k_pool || !sz_pool)
     return cudaErrorInvalidValue;

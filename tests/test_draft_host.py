@@ -1,9 +1,10 @@
 """Host side of the draft operators without a GPU: what ``PagedKVCache`` hands to
-the binding (replaced by a recorder), on CPU tensors."""
+the binding (replaced by a recorder), on CPU tensors, and limits of the C entry points."""
 
 import pytest
 
 from helpers import pkg
+from test_draft_refusals import INVALID, OK, aligned, extend, lib, read  # noqa: F401 (lib: a fixture)
 
 torch = pytest.importorskip("torch")
 C = pkg("_C")
@@ -55,3 +56,13 @@ def test_extend_passes_equal_types_on(calls, dtype):
     cache().extend([4], [3], k, v)
     (_, args, _), = calls
     assert args[0].dtype == args[1].dtype == dtype
+
+
+def test_tables_end_before_positions_do(lib):  # noqa: F811
+    """The longest table leaves the kernels' positions room below 2^31."""
+    keep, p = aligned()
+    longest = (2 ** 31 - 1025) // 16
+    for call in (extend, read):
+        assert call(lib, p, max_pages=longest + 1) == INVALID
+        assert call(lib, p, max_pages=2 ** 31 - 1024, page=1, group=64) == INVALID
+        assert call(lib, p, max_pages=longest, max_rows=0) == OK

@@ -1,5 +1,5 @@
 """The draft operators in corners of what they allow: mixed types, weights that sum to one,
-logits of any size."""
+logits of any size, the end of the longest tables."""
 
 import pytest
 
@@ -87,3 +87,29 @@ def test_logits_of_any_size(dtype, size):
     q = torch.full((5, 8, 128), size, device="cuda").to(dtype)
     out = C.paged_window_decode(q, *s.pools[:5], window=1, group_tokens=64)
     assert torch.equal(out[4].view(2, 4, 128), v_pool[bt[4, 39 // 16], :, 39 % 16][:, None].expand(2, 4, 128))
+
+
+@pytest.mark.parametrize("bound", [40, 4000])  # the rows there are, and a bound that reaches past 2^31
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_end_of_the_longest_table(dtype, bound):
+    """The last 40 tokens of the longest table there may be: as the same tokens of a short one."""
+    heads, d, group, n = 2, 64, 128, 40
+    pages = (2 ** 31 - 1025) // 16
+    first = pages * 16 // group * group  # the last group, of 112 tokens
+    start = pages * 16 - n
+    k, v = (torch.randn((n, heads, d), device="cuda").to(dtype) for _ in range(2))
+    stage = torch.randn((1, group, heads * d), device="cuda")
+    longest = torch.full((1, pages), -1, dtype=torch.int32, device="cuda")
+    short = i32([[3, 1, 0, 5, 2, 6, 4]])
+    longest[:, first // 16:] = short
+    got = []
+    for table, at in ((longest, start), (short, start - first)):
+        pools = [torch.zeros((8, heads, 16, d // 2), dtype=torch.uint8, device="cuda"),
+                 torch.zeros((8, heads, 16, d), dtype=dtype, device="cuda"), torch.zeros((8, heads, 2, d), device="cuda")]
+        staged, status = stage.clone(), i32([0])
+        C.cache_extend(k, v, i32([0, n]), i32([at]), i32([0]), staged, table, *pools, bound, group, status=status)
+        out = C.cache_read(*pools, table, i32([at]), i32([0, n]), n, bound, group, dtype=dtype, status=status)
+        assert status.item() == 0
+        got.append((*pools, staged, *out))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert torch.equal(got[0][5], v)
