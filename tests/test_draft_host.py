@@ -1,6 +1,9 @@
 """Host side of the draft operators without a GPU: what ``PagedKVCache`` hands to
 the binding (replaced by a recorder), on CPU tensors, and limits of the C entry points."""
 
+import contextlib
+import ctypes
+
 import pytest
 
 from helpers import pkg
@@ -8,6 +11,7 @@ from test_draft_refusals import INVALID, OK, aligned, extend, lib, read  # noqa:
 
 torch = pytest.importorskip("torch")
 C = pkg("_C")
+L = pkg("_lib")
 P = pkg("paged")
 
 F32, F16, BF16, F64 = torch.float32, torch.float16, torch.bfloat16, torch.float64
@@ -66,3 +70,44 @@ def test_tables_end_before_positions_do(lib):  # noqa: F811
         assert call(lib, p, max_pages=longest + 1) == INVALID
         assert call(lib, p, max_pages=2 ** 31 - 1024, page=1, group=64) == INVALID
         assert call(lib, p, max_pages=longest, max_rows=0) == OK
+
+
+@pytest.fixture
+def bound(monkeypatch):
+    """(window, sinks) as the C entry points receive them from the binding, with CPU tensors let through."""
+    got = []
+
+    class Lib:
+        def int4kv_paged_tree_decode(self, *a):
+            got.append((ctypes.c_int(a[22]).value, ctypes.c_int(a[23]).value))
+            return 0
+
+        def int4kv_paged_window_decode(self, *a):
+            got.append((ctypes.c_int(a[16]).value, ctypes.c_int(a[17]).value))
+            return 0
+
+    monkeypatch.setattr(L, "load", lambda: Lib())
+    monkeypatch.setattr(C, "_check_input", lambda t, name: None)
+    monkeypatch.setattr(C, "_check_pools", lambda k, v, sz: (k.shape[0], k.shape[1], 16, k.shape[3] * 2))
+    monkeypatch.setattr(C, "_check_table", lambda bt, b: bt.shape[1])
+    monkeypatch.setattr(C, "_guard", lambda i: contextlib.nullcontext())
+    monkeypatch.setattr(C, "_attention_need", lambda *a: 16)
+    monkeypatch.setattr(C, "_stream", lambda t: 0)
+    return got
+
+
+MOST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("window,sinks,want", [
+    (5, 3, (5, 3)), (MOST, MOST, (MOST, MOST)), (2 ** 31, 0, (MOST, 0)), (2 ** 32 + 7, 2 ** 32 + 1, (MOST, MOST)),
+    (10 ** 12, 2 ** 40, (MOST, MOST)), (2 ** 63 - 1, 2 ** 63 - 1, (MOST, MOST))])
+def test_window_and_sinks_past_32_bits_reach_over_everything(bound, window, sinks, want):
+    q = torch.zeros((1, 2, 64))
+    k_pool = torch.zeros((2, 2, 16, 32), dtype=torch.uint8)
+    v_pool, sz = torch.zeros((2, 2, 16, 64)), torch.zeros((2, 2, 2, 64))
+    bt, sl, offs = (torch.zeros(s, dtype=torch.int32) for s in ((1, 2), (1,), (2,)))
+    C.paged_window_decode(q, k_pool, v_pool, sz, bt, sl, window, sinks)
+    C.paged_tree_decode(q, q, q, torch.zeros(1, dtype=torch.int64), offs, k_pool, v_pool, sz, bt, sl, 1, window=window,
+                        sinks=sinks)
+    assert bound == [want, want]
