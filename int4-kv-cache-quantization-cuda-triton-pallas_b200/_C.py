@@ -623,6 +623,15 @@ def paged_decode_split(query, k_pool, v_pool, sz_pool, block_table, seq_lens, pe
 MAX_DRAFTS = 64
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _bound(n):
+    """An upper bound (a window, a count of sinks or rows) as a C int; ctypes would wrap it. No
+    position or row is past 2^31, so a larger bound bounds nothing more."""
+    return min(int(n), _INT_MAX)
+
+
 def _check_int32(t, name, n=None):
     _check_input(t, name)
     if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
@@ -687,7 +696,7 @@ def cache_extend(k, v, tok_offsets, start_pos, stage_slots, k_stage, block_table
         _lib.check(lib.int4kv_cache_extend(
             _p(k), _p(v), VALUE_KINDS[k.dtype], k.shape[0], _p(tok_offsets), _p(start_pos),
             _p(rows), rows.shape[0] if rows is not None else k.shape[0],
-            _p(stage_slots), _p(k_stage), k_stage.shape[0], b, int(max_rows_per_seq), hkv, d,
+            _p(stage_slots), _p(k_stage), k_stage.shape[0], b, _bound(max_rows_per_seq), hkv, d,
             group_tokens, page, _p(block_table), max_pages, num_pages, _p(k_pool), _p(v_pool), vk,
             _p(sz_pool), _p(status), _stream(k)), "cache_extend")
 
@@ -734,7 +743,7 @@ def cache_read(k_pool, v_pool, sz_pool, block_table, start_pos, tok_offsets, num
         _lib.check(lib.int4kv_cache_read(
             _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype] if v_pool is not None else 0,
             _p(sz_pool), _p(block_table), _p(start_pos), _p(tok_offsets), b, shape[0],
-            int(max_rows_per_seq), hkv, d, group_tokens, page, max_pages, num_pages,
+            _bound(max_rows_per_seq), hkv, d, group_tokens, page, max_pages, num_pages,
             VALUE_KINDS[dtype], _p(k_out), _p(v_out), _p(status), _stream(k_pool)), "cache_read")
     return k_out, v_out
 
@@ -839,7 +848,7 @@ def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool,
             _p(query), _p(k_draft), _p(v_draft), VALUE_KINDS[query.dtype], _p(tree_mask),
             _p(draft_offsets), rows, int(max_drafts), _p(k_pool), _p(v_pool),
             VALUE_KINDS[v_pool.dtype], _p(sz_pool), _p(block_table), _p(seq_lens), b, hq, hkv, d,
-            page, group_tokens, max_pages, num_pages, int(window or 0), int(sinks), _p(out),
+            page, group_tokens, max_pages, num_pages, _bound(window or 0), _bound(sinks), _p(out),
             _p(workspace), workspace.numel() * workspace.element_size(), _p(status),
             _stream(query)), "paged_tree_decode")
     return out
@@ -868,7 +877,7 @@ def paged_window_decode(query, k_pool, v_pool, sz_pool, block_table, seq_lens, w
         _lib.check(lib.int4kv_paged_window_decode(
             _p(query), VALUE_KINDS[query.dtype], _p(k_pool), _p(v_pool), VALUE_KINDS[v_pool.dtype],
             _p(sz_pool), _p(block_table), _p(seq_lens), b, hq, hkv, d, page, group_tokens,
-            max_pages, num_pages, int(window), int(sinks), _p(out), _p(workspace),
+            max_pages, num_pages, _bound(window), _bound(sinks), _p(out), _p(workspace),
             workspace.numel() * workspace.element_size(), _p(status), _stream(query)),
             "paged_window_decode")
     return out
