@@ -643,10 +643,10 @@ def _check_status(status):
         raise RuntimeError("status must be an int32 CUDA tensor")
 
 
-def _check_groups(group_tokens, most=None):
-    if group_tokens <= 0 or group_tokens % PAGE_TOKENS or (most and group_tokens > most):
-        raise RuntimeError(f"group_tokens must be a positive multiple of {PAGE_TOKENS}"
-                           + (f" up to {most}" if most else "") + f", got {group_tokens}")
+def _check_groups(group_tokens, most=_INT_MAX):
+    if group_tokens <= 0 or group_tokens % PAGE_TOKENS or group_tokens > most:
+        raise RuntimeError(f"group_tokens must be a positive multiple of {PAGE_TOKENS} up to {most}, "
+                           f"got {group_tokens}")
 
 
 def cache_extend(k, v, tok_offsets, start_pos, stage_slots, k_stage, block_table, k_pool, v_pool,

@@ -111,3 +111,13 @@ def test_window_and_sinks_past_32_bits_reach_over_everything(bound, window, sink
     C.paged_tree_decode(q, q, q, torch.zeros(1, dtype=torch.int64), offs, k_pool, v_pool, sz, bt, sl, 1, window=window,
                         sinks=sinks)
     assert bound == [want, want]
+
+
+@pytest.mark.parametrize("group", [2 ** 31, 2 ** 32 + 16])
+def test_groups_past_32_bits_are_refused(bound, group):
+    q = torch.zeros((1, 2, 64))
+    pools = torch.zeros((2, 2, 16, 32), dtype=torch.uint8), torch.zeros((2, 2, 16, 64)), torch.zeros((2, 2, 2, 64))
+    bt, sl = torch.zeros((1, 2), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="group_tokens"):
+        C.paged_window_decode(q, *pools, bt, sl, 5, group_tokens=group)
+    assert not bound
