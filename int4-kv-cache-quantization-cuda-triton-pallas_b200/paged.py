@@ -201,7 +201,9 @@ class PagedKVCache:
         necessarily the same) hold the sequences' new tokens one after another; with ``rows`` (int32
         [sum of counts]) the new tokens are those rows of ``keys`` in that order:
         the accepted paths out of all drafted rows. Sequences may be new. The
-        cache equals a bulk write of the same tokens bit for bit.
+        cache equals a bulk write of the same tokens bit for bit. ``rows`` on the
+        host are checked; an entry of ``rows`` on the device that names no row of
+        ``keys`` writes a token of zeros.
         """
         ids, n_new = list(seq_ids), [int(n) for n in counts]
         if len(set(ids)) != len(ids):
@@ -213,14 +215,31 @@ class PagedKVCache:
             raise ValueError(f"keys must be [rows, {self.heads}, {self.head_dim}]")
         if values is not None and values.shape != keys.shape:
             raise ValueError("values must have the shape of keys")
+        if rows is not None and (rows.dim() != 1 or rows.dtype.is_floating_point or rows.dtype == torch.bool):
+            raise ValueError("rows must be integers [sum of counts]")
         if (rows.shape[0] if rows is not None else keys.shape[0]) < total:
             raise ValueError(f"{total} new tokens need as many rows")
         if total == 0:
             return
+        if keys.dtype not in _C.VALUE_KINDS:
+            raise ValueError(f"keys must be one of {list(_C.VALUE_KINDS)}, got {keys.dtype}")
+        if rows is not None and not rows.is_cuda:
+            if int(rows[:total].min()) < 0 or int(rows[:total].max()) >= keys.shape[0]:
+                raise ValueError(f"rows must lie in [0, {keys.shape[0]})")
         need = [-(-(self.lens.get(s, 0) + n) // PAGE_TOKENS) - len(self.pages.get(s, []))
                 for s, n in zip(ids, n_new)]
         if sum(max(0, n) for n in need) > len(self._free):
             raise MemoryError(f"paged KV cache out of pages: need {sum(need)}, {len(self._free)} free")
+        k = keys.to(self.device).contiguous()
+        v = None
+        if values is not None and self.v_pool is not None:
+            v = values.to(self.device).contiguous()
+            if v.dtype != k.dtype:  # float32 holds either: neither is rounded to the other's type
+                k, v = k.float(), v.float()
+        if rows is not None:
+            if rows.dtype != torch.int32:  # (what does not fit names no row either)
+                rows = rows.long().clamp(-1, keys.shape[0]).int()
+            rows = rows.to(self.device).contiguous()
         start = []
         for s, n in zip(ids, need):
             start.append(self.lens.setdefault(s, 0))
@@ -228,19 +247,12 @@ class PagedKVCache:
         # a sequence that takes no token has no open group to stage for: any slot names it
         slots = [self._slot_of(s) if n else 0 for s, n in zip(ids, n_new)]
         bt, _ = self.block_table(ids)
-        k = keys.to(self.device).contiguous()
-        v = None
-        if values is not None and self.v_pool is not None:
-            v = values.to(self.device).contiguous()
-            if v.dtype != k.dtype:  # float32 holds either: neither is rounded to the other's type
-                k, v = k.float(), v.float()
         offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n_new)]).astype(np.int32))
         _C.cache_extend(k, v, offs.to(self.device),
                         torch.tensor(start, dtype=torch.int32, device=self.device),
                         torch.tensor(slots, dtype=torch.int32, device=self.device), self.k_stage, bt,
                         self.k_pool, self.v_pool, self.sz_pool, max_rows_per_seq=max(n_new),
-                        group_tokens=self.group_tokens,
-                        rows=rows.to(self.device, torch.int32).contiguous() if rows is not None else None)
+                        group_tokens=self.group_tokens, rows=rows)
         for s, n in zip(ids, n_new):
             self.lens[s] += n
 

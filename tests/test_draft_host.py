@@ -121,3 +121,40 @@ def test_groups_past_32_bits_are_refused(bound, group):
     with pytest.raises(RuntimeError, match="group_tokens"):
         C.paged_window_decode(q, *pools, bt, sl, 5, group_tokens=group)
     assert not bound
+
+
+def state(c):
+    return (dict(c.lens), {s: list(p) for s, p in c.pages.items()}, list(c._free), dict(c._stage_slot),
+            list(c._stage_free))
+
+
+REFUSED = {
+    "keys of float64": dict(keys=rows(4, F64)), "both of float64": dict(keys=rows(4, F64), values=rows(4, F64)),
+    "integer keys": dict(keys=rows(4, F32).int()), "fewer values": dict(values=rows(4, F32)[:3]),
+    "row past the keys": dict(rows=torch.tensor([0, 1, 4])),
+    "negative row": dict(rows=torch.tensor([0, -1, 2], dtype=torch.int32)),
+    "fractional rows": dict(rows=torch.tensor([0.0, 1.0, 2.0])), "rows of two axes": dict(rows=torch.tensor([[0], [1], [2]])),
+    "too few rows": dict(rows=torch.tensor([0, 1])), "row past 32 bits": dict(rows=torch.tensor([0, 1, 2 ** 32 + 2])),
+    "twice the same": dict(ids=[7, 7]), "negative count": dict(counts=[1, -1]), "too many": dict(counts=[4, 4]),
+    "a count too few": dict(counts=[1]),
+}
+
+
+@pytest.mark.parametrize("what", REFUSED)
+def test_a_refused_extend_leaves_the_cache_as_it_was(calls, what):
+    c = cache()
+    c.extend([7], [20], rows(20, F32), rows(20, F32))
+    before = state(c)
+    a = dict(ids=[7, 9], counts=[1, 2], keys=rows(4, F32), values=rows(4, F32, 1), rows=None)
+    a.update(REFUSED[what])
+    with pytest.raises(ValueError):
+        c.extend(a["ids"], a["counts"], a["keys"], a["values"], rows=a["rows"])
+    assert state(c) == before and len(calls) == 1
+
+
+def test_rows_of_any_integer_type_name_the_new_tokens(calls):
+    for dtype in (torch.int32, torch.int64, torch.int16, torch.uint8):
+        # (entries past the counts' sum name no token: any value)
+        cache().extend([1, 2], [2, 1], rows(4, F32), rows(4, F32), rows=torch.tensor([3, 0, 3, 77], dtype=dtype))
+        passed = calls[-1][2]["rows"]
+        assert passed.dtype == torch.int32 and passed[:3].tolist() == [3, 0, 3]
