@@ -67,6 +67,8 @@ class PagedKVCache:
                                    dtype=value_dtype, device=self.device) if values else None)
         self.sz_pool = torch.zeros((num_pages, num_kv_heads, 2, head_dim), dtype=torch.float32,
                                    device=self.device)
+        # what the draft operators met (extend, tree_decode, window_decode, read): see check
+        self.status = torch.zeros((1,), dtype=torch.int32, device=self.device)
         order = (np.random.default_rng(seed).permutation(num_pages) if seed is not None
                  else np.arange(num_pages))
         self._free: List[int] = [int(p) for p in order[::-1]]
@@ -78,6 +80,17 @@ class PagedKVCache:
         self.k_stage: Optional[torch.Tensor] = None
         self._stage_slot: Dict[int, int] = {}
         self._stage_free: List[int] = list(range(max_open_sequences - 1, -1, -1))
+
+    def check(self) -> None:
+        """Raise if an ``extend``, ``tree_decode``, ``window_decode`` or ``read`` since the last check
+        met a page outside the pool, a bad length or row index, or a wait that ran out. Waits for
+        the current stream; the calls themselves do not."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            met = [text for bit, text in ((1, "a page outside the pool"), (2, "a bad length or row index"),
+                                          (4, "a wait that ran out")) if bits & bit]
+            raise RuntimeError("paged KV cache met " + ", ".join(met))
 
     # ---- page allocation ----
     def _alloc(self, n: int) -> List[int]:
@@ -203,7 +216,7 @@ class PagedKVCache:
         the accepted paths out of all drafted rows. Sequences may be new. The
         cache equals a bulk write of the same tokens bit for bit. ``rows`` on the
         host are checked; an entry of ``rows`` on the device that names no row of
-        ``keys`` writes a token of zeros.
+        ``keys`` writes a token of zeros, and ``check`` tells.
         """
         ids, n_new = list(seq_ids), [int(n) for n in counts]
         if len(set(ids)) != len(ids):
@@ -252,7 +265,7 @@ class PagedKVCache:
                         torch.tensor(start, dtype=torch.int32, device=self.device),
                         torch.tensor(slots, dtype=torch.int32, device=self.device), self.k_stage, bt,
                         self.k_pool, self.v_pool, self.sz_pool, max_rows_per_seq=max(n_new),
-                        group_tokens=self.group_tokens, rows=rows)
+                        group_tokens=self.group_tokens, rows=rows, status=self.status)
         for s, n in zip(ids, n_new):
             self.lens[s] += n
 
@@ -292,7 +305,7 @@ class PagedKVCache:
         bt, sl = self.block_table(list(seq_ids))
         return _C.paged_window_decode(query.to(self.device).contiguous(), self.k_pool, self.v_pool,
                                       self.sz_pool, bt, sl, window=window, sinks=sinks,
-                                      group_tokens=self.group_tokens)
+                                      group_tokens=self.group_tokens, status=self.status)
 
     def tree_decode(self, query: torch.Tensor, k_draft: torch.Tensor, v_draft: torch.Tensor,
                     seq_ids: Sequence[int], counts: Sequence[int], mask: torch.Tensor,
@@ -312,7 +325,7 @@ class PagedKVCache:
             query.to(self.device).contiguous(), k_draft.to(self.device).contiguous(),
             v_draft.to(self.device).contiguous(), mask.to(self.device), offs.to(self.device),
             self.k_pool, self.v_pool, self.sz_pool, bt, sl, max_drafts=max(n),
-            group_tokens=self.group_tokens, window=window, sinks=sinks)
+            group_tokens=self.group_tokens, window=window, sinks=sinks, status=self.status)
 
     def read(self, seq_id: int, start: int = 0, stop: Optional[int] = None,
              dtype=torch.float32):
@@ -326,7 +339,7 @@ class PagedKVCache:
         one = torch.tensor([start, 0, stop - start], dtype=torch.int32, device=self.device)
         return _C.cache_read(self.k_pool, self.v_pool, self.sz_pool, bt, one[:1], one[1:],
                              num_rows=stop - start, max_rows_per_seq=stop - start,
-                             group_tokens=self.group_tokens, dtype=dtype)
+                             group_tokens=self.group_tokens, dtype=dtype, status=self.status)
 
     def memory_stats(self) -> dict:
         used = sum(len(p) for p in self.pages.values())

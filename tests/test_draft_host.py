@@ -158,3 +158,20 @@ def test_rows_of_any_integer_type_name_the_new_tokens(calls):
         cache().extend([1, 2], [2, 1], rows(4, F32), rows(4, F32), rows=torch.tensor([3, 0, 3, 77], dtype=dtype))
         passed = calls[-1][2]["rows"]
         assert passed.dtype == torch.int32 and passed[:3].tolist() == [3, 0, 3]
+
+
+def test_draft_calls_share_the_cache_s_status_word(calls):
+    c = cache()
+    c.extend([1], [3], rows(3, F32), rows(3, F32))
+    q = torch.zeros((1, 2, 8))
+    c.window_decode(q, [1], 4)
+    c.tree_decode(q, q, q, [1], [1], torch.ones(1, dtype=torch.int64))
+    c.read(1)
+    assert [name for name, _, _ in calls] == ["cache_extend", "paged_window_decode", "paged_tree_decode", "cache_read"]
+    assert all(kw["status"] is c.status for _, _, kw in calls)
+    c.check()
+    for bits, words in ((1, "page"), (2, "length"), (4, "wait"), (3, "page")):
+        c.status.fill_(bits)
+        with pytest.raises(RuntimeError, match=words):
+            c.check()
+        c.check()  # told once

@@ -113,3 +113,27 @@ def test_the_end_of_the_longest_table(dtype, bound):
         got.append((*pools, staged, *out))
     assert all(torch.equal(x, y) for x, y in zip(*got))
     assert torch.equal(got[0][5], v)
+
+
+def test_the_cache_reports_what_its_calls_met():
+    """A row index on the device that names no row, a page outside the pool: found by ``check``."""
+    k = torch.randn((4, 2, 64), device="cuda")
+    cache = P.PagedKVCache(8, 2, 64, group_tokens=32, device="cuda")
+    cache.extend([1], [3], k, k, rows=i32([0, 3, 1]))
+    q = torch.randn((1, 4, 64), device="cuda")
+    cache.window_decode(q, [1], 2)
+    cache.read(1)
+    cache.check()
+    cache.extend([1], [2], k, k, rows=i32([4, 0]))
+    with pytest.raises(RuntimeError, match="length"):
+        cache.check()
+    cache.extend([1], [1], k, k, rows=torch.tensor([2 ** 32 + 1], device="cuda"))
+    with pytest.raises(RuntimeError, match="length"):
+        cache.check()
+    cache.check()
+    cache.pages[1][0] = 8
+    for call in (lambda: cache.window_decode(q, [1], 2), lambda: cache.read(1), lambda: cache.extend([1], [1], k, k),
+                 lambda: cache.tree_decode(q, k[:1], k[:1], [1], [1], P.tree_mask([[-1]]))):
+        call()
+        with pytest.raises(RuntimeError, match="page"):
+            cache.check()
