@@ -817,8 +817,8 @@ def paged_tree_decode(query, k_draft, v_draft, tree_mask, draft_offsets, k_pool,
     ``tree_mask[row]`` (int64; ``paged.tree_mask``) lets a draft see draft u of its sequence. With
     ``window`` a query at position p sees positions above p - window and the first ``sinks`` only.
     float32 with any value pool, or float16 / bfloat16 with a value pool of the same type. Rows
-    past the last sequence's are left as ``out`` (not one of the inputs) held them. A ``workspace``
-    belongs to one call at a time; None allocates one.
+    past the last sequence's are left as ``out`` (not one of the inputs) held them (a new output:
+    unspecified). A ``workspace`` belongs to one call at a time; None allocates one.
     """
     lib = _lib.load()
     num_pages, hkv, page, d = _check_pools(k_pool, v_pool, sz_pool)

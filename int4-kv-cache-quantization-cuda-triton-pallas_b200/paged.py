@@ -314,18 +314,22 @@ class PagedKVCache:
 
         query [n, heads, head_dim], k_draft / v_draft [n, kv_heads, head_dim]
         (rotated, not in the cache), ``mask`` from ``tree_mask``. float32, or of
-        the value pool's 16-bit type. ``extend`` then writes the accepted path.
+        the value pool's 16-bit type. ``extend`` then writes the accepted path. Rows
+        past the counts' sum (a padded batch) come back as zeros.
         """
         ids, n = list(seq_ids), [int(c) for c in counts]
         if not ids or len(n) != len(ids) or any(c < 0 for c in n) or sum(n) > query.shape[0]:
             raise ValueError("counts must give the number of drafts of each sequence")
         bt, sl = self.block_table(ids)
         offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n)]).astype(np.int32))
-        return _C.paged_tree_decode(
+        out = _C.paged_tree_decode(
             query.to(self.device).contiguous(), k_draft.to(self.device).contiguous(),
             v_draft.to(self.device).contiguous(), mask.to(self.device), offs.to(self.device),
             self.k_pool, self.v_pool, self.sz_pool, bt, sl, max_drafts=max(n),
             group_tokens=self.group_tokens, window=window, sinks=sinks, status=self.status)
+        if sum(n) < out.shape[0]:
+            out[sum(n):] = 0
+        return out
 
     def read(self, seq_id: int, start: int = 0, stop: Optional[int] = None,
              dtype=torch.float32):

@@ -175,3 +175,11 @@ def test_draft_calls_share_the_cache_s_status_word(calls):
         with pytest.raises(RuntimeError, match=words):
             c.check()
         c.check()  # told once
+
+
+def test_tree_rows_that_no_sequence_has_are_zeros(calls):
+    c = cache()
+    c.extend([1, 2], [3, 1], rows(4, F32), rows(4, F32))
+    q = torch.ones((7, 2, 8))
+    out = c.tree_decode(q, q, q, [1, 2], [2, 3], torch.ones(7, dtype=torch.int64))
+    assert (out[:5] == 7).all() and (out[5:] == 0).all()

@@ -137,3 +137,19 @@ def test_the_cache_reports_what_its_calls_met():
         call()
         with pytest.raises(RuntimeError, match="page"):
             cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_padded_drafts_come_back_as_zeros(dtype):
+    """More query rows than the counts add up to (a batch of fixed size)."""
+    cache = P.PagedKVCache(16, 2, 64, group_tokens=32, device="cuda", value_dtype=dtype)
+    k = torch.randn((40, 2, 64), device="cuda").to(dtype)
+    cache.extend([1, 2], [20, 3], k, k)
+    q = torch.randn((12, 4, 64), device="cuda").to(dtype)
+    mask = torch.cat([P.tree_mask([[-1, 0, 1], [-1, -1]]), torch.zeros(7, dtype=torch.int64, device="cuda")])
+    want = cache.tree_decode(q[:5], k[:5], k[:5], [1, 2], [3, 2], mask[:5])
+    for _ in range(3):
+        torch.full_like(q, 9.0)  # (memory that the allocator may hand out next)
+        out = cache.tree_decode(q, k[:12], k[:12], [1, 2], [3, 2], mask)
+        assert torch.equal(out[:5], want) and (out[5:] == 0).all()
+    assert (cache.tree_decode(q, k[:12], k[:12], [1, 2], [0, 0], mask) == 0).all()
