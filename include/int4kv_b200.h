@@ -503,7 +503,9 @@ cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, in
  * tokens are not seen (INT4KV_STATUS_BAD_PAGE); nor are those of a group whose first
  * page, which keeps its scales, is outside (with a window, that page may lie before it). Offsets outside [0, num_rows] or
  * too many drafts skip the sequence's drafts, a bad length is clamped to the
- * table (INT4KV_STATUS_BAD_LENGTH). Results do not depend on the order of any
+ * table (INT4KV_STATUS_BAD_LENGTH). A batch of more than 2^31 - 1 tiles (of 128 cached
+ * tokens and up to 128 rows of a kv head, 64 and 16 in float32, counted from the table's
+ * width or the window) is refused. Results do not depend on the order of any
  * atomics: equal calls on equal devices give equal bits. */
 cudaError_t int4kv_paged_tree_decode(const void* query, const void* k_draft, const void* v_draft,
                                      int qkv_dtype, const int64_t* tree_mask,

@@ -7,6 +7,8 @@
 using namespace i4kv;
 
 namespace i4kv {
+double multi_query_f32_units(const MultiQueryArgs& a, int dim);
+double multi_query_tc_units(const MultiQueryArgs& a, int dim);
 size_t multi_query_f32_workspace(int dim, int sms);
 cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, void* ws, size_t ws_bytes,
                             cudaStream_t stream);
@@ -26,7 +28,7 @@ cudaError_t sm_count(int* sms) {
   return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
 }
 
-// The sizes shared by both entry points; work is counted in 32-bit tile counts.
+// The sizes shared by both entry points.
 bool sizes_ok(int batch, int hq, int hkv, int dim, int page, int group, int max_pages, int num_pages,
               int max_drafts) {
   if (batch <= 0 || batch > 65535 || hkv <= 0 || hq < hkv || hq % hkv != 0) return false;
@@ -40,9 +42,8 @@ cudaError_t run(const MultiQueryArgs& a, int dim, int vk, void* workspace, size_
   if (!aligned16(workspace) || !workspace) return cudaErrorInvalidValue;
   int sms = 0;
   if ((long long)a.total_rows * a.kv_heads * a.group_q > 0x7fffffffll) return cudaErrorInvalidValue;
-  // the kernels count tiles of at least 32 tokens and chunks of at least 4 rows in 31 bits
-  const double tiles = (a.max_pages / 2 + 12.0) * ((double)std::max(1, a.max_drafts) * a.group_q / 4 + 1);
-  if (tiles * a.batch * a.kv_heads > 2e9) return cudaErrorInvalidValue;
+  if ((a.qk != INT4KV_VALUES_F32 ? multi_query_tc_units(a, dim) : multi_query_f32_units(a, dim)) > kMqMostUnits)
+    return cudaErrorInvalidValue;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   if (a.qk != INT4KV_VALUES_F32) return multi_query_tc(a, dim, sms, workspace, bytes, stream);

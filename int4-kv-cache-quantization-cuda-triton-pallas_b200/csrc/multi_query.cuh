@@ -22,6 +22,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <mutex>
 
 #include "common.cuh"
@@ -331,6 +332,19 @@ I4KV_DEVINL float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+
+// Units of all streams together at most, in chunks of `nr` rows and tiles of `tp` pages;
+// the kernels count them in 31 bits. (From the table's width, or the window and the
+// sinks, for every sequence: what the host knows.)
+inline double mq_most_units(const MultiQueryArgs& a, long long rows, int nr, int tp, int extra) {
+  const auto blocks = [&](long long pages) { return (double)((pages + tp - 1) / tp); };
+  double tiles = blocks(a.max_pages);
+  if (a.window > 0)  // (their first and last pages, and blocks, may be parts)
+    tiles = std::min(tiles, blocks(a.window / kMqPage + 2) + 1 + blocks(a.sinks / kMqPage + 1));
+  tiles += blocks((a.max_drafts + kMqPage - 1) / kMqPage) + extra;
+  return tiles * (double)((rows + nr - 1) / nr) * a.batch * a.kv_heads;
+}
+constexpr double kMqMostUnits = 2147483647.;
 
 // Workspace of `runs` runs: their notes, then two records each.
 inline size_t mq_workspace_bytes(int runs, int record_floats) {

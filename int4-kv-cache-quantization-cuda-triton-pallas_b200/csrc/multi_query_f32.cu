@@ -38,6 +38,7 @@ using namespace i4kv;
 namespace {
 
 constexpr int kWarps = 8, kConsumers = 32 * kWarps, kThreads = kConsumers + 32;
+constexpr int kStreamUnits = 1, kDraftUnits = 1;  // what a stream costs besides its tiles, in tiles
 constexpr int kMaxPerSm = 4;                  // CTAs per SM the workspace is sized for
 constexpr uint64_t kWaitNs = 2000000000ull;  // bounded waits: 2 s
 
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) multi_query_f32_kernel(MultiQueryArg
   zero_idle_rows<NR, TP, D>(a);
   const int cta = blockIdx.x;
   if (warp == 0) {
-    const RunPlan mine = plan_run<NR, TP, 1, 1>(a, cta, gridDim.x);
+    const RunPlan mine = plan_run<NR, TP, kStreamUnits, kDraftUnits>(a, cta, gridDim.x);
     if (lane == 0) s_plan = mine;
   }
   __syncthreads();
@@ -517,12 +518,16 @@ cudaError_t launch_vk(int vk, const MultiQueryArgs& a, int sms, void* ws, size_t
   return launch<D, NR, INT4KV_VALUES_BF16>(a, sms, ws, n, st);
 }
 
+// Rows of a chunk.
+int chunk_of(long long rows, int dim) { return rows == 1 ? 1 : (rows <= 4 ? 4 : (rows <= 8 || dim == 256 ? 8 : 16)); }
+long long rows_of(const MultiQueryArgs& a) { return (long long)std::max(1, a.max_drafts) * a.group_q; }
+
 template <int D>
-cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
-  if (rows == 1) return launch_vk<D, 1>(vk, a, sms, ws, n, st);
-  if (rows <= 4) return launch_vk<D, 4>(vk, a, sms, ws, n, st);
+cudaError_t launch_rows(int nr, int vk, const MultiQueryArgs& a, int sms, void* ws, size_t n, cudaStream_t st) {
+  if (nr == 1) return launch_vk<D, 1>(vk, a, sms, ws, n, st);
+  if (nr == 4) return launch_vk<D, 4>(vk, a, sms, ws, n, st);
   if constexpr (D < 256) {
-    if (rows > 8) return launch_vk<D, 16>(vk, a, sms, ws, n, st);
+    if (nr == 16) return launch_vk<D, 16>(vk, a, sms, ws, n, st);
   }
   return launch_vk<D, 8>(vk, a, sms, ws, n, st);
 }
@@ -531,17 +536,20 @@ cudaError_t launch_rows(int rows, int vk, const MultiQueryArgs& a, int sms, void
 
 namespace i4kv {
 
+double multi_query_f32_units(const MultiQueryArgs& a, int dim) {
+  return mq_most_units(a, rows_of(a), chunk_of(rows_of(a), dim), 64 / kMqPage, kStreamUnits + kDraftUnits);
+}
+
 size_t multi_query_f32_workspace(int dim, int sms) {
   return mq_workspace_bytes(sms * kMaxPerSm, 2 * 16 + 16 * dim);
 }
 
 cudaError_t multi_query_f32(const MultiQueryArgs& a, int dim, int vk, int sms, void* ws, size_t ws_bytes,
                             cudaStream_t stream) {
-  const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
-  const int r = (int)std::min<long long>(rows, 1 << 20);
-  if (dim == 64) return launch_rows<64>(r, vk, a, sms, ws, ws_bytes, stream);
-  if (dim == 128) return launch_rows<128>(r, vk, a, sms, ws, ws_bytes, stream);
-  return launch_rows<256>(r, vk, a, sms, ws, ws_bytes, stream);
+  const int nr = chunk_of(rows_of(a), dim);
+  if (dim == 64) return launch_rows<64>(nr, vk, a, sms, ws, ws_bytes, stream);
+  if (dim == 128) return launch_rows<128>(nr, vk, a, sms, ws, ws_bytes, stream);
+  return launch_rows<256>(nr, vk, a, sms, ws, ws_bytes, stream);
 }
 
 }  // namespace i4kv

@@ -1591,6 +1591,12 @@ cudaError_t launch_rows(int nr, const MultiQueryArgs& a, int sms, void* ws, size
 
 namespace i4kv {
 
+double multi_query_tc_units(const MultiQueryArgs& a, int dim) {
+  const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
+  // (with the larger choice of rows: the smaller is for a few units a CTA)
+  return mq_most_units(a, rows, rows_of(rows, dim, kFewUnits), kTilePages, kStreamUnits + kDraftUnits);
+}
+
 size_t multi_query_tc_workspace(int dim, long long rows, int sms) {
   const int nr = rows_of(rows, dim, kFewUnits);  // (the larger choice)
   return mq_workspace_bytes(sms, 2 * nr + nr * dim);

@@ -7,7 +7,8 @@ import ctypes
 import pytest
 
 from helpers import pkg
-from test_draft_refusals import INVALID, OK, aligned, extend, lib, read  # noqa: F401 (lib: a fixture)
+from test_draft_refusals import (BF16 as K_BF16, F16 as K_F16, INVALID, OK, aligned, extend,  # noqa: F401
+                                 lib, read, tree)  # (lib: a fixture)
 
 torch = pytest.importorskip("torch")
 C = pkg("_C")
@@ -183,3 +184,23 @@ def test_tree_rows_that_no_sequence_has_are_zeros(calls):
     q = torch.ones((7, 2, 8))
     out = c.tree_decode(q, q, q, [1, 2], [2, 3], torch.ones(7, dtype=torch.int64))
     assert (out[:5] == 7).all() and (out[5:] == 0).all()
+
+
+def test_no_batch_is_refused_that_the_kernels_can_count(lib):  # noqa: F811
+    """Units of work are counted in 31 bits, in tiles and chunks of the kernel that runs: a large
+    serving batch (64 drafts, 8 query heads a kv head, tables of 131072 tokens) is none too many.
+    (Without a GPU what passes the checks ends at the device; with one, at the empty workspace.)"""
+    if torch.cuda.is_available():
+        pytest.skip("the answer without a GPU is asked for")
+    keep, p = aligned()
+    big = dict(d=128, max_drafts=64, rows=64, max_pages=8192, num_pages=1 << 20)
+    for kw in (dict(batch=512, hq=64, hkv=8), dict(batch=4096, hq=64, hkv=8), dict(batch=1024, hq=32, hkv=32),
+               dict(batch=65535, hq=8, hkv=1)):
+        for dtype in (K_F16, K_BF16):
+            assert tree(lib, p, **{**big, **kw}, dtype=dtype, vk=dtype) != INVALID
+    # behind a window only its tiles count
+    assert tree(lib, p, **{**big, "max_pages": 1 << 26}, batch=4096, hq=64, hkv=8, dtype=K_BF16, vk=K_BF16, window=4096,
+                sinks=64) != INVALID
+    # what is past 31 bits stays refused, in either kernel
+    assert tree(lib, p, **{**big, "max_pages": 1 << 26}, batch=4096, hq=64, hkv=8, dtype=K_BF16, vk=K_BF16) == INVALID
+    assert tree(lib, p, **{**big, "max_pages": 1 << 20}, batch=4096, hq=64, hkv=8) == INVALID
