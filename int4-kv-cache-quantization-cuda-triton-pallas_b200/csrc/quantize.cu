@@ -619,12 +619,11 @@ append_quant_kernel(AppendArgs ap, int C, int R, OutPaged op) {
 // staged rows of the old open group are read by the y = 0 CTA alone, and the
 // same CTA writes those of the new one after the barrier that follows its
 // reads: when the rows cross a group boundary the slot is reused in place.
-// Values are copied by CTAs of their own (x = slabs ..): they need no barrier, and
-// without their registers more CTAs share an SM, so one's loads meet another's
-// stores. Where each row comes from and goes to is looked up once, by the lanes of a
-// warp side by side, and every load of a CTA is in flight before the first is used.
-// Bound by HBM bytes for long chunks, by launch and three dependent loads (metadata,
-// page and row, data) for a few tokens.
+// Values are copied with the keys, or by CTAs of their own (x = slabs ..): those need no
+// barrier, and one's loads meet another's stores. Where each row comes from and goes to
+// is looked up once, by the lanes of a warp side by side, and every load of a CTA's keys
+// is in flight before the first is used. Bound by HBM bytes for long chunks, by launch
+// and three dependent loads (metadata, page and row, data) for a few tokens.
 struct ExtendArgs {
   const void* k;             // [num_src, C] keys of the kernel's input type
   const void* v;             // [num_src, C] (nullable)
@@ -673,7 +672,7 @@ __device__ __forceinline__ void store_value4(const OutPaged& op, size_t vi, cons
 // WARPS: 8 for groups of up to 64 tokens, else 16, so that a thread never holds more
 // than 8 rows' keys: with 16 rows and their values a thread, one CTA of 8 warps
 // filled an SM's registers (8 x 1000 rows of 32 heads x 128 float32 in groups of 128:
-// 140 us, now 105 us = 3.9 TB/s).
+// 140 us, now 107 us = 3.9 TB/s).
 template <int KIND, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, WARPS == 8 ? 3 : 2)
 extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
@@ -749,7 +748,7 @@ extend_quant_kernel(ExtendArgs ea, int C, int R, int slabs, OutPaged op) {
     }
     return;
   }
-  if (ea.v && (int)gridDim.x == slabs) {  // few new rows: copied here, while the keys arrive
+  if (ea.v && (int)gridDim.x == slabs) {  // copied here, while the keys arrive
 #pragma unroll 1
     for (int pos = max(start, gpos) + warp; pos < gpos + rows; pos += WARPS) {
       const int page = row_bt[pos / op.page], src = source(pos);
@@ -1366,9 +1365,14 @@ cudaError_t int4kv_cache_extend(const void* k, const void* v, int kv_dtype, int 
   if (groups > 65535) return cudaErrorInvalidValue;
   const int slabs = (int)((C + kSlab - 1) / kSlab);
   const int warps = group_tokens <= 64 ? 8 : 16;
-  // values by CTAs of their own, but for few new rows a sequence, where those CTAs would
-  // mostly look metadata up (64 x 8 rows and the read after them: 45 us with, 39 without)
-  const bool apart = v && max_rows_per_seq > 2 * warps;
+  // Values by CTAs of their own where float32 rows fill groups of 64 or more, which is
+  // bound by HBM (8 x 1000 rows of 32 x 128, groups of 128: 107 us apart, 128 with the
+  // keys; of 64: 95 and 132; 64 x 300 of 8 x 128: 87 and 93; 64 x 128: 54 and 57). Fewer
+  // rows, 16-bit ones and small groups go with the keys: those CTAs would mostly look
+  // metadata up (float32, 64 x 64 of 8 x 128: 44 us apart, 39 with; 8 x 1000 of 32 x 128 in
+  // groups of 16: 221 and 195; bfloat16, 64 x 16 of 8 x 128: 30 and 24; 8 x 1000 of 32 x 128:
+  // 144 and 135, in groups of 64 144 and 146).
+  const bool apart = v && kv_dtype == INT4KV_VALUES_F32 && group_tokens >= 64 && max_rows_per_seq >= group_tokens;
   dim3 grid((unsigned)(apart ? 2 * slabs : slabs), (unsigned)groups, batch);
   ExtendArgs ea{k, v, tok_offsets, start_pos, rows, num_src, rows ? num_rows : num_src,
                 stage_slots, k_stage, num_slots, max_rows_per_seq};

@@ -153,3 +153,43 @@ def test_padded_drafts_come_back_as_zeros(dtype):
         out = cache.tree_decode(q, k[:12], k[:12], [1, 2], [3, 2], mask)
         assert torch.equal(out[:5], want) and (out[5:] == 0).all()
     assert (cache.tree_decode(q, k[:12], k[:12], [1, 2], [0, 0], mask) == 0).all()
+
+
+@pytest.mark.parametrize("bound", [64, 63])  # values by blocks of their own, and with the keys
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_malformed_rows_and_pages_leave_the_rest(dtype, bound):
+    """Groups of 64 tokens: a row index that names no row writes zeros, a page outside the pool is
+    not written, and everything else is as it is without them."""
+    heads, d, group, n = 2, 64, 64, 40
+    k, v = (torch.randn((2 * n, heads, d), device="cuda").to(dtype) for _ in range(2))
+    rows = torch.arange(2 * n, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    table = i32([[5, 0, 3, 1], [2, 7, 4, 6]])
+
+    def go(rows, table):
+        pools = [torch.zeros((8, heads, 16, d // 2), dtype=torch.uint8, device="cuda"),
+                 torch.full((8, heads, 16, d), 5.0, dtype=dtype, device="cuda"),
+                 torch.full((8, heads, 2, d), 5.0, device="cuda")]
+        stage, status = torch.zeros((2, group, heads * d), device="cuda"), i32([0])
+        C.cache_extend(k, v, i32([0, n, 2 * n]), i32([0, 0]), i32([1, 0]), stage, table, *pools, bound, group, rows=rows,
+                       status=status)
+        return status.item(), *pools, stage
+
+    ok = go(rows, table)
+    assert ok[0] == 0
+    assert torch.equal(ok[2][table[1, :2].long()].transpose(1, 2).reshape(-1, heads, d), v.flip(0)[n:n + 32])
+    bad = rows.clone()
+    bad[3], bad[n + 17] = -1, 2 * n
+    got = go(bad, table)
+    assert got[0] == 2
+    assert (got[2][5, :, 3] == 0).all() and (got[2][7, :, 1] == 0).all()
+    same = torch.ones_like(ok[2], dtype=torch.bool)
+    same[5, :, 3] = same[7, :, 1] = False
+    assert torch.equal(got[2][same], ok[2][same])
+    broken = table.clone()
+    broken[0, 1] = 8
+    got = go(rows, broken)
+    assert got[0] == 1 and (got[2][0] == 5).all()
+    rest = [p for p in range(8) if p != 0]
+    for x, y in zip(got[1:4], ok[1:4]):
+        assert torch.equal(x[rest], y[rest])
+    assert torch.equal(got[4], ok[4])
