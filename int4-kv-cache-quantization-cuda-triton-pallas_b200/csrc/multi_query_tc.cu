@@ -1551,24 +1551,26 @@ cudaError_t launch(const MultiQueryArgs& args, int sms, void* ws, size_t ws_byte
 
 // Rows of one kv head's chunk: the smallest of 16, 32, 64, 128 that holds them
 // (head_dim 256: at most 64, the most its shared memory holds). More than 64 rows go in
-// chunks of 64 all the same where a CTA has little to do (`units` of 128-row tiles, at
-// most): a tile of 64 is not half as dear, but a stream's start and end are. (drafts
-// over 8 sequences, 128 rows a kv head, 64 against 128: 5.6 units 43 and 47 us, 12 units
-// 66 and 74; 16 x 1000 tokens, 256 rows, 21 units 135 and 115; 8 x 8192, 30 units 113 and
-// 109; 32 x 8192 410 and 320.)
-constexpr double kFewUnits = 12;
-int rows_of(long long rows, int dim, double units) {
+// chunks of 64 all the same where chunks of 128 would be `few` streams: fewer than half of
+// the CTAs, and with little to do for each (units of 128-row tiles a CTA, at most). A tile
+// of 64 rows is not half as dear, but a stream's start and end are, and where a stream is
+// shared by many CTAs each of them pays for those. (64 against 128 rows a chunk, bfloat16,
+// head_dim 128, 8 kv heads: 64 streams, 128 rows: 8 x 300 31 and 43 us, 8 x 4096 71 and
+// 75, 8 x 6000, 22 units a CTA, 89 and 91, but 8 x 8192, 30 units, 110 and 103. 32 streams of
+// 256 rows: 2 x 2048 38 and 43. 128 streams of 256 rows: 8 x 300 51 and 48, 8 x 1000 73 and
+// 67, 8 x 4096 124 and 111. 192 streams and more: 24 x 1000 105 and 87, 32 x 8192 378 and 301.)
+constexpr double kFewUnits = 24;
+int rows_of(long long rows, int dim, bool few) {
   if (rows <= 16) return 16;
   if (rows <= 32) return 32;
-  return rows <= 64 || dim == 256 || units < kFewUnits ? 64 : 128;
+  return rows <= 64 || dim == 256 || few ? 64 : 128;
 }
-// Units of a CTA in tiles of 128 rows, from the sizes that the host knows: the table's
-// width, or the window, for every sequence.
-double units_of(const MultiQueryArgs& a, long long rows, int sms) {
+// From the sizes that the host knows: the table's width, or the window, for every sequence.
+bool few_streams(const MultiQueryArgs& a, long long rows, int sms) {
   double pages = a.max_pages;
   if (a.window > 0) pages = std::min(pages, ((double)a.window + a.sinks) / kMqPage + 2);
-  return (double)a.batch * a.kv_heads * (double)((rows + 127) / 128) *
-         (std::ceil(pages / kTilePages) + 1 + kStreamUnits + kDraftUnits) / sms;
+  const double streams = (double)a.batch * a.kv_heads * (double)((rows + 127) / 128);
+  return 2 * streams < sms && streams * (std::ceil(pages / kTilePages) + 1 + kStreamUnits + kDraftUnits) / sms < kFewUnits;
 }
 
 template <int D, int NR>
@@ -1594,17 +1596,17 @@ namespace i4kv {
 double multi_query_tc_units(const MultiQueryArgs& a, int dim) {
   const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
   // (with the larger choice of rows: the smaller is for a few units a CTA)
-  return mq_most_units(a, rows, rows_of(rows, dim, kFewUnits), kTilePages, kStreamUnits + kDraftUnits);
+  return mq_most_units(a, rows, rows_of(rows, dim, false), kTilePages, kStreamUnits + kDraftUnits);
 }
 
 size_t multi_query_tc_workspace(int dim, long long rows, int sms) {
-  const int nr = rows_of(rows, dim, kFewUnits);  // (the larger choice)
+  const int nr = rows_of(rows, dim, false);  // (the larger choice)
   return mq_workspace_bytes(sms, 2 * nr + nr * dim);
 }
 
 cudaError_t multi_query_tc(const MultiQueryArgs& a, int dim, int sms, void* ws, size_t ws_bytes, cudaStream_t stream) {
   const long long rows = (long long)std::max(1, a.max_drafts) * a.group_q;
-  const int nr = rows_of(rows, dim, units_of(a, rows, sms));
+  const int nr = rows_of(rows, dim, few_streams(a, rows, sms));
   if (dim == 64) return launch_rows<64>(nr, a, sms, ws, ws_bytes, stream);
   if (dim == 128) return launch_rows<128>(nr, a, sms, ws, ws_bytes, stream);
   return launch_rows<256>(nr, a, sms, ws, ws_bytes, stream);
