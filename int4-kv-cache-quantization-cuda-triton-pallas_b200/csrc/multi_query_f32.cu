@@ -27,8 +27,11 @@
 // 16 that holds the rows of one kv head (head_dim 256: at most 8, what its
 // accumulators leave of the registers).
 // Measured (B200, 32 heads, head_dim 128, float32 values): window of 2000 over 32 x
-// 4096 tokens 220 us (5.5 TB/s, HBM and the logits' arithmetic); 4 drafts over 8 x
-// 2048 90 us (3.4 TB/s, issue and shared-memory reads).
+// 4096 tokens 217 to 234 us on different machines (5.1 to 5.5 TB/s, HBM and the logits'
+// arithmetic); 4 drafts over 8 x 2048 90 us (3.4 TB/s, issue and shared-memory reads).
+// With bfloat16 values, half the bytes, 221 and 92 us: the arithmetic alone. 16 drafts of
+// 32 query heads over 8, 8 x 2048: 257 us, four chunks of 16 rows that each read and
+// dequantize the cache again.
 #include <algorithm>
 
 #include "multi_query.cuh"
