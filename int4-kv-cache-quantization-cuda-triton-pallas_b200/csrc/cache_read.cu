@@ -205,8 +205,8 @@ extern "C" cudaError_t int4kv_cache_read(const uint8_t* k_pool, const void* v_po
     if (kind != INT4KV_VALUES_F32 && kind != INT4KV_VALUES_F16 && kind != INT4KV_VALUES_BF16)
       return cudaErrorInvalidValue;
   if (!k_pool || !sz_pool || !block_table || !start_pos || !tok_offsets) return cudaErrorInvalidValue;
+  if (num_rows == 0 || max_rows_per_seq == 0) return cudaSuccess;  // (outputs of no rows may have no address)
   if ((v_pool != nullptr) != (v_out != nullptr)) return cudaErrorInvalidValue;
-  if (num_rows == 0 || max_rows_per_seq == 0) return cudaSuccess;
   if (!k_out || !aligned16(k_pool) || !aligned16(sz_pool) || !aligned16(v_pool) || !aligned16(k_out) ||
       !aligned16(v_out))
     return cudaErrorInvalidValue;

@@ -204,3 +204,12 @@ def test_no_batch_is_refused_that_the_kernels_can_count(lib):  # noqa: F811
     # what is past 31 bits stays refused, in either kernel
     assert tree(lib, p, **{**big, "max_pages": 1 << 26}, batch=4096, hq=64, hkv=8, dtype=K_BF16, vk=K_BF16) == INVALID
     assert tree(lib, p, **{**big, "max_pages": 1 << 20}, batch=4096, hq=64, hkv=8) == INVALID
+
+
+def test_an_empty_read_is_no_error(lib):  # noqa: F811
+    """Outputs of no rows have no address."""
+    keep, p = aligned()
+    assert read(lib, p, rows=0, ko=None, vo=None) == OK
+    assert read(lib, p, max_rows=0, ko=None, vo=None) == OK
+    assert read(lib, p, rows=0, vp=None, ko=None, vo=None) == OK
+    assert read(lib, p, vo=None) == INVALID and read(lib, p, vp=None) == INVALID

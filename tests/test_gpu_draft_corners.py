@@ -193,3 +193,16 @@ def test_malformed_rows_and_pages_leave_the_rest(dtype, bound):
     for x, y in zip(got[1:4], ok[1:4]):
         assert torch.equal(x[rest], y[rest])
     assert torch.equal(got[4], ok[4])
+
+
+@pytest.mark.parametrize("values", [F32, BF16, None])
+def test_an_empty_range_reads_as_no_rows(values):
+    cache = P.PagedKVCache(8, 2, 64, group_tokens=32, device="cuda", values=values is not None,
+                           value_dtype=values or F32)
+    k = torch.randn((20, 2, 64), device="cuda")
+    cache.extend([1, 2], [20, 0], k, k if values is not None else None)
+    for seq, start, stop in ((1, 0, 0), (1, 20, 20), (1, 7, 7), (2, 0, None)):
+        got_k, got_v = cache.read(seq, start, stop, dtype=BF16)
+        assert got_k.shape == (0, 2, 64) and got_k.dtype == BF16
+        assert got_v is None if values is None else got_v.shape == (0, 2, 64)
+    cache.check()
