@@ -92,6 +92,11 @@ class PagedKVCache:
                                           (4, "a wait that ran out")) if bits & bit]
             raise RuntimeError("paged KV cache met " + ", ".join(met))
 
+    def _ready(self, t: torch.Tensor) -> torch.Tensor:
+        """``t`` on the device, contiguous and on a 16-byte boundary, as the draft operators read it."""
+        t = t.to(self.device).contiguous()
+        return t.clone() if t.data_ptr() % 16 else t
+
     # ---- page allocation ----
     def _alloc(self, n: int) -> List[int]:
         if n > len(self._free):
@@ -243,10 +248,10 @@ class PagedKVCache:
                 for s, n in zip(ids, n_new)]
         if sum(max(0, n) for n in need) > len(self._free):
             raise MemoryError(f"paged KV cache out of pages: need {sum(need)}, {len(self._free)} free")
-        k = keys.to(self.device).contiguous()
+        k = self._ready(keys)
         v = None
         if values is not None and self.v_pool is not None:
-            v = values.to(self.device).contiguous()
+            v = self._ready(values)
             if v.dtype != k.dtype:  # float32 holds either: neither is rounded to the other's type
                 k, v = k.float(), v.float()
         if rows is not None:
@@ -303,7 +308,7 @@ class PagedKVCache:
         query [B, heads, head_dim] float32, or of the value pool's 16-bit type.
         """
         bt, sl = self.block_table(list(seq_ids))
-        return _C.paged_window_decode(query.to(self.device).contiguous(), self.k_pool, self.v_pool,
+        return _C.paged_window_decode(self._ready(query), self.k_pool, self.v_pool,
                                       self.sz_pool, bt, sl, window=window, sinks=sinks,
                                       group_tokens=self.group_tokens, status=self.status)
 
@@ -323,8 +328,8 @@ class PagedKVCache:
         bt, sl = self.block_table(ids)
         offs = torch.from_numpy(np.concatenate([[0], np.cumsum(n)]).astype(np.int32))
         out = _C.paged_tree_decode(
-            query.to(self.device).contiguous(), k_draft.to(self.device).contiguous(),
-            v_draft.to(self.device).contiguous(), mask.to(self.device), offs.to(self.device),
+            self._ready(query), self._ready(k_draft), self._ready(v_draft),
+            mask.to(self.device).contiguous(), offs.to(self.device),
             self.k_pool, self.v_pool, self.sz_pool, bt, sl, max_drafts=max(n),
             group_tokens=self.group_tokens, window=window, sinks=sinks, status=self.status)
         if sum(n) < out.shape[0]:

@@ -213,3 +213,21 @@ def test_an_empty_read_is_no_error(lib):  # noqa: F811
     assert read(lib, p, max_rows=0, ko=None, vo=None) == OK
     assert read(lib, p, rows=0, vp=None, ko=None, vo=None) == OK
     assert read(lib, p, vo=None) == INVALID and read(lib, p, vp=None) == INVALID
+
+
+def misaligned(t):
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape)
+    assert flat.copy_(t).data_ptr() % 16
+    return flat
+
+
+def test_tensors_that_start_anywhere_are_taken(calls):
+    """The kernels load 16 bytes at a time: what does not start on such a boundary is copied."""
+    c = cache()
+    c.extend([1], [3], misaligned(rows(3, BF16)), misaligned(rows(3, BF16, 1)))
+    q = misaligned(rows(1, F32))
+    c.tree_decode(q, q, q, [1], [1], torch.ones(1, dtype=torch.int64))
+    c.window_decode(q, [1], 5)
+    for (_, args, _), n in zip(calls, (2, 3, 1)):
+        assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() for t in args[:n])
+    assert torch.equal(calls[0][1][0], rows(3, BF16)) and torch.equal(calls[0][1][1], rows(3, BF16, 1))
