@@ -206,3 +206,18 @@ def test_an_empty_range_reads_as_no_rows(values):
         assert got_k.shape == (0, 2, 64) and got_k.dtype == BF16
         assert got_v is None if values is None else got_v.shape == (0, 2, 64)
     cache.check()
+
+
+@pytest.mark.parametrize("dtype,values", [(F32, F32), (F32, F16), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("lens,counts", [([3000, 20, 0], [9, 3, 1]), ([17], [2]), ([100] * 40, [5] * 40), ([0, 0], [1, 0])])
+def test_a_workspace_may_hold_anything(dtype, values, lens, counts):
+    """Leftovers of other calls, notes of streams among them: the results are the same bits."""
+    s = Step(lens, counts, 8, 2, 128, 64, dtype, values, seed=7)
+    other = Step([2500, 2500], [60, 64], 8, 2, 128, 64, dtype, values, seed=8)
+    need = C.paged_attention_workspace_bytes(max(len(lens), 2), 8, 2, 128, 64)
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    want = s.run(workspace=ws, max_drafts=64)
+    for leave in (lambda: ws.fill_(255), lambda: ws.fill_(1), lambda: ws.view(torch.int32)[:need // 4].random_(0, 200),
+                  lambda: ws.random_(0, 256), lambda: other.run(workspace=ws)):
+        leave()
+        assert torch.equal(s.run(workspace=ws, max_drafts=64), want)
