@@ -480,33 +480,31 @@ cudaError_t int4kv_cache_read(const uint8_t* k_pool, const void* v_pool, int val
 cudaError_t int4kv_paged_attention_workspace_size(int batch, int num_q_heads, int num_kv_heads,
                                                   int head_dim, int max_drafts, size_t* bytes);
 
-/* Attention of each sequence's drafted tokens over its cache and, through
- * tree_mask, over one another: the verification step of speculative decoding.
- * Rows draft_offsets[b] .. draft_offsets[b+1]-1 (at most max_drafts <=
- * INT4KV_MAX_DRAFTS; rows of query / k_draft / v_draft / out past the last
- * sequence's are left as they were) are the drafts of sequence b, whose cache
- * holds seq_lens[b] tokens, none of them drafts. Draft t sees draft u of its
- * sequence iff bit u of tree_mask[row of t] is set (its own bit included, if it
- * is to see itself), and its position is seq_lens[b] + its ancestors, the
- * other bits set. With window > 0 a query at position p sees position j only
- * if j > p - window or j < sinks, cached and drafted alike; window 0: all. No
- * softmax scale (the queries carry it); a row that sees nothing gives zeros.
- * query / out [num_rows, num_q_heads, head_dim], k_draft / v_draft [num_rows,
- * num_kv_heads, head_dim], all of type qkv_dtype: float32 with any value pool,
- * or float16 / bfloat16 with a value pool of the same type (keys and softmax
- * weights are then rounded to 16 bits for the tensor cores, sums stay
- * float32; bfloat16 logits must stay within +- 2^29). head_dim 64, 128 or 256,
- * pages of 16 tokens, tensors 16-byte aligned, `out` apart from the inputs. What stands behind a sequence's length,
- * outside every window or in drafts nobody sees is never part of a result, even
- * NaN; a 16-bit cached value that some row of a sequence sees must be finite for
- * the results of its other rows to be. Pages outside the pool are not read: their
- * tokens are not seen (INT4KV_STATUS_BAD_PAGE); nor are those of a group whose first
- * page, which keeps its scales, is outside (with a window, that page may lie before it). Offsets outside [0, num_rows] or
- * too many drafts skip the sequence's drafts, a bad length is clamped to the
- * table (INT4KV_STATUS_BAD_LENGTH). A batch of more than 2^31 - 1 tiles (of 128 cached
- * tokens and up to 128 rows of a kv head, 64 and 16 in float32, counted from the table's
- * width or the window) is refused. Results do not depend on the order of any
- * atomics: equal calls on equal devices give equal bits. */
+/* Attention of each sequence's drafted tokens over its cache and, through tree_mask,
+ * over one another: the verification step of speculative decoding. Rows draft_offsets[b]
+ * .. draft_offsets[b+1]-1 (at most max_drafts <= INT4KV_MAX_DRAFTS; rows of query /
+ * k_draft / v_draft / out past the last sequence's are left as they were) are the drafts
+ * of sequence b, whose cache holds seq_lens[b] tokens, none of them drafts. Draft t sees
+ * draft u of its sequence iff bit u of tree_mask[row of t] is set (its own bit included,
+ * if it is to see itself), and its position is seq_lens[b] + its ancestors, the other
+ * bits set. With window > 0 a query at position p sees position j only if j > p - window
+ * or j < sinks, cached and drafted alike; window 0: all. No softmax scale (the queries
+ * carry it); a row that sees nothing gives zeros. query / out [num_rows, num_q_heads,
+ * head_dim], k_draft / v_draft [num_rows, num_kv_heads, head_dim], all of type
+ * qkv_dtype: float32 with any value pool, or float16 / bfloat16 with a value pool of the
+ * same type (keys and softmax weights are then rounded to 16 bits for the tensor cores,
+ * sums stay float32; bfloat16 logits must stay within +- 2^29). head_dim 64, 128 or 256,
+ * pages of 16 tokens, tensors 16-byte aligned, `out` apart from the inputs. What stands
+ * behind a sequence's length, outside every window or in drafts nobody sees is never
+ * part of a result, even NaN; a 16-bit cached value that some row of a sequence sees
+ * must be finite for the results of its other rows to be. Pages outside the pool are not
+ * read: their tokens are not seen (INT4KV_STATUS_BAD_PAGE); nor are those of a group
+ * whose first page, which keeps its scales, is outside (with a window, that page may lie
+ * before it). Offsets outside [0, num_rows] or too many drafts skip the sequence's
+ * drafts, a bad length is clamped to the table (INT4KV_STATUS_BAD_LENGTH). A batch of
+ * more than 2^31 - 1 tiles (of 128 cached tokens and up to 128 rows of a kv head, 64 and
+ * 16 in float32, counted from the table's width or the window) is refused. Results do
+ * not depend on the order of any atomics: equal calls on equal devices give equal bits. */
 cudaError_t int4kv_paged_tree_decode(const void* query, const void* k_draft, const void* v_draft,
                                      int qkv_dtype, const int64_t* tree_mask,
                                      const int32_t* draft_offsets, int num_rows, int max_drafts,

@@ -47,7 +47,8 @@
 // over 32 x 8192 tokens 84 us (4.1 TB/s of the cache), 16 drafts over 8 x 8192 68 us,
 // 32 drafts over 32 x 8192 300 to 318 us on different machines (430 to 460 TFLOP/s);
 // the float32 kernel took 9614 us for the last. float16 at head_dim 64, the same
-// window: 68 us (2.6 TB/s: a tile has half the bytes and the same chain). Bound by a tile's chain through the roles, foremost the softmax
+// window: 68 us (2.6 TB/s: a tile has half the bytes and the same chain).
+// Bound by a tile's chain through the roles, foremost the softmax
 // (1.15 us a tile at 16 rows, 2 us at 128, 0.5 us of which are exponentials), not by
 // HBM or the tensor pipe (under 13 % active).
 #include <cuda.h>
